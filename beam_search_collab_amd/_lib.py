@@ -1,6 +1,7 @@
 """ctypes bindings of the two C-ABI libraries built in-tree.
 
 libbs_hip.so  (include/bs_hip.h)   gfx950 search kernels
+              (include/bs_embed.h) encoder operators
 libbs_host.so (include/bs_host.h)  host formats, index construction, input preparation
 
 Loading fails loudly when a library is missing: there is no CPU fallback for the
@@ -50,6 +51,20 @@ class Stats(C.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_}
 
 
+i64 = C.c_int64
+
+
+class AttentionArgs(C.Structure):
+    """bs_attention_args (include/bs_embed.h)."""
+    _fields_ = (
+        [(n, vp) for n in ("q", "k", "v", "out", "lse", "q_offsets", "k_offsets")]
+        + [(n, i64) for n in ("q_stride", "q_head_stride", "k_stride", "k_head_stride", "v_stride", "v_head_stride",
+                              "out_stride", "out_head_stride")]
+        + [(n, u32) for n in ("q_tokens", "k_tokens", "sequences", "heads", "kv_heads", "head_dim", "longest_q", "longest_k")]
+        + [("type", i32), ("causal", i32), ("scale", f32)]
+    )
+
+
 # name -> (restype, argtypes)
 HIP_API = {
     "bs_index_create": (C.c_int, [vp, vp, u64, u32, u32, P(vp)]),
@@ -81,6 +96,17 @@ HIP_API = {
     "bs_debug_groundtruth": (C.c_int, [vp, vp, u64, u32, u64, vp, vp]),
     "bs_debug_gt_plan": (C.c_int, [u64, u64, u32, vp]),
     "bs_debug_gt_products": (C.c_int, [vp, u32, vp, u32, C.c_int, vp]),
+}
+
+# include/bs_embed.h, in libbs_hip.so too
+EMBED_API = {
+    "bs_layer_norm": (C.c_int, [vp, i64, vp, vp, C.c_int, f32, vp, i64, vp, vp, u64, u32, C.c_int, vp]),
+    "bs_layer_norm_backward": (C.c_int, [vp, i64, vp, i64, vp, vp, vp, C.c_int, vp, i64, vp, vp, u64, u32, C.c_int, vp, u64, vp]),
+    "bs_layer_norm_backward_workspace": (C.c_int, [u64, u32, C.c_int, P(u64)]),
+    "bs_linear": (C.c_int, [vp, i64, vp, i64, vp, vp, i64, vp, i64, u64, u32, u32, C.c_int, C.c_int, C.c_int, vp, u64, vp]),
+    "bs_linear_workspace": (C.c_int, [u64, u32, u32, P(u64)]),
+    "bs_attention": (C.c_int, [P(AttentionArgs), vp, u64, vp]),
+    "bs_attention_workspace": (C.c_int, [P(AttentionArgs), P(u64)]),
 }
 
 HOST_API = {
@@ -124,7 +150,7 @@ def hip():
             raise ImportError(
                 f"{HIP_LIB_PATH} is missing: build it with "
                 "`python -c 'import __graft_entry__ as g; g.build()'` (make -C beam_search_collab_amd/csrc)")
-        _hip = _bind(C.CDLL(HIP_LIB_PATH), HIP_API)
+        _hip = _bind(C.CDLL(HIP_LIB_PATH), {**HIP_API, **EMBED_API})
     return _hip
 
 

@@ -6,6 +6,8 @@
 // adjacent columns.
 #include "bs_embed.hpp"
 
+#include <type_traits>
+
 namespace {
 using namespace bse;
 
@@ -32,103 +34,466 @@ struct Params {
     int act;
 };
 
-__device__ inline float activate(float z, int act) {
-    switch (act) {
-        case BS_ACT_RELU: return z < 0.0f ? 0.0f : z;
-        case BS_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case BS_ACT_GELU_TANH: {
+// one branch for all values: the branches are the call's, not the lanes'
+template <int N>
+__device__ inline void activate(float (&z)[N], int act) {
+    if (act == BS_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] = z[j] < 0.0f ? 0.0f : z[j];
+    } else if (act == BS_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] = 0.5f * z[j] * (1.0f + erff(z[j] * 0.70710678118654752f));
+    } else if (act == BS_ACT_GELU_TANH) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
             // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
-            const float u = 0.79788456080286536f * fmaf(0.044715f * z * z, z, z);
-            return z / (1.0f + __expf(-2.0f * u));
+            const float u = 0.79788456080286536f * fmaf(0.044715f * z[j] * z[j], z[j], z[j]);
+            z[j] = z[j] / (1.0f + __expf(-2.0f * u));
         }
-        case BS_ACT_SILU: return z / (1.0f + __expf(-z));
-        default: return z;
+    } else if (act == BS_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] = z[j] / (1.0f + __expf(-z[j]));
     }
 }
 
-// four adjacent columns of one row: n of them are inside
+// eight adjacent columns of one row: those from `first` on, and inside
 template <typename T, typename O>
-__device__ inline void finish(const Params& p, uint32_t row, uint32_t col, f32x4 z) {
-    if (row >= p.rows || col >= p.cols) return;
+__device__ inline void finish(const Params& p, uint32_t row, uint32_t col, float (&z)[8], int first = 0) {
     const int n = static_cast<int>(p.cols - col);
     if (p.bias) {
-        const Vec<T, 4> b = load_some<T, 4>(static_cast<const T*>(p.bias) + col, n);
+        const Vec<T, 8> b = load_some<T, 8>(static_cast<const T*>(p.bias) + col, n);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[j] += static_cast<float>(b[j]);
+        for (int j = 0; j < 8; ++j) z[j] += static_cast<float>(b[j]);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) z[j] = activate(z[j], p.act);
+    activate(z, p.act);
     if (p.residual) {
-        const Vec<O, 4> r = load_some<O, 4>(static_cast<const O*>(p.residual) + static_cast<int64_t>(row) * p.rs + col, n);
+        const Vec<O, 8> r = load_some<O, 8>(static_cast<const O*>(p.residual) + static_cast<int64_t>(row) * p.rs + col, n);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[j] += static_cast<float>(r[j]);
+        for (int j = 0; j < 8; ++j) z[j] += static_cast<float>(r[j]);
     }
-    Vec<O, 4> o;
+    Vec<O, 8> o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = static_cast<O>(z[j]);
-    store_some<O, 4>(static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.os + col, o, n);
+    for (int j = 0; j < 8; ++j) o[j] = static_cast<O>(z[j]);
+    O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.os + col;
+    if (first <= 0 && n >= 8) {
+        store_any<O, 8>(out, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j >= first && j < n) out[j] = o[j];
+    }
 }
 
-// 16-byte chunk c (0..7) of tile row r (64 inner elements = 128 bytes): the 16 lanes of a quarter wave
-// read one chunk of 16 rows, which this spreads over all banks
-__device__ inline int place(int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 7)) << 3); }
+typedef __attribute__((address_space(1))) const void* global_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr;
 
-// Any sizes, strides and alignments: tiles of 128 x 128, inner steps of 64, through registers.
-template <typename T, typename O>
-__global__ __launch_bounds__(256) void linear_kernel(Params p) {
-    __shared__ __attribute__((aligned(16))) T tx[128 * 64], tw[128 * 64];
+// Meets the workgroup's other waves once all but this wave's N youngest moves to LDS are done.  Products
+// written before it stay before it, and with them the waits for the LDS reads that feed them; reads that
+// are still on their way at the meeting are of a step that nobody overwrites yet.
+template <int N>
+__device__ inline void meet() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);  // vmcnt(N)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Tiles of BM rows of x by BN rows of w; WM x WN waves; inner steps of BK; NS steps in LDS.
+template <int BM_, int BN_, int WM_, int WN_, int BK_, int NS_, int PER_CU_>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_, NS = NS_, PER_CU = PER_CU_;
+    static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
+    static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 results of a wave
+    static constexpr int CH = BK / 8;                           // 16-byte chunks of a row
+    static constexpr int STEP = (BM + BN) * BK;                 // elements of a step: rows of x, then of w
+    static constexpr int MOVES = (BM + BN) * CH / THREADS;      // 16-byte moves of a thread per step
+    static constexpr int JOIN = 32 * (TN * 32 + 4) * 4;         // bytes in which a wave turns 32 rows of results
+    static constexpr int LDS = NS * STEP * 2 > WAVES * JOIN ? NS * STEP * 2 : WAVES * JOIN;
+    // the 16 lanes of a quarter wave read one chunk of 16 rows: spread over the 256 bytes of all banks
+    __device__ static int swizzle(int r, int c) { return BK == 64 ? c ^ ((r >> 1) & 7) : c ^ ((r >> 2) & 3); }
+    __device__ static int place(int r, int c) { return r * BK + swizzle(r, c) * 8; }
+};
+
+// Direct: rows are 16-byte aligned, whole steps go from memory to LDS without registers
+template <typename T, typename O, typename C, bool Direct>
+__global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void linear_kernel(Params p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    T* buf = reinterpret_cast<T*>(lds);
     const T* x = static_cast<const T*>(p.x);
     const T* w = static_cast<const T*>(p.w);
-    const uint32_t across = (p.cols + 127) / 128, m0 = blockIdx.x / across * 128, n0 = blockIdx.x % across * 128;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, h = lane >> 5;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    f32x16 acc[2][2] = {};
-    for (uint32_t k0 = 0; k0 < p.inner; k0 += 64) {
-        __syncthreads();
+    // Workgroup b runs on XCD b mod 8: each XCD takes a contiguous run of tiles, 8 tile rows high, so that
+    // the tiles in flight on it share operands in its L2.
+    const uint32_t mt = (p.rows + C::BM - 1) / C::BM, nt = (p.cols + C::BN - 1) / C::BN, total = mt * nt;
+    const uint32_t xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+    const uint32_t id = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
+    const uint32_t band = id / (8 * nt), high = mt - band * 8 < 8 ? mt - band * 8 : 8, in = id - band * 8 * nt;
+    const uint32_t m0 = (band * 8 + in % high) * C::BM, n0 = in / high * C::BN;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
+    const int wm = wave / C::WN * C::TM * 32, wn = wave % C::WN * C::TN * 32;
+
+    // this thread's moves: 16 bytes each, to LDS positions that are linear over the workgroup
+    const T* from[C::MOVES];
+    int chunk[C::MOVES];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = i * 256 + threadIdx.x, r = at >> 3, c = at & 7;
-            const uint32_t k = k0 + c * 8;
-            const int n = static_cast<int>(p.inner) - static_cast<int>(k);
-            // rows past the end repeat the last one: their products are not stored
-            const uint32_t m = m0 + r < p.rows ? m0 + r : p.rows - 1, v = n0 + r < p.cols ? n0 + r : p.cols - 1;
-            Vec<T, 8> a = {}, b = {};
-            if (n > 0) {
-                a = load_some<T, 8>(x + static_cast<int64_t>(m) * p.xs + k, n);
-                b = load_some<T, 8>(w + static_cast<int64_t>(v) * p.ws + k, n);
-            }
-            *reinterpret_cast<Vec<T, 8>*>(tx + place(r, c)) = a;
-            *reinterpret_cast<Vec<T, 8>*>(tw + place(r, c)) = b;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            Vec<T, 8> a[2], b[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i] = *reinterpret_cast<const Vec<T, 8>*>(tw + place(wn + i * 32 + l, s * 2 + h));
-                b[i] = *reinterpret_cast<const Vec<T, 8>*>(tx + place(wm + i * 32 + l, s * 2 + h));
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = Mma<T>::go(a[i], b[j], acc[i][j]);
+    for (int i = 0; i < C::MOVES; ++i) {
+        const int at = i * C::THREADS + threadIdx.x, r = at / C::CH;
+        chunk[i] = C::swizzle(r, at % C::CH);
+        // rows past the end repeat the last one: their products are not stored
+        if (r < C::BM) {
+            const uint32_t m = m0 + r < p.rows ? m0 + r : p.rows - 1;
+            from[i] = x + static_cast<int64_t>(m) * p.xs + chunk[i] * 8;
+        } else {
+            const uint32_t n = n0 + r - C::BM < p.cols ? n0 + r - C::BM : p.cols - 1;
+            from[i] = w + static_cast<int64_t>(n) * p.ws + chunk[i] * 8;
         }
     }
+    const uint32_t whole = p.inner / C::BK, steps = (p.inner + C::BK - 1) / C::BK;
+    auto move = [&](uint32_t t, int slot, int first = 0, int n = C::MOVES) {  // Direct
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = first; i < first + n; ++i)
+            __builtin_amdgcn_global_load_lds((global_ptr)(from[i] + static_cast<size_t>(t) * C::BK),
+                                             (lds_ptr)(buf + slot * C::STEP + (i * C::THREADS + wave * 64) * 8), 16, 0, 0);
+    };
+    auto fetch = [&](uint32_t t, Vec<T, 8> (&v)[C::MOVES]) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < C::MOVES; ++i) {
+            const int left = static_cast<int>(p.inner) - static_cast<int>(t * C::BK) - chunk[i] * 8;
+            v[i] = left > 0 ? load_some<T, 8>(from[i] + static_cast<size_t>(t) * C::BK, left) : Vec<T, 8>{};
+        }
+    };
+    auto put = [&](int slot, const Vec<T, 8> (&v)[C::MOVES]) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 z = {acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
-                finish<T, O>(p, m0 + wm + j * 32 + l, n0 + wn + i * 32 + q * 8 + h * 4, z);
+        for (int i = 0; i < C::MOVES; ++i)
+            *reinterpret_cast<Vec<T, 8>*>(buf + slot * C::STEP + (i * C::THREADS + threadIdx.x) * 8) = v[i];
+    };
+    f32x16 acc[C::TN][C::TM] = {};
+    struct Parts {
+        Vec<T, 8> a[C::TN], b[C::TM];
+    };
+    auto read = [&](int slot, int s, Parts& f) {  // 16 inner elements
+        const T* tx = buf + slot * C::STEP;
+        const T* tw = tx + C::BM * C::BK;
+#pragma unroll
+        for (int i = 0; i < C::TN; ++i) f.a[i] = *reinterpret_cast<const Vec<T, 8>*>(tw + C::place(wn + i * 32 + l, s * 2 + h));
+#pragma unroll
+        for (int j = 0; j < C::TM; ++j) f.b[j] = *reinterpret_cast<const Vec<T, 8>*>(tx + C::place(wm + j * 32 + l, s * 2 + h));
+    };
+    auto product = [&](const Parts& f, int from_, int to) {
+#pragma unroll
+        for (int i = from_; i < to; ++i)
+#pragma unroll
+            for (int j = 0; j < C::TM; ++j) acc[i][j] = Mma<T>::go(f.a[i], f.b[j], acc[i][j]);
+    };
+    auto multiply = [&](int slot) {
+        Parts f;
+#pragma unroll
+        for (int s = 0; s < C::BK / 16; ++s) {
+            read(slot, s, f);
+            product(f, 0, C::TN);
+        }
+    };
+    if (Direct) {
+        // At meeting t steps t and t + 1 are in LDS and nobody reads step t - 1 any more, whose place step
+        // t + NS - 1 gets.  Operands are read one part (16 inner elements) ahead of their products, across the
+        // meeting too.  A move past the last step repeats the last one, so that every wait counts the same.
+        const uint32_t last = whole ? whole - 1 : 0;
+        if (whole) {
+            Parts f[2];
+#pragma unroll
+            for (int i = 0; i < C::NS - 1; ++i) move(min(static_cast<uint32_t>(i), last), i);
+            meet<(C::NS - 2) * C::MOVES>();
+            read(0, 0, f[0]);
+            int slot = 0;
+            for (uint32_t t = 0; t < whole; ++t) {
+                meet<(C::NS - 3) * C::MOVES>();
+                move(min(t + C::NS - 1, last), slot == 0 ? C::NS - 1 : slot - 1);
+                const int next = slot == C::NS - 1 ? 0 : slot + 1;
+#pragma unroll
+                for (int s = 0; s < C::BK / 16; ++s) {
+                    product(f[s & 1], 0, C::TN / 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (s + 1 < C::BK / 16)
+                        read(slot, s + 1, f[(s + 1) & 1]);
+                    else
+                        read(next, 0, f[(s + 1) & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    product(f[s & 1], C::TN / 2, C::TN);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                slot = next;
             }
+        }
+        meet<0>();
+        __syncthreads();
+        if (steps > whole) {
+            Vec<T, 8> v[C::MOVES];
+            fetch(whole, v);
+            put(0, v);
+            __syncthreads();
+            multiply(0);
+            __syncthreads();
+        }
+    } else {
+        Vec<T, 8> v[C::MOVES];
+        fetch(0, v);
+        put(0, v);
+        for (uint32_t t = 0; t < steps; ++t) {
+            __syncthreads();
+            if (t + 1 < steps) fetch(t + 1, v);
+            multiply(t & 1);
+            if (t + 1 < steps) put(~t & 1, v);
+        }
+        __syncthreads();
+    }
+    // a wave turns 32 rows of its results at a time: a lane then has 8 adjacent columns
+    constexpr int W = C::TN * 32, PITCH = W + 4, LANES = W / 8;
+    float* turn = reinterpret_cast<float*>(lds + wave * C::JOIN);
+    auto spread = [&](auto J) {
+        constexpr int j = decltype(J)::value;
+        if constexpr (j < C::TM) {
+#pragma unroll
+            for (int i = 0; i < C::TN; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4*>(turn + l * PITCH + i * 32 + q * 8 + h * 4) =
+                        f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+        }
+    };
+    static_assert(C::TM <= 4, "cases below");
+#pragma unroll 1
+    for (int j = 0; j < C::TM; ++j) {  // not unrolled: the epilogue's code stays in the instruction cache
+        switch (j) {
+            case 0: spread(std::integral_constant<int, 0>()); break;
+            case 1: spread(std::integral_constant<int, 1>()); break;
+            case 2: spread(std::integral_constant<int, 2>()); break;
+            default: spread(std::integral_constant<int, 3>()); break;
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int k = 0; k < 32 * LANES / 64; ++k) {
+            const int r = k * (64 / LANES) + lane / LANES, c = lane % LANES * 8;
+            const uint32_t row = m0 + wm + j * 32 + r, col = n0 + wn + c;
+            float z[8];
+            const f32x4 z0 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + c), z1 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + c + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = z0[e], z[4 + e] = z1[e];
+            if (row < p.rows && col < p.cols) finish<T, O>(p, row, col, z);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+using Mid = Tile<128, 128, 2, 2, 32, 4, 2>;
+
+// Large products: tiles of 256 x 256 by 8 waves of 128 (rows of x) x 64 (rows of w), inner steps of 64.
+//
+// A step's operands take 64 KB of LDS and two steps fit, so that the way from memory to LDS would have one
+// step's time.  It has one and a half: a step is four phases, and the quarters of its operands (x0, x1: the
+// first and second 64 rows of every wave; w0, w1: the first and second 32) are read into registers a phase
+// before their products, whereupon the moves of step t + 2 into that quarter start.
+//   phase 0: read w1(t)              products w0 x0
+//   phase 1: read x1(t)              products w1 x0    move x0, w0 (t + 2)
+//   phase 2:                         products w0 x1    move w1 (t + 2)
+//   phase 3: read x0, w0 (t + 1)     products w1 x1    move x1 (t + 2)
+// A workgroup per CU goes through its tiles without a break: the moves of the next tile's first steps are
+// under way while a tile's results are written.  A tile that would pass an edge is shifted back inside and
+// does not write what its neighbour writes.
+template <typename T, typename O>
+__global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int STEP = 512 * 64;  // elements: 256 rows of x, then 256 of w
+    T* buf = reinterpret_cast<T*>(lds);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
+    float* turn = reinterpret_cast<float*>(lds + 2 * STEP * 2) + wave * 1024;
+    const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+    auto swizzle = [](int r, int c) { return c ^ ((r >> 1) & 7); };
+
+    const uint32_t mt = (p.rows + 255) / 256, nt = (p.cols + 255) / 256, total = mt * nt;
+    // Workgroup b runs on XCD b mod 8: each XCD takes a contiguous run of tiles, 8 tile rows high, so that
+    // the tiles in flight on it share operands in its L2.
+    const uint32_t xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+    const uint32_t run = xcd * q8 + (xcd < r8 ? xcd : r8), end = run + q8 + (xcd < r8 ? 1 : 0), stride = gridDim.x >> 3;
+    uint32_t id = run + (blockIdx.x >> 3);
+    if (id >= end) return;
+    auto origin = [&](uint32_t i, uint32_t& m, uint32_t& n) {
+        const uint32_t band = i / (8 * nt), high = min(mt - band * 8, 8u), in = i - band * 8 * nt;
+        m = (band * 8 + in % high) * 256;
+        n = in / high * 256;
+    };
+
+    // this thread's part of a move of 64 rows; those of w are 32 rows of each of two waves' 64
+    const int r = threadIdx.x >> 3, c = swizzle(r, threadIdx.x & 7), rw = (r & 31) + (r >> 5) * 64;
+    const uint32_t vx = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.xs) * 2 + c * 16;
+    const uint32_t vw = static_cast<uint32_t>(rw) * static_cast<uint32_t>(p.ws) * 2 + c * 16;
+    const int rows8 = wave * 8, rows8w = (rows8 & 31) + (rows8 >> 5) * 64;
+    struct Source {
+        const char *x, *w;  // the tile's first rows, at the step to be moved
+    };
+    const uint64_t xhop = static_cast<uint64_t>(p.xs) * 2, whop = static_cast<uint64_t>(p.ws) * 2;
+    auto move_x = [&](const Source& f, int slot, int g, int i) {
+        __builtin_amdgcn_global_load_lds((global_ptr)(f.x + (i * 128 + g * 64) * xhop + vx),
+                                         (lds_ptr)(buf + slot * STEP + (i * 128 + g * 64 + rows8) * 64), 16, 0, 0);
+    };
+    auto move_w = [&](const Source& f, int slot, int g, int i) {
+        __builtin_amdgcn_global_load_lds((global_ptr)(f.w + (i * 128 + g * 32) * whop + vw),
+                                         (lds_ptr)(buf + slot * STEP + (256 + i * 128 + g * 32 + rows8w) * 64), 16, 0, 0);
+    };
+    Vec<T, 8> fx[4][4], fw[2][4];
+    // a lane's place in a row of LDS: rows of operands differ by multiples of 32, so the swizzle is the lane's
+    int at[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) at[s] = l * 64 + swizzle(l, s * 2 + h) * 8;
+    auto read_x = [&](int slot, int j, int s) {
+        fx[j][s] = *reinterpret_cast<const Vec<T, 8>*>(buf + slot * STEP + (wm + j * 32) * 64 + at[s]);
+    };
+    auto read_w = [&](int slot, int i, int s) {
+        fw[i][s] = *reinterpret_cast<const Vec<T, 8>*>(buf + slot * STEP + (256 + wn + i * 32) * 64 + at[s]);
+    };
+    f32x16 acc[2][4];
+    // Eight matrix instructions; `between` puts the phase's reads and moves between them, one or two at a time:
+    // issued in a row they would keep the wave from its products until the memory pipes have taken them all.
+    auto product = [&](int i, int j, auto between) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            acc[i][j + (n & 1)] = Mma<T>::go(fw[i][n >> 1], fx[j + (n & 1)][n >> 1], acc[i][j + (n & 1)]);
+            __builtin_amdgcn_sched_barrier(0);
+            between(n);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    const uint32_t steps = p.inner / 64;
+    uint32_t m0, n0;
+    origin(id, m0, n0);
+    auto source = [&](uint32_t m, uint32_t n) {
+        return Source{static_cast<const char*>(p.x) + min(m, p.rows - 256) * xhop, static_cast<const char*>(p.w) + min(n, p.cols - 256) * whop};
+    };
+    Source from = source(m0, n0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) move_x(from, t, 0, i), move_w(from, t, 0, i);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) move_w(from, t, 1, i);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) move_x(from, t, 1, i);
+        from.x += 128;
+        from.w += 128;
+    }
+    meet<12>();
+    int slot = 0;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) read_x(0, 0, n), read_x(0, 1, n), read_w(0, 0, n);
+    while (true) {
+        const uint32_t next = id + stride;
+        uint32_t mn = m0, nn = n0;
+        if (next < end) origin(next, mn, nn);  // else the moves past the end repeat this tile's, unread
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
+        for (uint32_t t = 0; t < steps; ++t) {
+            if (t + 2 == steps) from = source(mn, nn);
+            // the moves in flight at a meeting, from the oldest: the quarter that the phase reads is the first of them
+            meet<10>();
+            product(0, 0, [&](int n) {
+                if (n < 4) read_w(slot, 1, n);
+            });
+            meet<8>();
+            product(1, 0, [&](int n) {
+                read_x(slot, 2 + (n & 1), n >> 1);
+                if (n & 1) (n & 2) ? move_w(from, slot, 0, n >> 2) : move_x(from, slot, 0, n >> 2);
+            });
+            meet<12>();
+            product(0, 2, [&](int n) {
+                if ((n & 3) == 1) move_w(from, slot, 1, n >> 2);
+            });
+            meet<10>();
+            product(1, 2, [&](int n) {
+                if (n < 4) {
+                    read_w(slot ^ 1, 0, n);
+                    read_x(slot ^ 1, 0, n);
+                } else {
+                    read_x(slot ^ 1, 1, n - 4);
+                    if (n & 1) move_x(from, slot, 1, (n - 4) >> 1);
+                }
+            });
+            from.x += 128;
+            from.w += 128;
+            slot ^= 1;
+        }
+        // results: 16 rows at a time through the wave's 4 KB, then 8 adjacent columns a lane
+        const uint32_t ms = min(m0, p.rows - 256), ns = min(n0, p.cols - 256);
+        auto put = [&](auto J, int half) {
+            constexpr int j = decltype(J)::value;
+            if ((l >> 4) == half) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<f32x4*>(turn + (l & 15) * 64 + ((i * 8 + q * 2 + h) ^ (l & 15)) * 4) =
+                            f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+            }
+        };
+#pragma unroll 1
+        for (int g = 0; g < 8; ++g) {  // not unrolled: the epilogue's code stays in the instruction cache
+            const int half = g & 1;
+            switch (g >> 1) {
+                case 0: put(std::integral_constant<int, 0>(), half); break;
+                case 1: put(std::integral_constant<int, 1>(), half); break;
+                case 2: put(std::integral_constant<int, 2>(), half); break;
+                default: put(std::integral_constant<int, 3>(), half); break;
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int rr = k * 8 + (lane >> 3), cc = (lane & 7) * 2;
+                const f32x4 z0 = *reinterpret_cast<const f32x4*>(turn + rr * 64 + (cc ^ rr) * 4);
+                const f32x4 z1 = *reinterpret_cast<const f32x4*>(turn + rr * 64 + ((cc + 1) ^ rr) * 4);
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[e] = z0[e], z[4 + e] = z1[e];
+                const uint32_t row = ms + wm + g * 16 + rr, col = ns + wn + cc * 4;
+                if (row >= m0 && col + 8 > n0) finish<T, O>(p, row, col, z, col < n0 ? n0 - col : 0);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        if (next >= end) break;
+        id = next;
+        m0 = mn;
+        n0 = nn;
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // moves into this workgroup's LDS end before it does
+}
+
+template <typename T, typename O, typename C, bool Direct>
+void start(const Params& p, hipStream_t s) {
+    const uint32_t tiles = (p.cols + C::BN - 1) / C::BN * ((p.rows + C::BM - 1) / C::BM);
+    auto* k = linear_kernel<T, O, C, Direct>;
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+    (void)once;
+    k<<<tiles, C::THREADS, C::LDS, s>>>(p);
+}
+
+template <typename T, typename O>
+void start_big(const Params& p, hipStream_t s) {
+    constexpr int LDS = 160 * 1024;
+    auto* k = linear_big_kernel<T, O>;
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    (void)once;
+    const uint32_t tiles = (p.cols + 255) / 256 * ((p.rows + 255) / 256);
+    k<<<tiles < CUS ? (tiles + 7) / 8 * 8 : CUS, 512, LDS, s>>>(p);
 }
 
 template <typename T, typename O>
 void launch(const Params& p, hipStream_t s) {
-    linear_kernel<T, O><<<(p.cols + 127) / 128 * ((p.rows + 127) / 128), 256, 0, s>>>(p);
+    const bool direct = aligned16(p.x) && aligned16(p.w) && p.xs % 8 == 0 && p.ws % 8 == 0;
+    const bool big = static_cast<uint64_t>((p.cols + 255) / 256) * ((p.rows + 255) / 256) >= CUS;
+    if (big && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 && p.xs < (1 << 22) && p.ws < (1 << 22))
+        start_big<T, O>(p, s);
+    else
+        direct ? start<T, O, Mid, true>(p, s) : start<T, O, Mid, false>(p, s);
 }
 
 int check(const char* what, uint64_t rows, uint32_t inner, uint32_t cols) {

@@ -23,58 +23,63 @@ import torch
 from . import _lib
 from .search import BeamSearchError, _check
 
+_HALF = (torch.float16, torch.bfloat16)
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 __all__ = ["attention", "layer_norm", "layer_norm_backward", "linear", "ACTIVATIONS", "BeamSearchError"]
 
 
-def _want(ok, message):
-    if not ok:
-        raise ValueError(message)
+# the current stream's handle: torch.cuda.current_stream() makes an object for it (2.9 us a call against 0.1)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _gpu(what: str, device, **tensors):
-    """every tensor given is on `device`, a GPU that is the current one"""
-    for name, t in tensors.items():
-        if t is not None and (not isinstance(t, torch.Tensor) or t.device != device):
-            raise ValueError(f"{what}: {name} must be a tensor on {device}")
-    if device.type != "cuda":
-        raise ValueError(f"{what}: the tensors must be on a GPU")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: the tensors are on {device}, the current device is {torch.cuda.current_device()}")
+def _fail(message):
+    raise ValueError(message)
 
 
-def _rows(what: str, name: str, t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """`t` as rows x features (leading dimensions joined) and the distance of its rows; what cannot be
-    viewed so, or has strided features, is refused"""
-    _want(t.dim() >= 1, f"{what}: {name} must have at least one dimension")
+def _gpu(what: str, x: torch.Tensor, *tensors) -> int:
+    """the GPU that all tensors given are on, which must be the current one"""
+    dev = x.get_device()
+    if dev < 0:
+        _fail(f"{what}: the tensors must be on a GPU")
+    for t in tensors:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != dev):
+            _fail(f"{what}: every argument must be a tensor on {x.device}, got {getattr(t, 'device', type(t))}")
+    if dev != torch.cuda.current_device():
+        _fail(f"{what}: the tensors are on {x.device}, the current device is {torch.cuda.current_device()}")
+    return dev
+
+
+def _rows(what: str, name: str, t: torch.Tensor) -> Tuple[int, int, int]:
+    """`t` as rows x features (leading dimensions joined): rows, features and the distance of the rows.
+    What cannot be seen so, or has strided features, is refused."""
+    if t.dim() == 0:
+        _fail(f"{what}: {name} must have at least one dimension")
+    m = t.shape[-1]
+    if t.is_contiguous():
+        return (t.numel() // m if m else 0), m, m
     if t.dim() != 2:
         try:
-            t = t.view(-1, t.shape[-1]) if t.shape[-1] else t.view(0, 0)
+            t = t.view(-1, m) if m else t.view(0, 0)
         except RuntimeError:
-            raise ValueError(f"{what}: the rows of {name} must lie at one distance") from None
-    n, m = t.shape
-    _want(m <= 1 or t.stride(1) == 1, f"{what}: the features of {name} must be contiguous")
+            _fail(f"{what}: the rows of {name} must lie at one distance")
+    n = t.shape[0]
+    s, f = t.stride()
+    if f != 1 and m > 1:
+        _fail(f"{what}: the features of {name} must be contiguous")
     if n <= 1:
-        return t, m
-    s = t.stride(0)
-    _want(s >= m, f"{what}: the rows of {name} overlap")
-    return t, s
+        return n, m, m
+    if s < m:
+        _fail(f"{what}: the rows of {name} overlap")
+    return n, m, s
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
-
-
-def _vector(what: str, name: str, t: Optional[torch.Tensor], n: int, types):
-    if t is not None:
-        _want(t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), f"{what}: {name} must be {n} contiguous elements")
-        _want(t.dtype in types, f"{what}: {name} must be of {' or '.join(str(x) for x in types)}")
+def _vector(what: str, name: str, t: torch.Tensor, n: int, *types):
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        _fail(f"{what}: {name} must be {n} contiguous elements")
+    if t.dtype not in types:
+        _fail(f"{what}: {name} must be of {' or '.join(str(x) for x in types)}")
 
 
 @lru_cache(maxsize=1024)
@@ -98,22 +103,37 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     (y, mean, rstd), float32 of x's leading shape, as layer_norm_backward takes them.  out: where to
     write y (may be x)."""
     what = "layer_norm"
-    _want(isinstance(x, torch.Tensor) and x.dtype in TYPES, f"{what}: x must be a float32, float16 or bfloat16 tensor")
-    _gpu(what, x.device, weight=weight, bias=bias, out=out)
-    r, xs = _rows(what, "x", x)
-    n, m = r.shape
-    wt = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-    _vector(what, "weight", weight, m, (x.dtype, torch.float32))
-    _vector(what, "bias", bias, m, (wt,))
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    _want(y.shape == x.shape and y.dtype == x.dtype, f"{what}: out must have x's shape and type")
-    o, ys = _rows(what, "out", y)
+    type_ = x.dtype
+    code = TYPES.get(type_)
+    if code is None:
+        _fail(f"{what}: x must be a float32, float16 or bfloat16 tensor")
+    dev = _gpu(what, x, weight, bias, out)
+    n, m, xs = _rows(what, "x", x)
+    wt = type_
+    if weight is not None:
+        wt = weight.dtype
+        _vector(what, "weight", weight, m, type_, torch.float32)
+    if bias is not None:
+        if weight is None:
+            wt = bias.dtype
+        _vector(what, "bias", bias, m, *((type_, torch.float32) if weight is None else (wt,)))
+    if out is None:
+        y, ys = x.new_empty(x.shape), m
+    else:
+        y = out
+        if y.shape != x.shape or y.dtype != type_:
+            _fail(f"{what}: out must have x's shape and type")
+        ys = _rows(what, "out", y)[2]
     mean = rstd = None
     if stats:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
-    _check(_lib.hip().bs_layer_norm(r.data_ptr(), xs, _ptr(weight), _ptr(bias), TYPES[wt], eps, o.data_ptr(), ys, _ptr(mean),
-                                    _ptr(rstd), n, m, TYPES[x.dtype], _stream()), what)
+    rc = _lib.hip().bs_layer_norm(x.data_ptr(), xs, None if weight is None else weight.data_ptr(),
+                                  None if bias is None else bias.data_ptr(), TYPES[wt], eps, y.data_ptr(), ys,
+                                  mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None, n, m, code,
+                                  _raw_stream(dev))
+    if rc:
+        _check(rc, what)
     return (y, mean, rstd) if stats else y
 
 
@@ -123,28 +143,35 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     dweight and dbias of weight's (float32 without one), None if params is False.  The sums over the
     rows have a fixed order."""
     what = "layer_norm_backward"
-    _want(isinstance(x, torch.Tensor) and x.dtype in TYPES, f"{what}: x must be a float32, float16 or bfloat16 tensor")
-    _gpu(what, x.device, dy=dy, mean=mean, rstd=rstd, weight=weight)
-    _want(dy.shape == x.shape and dy.dtype == x.dtype, f"{what}: dy must have x's shape and type")
-    r, xs = _rows(what, "x", x)
-    g, gs = _rows(what, "dy", dy)
-    n, m = r.shape
-    _vector(what, "weight", weight, m, (x.dtype, torch.float32))
+    type_ = x.dtype
+    code = TYPES.get(type_)
+    if code is None:
+        _fail(f"{what}: x must be a float32, float16 or bfloat16 tensor")
+    dev = _gpu(what, x, dy, mean, rstd, weight)
+    if dy.shape != x.shape or dy.dtype != type_:
+        _fail(f"{what}: dy must have x's shape and type")
+    n, m, xs = _rows(what, "x", x)
+    gs = _rows(what, "dy", dy)[2]
+    if weight is not None:
+        _vector(what, "weight", weight, m, type_, torch.float32)
     for name, t in (("mean", mean), ("rstd", rstd)):
-        _want(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous(),
-              f"{what}: {name} must be {n} contiguous float32 values")
-    wt = weight.dtype if weight is not None else torch.float32
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+            _fail(f"{what}: {name} must be {n} contiguous float32 values")
+    wt = torch.float32 if weight is None else weight.dtype
+    dx = x.new_empty(x.shape)
     dw = db = ws = None
     size = 0
     if params:
-        dw = torch.empty(m, dtype=wt, device=x.device)
+        dw = x.new_empty((m,), dtype=wt)
         db = torch.empty_like(dw)
-        size = _norm_workspace(n, m, TYPES[x.dtype])
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    _check(_lib.hip().bs_layer_norm_backward(g.data_ptr(), gs, r.data_ptr(), xs, mean.data_ptr(), rstd.data_ptr(), _ptr(weight),
-                                             TYPES[wt], dx.data_ptr(), m, _ptr(dw), _ptr(db), n, m, TYPES[x.dtype], _ptr(ws),
-                                             size, _stream()), what)
+        size = _norm_workspace(n, m, code)
+        ws = x.new_empty((size,), dtype=torch.uint8)
+    rc = _lib.hip().bs_layer_norm_backward(dy.data_ptr(), gs, x.data_ptr(), xs, mean.data_ptr(), rstd.data_ptr(),
+                                           None if weight is None else weight.data_ptr(), TYPES[wt], dx.data_ptr(), m,
+                                           dw.data_ptr() if params else None, db.data_ptr() if params else None, n, m, code,
+                                           ws.data_ptr() if params else None, size, _raw_stream(dev))
+    if rc:
+        _check(rc, what)
     return dx, dw, db
 
 
@@ -156,39 +183,51 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     float32 (what an index takes).  activation: none, relu, gelu, gelu_tanh or silu.  out: where to
     write the result (may be the residual)."""
     what = "linear"
-    _want(isinstance(x, torch.Tensor) and x.dtype in (torch.float16, torch.bfloat16),
-          f"{what}: x must be a float16 or bfloat16 tensor")
-    _gpu(what, x.device, weight=weight, bias=bias, residual=residual, out=out)
-    _want(activation in ACTIVATIONS, f"{what}: unknown activation {activation!r}")
-    _want(weight.dim() == 2 and weight.dtype == x.dtype, f"{what}: weight must be cols x inner of x's type")
-    r, xs = _rows(what, "x", x)
-    w, ws = _rows(what, "weight", weight)
-    n, inner = r.shape
-    cols = w.shape[0]
-    _want(w.shape[1] == inner, f"{what}: x has {inner} features, weight {w.shape[1]}")
-    _vector(what, "bias", bias, cols, (x.dtype,))
+    type_ = x.dtype
+    if type_ not in _HALF:
+        _fail(f"{what}: x must be a float16 or bfloat16 tensor")
+    dev = _gpu(what, x, weight, bias, residual, out)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        _fail(f"{what}: unknown activation {activation!r}")
+    if weight.dim() != 2 or weight.dtype != type_:
+        _fail(f"{what}: weight must be cols x inner of x's type")
+    n, inner, xs = _rows(what, "x", x)
+    cols, k, ws = _rows(what, "weight", weight)
+    if k != inner:
+        _fail(f"{what}: x has {inner} features, weight {k}")
+    if bias is not None:
+        _vector(what, "bias", bias, cols, type_)
     if out_dtype is None:
-        out_dtype = x.dtype if out is None else out.dtype
-    _want(out_dtype in (x.dtype, torch.float32), f"{what}: out_dtype must be x's type or float32")
-    shape = x.shape[:-1] + (cols,)
-    y = torch.empty(shape, dtype=out_dtype, device=x.device) if out is None else out
-    _want(y.shape == shape and y.dtype == out_dtype, f"{what}: out must be {tuple(shape)} of {out_dtype}")
-    o, os_ = _rows(what, "out", y)
-    res, rs = None, 0
+        out_dtype = type_ if out is None else out.dtype
+    elif out_dtype != type_ and out_dtype != torch.float32:
+        _fail(f"{what}: out_dtype must be x's type or float32")
+    shape = (n, cols) if x.dim() == 2 else (*x.shape[:-1], cols)
+    if out is None:
+        y, ys = x.new_empty(shape, dtype=out_dtype), cols
+    else:
+        y = out
+        if y.shape != shape or y.dtype != out_dtype:
+            _fail(f"{what}: out must be {tuple(shape)} of {out_dtype}")
+        ys = _rows(what, "out", y)[2]
+    rs = 0
     if residual is not None:
-        _want(residual.shape == shape and residual.dtype == out_dtype,
-              f"{what}: residual must be {tuple(shape)} of {out_dtype}")
-        res, rs = _rows(what, "residual", residual)
+        if residual.shape != shape or residual.dtype != out_dtype:
+            _fail(f"{what}: residual must be {tuple(shape)} of {out_dtype}")
+        rs = _rows(what, "residual", residual)[2]
     size = _linear_workspace(n, inner, cols)
-    space = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    _check(_lib.hip().bs_linear(r.data_ptr(), xs, w.data_ptr(), ws, _ptr(bias), _ptr(res), rs, o.data_ptr(), os_, n, inner, cols,
-                                TYPES[x.dtype], TYPES[out_dtype], ACTIVATIONS[activation], _ptr(space), size, _stream()), what)
+    space = x.new_empty((size,), dtype=torch.uint8) if size else None
+    rc = _lib.hip().bs_linear(x.data_ptr(), xs, weight.data_ptr(), ws, None if bias is None else bias.data_ptr(),
+                              None if residual is None else residual.data_ptr(), rs, y.data_ptr(), ys, n, inner, cols, TYPES[type_],
+                              TYPES[out_dtype], act, space.data_ptr() if size else None, size, _raw_stream(dev))
+    if rc:
+        _check(rc, what)
     return y
 
 
 def _offsets(what: str, name: str, t: torch.Tensor, n: int):
-    _want(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.shape[0] == n + 1 and n >= 1,
-          f"{what}: {name} must be sequences + 1 contiguous int32 values")
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.shape[0] != n + 1 or n < 1:
+        _fail(f"{what}: {name} must be sequences + 1 contiguous int32 values")
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: Optional[torch.Tensor] = None,
@@ -203,34 +242,52 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: Opti
     lse), lse (tokens, heads) float32 the log of the sum of the exponentials.  A query that sees no key
     gets 0 and -inf.  out: where to write the result."""
     what = "attention"
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _want(isinstance(t, torch.Tensor) and t.dim() == 3, f"{what}: {name} must be tokens x heads x head_dim")
-        _want(t.dtype in (torch.float16, torch.bfloat16) and t.dtype == q.dtype, f"{what}: q, k and v must be of one type, float16 or bfloat16")
-        _want(t.shape[2] <= 1 or t.stride(2) == 1, f"{what}: the elements of a head of {name} must be contiguous")
-    _gpu(what, q.device, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, out=out)
+    type_ = q.dtype
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        _fail(f"{what}: q, k and v must be tokens x heads x head_dim")
+    if type_ not in _HALF or k.dtype != type_ or v.dtype != type_:
+        _fail(f"{what}: q, k and v must be of one type, float16 or bfloat16")
+    dev = _gpu(what, q, k, v, q_offsets, k_offsets, out)
     tq, heads, dim = q.shape
-    tk, kv_heads = k.shape[0], k.shape[1]
-    _want(k.shape == v.shape and k.shape[2] == dim, f"{what}: k and v must have one shape and q's head_dim")
+    tk, kv_heads, kdim = k.shape
+    qt, qh, qe = q.stride()
+    kt, kh, ke = k.stride()
+    vt, vh, ve = v.stride()
+    if dim > 1 and not qe == ke == ve == 1:
+        _fail(f"{what}: the elements of a head of q, k and v must be contiguous")
+    if v.shape != k.shape or kdim != dim:
+        _fail(f"{what}: k and v must have one shape and q's head_dim")
     n = 1
-    if k_offsets is None and q_offsets is not None:
-        _want(tq == tk, f"{what}: k_offsets must be given where k has other tokens than q")
-        k_offsets = q_offsets
-    _want((q_offsets is None) == (k_offsets is None), f"{what}: k_offsets without q_offsets")
-    if q_offsets is not None:
+    if q_offsets is None:
+        if k_offsets is not None:
+            _fail(f"{what}: k_offsets without q_offsets")
+    else:
+        if k_offsets is None:
+            if tq != tk:
+                _fail(f"{what}: k_offsets must be given where k has other tokens than q")
+            k_offsets = q_offsets
         n = q_offsets.shape[0] - 1 if q_offsets.dim() == 1 else 0
         _offsets(what, "q_offsets", q_offsets, n)
-        _offsets(what, "k_offsets", k_offsets, n)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    _want(o.shape == q.shape and o.dtype == q.dtype and (dim <= 1 or o.stride(2) == 1),
-          f"{what}: out must have q's shape and type, the elements of a head contiguous")
-    stat = torch.empty((tq, heads), dtype=torch.float32, device=q.device) if lse else None
-    a = _lib.AttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(stat), _ptr(q_offsets), _ptr(k_offsets),
-                           q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), o.stride(0),
-                           o.stride(1), tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, TYPES[q.dtype], 1 if causal else 0,
-                           dim ** -0.5 if scale is None and dim else scale or 0.0)
-    size = _attention_workspace(tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, TYPES[q.dtype], bool(causal))
-    space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _check(_lib.hip().bs_attention(C.byref(a), _ptr(space), size, _stream()), what)
+        if k_offsets is not q_offsets:
+            _offsets(what, "k_offsets", k_offsets, n)
+    if out is None:
+        o, ot, oh = q.new_empty((tq, heads, dim)), heads * dim, dim
+    else:
+        o = out
+        if o.shape != q.shape or o.dtype != type_ or (dim > 1 and o.stride(2) != 1):
+            _fail(f"{what}: out must have q's shape and type, the elements of a head contiguous")
+        ot, oh = o.stride(0), o.stride(1)
+    stat = q.new_empty((tq, heads), dtype=torch.float32) if lse else None
+    code = TYPES[type_]
+    a = _lib.AttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), stat.data_ptr() if lse else None,
+                           None if q_offsets is None else q_offsets.data_ptr(), None if k_offsets is None else k_offsets.data_ptr(),
+                           qt, qh, kt, kh, vt, vh, ot, oh, tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, code,
+                           1 if causal else 0, (dim ** -0.5 if dim else 0.0) if scale is None else scale)
+    size = _attention_workspace(tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, code, causal)
+    space = q.new_empty((size,), dtype=torch.uint8) if size else None
+    rc = _lib.hip().bs_attention(C.byref(a), space.data_ptr() if size else None, size, _raw_stream(dev))
+    if rc:
+        _check(rc, what)
     return (o, stat) if lse else o
 
 

@@ -238,6 +238,23 @@ def test_linear(gpu, rows, inner, cols, dtype, full):
         assert torch.equal(got, embed.linear(x, w, b, activation=act, residual=r, out_dtype=out))
 
 
+@pytest.mark.parametrize("rows,inner,cols", [(4096, 128, 4096), (4111, 192, 4203), (300, 320, 33000), (17000, 256, 1001)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_linear_of_many_tiles(gpu, rows, inner, cols, dtype):
+    """more tiles than compute units, shifted ones at the edges; the residual is the result's own buffer"""
+    x, w = rand(44, rows, inner, dtype=dtype), rand(45, cols, inner, dtype=dtype, std=inner ** -0.5)
+    b, r = rand(46, cols, dtype=dtype), rand(47, rows, cols, dtype=dtype)
+    want = embed.linear(x, w, b, activation="silu", residual=r)
+    check_linear(x, w, b, "silu", r, want)
+    got = r.clone()
+    embed.linear(x, w, b, activation="silu", residual=got, out=got)
+    assert torch.equal(got, want)
+    check_linear(x, w, None, "none", None, embed.linear(x, w, out_dtype=F32))
+    wide = torch.full((rows, cols + 9), 7.0, dtype=dtype, device="cuda")
+    embed.linear(x, w, b, activation="silu", residual=r, out=wide[:, 3:cols + 3])
+    assert torch.equal(wide[:, 3:cols + 3], want) and (wide[:, :3] == 7).all() and (wide[:, cols + 3:] == 7).all()
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("rows,inner,cols", [(4, 128, 64), (300, 256, 384), (600, 100, 130)])
 def test_linear_activations(gpu, act, rows, inner, cols):
@@ -504,7 +521,7 @@ def test_python_refusals(gpu):
         (lambda: embed.layer_norm(x, x[0], x[0].float()), "bias must be of"),
         (lambda: embed.layer_norm(x, out=x.float()), "x's shape and type"),
         (lambda: embed.layer_norm(x[:1].expand(4, 64)), "rows of x overlap"),
-        (lambda: embed.layer_norm(x, x[0].cpu()), "weight must be a tensor on"),
+        (lambda: embed.layer_norm(x, x[0].cpu()), "must be a tensor on"),
         (lambda: embed.layer_norm_backward(x.float(), x, x[:, 0], x[:, 0]), "dy must have"),
         (lambda: embed.layer_norm_backward(x, x, x[:, 0], x[:, 0]), "mean must be"),
         (lambda: embed.linear(x, w[:, :32]), "x has 64 features"),
@@ -512,13 +529,14 @@ def test_python_refusals(gpu):
         (lambda: embed.linear(x, w, activation="tanh"), "unknown activation"),
         (lambda: embed.linear(x, w, residual=x), "residual must be"),
         (lambda: embed.linear(x, w, out_dtype=F16), "out_dtype must be"),
+        (lambda: embed.linear(x, w, out=rand(4, 4, 32, dtype=F16)), "out must be|out_type must be"),
         (lambda: embed.linear(x, w, x[0]), "bias must be 32"),
         (lambda: embed.attention(q, q[:, :, :16], q), "k and v must have one shape"),
         (lambda: embed.attention(q, q[:3], q[:3], off), "k_offsets must be given"),
         (lambda: embed.attention(q, q, q, None, off), "k_offsets without q_offsets"),
         (lambda: embed.attention(q, q, q, off.long()), "int32"),
         (lambda: embed.attention(q, q, q, off, offsets([2, 2])), "k_offsets must be"),
-        (lambda: embed.attention(q.transpose(1, 2), q, q), "elements of a head of q"),
+        (lambda: embed.attention(q.transpose(1, 2), q, q), "elements of a head of q, k and v"),
         (lambda: embed.attention(q[:, :, 1:25], q[:, :, :24], q[:, :, :24]), "multiples of 16 bytes"),
         (lambda: embed.attention(q, torch.cat([q, q[:, :1]], 1), torch.cat([q, q[:, :1]], 1)), "multiple of kv_heads"),
     ]:

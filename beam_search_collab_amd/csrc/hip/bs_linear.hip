@@ -6,6 +6,7 @@
 // adjacent columns.
 #include "bs_embed.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -32,6 +33,8 @@ struct Params {
     int64_t xs, ws, rs, os;
     uint32_t rows, inner, cols;
     int act;
+    uint32_t splits;  // pieces of the inner dimension; > 1: their sums go to `parts`, splits x rows x cols
+    float* parts;
 };
 
 // one branch for all values: the branches are the call's, not the lanes'
@@ -56,30 +59,30 @@ __device__ inline void activate(float (&z)[N], int act) {
     }
 }
 
-// eight adjacent columns of one row: those from `first` on, and inside
-template <typename T, typename O>
-__device__ inline void finish(const Params& p, uint32_t row, uint32_t col, float (&z)[8], int first = 0) {
+// N adjacent columns of one row: those from `first` on, and inside
+template <typename T, typename O, int N>
+__device__ inline void finish(const Params& p, uint32_t row, uint32_t col, float (&z)[N], int first = 0) {
     const int n = static_cast<int>(p.cols - col);
     if (p.bias) {
-        const Vec<T, 8> b = load_some<T, 8>(static_cast<const T*>(p.bias) + col, n);
+        const Vec<T, N> b = load_some<T, N>(static_cast<const T*>(p.bias) + col, n);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] += static_cast<float>(b[j]);
+        for (int j = 0; j < N; ++j) z[j] += static_cast<float>(b[j]);
     }
     activate(z, p.act);
     if (p.residual) {
-        const Vec<O, 8> r = load_some<O, 8>(static_cast<const O*>(p.residual) + static_cast<int64_t>(row) * p.rs + col, n);
+        const Vec<O, N> r = load_some<O, N>(static_cast<const O*>(p.residual) + static_cast<int64_t>(row) * p.rs + col, n);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] += static_cast<float>(r[j]);
+        for (int j = 0; j < N; ++j) z[j] += static_cast<float>(r[j]);
     }
-    Vec<O, 8> o;
+    Vec<O, N> o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = static_cast<O>(z[j]);
+    for (int j = 0; j < N; ++j) o[j] = static_cast<O>(z[j]);
     O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.os + col;
-    if (first <= 0 && n >= 8) {
-        store_any<O, 8>(out, o);
+    if (first <= 0 && n >= N) {
+        store_any<O, N>(out, o);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < N; ++j)
             if (j >= first && j < n) out[j] = o[j];
     }
 }
@@ -148,7 +151,9 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void linear_k
             from[i] = w + static_cast<int64_t>(n) * p.ws + chunk[i] * 8;
         }
     }
-    const uint32_t whole = p.inner / C::BK, steps = (p.inner + C::BK - 1) / C::BK;
+    // this workgroup's piece: whole steps [begin, whole), and for the last piece what is left after them
+    const uint32_t allsteps = (p.inner + C::BK - 1) / C::BK, piece = (allsteps + p.splits - 1) / p.splits;
+    const uint32_t begin = blockIdx.y * piece, steps = min(begin + piece, allsteps), whole = min(steps, p.inner / C::BK);
     auto move = [&](uint32_t t, int slot, int first = 0, int n = C::MOVES) {  // Direct
 #pragma unroll
         for (int i = first; i < first + n; ++i)
@@ -198,14 +203,14 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void linear_k
         // t + NS - 1 gets.  Operands are read one part (16 inner elements) ahead of their products, across the
         // meeting too.  A move past the last step repeats the last one, so that every wait counts the same.
         const uint32_t last = whole ? whole - 1 : 0;
-        if (whole) {
+        if (whole > begin) {
             Parts f[2];
 #pragma unroll
-            for (int i = 0; i < C::NS - 1; ++i) move(min(static_cast<uint32_t>(i), last), i);
+            for (int i = 0; i < C::NS - 1; ++i) move(min(begin + i, last), i);
             meet<(C::NS - 2) * C::MOVES>();
             read(0, 0, f[0]);
             int slot = 0;
-            for (uint32_t t = 0; t < whole; ++t) {
+            for (uint32_t t = begin; t < whole; ++t) {
                 meet<(C::NS - 3) * C::MOVES>();
                 move(min(t + C::NS - 1, last), slot == 0 ? C::NS - 1 : slot - 1);
                 const int next = slot == C::NS - 1 ? 0 : slot + 1;
@@ -236,9 +241,9 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void linear_k
         }
     } else {
         Vec<T, 8> v[C::MOVES];
-        fetch(0, v);
-        put(0, v);
-        for (uint32_t t = 0; t < steps; ++t) {
+        fetch(begin, v);
+        put(begin & 1, v);
+        for (uint32_t t = begin; t < steps; ++t) {
             __syncthreads();
             if (t + 1 < steps) fetch(t + 1, v);
             multiply(t & 1);
@@ -278,13 +283,110 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void linear_k
             const f32x4 z0 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + c), z1 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + c + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[e] = z0[e], z[4 + e] = z1[e];
-            if (row < p.rows && col < p.cols) finish<T, O>(p, row, col, z);
+            if (row >= p.rows || col >= p.cols) continue;
+            if (p.splits > 1) {
+                float* part = p.parts + (static_cast<size_t>(blockIdx.y) * p.rows + row) * p.cols + col;
+                store_some<float, 4>(part, z0, static_cast<int>(p.cols - col));
+                if (p.cols - col > 4) store_some<float, 4>(part + 4, z1, static_cast<int>(p.cols - col) - 4);
+            } else {
+                finish<T, O>(p, row, col, z);
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
+// the pieces' sums in order, and the epilogue: a thread takes four adjacent columns of a row
+template <typename T, typename O>
+__global__ __launch_bounds__(256) void linear_join_kernel(Params p) {
+    const uint32_t across = (p.cols + 3) / 4;
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const uint32_t row = static_cast<uint32_t>(at / across), col = static_cast<uint32_t>(at % across) * 4;
+    if (row >= p.rows) return;
+    const int n = static_cast<int>(p.cols - col);
+    const float* part = p.parts + static_cast<size_t>(row) * p.cols + col;
+    f32x4 s = load_some<float, 4>(part, n);
+    for (uint32_t i = 1; i < p.splits; ++i) s += load_some<float, 4>(part + static_cast<size_t>(i) * p.rows * p.cols, n);
+    float z[4] = {s[0], s[1], s[2], s[3]};
+    finish<T, O>(p, row, col, z);
+}
+
+template <typename T>
+struct Mma16;
+template <>
+struct Mma16<f16> {
+    __device__ static f32x4 go(Vec<f16, 8> a, Vec<f16, 8> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma16<bf16> {
+    __device__ static f32x4 go(Vec<bf16, 8> a, Vec<bf16, 8> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// Few rows: the weight is read once, from memory to registers, and bounds the time.  A workgroup has NT x 16 of
+// its rows, its eight waves a contiguous piece each of the inner dimension, so that 16 columns are enough work
+// for a compute unit and nothing is joined across workgroups; x (MT x 16 rows) comes from the L2.
+template <typename T, typename O, int MT, int NT>
+__global__ __launch_bounds__(512) void linear_few_kernel(Params p) {
+    __shared__ f32x4 join[8][NT * MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const uint32_t n0 = blockIdx.x * (NT * 16);
+    // rows past the end repeat the last one: their products are not stored
+    const T *wp[NT], *xp[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) wp[i] = static_cast<const T*>(p.w) + static_cast<int64_t>(min(n0 + i * 16 + l, p.cols - 1)) * p.ws + g * 8;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+        xp[i] = static_cast<const T*>(p.x) + static_cast<int64_t>(min(static_cast<uint32_t>(i * 16 + l), p.rows - 1)) * p.xs + g * 8;
+    f32x4 acc[NT][MT] = {};
+    const uint32_t steps = (p.inner + 31) / 32, piece = (steps + 7) / 8, begin = wave * piece;
+    const uint32_t end = min(begin + piece, steps), whole = min(end, p.inner / 32);
+    constexpr int U = 8;  // steps in flight
+    uint32_t t = begin;
+    for (; t + U <= whole; t += U) {
+        Vec<T, 8> a[U][NT], b[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) a[u][i] = load_any<T, 8>(wp[i] + (t + u) * 32);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) b[u][i] = load_any<T, 8>(xp[i] + (t + u) * 32);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) acc[i][j] = Mma16<T>::go(a[u][i], b[u][j], acc[i][j]);
+    }
+    for (; t < end; ++t) {
+        const int left = static_cast<int>(p.inner - t * 32) - g * 8;
+        Vec<T, 8> a[NT], b[MT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) a[i] = left > 0 ? load_some<T, 8>(wp[i] + t * 32, left) : Vec<T, 8>{};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) b[i] = left > 0 ? load_some<T, 8>(xp[i] + t * 32, left) : Vec<T, 8>{};
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] = Mma16<T>::go(a[i], b[j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) join[wave][i * MT + j][lane] = acc[i][j];
+    __syncthreads();
+    if (wave >= NT * MT) return;
+    // wave i MT + j: rows 16 j + l, columns 16 i + 4 g to + 3; the waves' sums in order
+    f32x4 s = join[0][wave][lane];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += join[k][wave][lane];
+    const uint32_t row = wave % MT * 16 + l, col = n0 + wave / MT * 16 + g * 4;
+    float z[4] = {s[0], s[1], s[2], s[3]};
+    if (row < p.rows && col < p.cols) finish<T, O>(p, row, col, z);
+}
+
 using Mid = Tile<128, 128, 2, 2, 32, 4, 2>;
+using Small = Tile<64, 64, 2, 2, 64, 4, 2>;
 
 // Large products: tiles of 256 x 256 by 8 waves of 128 (rows of x) x 64 (rows of w), inner steps of 64.
 //
@@ -455,7 +557,7 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) z[e] = z0[e], z[4 + e] = z1[e];
                 const uint32_t row = ms + wm + g * 16 + rr, col = ns + wn + cc * 4;
-                if (row >= m0 && col + 8 > n0) finish<T, O>(p, row, col, z, col < n0 ? n0 - col : 0);
+                if (row >= m0 && col + 8 > n0) finish<T, O>(p, row, col, z, col < n0 ? static_cast<int>(n0 - col) : 0);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -473,7 +575,11 @@ void start(const Params& p, hipStream_t s) {
     auto* k = linear_kernel<T, O, C, Direct>;
     static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
     (void)once;
-    k<<<tiles, C::THREADS, C::LDS, s>>>(p);
+    k<<<dim3(tiles, p.splits), C::THREADS, C::LDS, s>>>(p);
+    if (p.splits > 1) {
+        const uint64_t quads = static_cast<uint64_t>(p.rows) * ((p.cols + 3) / 4);
+        linear_join_kernel<T, O><<<static_cast<uint32_t>((quads + 255) / 256), 256, 0, s>>>(p);
+    }
 }
 
 template <typename T, typename O>
@@ -486,21 +592,51 @@ void start_big(const Params& p, hipStream_t s) {
     k<<<tiles < CUS ? (tiles + 7) / 8 * 8 : CUS, 512, LDS, s>>>(p);
 }
 
+constexpr uint32_t FEW = 32;  // rows up to which the weight is streamed
+
+uint64_t tiles_of(uint64_t rows, uint32_t cols, uint32_t size) { return (rows + size - 1) / size * ((cols + size - 1) / size); }
+
+// Pieces of the inner dimension for tiles of 64: where they leave compute units idle, pieces of 512 elements
+// at least.
+uint32_t splits_of(uint64_t rows, uint32_t inner, uint32_t cols) {
+    if (rows <= FEW) return 1;
+    const uint64_t tiles = tiles_of(rows, cols, 64);
+    if (tiles >= CUS || inner < 1024) return 1;
+    const uint32_t want = static_cast<uint32_t>(std::min<uint64_t>(2 * CUS / tiles, inner / 512));
+    const uint32_t steps = (inner + 63) / 64, piece = (steps + want - 1) / want;
+    return (steps + piece - 1) / piece;
+}
+
+template <typename T, typename O, int MT>
+void start_few(const Params& p, hipStream_t s) {
+    // 32 columns a workgroup, half the reads of x, where that leaves a workgroup for every compute unit
+    if (p.cols >= 32 * CUS)
+        linear_few_kernel<T, O, MT, 2><<<(p.cols + 31) / 32, 512, 0, s>>>(p);
+    else
+        linear_few_kernel<T, O, MT, 1><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
+}
+
 template <typename T, typename O>
 void launch(const Params& p, hipStream_t s) {
+    if (p.rows <= FEW) {
+        p.rows <= 16 ? start_few<T, O, 1>(p, s) : start_few<T, O, 2>(p, s);
+        return;
+    }
     const bool direct = aligned16(p.x) && aligned16(p.w) && p.xs % 8 == 0 && p.ws % 8 == 0;
-    const bool big = static_cast<uint64_t>((p.cols + 255) / 256) * ((p.rows + 255) / 256) >= CUS;
-    if (big && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 && p.xs < (1 << 22) && p.ws < (1 << 22))
+    if (tiles_of(p.rows, p.cols, 256) >= CUS && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 &&
+        p.xs < (1 << 22) && p.ws < (1 << 22))
         start_big<T, O>(p, s);
-    else
+    else if (tiles_of(p.rows, p.cols, 128) >= CUS)
         direct ? start<T, O, Mid, true>(p, s) : start<T, O, Mid, false>(p, s);
+    else
+        direct ? start<T, O, Small, true>(p, s) : start<T, O, Small, false>(p, s);
 }
 
 int check(const char* what, uint64_t rows, uint32_t inner, uint32_t cols) {
     const std::string w = what;
     if (rows > 0x7FFFFFFFull) return refuse(w + ": rows must be < 2^31");
     if (inner == 0 || inner > (1u << 24) || cols == 0 || cols > (1u << 24)) return refuse(w + ": inner and cols must be in 1..2^24");
-    if (((rows + 127) >> 7) * ((cols + 127) >> 7) > 0x7FFFFFFFull) return refuse(w + ": rows x cols is too large for one launch");
+    if (((rows + 63) >> 6) * ((cols + 63) >> 6) > 0x7FFFFFFFull) return refuse(w + ": rows x cols is too large for one launch");
     return BS_OK;
 }
 
@@ -509,7 +645,8 @@ int check(const char* what, uint64_t rows, uint32_t inner, uint32_t cols) {
 extern "C" int bs_linear_workspace(uint64_t rows, uint32_t inner, uint32_t cols, uint64_t* bytes) try {
     if (!bytes) return refuse("bs_linear_workspace: bytes is null");
     if (const int rc = check("bs_linear_workspace", rows, inner, cols)) return rc;
-    *bytes = 0;
+    const uint32_t splits = splits_of(rows, inner, cols);
+    *bytes = splits > 1 ? splits * rows * cols * sizeof(float) : 0;
     return BS_OK;
 } catch (...) {
     return bs_internal_exception();
@@ -528,7 +665,14 @@ extern "C" int bs_linear(const void* x, int64_t x_stride, const void* w, int64_t
         return refuse("bs_linear: rows overlap (a stride is shorter than its row)");
     if (x_stride >= (1 << 24) || w_stride >= (1 << 24) || out_stride >= (1 << 24) || (residual && residual_stride >= (1 << 24)))
         return refuse("bs_linear: strides must be < 2^24");
-    const Params p{x, w, bias, residual, out, x_stride, w_stride, residual_stride, out_stride, static_cast<uint32_t>(rows), inner, cols, activation};
+    const uint32_t splits = splits_of(rows, inner, cols);
+    if (splits > 1) {
+        const uint64_t need = splits * rows * cols * sizeof(float);
+        if (!workspace || workspace_bytes < need) return refuse("bs_linear: the workspace must hold " + std::to_string(need) + " bytes");
+        if (!aligned16(workspace)) return refuse("bs_linear: the workspace must be 16-byte aligned");
+    }
+    const Params p{x, w, bias, residual, out, x_stride, w_stride, residual_stride, out_stride, static_cast<uint32_t>(rows), inner, cols, activation,
+                   splits, static_cast<float*>(workspace)};
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (type == BS_F16)
         out_type == BS_F32 ? launch<f16, float>(p, s) : launch<f16, f16>(p, s);

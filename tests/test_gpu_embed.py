@@ -220,7 +220,7 @@ def check_linear(x, w, b, act, r, got):
 SIZES = [(1, 1, 1), (1, 1024, 128), (1, 960, 100), (2, 100, 3), (3, 8, 8), (5, 63, 65), (16, 64, 128), (17, 4096, 256),
          (31, 200, 96), (32, 256, 512), (33, 257, 131), (64, 1024, 64), (65, 72, 1000), (100, 1000, 300), (127, 128, 127),
          (128, 128, 128), (129, 192, 257), (200, 4096, 128), (255, 64, 255), (256, 512, 256), (257, 520, 264), (1000, 96, 777),
-         (1024, 1024, 1024), (1111, 333, 222), (0, 64, 32)]
+         (1024, 1024, 1024), (1111, 333, 222), (0, 64, 32), (5, 200, 8192), (29, 72, 8205), (65, 2050, 90), (90, 4096, 520)]
 
 
 @pytest.mark.parametrize("rows,inner,cols", SIZES)

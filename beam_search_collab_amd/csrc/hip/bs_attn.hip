@@ -95,186 +95,297 @@ __device__ inline s16x4 read_transposed(const char* p) {
         reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p)));
 }
 
-// DP: head_dim rounded up to 32.  Four waves of 32 rows.
+typedef __attribute__((address_space(1))) const void* global_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// waits until all but the wave's N youngest moves to LDS are done, and its reads of LDS
+template <int N>
+__device__ inline void landed() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);  // vmcnt(N) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// the same for all of them, and meets the workgroup's other waves
+__device__ inline void meet() {
+    landed<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ inline uint32_t keys_of(const bs_attention_args& a, const Sequence& sq, uint32_t t) {  // visible keys of query t
+    const int64_t e = a.causal ? min(static_cast<int64_t>(sq.nk), static_cast<int64_t>(sq.nk) - sq.nq + t + 1) : static_cast<int64_t>(sq.nk);
+    return static_cast<uint32_t>(e < 0 ? 0 : e);
+}
+
+template <int DP>
+constexpr int ROW = DP <= 32 ? 64 : DP <= 64 ? 128 : 256;  // bytes of a key or value in LDS
+
+// The rows of one wave: 32 of them, lanes l and l + 32 (half h) hold row l.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
-    constexpr int ROWS = 128, S = DP <= 32 ? 64 : DP <= 64 ? 128 : 256, CH = DP / 8;
-    __shared__ __attribute__((aligned(16))) char tk[BN * S], tv[BN * S];
-    const bs_attention_args& a = p.a;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, h = lane >> 5;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
-    const uint32_t seq = a.q_offsets ? find(a.q_offsets, a.sequences, tile, p.group, ROWS) : 0;
-    const uint64_t first = a.q_offsets ? first_tile(a.q_offsets, seq, p.group, ROWS) : 0;
-    const Sequence sq = sequence(a, seq);
-    const uint64_t rows = static_cast<uint64_t>(sq.nq) * p.group;
-    if (tile < first || (tile - first) * ROWS >= rows) return;
-    const uint64_t row0 = (tile - first) * ROWS;
-    const int64_t shift = static_cast<int64_t>(sq.nk) - sq.nq;  // query i sees the keys up to i + shift
-
-    // this lane's row
-    const uint64_t row = row0 + wave * 32 + l;
-    const bool live = row < rows;
-    const uint32_t tok = static_cast<uint32_t>((live ? row : rows - 1) / p.group);
-    const uint32_t head = kvh * p.group + static_cast<uint32_t>((live ? row : rows - 1) - static_cast<uint64_t>(tok) * p.group);
-    auto keys_of = [&](uint32_t t) {  // visible keys of query t
-        const int64_t e = a.causal ? min(static_cast<int64_t>(sq.nk), t + shift + 1) : static_cast<int64_t>(sq.nk);
-        return static_cast<uint32_t>(e < 0 ? 0 : e);
-    };
-    const uint32_t mine = keys_of(tok);
-    const uint64_t last_row = min(rows, row0 + ROWS) - 1;
-    const uint32_t all = keys_of(static_cast<uint32_t>(last_row / p.group));  // of the tile's last row: the most
-    uint32_t kb = 0, ke = all;
-    if (p.splits > 1) {
-        kb = min(all, blockIdx.y * p.piece);
-        if (blockIdx.y + 1 < p.splits) ke = min(all, kb + p.piece);
-        if (kb >= ke && blockIdx.y > 0) return;  // the join does not read it
-    }
-
+struct Rows {
+    static constexpr int S = ROW<DP>;
     Vec<T, 8> q[DP / 16];
-    const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + tok) * a.q_stride + static_cast<int64_t>(head) * a.q_head_stride;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-        const uint32_t d = s * 16 + h * 8;
-        q[s] = Vec<T, 8>{};
-        if (d < a.head_dim) q[s] = *reinterpret_cast<const Vec<T, 8>*>(qp + d);
-    }
-    const T* kp = static_cast<const T*>(a.k) + static_cast<int64_t>(sq.k0) * a.k_stride + static_cast<int64_t>(kvh) * a.k_head_stride;
-    const T* vp = static_cast<const T*>(a.v) + static_cast<int64_t>(sq.k0) * a.v_stride + static_cast<int64_t>(kvh) * a.v_head_stride;
-
     f32x16 o[DP / 32];
-    float top, sum;
-    auto clear = [&] {
+    float top, sum;  // what the weights are taken against, in units of log2, and their sum over this half's keys
+
+    __device__ void clear() {
         top = NONE;
         sum = 0.0f;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
-    };
-    const float scale = a.scale * LOG2E;
-    // one tile of keys; Masked: some row of the workgroup does not see all of them
-    auto step = [&](uint32_t j0, auto Masked, auto Careful) {
-        constexpr bool masked = decltype(Masked)::value, careful = decltype(Careful)::value;
-        __syncthreads();
-        for (int at = threadIdx.x; at < BN * CH; at += 256) {
-            const int r = at / CH, c = at % CH;
-            Vec<T, 8> x = {}, y = {};
-            if (j0 + r < sq.nk && static_cast<uint32_t>(c * 8) < a.head_dim) {
-                x = *reinterpret_cast<const Vec<T, 8>*>(kp + static_cast<int64_t>(j0 + r) * a.k_stride + c * 8);
-                y = *reinterpret_cast<const Vec<T, 8>*>(vp + static_cast<int64_t>(j0 + r) * a.v_stride + c * 8);
-            }
-            *reinterpret_cast<Vec<T, 8>*>(tk + place<S>(r, c)) = x;
-            *reinterpret_cast<Vec<T, 8>*>(tv + place<S>(r, c)) = y;
+    }
+    __device__ void load(const T* p, uint32_t head_dim, int h) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const uint32_t d = s * 16 + h * 8;
+            q[s] = Vec<T, 8>{};
+            if (d < head_dim) q[s] = *reinterpret_cast<const Vec<T, 8>*>(p + d);
         }
-        __syncthreads();
-        f32x16 z[2] = {};
+    }
+    __device__ bool odd() const {  // some result is not finite
+        bool is = false;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) is |= !(fabsf(o[d][r]) < INFINITY);
+        return is;
+    }
+    // KB x 32 keys from j0 on, in LDS.  Masked: only those below `mine` count.  Careful: values of weight 0
+    // that are not finite do not touch the result.
+    template <int KB, bool Masked, bool Careful>
+    __device__ void step(const char* tk, const char* tv, uint32_t j0, uint32_t mine, float scale, int lane) {
+        const int l = lane & 31, h = lane >> 5;
+        f32x16 z[KB] = {};
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < KB; ++b) {
                 const Vec<T, 8> k = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + l, s * 2 + h));
                 z[b] = Mma<T>::go(k, q[s], z[b]);
             }
         // result register r of block b: key b * 32 + r % 4 + 8 (r / 4) + 4 h
         float most = NONE;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const uint32_t j = j0 + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
                 z[b][r] *= scale;
-                if (masked && (j >= mine || j >= ke)) z[b][r] = NONE;
+                if (Masked && j0 + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * h >= mine) z[b][r] = NONE;
                 most = fmaxf(most, z[b][r]);
             }
         most = fmaxf(most, __shfl_xor(most, 32));
-        const float now = fmaxf(top, most);
-        const float base = now == NONE ? 0.0f : now;  // nothing visible yet: every weight is exp2(-inf) = 0
-        const float fade = exp2f(top - base);
-        float add = 0.0f;
-        Vec<T, 8> w[4];
+        // The weights may stand against an older maximum while they stay below 2^8: sums and results lose
+        // nothing by that, and the results are rescaled seldom.
+        if (__any(most > top + 8.0f)) {
+            const float now = fmaxf(top, most), fade = __builtin_amdgcn_exp2f(top - (now == NONE ? 0.0f : now));
+            top = now;
+            sum *= fade;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= fade;
+        }
+        const float base = top == NONE ? 0.0f : top;  // nothing visible yet: every weight is exp2(-inf) = 0
+        float add = 0.0f;
+        Vec<T, 8> w[2 * KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float e = exp2f(z[b][r] - base);
+                const float e = __builtin_amdgcn_exp2f(z[b][r] - base);
                 add += e;
                 w[b * 2 + (r >> 3)][r & 7] = static_cast<T>(e);
             }
-        add += __shfl_xor(add, 32);
-        sum = fmaf(sum, fade, add);
-        top = now;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] *= fade;
+        sum += add;
+        auto value = [&](int d, int s) {  // 16 keys of 32 elements
+            // lanes 16g .. 16g + 15 read 4 keys x 16 elements and get an element's 4 keys each
+            const int key = s * 16 + h * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            const s16x4 lo = read_transposed(tv + place<S>(key, e >> 3) + (e & 7) * 2);
+            const s16x4 hi = read_transposed(tv + place<S>(key + 8, e >> 3) + (e & 7) * 2);
+            return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+        };
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-            Vec<T, 8> v[4];
+            if (!Careful) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                // lanes 16g .. 16g + 15 read 4 keys x 16 elements and get an element's 4 keys each
-                const int key = s * 16 + h * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-                const s16x4 lo = read_transposed(tv + place<S>(key, e >> 3) + (e & 7) * 2);
-                const s16x4 hi = read_transposed(tv + place<S>(key + 8, e >> 3) + (e & 7) * 2);
-                v[s] = __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-                if (!careful) o[d] = Mma<T>::go(v[s], w[s], o[d]);
+                for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(value(d, s), w[s], o[d]);
+                continue;
             }
-            if (careful) {
-                // a weight of 0 times NaN or an infinity is NaN: what is not finite is left out of the product and
-                // its kind brought in where the weights of such values sum to more than 0
-                for (int kind = 0; kind < 4; ++kind) {
-                    f32x16 c = {};
+            // a weight of 0 times NaN or an infinity is NaN: what is not finite is left out of the product and
+            // its kind brought in where the weights of such values sum to more than 0
+#pragma unroll 1
+            for (int kind = 0; kind < 4; ++kind) {
+                f32x16 c = {};
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        Vec<T, 8> x;
+                for (int s = 0; s < 2 * KB; ++s) {
+                    Vec<T, 8> x = value(d, s);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float f = static_cast<float>(v[s][i]);
-                            const int is = f != f ? 1 : f == INFINITY ? 2 : f == NONE ? 3 : 0;
-                            x[i] = static_cast<T>(kind == 0 ? (is ? 0.0f : f) : is == kind ? 1.0f : 0.0f);
-                        }
-                        c = Mma<T>::go(x, w[s], c);
+                    for (int i = 0; i < 8; ++i) {
+                        const float f = static_cast<float>(x[i]);
+                        const int is = f != f ? 1 : f == INFINITY ? 2 : f == NONE ? 3 : 0;
+                        x[i] = static_cast<T>(kind == 0 ? (is ? 0.0f : f) : is == kind ? 1.0f : 0.0f);
                     }
+                    c = Mma<T>::go(x, w[s], c);
+                }
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        o[d][r] += kind == 0 ? c[r] : !(c[r] > 0.0f) ? 0.0f : kind == 1 ? NAN : kind == 2 ? INFINITY : NONE;
+                for (int r = 0; r < 16; ++r)
+                    o[d][r] += kind == 0 ? c[r] : !(c[r] > 0.0f) ? 0.0f : kind == 1 ? NAN : kind == 2 ? INFINITY : NONE;
+            }
+        }
+    }
+    __device__ void join_halves() { sum += __shfl_xor(sum, 32); }
+};
+
+__device__ inline float reciprocal_of(float sum) { return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum; }
+__device__ inline float log_of(float top, float sum) { return sum == 0.0f ? NONE : (top + log2f(sum)) * LN2; }
+
+// Moves KEYS rows of keys and of values to LDS, 16 bytes a lane; THREADS threads (whole waves) share them.
+template <int S, int KEYS, int THREADS>
+struct Mover {
+    static constexpr int CH = S / 16, N = THREADS / CH, MOVES = KEYS / N;  // rows of a move; moves of each kind
+    const char *k, *v;
+    int64_t khop, vhop, kat, vat;  // bytes between rows; to this thread's row of a move
+    uint32_t nk;
+    int row, slot, wave;
+    uint32_t chunks;
+
+    __device__ Mover(const bs_attention_args& a, const Sequence& sq, uint32_t kvh, int thread)
+        : khop(a.k_stride * 2), vhop(a.v_stride * 2), nk(sq.nk), row(thread / CH), slot(thread % CH),
+          wave(__builtin_amdgcn_readfirstlane(thread >> 6)), chunks(a.head_dim / 8) {
+        k = static_cast<const char*>(a.k) + static_cast<int64_t>(sq.k0) * khop + static_cast<int64_t>(kvh) * a.k_head_stride * 2;
+        v = static_cast<const char*>(a.v) + static_cast<int64_t>(sq.k0) * vhop + static_cast<int64_t>(kvh) * a.v_head_stride * 2;
+        kat = row * khop;
+        vat = row * vhop;
+    }
+    // keys j0 .. j0 + KEYS - 1; those past the sequence's end repeat its last one, and no row sees them
+    __device__ void go(uint32_t j0, char* tk, char* tv) const {
+        const bool past = j0 + KEYS > nk;
+#pragma unroll
+        for (int i = 0; i < MOVES; ++i) {
+            const int r = i * N + row;
+            const uint32_t c = (place<S>(r, slot) - r * S) >> 4;  // the chunk whose place this slot is
+            const char *kp, *vp;
+            if (past) {
+                const int64_t key = min(j0 + r, nk - 1);
+                kp = k + key * khop;
+                vp = v + key * vhop;
+            } else {
+                kp = k + static_cast<int64_t>(j0 + i * N) * khop + kat;
+                vp = v + static_cast<int64_t>(j0 + i * N) * vhop + vat;
+            }
+            if (c < chunks) {
+                __builtin_amdgcn_global_load_lds((global_ptr)(kp + c * 16), (lds_ptr)(tk + i * N * S + wave * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_ptr)(vp + c * 16), (lds_ptr)(tv + i * N * S + wave * 1024), 16, 0, 0);
+            }
+        }
+    }
+};
+
+struct Place {  // of a row: its query token in the sequence, its head, the keys that it sees
+    uint32_t tok, head, keys;
+    bool live;
+};
+// row of a sequence's (token, head of the group) pairs; past the end the last one, not live
+__device__ inline Place place_of(const Params& p, const Sequence& sq, uint32_t kvh, uint64_t row, uint64_t rows) {
+    Place x;
+    x.live = row < rows;
+    const uint64_t r = x.live ? row : rows - 1;
+    x.tok = static_cast<uint32_t>(r / p.group);
+    x.head = kvh * p.group + static_cast<uint32_t>(r - static_cast<uint64_t>(x.tok) * p.group);
+    x.keys = keys_of(p.a, sq, x.tok);
+    return x;
+}
+
+// Whole prompts.  Four waves of 32 rows share the tiles of 64 keys in LDS, two of them: the next tile's moves
+// run under a tile's products.  Two workgroups per compute unit: one's matrix instructions run under the
+// other's exponentials.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
+    constexpr int ROWS = 128, S = ROW<DP>, TILE = BN * S;
+    __shared__ __attribute__((aligned(16))) char lds[2][2 * TILE];
+    __shared__ int flag;
+    const bs_attention_args& a = p.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+    const uint32_t seq = a.q_offsets ? find(a.q_offsets, a.sequences, tile, p.group, ROWS) : 0;
+    const uint64_t first = a.q_offsets ? first_tile(a.q_offsets, seq, p.group, ROWS) : 0;
+    const Sequence sq = sequence(a, seq);
+    const uint64_t rows = static_cast<uint64_t>(sq.nq) * p.group;
+    if (tile < first || (tile - first) * ROWS >= rows) return;
+    // the tiles that see most keys start first
+    const uint64_t row0 = ((rows - 1) / ROWS - (tile - first)) * ROWS;
+    const Place me = place_of(p, sq, kvh, row0 + wave * 32 + l, rows);
+    const uint64_t last_row = min(rows, row0 + ROWS) - 1;
+    const uint32_t all = keys_of(a, sq, static_cast<uint32_t>(last_row / p.group));  // of the tile's last row: the most
+    uint32_t kb = 0, ke = all;
+    if (p.splits > 1) {
+        kb = min(all, blockIdx.y * p.piece);
+        if (blockIdx.y + 1 < p.splits) ke = min(all, kb + p.piece);
+        if (kb >= ke && blockIdx.y > 0) return;  // the join does not read it
+    }
+    Rows<T, DP> me_;
+    me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
+             a.head_dim, h);
+    me_.clear();
+    if (a.head_dim != DP) {  // the padding of the heads is never moved to
+        for (int i = threadIdx.x; i < 2 * 2 * TILE / 16; i += 256) reinterpret_cast<Vec<float, 4>*>(lds[0])[i] = Vec<float, 4>{};
+    }
+    if (threadIdx.x == 0) flag = 0;
+    __syncthreads();
+    const Mover<S, BN, 256> mover(a, sq, kvh, threadIdx.x);
+    const float scale = a.scale * LOG2E;
+    const uint32_t mine = min(me.keys, ke);
+    // The tiles that some row does not see whole come first, on a state of zeros: if a result is then not
+    // finite, they are taken again with care, so that a row is never touched by a value it does not see.
+    const uint32_t seen = keys_of(a, sq, static_cast<uint32_t>(row0 / p.group));  // by every row of the tile
+    const uint32_t full = max(kb, min(ke, seen) / BN * BN);                      // kb and pieces are multiples of BN
+    const uint32_t parts = (ke - full + BN - 1) / BN, tiles = parts + (full - kb) / BN;
+    auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
+    if (tiles) mover.go(start(0), lds[0], lds[0] + TILE);
+    for (uint32_t t = 0; t < tiles; ++t) {
+        char* tk = lds[t & 1];
+        meet();  // tile t is in LDS, and nobody reads tile t - 1 any more
+        if (t + 1 < tiles) mover.go(start(t + 1), lds[~t & 1], lds[~t & 1] + TILE);
+        if (t >= parts) {
+            me_.template step<2, false, false>(tk, tk + TILE, start(t), mine, scale, lane);
+            continue;
+        }
+        me_.template step<2, true, false>(tk, tk + TILE, start(t), mine, scale, lane);
+        if (t + 1 == parts) {
+            if (me_.odd()) flag = 1;
+            meet();
+            if (flag) {
+                me_.clear();
+                for (uint32_t u = 0; u < parts; ++u) {
+                    meet();
+                    mover.go(start(u), tk, tk + TILE);
+                    meet();
+                    me_.template step<2, true, true>(tk, tk + TILE, start(u), mine, scale, lane);
                 }
             }
         }
-    };
-    // The tiles that some row does not see whole come first, on a state of zeros: if a result is then not
-    // finite, they are taken again with care, so that a row is never touched by a value it does not see.
-    const uint32_t seen = keys_of(static_cast<uint32_t>(row0 / p.group));  // by every row of the tile
-    const uint32_t full = max(kb, min(ke, seen) / BN * BN);                // kb and pieces are multiples of BN
-    clear();
-    for (uint32_t j0 = full; j0 < ke; j0 += BN) step(j0, std::true_type(), std::false_type());
-    if (full < ke) {
-        bool odd = false;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) odd |= !(fabsf(o[d][r]) < INFINITY);
-        if (__syncthreads_or(odd)) {
-            clear();
-            for (uint32_t j0 = full; j0 < ke; j0 += BN) step(j0, std::true_type(), std::true_type());
-        }
     }
-    for (uint32_t j0 = kb; j0 < full; j0 += BN) step(j0, std::false_type(), std::false_type());
-    if (!live) return;
-    const int64_t at = static_cast<int64_t>(sq.q0 + tok) * a.heads + head;
+    me_.join_halves();
+    if (!me.live) return;
+    const int64_t at = static_cast<int64_t>(sq.q0 + me.tok) * a.heads + me.head;
     if (p.splits > 1) {
         const int64_t slot = static_cast<int64_t>(blockIdx.y) * a.q_tokens * a.heads + at;
-        if (h == 0) p.part_stat[slot] = make_float2(top, sum);
+        if (h == 0) p.part_stat[slot] = make_float2(me_.top, me_.sum);
         float* out = p.part_out + slot * a.head_dim;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const uint32_t e = d * 32 + r * 8 + h * 4;
-                if (e < a.head_dim) *reinterpret_cast<f32x4*>(out + e) = f32x4{o[d][r * 4], o[d][r * 4 + 1], o[d][r * 4 + 2], o[d][r * 4 + 3]};
+                const f32x4 v = {me_.o[d][r * 4], me_.o[d][r * 4 + 1], me_.o[d][r * 4 + 2], me_.o[d][r * 4 + 3]};
+                if (e < a.head_dim) *reinterpret_cast<f32x4*>(out + e) = v;
             }
         return;
     }
-    const float over = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(sq.q0 + tok) * a.out_stride + static_cast<int64_t>(head) * a.out_head_stride;
+    const float over = reciprocal_of(me_.sum);
+    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(sq.q0 + me.tok) * a.out_stride + static_cast<int64_t>(me.head) * a.out_head_stride;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -282,10 +393,122 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
             const uint32_t e = d * 32 + r * 8 + h * 4;
             Vec<T, 4> v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = static_cast<T>(o[d][r * 4 + i] * over);
+            for (int i = 0; i < 4; ++i) v[i] = static_cast<T>(me_.o[d][r * 4 + i] * over);
             if (e < a.head_dim) *reinterpret_cast<Vec<T, 4>*>(out + e) = v;
         }
-    if (a.lse && h == 0) a.lse[at] = sum == 0.0f ? NONE : (top + log2f(sum)) * LN2;
+    if (a.lse && h == 0) a.lse[at] = log_of(me_.top, me_.sum);
+}
+
+// Few rows per sequence (single tokens): the keys' bytes bound the time.  A tile has at most 32 rows, and the
+// four waves of a workgroup take every fourth tile of 32 keys each, through LDS of their own, without meeting;
+// their results are joined at the end.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 1) void attention_few_kernel(Params p) {
+    constexpr int ROWS = 32, KN = 32, S = ROW<DP>, TILE = KN * S, NB = 32768 / (2 * TILE);  // NB tiles of a wave in LDS
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const bs_attention_args& a = p.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+    const uint32_t seq = a.q_offsets ? find(a.q_offsets, a.sequences, tile, p.group, ROWS) : 0;
+    const uint64_t first = a.q_offsets ? first_tile(a.q_offsets, seq, p.group, ROWS) : 0;
+    const Sequence sq = sequence(a, seq);
+    const uint64_t rows = static_cast<uint64_t>(sq.nq) * p.group;
+    if (tile < first || (tile - first) * ROWS >= rows) return;
+    const uint64_t row0 = (tile - first) * ROWS;
+    const Place me = place_of(p, sq, kvh, row0 + l, rows);
+    const uint32_t here = static_cast<uint32_t>(min(rows - row0, static_cast<uint64_t>(ROWS)));  // rows of the tile
+    const uint32_t all = keys_of(a, sq, static_cast<uint32_t>((row0 + here - 1) / p.group));
+    const uint32_t kb = min(all, blockIdx.y * p.piece), ke = blockIdx.y + 1 < p.splits ? min(all, kb + p.piece) : all;
+    if (kb >= ke && blockIdx.y > 0) return;  // the join does not read it
+    Rows<T, DP> me_;
+    me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
+             a.head_dim, h);
+    me_.clear();
+    char* mem = lds + wave * 32768;
+    if (a.head_dim != DP) {  // the padding of the heads is never moved to
+        for (int i = lane; i < 32768 / 16; i += 64) reinterpret_cast<Vec<float, 4>*>(mem)[i] = Vec<float, 4>{};
+    }
+    const Mover<S, KN, 64> mover(a, sq, kvh, lane);
+    const float scale = a.scale * LOG2E;
+    const uint32_t mine = min(me.keys, ke), seen = keys_of(a, sq, static_cast<uint32_t>(row0 / p.group));
+    // tiles from the last to the first: of those that some row does not see whole (there are at most 3: a tile
+    // of rows has at most 32 tokens) a wave has at most one, its first
+    const uint32_t tiles = (ke - kb + KN - 1) / KN, n = tiles > static_cast<uint32_t>(wave) ? (tiles - wave + 3) / 4 : 0;
+    auto start = [&](uint32_t u) { return kb + (tiles - 1 - wave - 4 * u) * KN; };
+    auto buffer = [&](uint32_t u) { return mem + u % NB * (2 * TILE); };
+    constexpr int MOVES = 2 * Mover<S, KN, 64>::MOVES;  // of a tile
+    static_assert((NB - 1) * MOVES < 64, "counted by vmcnt");
+    landed<0>();
+#pragma unroll
+    for (int u = 0; u < NB - 1; ++u)
+        if (static_cast<uint32_t>(u) < n) mover.go(start(u), buffer(u), buffer(u) + TILE);
+    for (uint32_t u = 0; u < n; ++u) {
+        if (u + NB - 1 < n) {
+            landed<63>();  // reads of the tile before are done
+            mover.go(start(u + NB - 1), buffer(u + NB - 1), buffer(u + NB - 1) + TILE);
+            landed<(NB - 1) * MOVES>();
+        } else {
+            landed<0>();
+        }
+        const uint32_t j0 = start(u);
+        const char* tk = buffer(u);
+        if (j0 + KN <= min(seen, ke)) {
+            me_.template step<1, false, false>(tk, tk + TILE, j0, mine, scale, lane);
+        } else {
+            me_.template step<1, true, false>(tk, tk + TILE, j0, mine, scale, lane);
+            if (__any(me_.odd())) {  // as above
+                me_.clear();
+                me_.template step<1, true, true>(tk, tk + TILE, j0, mine, scale, lane);
+            }
+        }
+    }
+    me_.join_halves();
+    // joins the waves: every wave's results against the largest of their maxima, then a sum in wave order
+    __shared__ float2 stat[4][32];
+    landed<0>();
+    __syncthreads();  // nobody reads tiles any more
+    if (h == 0) stat[wave][l] = make_float2(me_.top, me_.sum);
+    float* all_o = reinterpret_cast<float*>(lds);  // 4 x 32 x (DP + 4)
+    __syncthreads();
+    float top = NONE;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][l].x);
+    const float gain = __builtin_amdgcn_exp2f(me_.top - (top == NONE ? 0.0f : top));
+    if (static_cast<uint32_t>(l) < here) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<f32x4*>(all_o + (wave * 32 + l) * (DP + 4) + d * 32 + r * 8 + h * 4) =
+                    f32x4{me_.o[d][r * 4] * gain, me_.o[d][r * 4 + 1] * gain, me_.o[d][r * 4 + 2] * gain, me_.o[d][r * 4 + 3] * gain};
+    }
+    __syncthreads();
+    const uint32_t quads = a.head_dim / 4;
+    for (uint32_t i = threadIdx.x; i < here * quads; i += 256) {
+        const uint32_t r = i / quads, e = i % quads * 4;
+        float t = NONE, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) t = fmaxf(t, stat[w][r].x);
+        f32x4 v = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            sum += stat[w][r].y * __builtin_amdgcn_exp2f(stat[w][r].x - (t == NONE ? 0.0f : t));
+            v += *reinterpret_cast<const f32x4*>(all_o + (w * 32 + r) * (DP + 4) + e);
+        }
+        const Place x = place_of(p, sq, kvh, row0 + r, rows);
+        const int64_t at = static_cast<int64_t>(sq.q0 + x.tok) * a.heads + x.head;
+        if (p.splits > 1) {
+            const int64_t slot = static_cast<int64_t>(blockIdx.y) * a.q_tokens * a.heads + at;
+            *reinterpret_cast<f32x4*>(p.part_out + slot * a.head_dim + e) = v;
+            if (e == 0) p.part_stat[slot] = make_float2(t, sum);
+        } else {
+            const float over = reciprocal_of(sum);
+            const Vec<T, 4> y = {static_cast<T>(v[0] * over), static_cast<T>(v[1] * over), static_cast<T>(v[2] * over), static_cast<T>(v[3] * over)};
+            *reinterpret_cast<Vec<T, 4>*>(static_cast<T*>(a.out) + static_cast<int64_t>(sq.q0 + x.tok) * a.out_stride +
+                                          static_cast<int64_t>(x.head) * a.out_head_stride + e) = y;
+            if (a.lse && e == 0) a.lse[at] = log_of(t, sum);
+        }
+    }
 }
 
 // joins the pieces of a row: a wave per (query token, head)
@@ -328,13 +551,13 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
             o[1] = o[1] * fade + v.y * gain;
         }
     }
-    const float over = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    const float over = reciprocal_of(sum);
     T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tok) * a.out_stride + static_cast<int64_t>(head) * a.out_head_stride;
     if (d < a.head_dim) {
         const Vec<T, 2> v = {static_cast<T>(o[0] * over), static_cast<T>(o[1] * over)};
         *reinterpret_cast<Vec<T, 2>*>(out + d) = v;
     }
-    if (a.lse && lane == 0) a.lse[at] = sum == 0.0f ? NONE : (top + log2f(sum)) * LN2;
+    if (a.lse && lane == 0) a.lse[at] = log_of(top, sum);
 }
 
 uint64_t tiles_of(const bs_attention_args& a, uint32_t rows) {
@@ -342,16 +565,33 @@ uint64_t tiles_of(const bs_attention_args& a, uint32_t rows) {
     return t / rows + a.sequences;
 }
 
-// pieces of the keys: enough workgroups for the chip, pieces of 256 keys at least
+// Few rows: sequences of two tiles of 32 rows at most, by the longest one where it is given, else by their mean.
+bool few_of(const bs_attention_args& a) {
+    const uint64_t group = a.heads / a.kv_heads;
+    const uint64_t tokens = a.longest_q ? a.longest_q : (a.q_tokens + a.sequences - 1) / a.sequences;
+    return tokens * group <= 64;
+}
+
+// Pieces of the keys, multiples of the keys that a workgroup takes at a time.  The last one takes what is left,
+// should a sequence be longer than longest_k said.
 void split(const bs_attention_args& a, uint32_t& splits, uint32_t& piece) {
-    const uint64_t groups = tiles_of(a, 128) * a.kv_heads;
     const uint32_t longest = a.longest_k ? std::min(a.longest_k, a.k_tokens) : a.k_tokens;
-    splits = 1;
-    piece = 0;
-    if (groups >= 2 * CUS || longest <= 512) return;
-    const uint64_t want = std::min<uint64_t>((4 * CUS + groups - 1) / groups, (longest + 255) / 256);
-    piece = static_cast<uint32_t>(((longest + want - 1) / want + BN - 1) / BN * BN);
-    splits = (longest + piece - 1) / piece;
+    uint64_t want;
+    if (few_of(a)) {
+        // about six workgroups per compute unit, so that sequences of different lengths even out
+        const uint64_t keys = static_cast<uint64_t>(a.k_tokens) * a.kv_heads * std::max<uint64_t>(1, (tiles_of(a, 32) - a.sequences) / a.sequences);
+        want = std::max<uint64_t>(keys / (6 * CUS), 256);
+    } else {
+        const uint64_t groups = tiles_of(a, 128) * a.kv_heads;
+        want = groups >= 2 * CUS ? longest : std::max<uint64_t>(longest * groups / (4 * CUS), 256);
+    }
+    piece = static_cast<uint32_t>(std::min<uint64_t>((want + 127) / 128 * 128, (static_cast<uint64_t>(longest) + 127) / 128 * 128));
+    if (piece == 0) piece = 128;
+    // at most 256 MB of parts: with many sequences the pieces are for their different lengths alone
+    const uint64_t row = static_cast<uint64_t>(a.q_tokens) * a.heads * (a.head_dim + 2) * sizeof(float);
+    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(65535, (1ull << 28) / std::max<uint64_t>(row, 1)));
+    if ((longest + piece - 1) / piece > most) piece = static_cast<uint32_t>((longest + most - 1) / most + 127) / 128 * 128;
+    splits = std::max(1u, (longest + piece - 1) / piece);
 }
 
 uint64_t workspace_of(const bs_attention_args& a) {
@@ -371,21 +611,35 @@ int check(const char* what, const bs_attention_args* a) {
     if (a->q_tokens > 0x7FFFFFFFu || a->k_tokens > 0x7FFFFFFFu) return refuse(w + ": q_tokens and k_tokens must be < 2^31");
     if (a->sequences == 0 || a->sequences > 0x7FFFFFFu) return refuse(w + ": sequences must be in 1..2^27");
     if (!(std::fabs(a->scale) < INFINITY)) return refuse(w + ": scale must be finite");
-    if (tiles_of(*a, 128) * a->kv_heads > 0x7FFFFFFFull) return refuse(w + ": too many tiles for one launch");
+    if (tiles_of(*a, 32) * a->kv_heads > 0x7FFFFFFFull) return refuse(w + ": too many tiles for one launch");
     return BS_OK;
+}
+
+template <typename T, int DP>
+void start(const Params& p, hipStream_t s) {
+    const bool few = few_of(p.a);
+    const dim3 grid(static_cast<uint32_t>(tiles_of(p.a, few ? 32 : 128) * p.a.kv_heads), p.splits);
+    if (few) {
+        constexpr int LDS = 4 * 32768;
+        auto* k = attention_few_kernel<T, DP>;
+        static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        (void)once;
+        k<<<grid, 256, LDS, s>>>(p);
+    } else {
+        attention_kernel<T, DP><<<grid, 256, 0, s>>>(p);
+    }
 }
 
 template <typename T>
 void launch(const Params& p, hipStream_t s) {
-    const dim3 grid(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits);
     if (p.a.head_dim <= 32)
-        attention_kernel<T, 32><<<grid, 256, 0, s>>>(p);
+        start<T, 32>(p, s);
     else if (p.a.head_dim <= 64)
-        attention_kernel<T, 64><<<grid, 256, 0, s>>>(p);
+        start<T, 64>(p, s);
     else if (p.a.head_dim <= 96)
-        attention_kernel<T, 96><<<grid, 256, 0, s>>>(p);
+        start<T, 96>(p, s);
     else
-        attention_kernel<T, 128><<<grid, 256, 0, s>>>(p);
+        start<T, 128>(p, s);
     if (p.splits > 1) {
         const uint64_t rows = static_cast<uint64_t>(p.a.q_tokens) * p.a.heads;
         join_kernel<T><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, s>>>(p);

@@ -80,6 +80,18 @@ __device__ inline uint32_t find(const int32_t* off, uint32_t n, uint64_t tile, u
     return lo;
 }
 
+// the last sequence that starts at or before the token
+__device__ inline uint32_t holder(const int32_t* off, uint32_t n, uint32_t tok) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 63) / 64, at = lo + (threadIdx.x & 63) * step;
+        const int k = __popcll(__ballot(at < hi && static_cast<uint32_t>(max(off[at], 0)) <= tok));
+        lo += (k > 0 ? k - 1 : 0) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
+}
+
 // chunk c of 16 bytes in row r of an LDS tile of S bytes per row (64, 128 or 256).  16 rows read at one
 // chunk (a quarter wave's operand of K) lie in 16 different chunks of the 256 bytes that all banks span,
 // and the 4 rows x 64 bytes of a transposed read of V in 4 different quarters of them.
@@ -400,11 +412,14 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
 }
 
 // Few rows per sequence (single tokens): the keys' bytes bound the time.  A tile has at most 32 rows, and the
-// four waves of a workgroup take every fourth tile of 32 keys each, through LDS of their own, without meeting;
+// FEW_WAVES waves of a workgroup take turns at its tiles of 32 keys, through LDS of their own, without meeting;
 // their results are joined at the end.
+constexpr int FEW_WAVES = 2;
+
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 1) void attention_few_kernel(Params p) {
+__global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params p) {
     constexpr int ROWS = 32, KN = 32, S = ROW<DP>, TILE = KN * S, NB = 32768 / (2 * TILE);  // NB tiles of a wave in LDS
+    constexpr int W = FEW_WAVES;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const bs_attention_args& a = p.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
@@ -431,25 +446,23 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Params p) {
     const Mover<S, KN, 64> mover(a, sq, kvh, lane);
     const float scale = a.scale * LOG2E;
     const uint32_t mine = min(me.keys, ke), seen = keys_of(a, sq, static_cast<uint32_t>(row0 / p.group));
-    // tiles from the last to the first: of those that some row does not see whole (there are at most 3: a tile
-    // of rows has at most 32 tokens) a wave has at most one, its first
-    const uint32_t tiles = (ke - kb + KN - 1) / KN, n = tiles > static_cast<uint32_t>(wave) ? (tiles - wave + 3) / 4 : 0;
-    auto start = [&](uint32_t u) { return kb + (tiles - 1 - wave - 4 * u) * KN; };
+    // tiles from the last to the first: of those that some row does not see whole (at most 2 in a row: a
+    // tile of rows has at most 32 tokens) a wave has at most one, its first
+    const uint32_t tiles = (ke - kb + KN - 1) / KN, n = tiles > static_cast<uint32_t>(wave) ? (tiles - wave + W - 1) / W : 0;
+    auto start = [&](uint32_t u) { return kb + (tiles - 1 - wave - W * u) * KN; };
     auto buffer = [&](uint32_t u) { return mem + u % NB * (2 * TILE); };
     constexpr int MOVES = 2 * Mover<S, KN, 64>::MOVES;  // of a tile
-    static_assert((NB - 1) * MOVES < 64, "counted by vmcnt");
+    static_assert(NB * MOVES < 64, "counted by vmcnt");
     landed<0>();
 #pragma unroll
-    for (int u = 0; u < NB - 1; ++u)
+    for (int u = 0; u < NB; ++u)
         if (static_cast<uint32_t>(u) < n) mover.go(start(u), buffer(u), buffer(u) + TILE);
     for (uint32_t u = 0; u < n; ++u) {
-        if (u + NB - 1 < n) {
-            landed<63>();  // reads of the tile before are done
-            mover.go(start(u + NB - 1), buffer(u + NB - 1), buffer(u + NB - 1) + TILE);
+        // the moves of tiles u + 1 .. u + NB - 1 may be on their way
+        if (u + NB <= n)
             landed<(NB - 1) * MOVES>();
-        } else {
+        else
             landed<0>();
-        }
         const uint32_t j0 = start(u);
         const char* tk = buffer(u);
         if (j0 + KN <= min(seen, ke)) {
@@ -461,18 +474,22 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Params p) {
                 me_.template step<1, true, true>(tk, tk + TILE, j0, mine, scale, lane);
             }
         }
+        if (u + NB < n) {
+            landed<63>();  // this tile's reads are done
+            mover.go(start(u + NB), buffer(u), buffer(u) + TILE);
+        }
     }
     me_.join_halves();
     // joins the waves: every wave's results against the largest of their maxima, then a sum in wave order
-    __shared__ float2 stat[4][32];
+    __shared__ float2 stat[W][32];
     landed<0>();
     __syncthreads();  // nobody reads tiles any more
     if (h == 0) stat[wave][l] = make_float2(me_.top, me_.sum);
-    float* all_o = reinterpret_cast<float*>(lds);  // 4 x 32 x (DP + 4)
+    float* all_o = reinterpret_cast<float*>(lds);  // W x 32 x (DP + 4)
     __syncthreads();
     float top = NONE;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][l].x);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, stat[w][l].x);
     const float gain = __builtin_amdgcn_exp2f(me_.top - (top == NONE ? 0.0f : top));
     if (static_cast<uint32_t>(l) < here) {
 #pragma unroll
@@ -484,14 +501,14 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Params p) {
     }
     __syncthreads();
     const uint32_t quads = a.head_dim / 4;
-    for (uint32_t i = threadIdx.x; i < here * quads; i += 256) {
+    for (uint32_t i = threadIdx.x; i < here * quads; i += W * 64) {
         const uint32_t r = i / quads, e = i % quads * 4;
         float t = NONE, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) t = fmaxf(t, stat[w][r].x);
+        for (int w = 0; w < W; ++w) t = fmaxf(t, stat[w][r].x);
         f32x4 v = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
             sum += stat[w][r].y * __builtin_amdgcn_exp2f(stat[w][r].x - (t == NONE ? 0.0f : t));
             v += *reinterpret_cast<const f32x4*>(all_o + (w * 32 + r) * (DP + 4) + e);
         }
@@ -511,51 +528,51 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Params p) {
     }
 }
 
-// joins the pieces of a row: a wave per (query token, head)
+// Joins the pieces of a row (query token, head): a workgroup each.  First the maximum of all pieces and the sum
+// against it, a piece per lane; then the results, the pieces in four contiguous runs, one per wave.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
+    __shared__ float2 half[4][64];
     const bs_attention_args& a = p.a;
-    const int lane = threadIdx.x & 63;
-    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6), rows = static_cast<uint64_t>(a.q_tokens) * a.heads;
-    if (at >= rows) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t at = blockIdx.x, rows = static_cast<uint64_t>(a.q_tokens) * a.heads;
     const uint32_t tok = static_cast<uint32_t>(at / a.heads), head = static_cast<uint32_t>(at % a.heads);
-    uint32_t seq = 0;
-    if (a.q_offsets) {
-        // the last sequence that starts at or before the token and holds it
-        uint32_t lo = 0, hi = a.sequences;
-        while (hi - lo > 1) {
-            const uint32_t step = (hi - lo + 63) / 64, x = lo + lane * step;
-            const int k = __popcll(__ballot(x < hi && static_cast<uint32_t>(max(a.q_offsets[x], 0)) <= tok));
-            lo += (k > 0 ? k - 1 : 0) * step;
-            hi = min(lo + step, hi);
-        }
-        seq = lo;
-    }
+    const uint32_t seq = a.q_offsets ? holder(a.q_offsets, a.sequences, tok) : 0;
     const Sequence sq = sequence(a, seq);
     if (tok < sq.q0 || tok - sq.q0 >= sq.nq) return;
-    int64_t e = a.causal ? min(static_cast<int64_t>(sq.nk), static_cast<int64_t>(tok - sq.q0) + sq.nk - sq.nq + 1) : static_cast<int64_t>(sq.nk);
-    const uint32_t keys = e < 0 ? 0 : static_cast<uint32_t>(e);
+    const uint32_t keys = keys_of(a, sq, tok - sq.q0);
     const uint32_t n = max(1u, min(p.splits, (keys + p.piece - 1) / p.piece));
-    float top = NONE, sum = 0.0f, o[2] = {0.0f, 0.0f};
-    const uint32_t d = lane * 2;
-    for (uint32_t s = 0; s < n; ++s) {
-        const uint64_t slot = s * rows + at;
-        const float2 st = p.part_stat[slot];
-        const float now = fmaxf(top, st.x), base = now == NONE ? 0.0f : now;
-        const float fade = exp2f(top - base), gain = exp2f(st.x - base);
-        sum = sum * fade + st.y * gain;
-        top = now;
-        if (d < a.head_dim) {
+    float top = NONE, sum = 0.0f;
+    for (uint32_t s = lane; s < n; s += 64) top = fmaxf(top, p.part_stat[s * rows + at].x);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    const float base = top == NONE ? 0.0f : top;
+    for (uint32_t s = lane; s < n; s += 64) {
+        const float2 st = p.part_stat[s * rows + at];
+        sum += st.y * __builtin_amdgcn_exp2f(st.x - base);
+    }
+    sum = wave_sum(sum);
+    const uint32_t d = lane * 2, run = (n + 3) / 4, begin = wave * run, end = min(begin + run, n);
+    float2 o = make_float2(0.0f, 0.0f);
+    if (d < a.head_dim) {
+#pragma unroll 4
+        for (uint32_t s = begin; s < end; ++s) {
+            const uint64_t slot = s * rows + at;
+            const float gain = __builtin_amdgcn_exp2f(p.part_stat[slot].x - base);
             const float2 v = *reinterpret_cast<const float2*>(p.part_out + slot * a.head_dim + d);
-            o[0] = o[0] * fade + v.x * gain;
-            o[1] = o[1] * fade + v.y * gain;
+            o.x = fmaf(v.x, gain, o.x);
+            o.y = fmaf(v.y, gain, o.y);
         }
     }
+    half[wave][lane] = o;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) o.x += half[w][lane].x, o.y += half[w][lane].y;
     const float over = reciprocal_of(sum);
-    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tok) * a.out_stride + static_cast<int64_t>(head) * a.out_head_stride;
     if (d < a.head_dim) {
-        const Vec<T, 2> v = {static_cast<T>(o[0] * over), static_cast<T>(o[1] * over)};
-        *reinterpret_cast<Vec<T, 2>*>(out + d) = v;
+        T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tok) * a.out_stride + static_cast<int64_t>(head) * a.out_head_stride;
+        *reinterpret_cast<Vec<T, 2>*>(out + d) = Vec<T, 2>{static_cast<T>(o.x * over), static_cast<T>(o.y * over)};
     }
     if (a.lse && lane == 0) a.lse[at] = log_of(top, sum);
 }
@@ -611,7 +628,7 @@ int check(const char* what, const bs_attention_args* a) {
     if (a->q_tokens > 0x7FFFFFFFu || a->k_tokens > 0x7FFFFFFFu) return refuse(w + ": q_tokens and k_tokens must be < 2^31");
     if (a->sequences == 0 || a->sequences > 0x7FFFFFFu) return refuse(w + ": sequences must be in 1..2^27");
     if (!(std::fabs(a->scale) < INFINITY)) return refuse(w + ": scale must be finite");
-    if (tiles_of(*a, 32) * a->kv_heads > 0x7FFFFFFFull) return refuse(w + ": too many tiles for one launch");
+    if (tiles_of(*a, 32) * a->kv_heads > 0x7FFFFFFFull || static_cast<uint64_t>(a->q_tokens) * a->heads > 0x7FFFFFFFull) return refuse(w + ": too many tiles for one launch");
     return BS_OK;
 }
 
@@ -620,11 +637,11 @@ void start(const Params& p, hipStream_t s) {
     const bool few = few_of(p.a);
     const dim3 grid(static_cast<uint32_t>(tiles_of(p.a, few ? 32 : 128) * p.a.kv_heads), p.splits);
     if (few) {
-        constexpr int LDS = 4 * 32768;
+        constexpr int LDS = FEW_WAVES * 32768;
         auto* k = attention_few_kernel<T, DP>;
         static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         (void)once;
-        k<<<grid, 256, LDS, s>>>(p);
+        k<<<grid, FEW_WAVES * 64, LDS, s>>>(p);
     } else {
         attention_kernel<T, DP><<<grid, 256, 0, s>>>(p);
     }
@@ -642,7 +659,7 @@ void launch(const Params& p, hipStream_t s) {
         start<T, 128>(p, s);
     if (p.splits > 1) {
         const uint64_t rows = static_cast<uint64_t>(p.a.q_tokens) * p.a.heads;
-        join_kernel<T><<<static_cast<uint32_t>((rows + 3) / 4), 256, 0, s>>>(p);
+        join_kernel<T><<<static_cast<uint32_t>(rows), 256, 0, s>>>(p);
     }
 }
 

@@ -131,6 +131,13 @@ __device__ inline uint32_t keys_of(const bs_attention_args& a, const Sequence& s
     return static_cast<uint32_t>(e < 0 ? 0 : e);
 }
 
+// the values of lanes l and l + 32, to both
+__device__ inline float2 halves(float v) {
+    const uint32_t b = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 template <int DP>
 constexpr int ROW = DP <= 32 ? 64 : DP <= 64 ? 128 : 256;  // bytes of a key or value in LDS
 
@@ -148,12 +155,14 @@ struct Rows {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
     }
-    __device__ void load(const T* p, uint32_t head_dim, int h) {
+    // scores are taken times a scale > 0: a negative one turns the sign of the query, for 0 the query is 0
+    __device__ void load(const T* p, uint32_t head_dim, float scale, int h) {
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
             const uint32_t d = s * 16 + h * 8;
             q[s] = Vec<T, 8>{};
-            if (d < head_dim) q[s] = *reinterpret_cast<const Vec<T, 8>*>(p + d);
+            if (d < head_dim && scale != 0.0f) q[s] = *reinterpret_cast<const Vec<T, 8>*>(p + d);
+            if (scale < 0.0f) q[s] = -q[s];
         }
     }
     __device__ bool odd() const {  // some result is not finite
@@ -164,30 +173,57 @@ struct Rows {
             for (int r = 0; r < 16; ++r) is |= !(fabsf(o[d][r]) < INFINITY);
         return is;
     }
-    // KB x 32 keys from j0 on, in LDS.  Masked: only those below `mine` count.  Careful: values of weight 0
-    // that are not finite do not touch the result.
-    template <int KB, bool Masked, bool Careful>
+    // KB x 32 keys from j0 on, in LDS.  Masked: only those below `mine` count.
+    template <int KB, bool Masked>
     __device__ void step(const char* tk, const char* tv, uint32_t j0, uint32_t mine, float scale, int lane) {
         const int l = lane & 31, h = lane >> 5;
-        f32x16 z[KB] = {};
+        // Operands are read a part ahead of their products: parts of 32 elements of the keys, then of 32
+        // elements of the values, the first of which comes in under the exponentials.
+        Vec<T, 8> k[2][2][KB];
+        auto read_keys = [&](int i) {
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                const Vec<T, 8> k = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + l, s * 2 + h));
-                z[b] = Mma<T>::go(k, q[s], z[b]);
-            }
+                for (int b = 0; b < KB; ++b)
+                    k[i & 1][s][b] = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + l, i * 4 + s * 2 + h));
+        };
+        f32x16 z[KB];
+        read_keys(0);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            if (i + 1 < DP / 32) read_keys(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int b = 0; b < KB; ++b) z[b] = Mma<T>::go(k[i & 1][s][b], q[i * 2 + s], i + s ? z[b] : f32x16{});
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        auto value = [&](int d, int s) {  // 16 keys of 32 elements
+            // lanes 16g .. 16g + 15 read 4 keys x 16 elements and get an element's 4 keys each
+            const int key = s * 16 + h * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            const s16x4 lo = read_transposed(tv + place<S>(key, e >> 3) + (e & 7) * 2);
+            const s16x4 hi = read_transposed(tv + place<S>(key + 8, e >> 3) + (e & 7) * 2);
+            return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+        };
+        Vec<T, 8> v[2][2 * KB];
+        auto read_values = [&](int d) {
+#pragma unroll
+            for (int s = 0; s < 2 * KB; ++s) v[d & 1][s] = value(d, s);
+        };
+        read_values(0);
+        __builtin_amdgcn_sched_barrier(0);
         // result register r of block b: key b * 32 + r % 4 + 8 (r / 4) + 4 h
         float most = NONE;
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                z[b][r] *= scale;
                 if (Masked && j0 + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * h >= mine) z[b][r] = NONE;
                 most = fmaxf(most, z[b][r]);
             }
-        most = fmaxf(most, __shfl_xor(most, 32));
+        const float2 two = halves(most);
+        most = fmaxf(two.x, two.y) * scale;  // scale > 0
         // The weights may stand against an older maximum while they stay below 2^8: sums and results lose
         // nothing by that, and the results are rescaled seldom.
         if (__any(most > top + 8.0f)) {
@@ -206,48 +242,74 @@ struct Rows {
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float e = __builtin_amdgcn_exp2f(z[b][r] - base);
+                const float e = __builtin_amdgcn_exp2f(fmaf(z[b][r], scale, -base));
                 add += e;
                 w[b * 2 + (r >> 3)][r & 7] = static_cast<T>(e);
             }
         sum += add;
-        auto value = [&](int d, int s) {  // 16 keys of 32 elements
-            // lanes 16g .. 16g + 15 read 4 keys x 16 elements and get an element's 4 keys each
-            const int key = s * 16 + h * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-            const s16x4 lo = read_transposed(tv + place<S>(key, e >> 3) + (e & 7) * 2);
-            const s16x4 hi = read_transposed(tv + place<S>(key + 8, e >> 3) + (e & 7) * 2);
-            return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-        };
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-            if (!Careful) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (d + 1 < DP / 32) read_values(d + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(value(d, s), w[s], o[d]);
-                continue;
-            }
-            // a weight of 0 times NaN or an infinity is NaN: what is not finite is left out of the product and
-            // its kind brought in where the weights of such values sum to more than 0
-#pragma unroll 1
-            for (int kind = 0; kind < 4; ++kind) {
-                f32x16 c = {};
-#pragma unroll
-                for (int s = 0; s < 2 * KB; ++s) {
-                    Vec<T, 8> x = value(d, s);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float f = static_cast<float>(x[i]);
-                        const int is = f != f ? 1 : f == INFINITY ? 2 : f == NONE ? 3 : 0;
-                        x[i] = static_cast<T>(kind == 0 ? (is ? 0.0f : f) : is == kind ? 1.0f : 0.0f);
-                    }
-                    c = Mma<T>::go(x, w[s], c);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    o[d][r] += kind == 0 ? c[r] : !(c[r] > 0.0f) ? 0.0f : kind == 1 ? NAN : kind == 2 ? INFINITY : NONE;
-            }
+            for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(v[d & 1][s], w[s], o[d]);
         }
     }
-    __device__ void join_halves() { sum += __shfl_xor(sum, 32); }
+    __device__ void join_halves() {
+        const float2 two = halves(sum);
+        sum = two.x + two.y;
+    }
+};
+
+// A weight of 0 times NaN or an infinity is NaN, so a row would be touched by values that it does not see.  Where
+// the tiles that some row does not see whole give a result that is not finite, they are taken five times:
+// as they are, with 1 for every NaN (+infinity, -infinity) and 0 for the rest, and with 0 for what is not
+// finite.  The last pass gives the sums; NaN and infinities are added where their passes gave more than 0.
+enum { PLAIN = 0, NANS = 1, HIGH = 2, LOW = 3, FINITE = 4 };
+
+// the values of a tile for a pass: 16 bytes at a time, by THREADS threads
+template <typename T>
+__device__ inline void sift(char* tv, int bytes, int pass, int thread, int threads) {
+    for (int i = thread; i < bytes / 16; i += threads) {
+        Vec<T, 8>* p = reinterpret_cast<Vec<T, 8>*>(tv) + i;
+        Vec<T, 8> x = *p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = static_cast<float>(x[j]);
+            const int is = f != f ? NANS : f == INFINITY ? HIGH : f == NONE ? LOW : FINITE;
+            x[j] = static_cast<T>(pass == FINITE ? (is == FINITE ? f : 0.0f) : is == pass ? 1.0f : 0.0f);
+        }
+        *p = x;
+    }
+}
+template <int N>
+struct Found {  // results with such values: a bit each, NaN and +infinity in one word, -infinity in the other
+    uint32_t one[N], two[N];
+    __device__ void clear() {
+#pragma unroll
+        for (int d = 0; d < N; ++d) one[d] = two[d] = 0;
+    }
+    __device__ void take(const f32x16 (&o)[N], int pass) {
+#pragma unroll
+        for (int d = 0; d < N; ++d) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bits |= o[d][r] > 0.0f ? 1u << r : 0u;
+            one[d] |= pass == NANS ? bits : pass == HIGH ? bits << 16 : 0u;
+            two[d] |= pass == LOW ? bits : 0u;
+        }
+    }
+    __device__ void give(f32x16 (&o)[N]) const {
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if (one[d] >> r & 1) o[d][r] = NAN;
+                if (one[d] >> (r + 16) & 1) o[d][r] += INFINITY;
+                if (two[d] >> r & 1) o[d][r] += NONE;
+            }
+    }
 };
 
 __device__ inline float reciprocal_of(float sum) { return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum; }
@@ -339,7 +401,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
     }
     Rows<T, DP> me_;
     me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
-             a.head_dim, h);
+             a.head_dim, a.scale, h);
     me_.clear();
     if (a.head_dim != DP) {  // the padding of the heads is never moved to
         for (int i = threadIdx.x; i < 2 * 2 * TILE / 16; i += 256) reinterpret_cast<Vec<float, 4>*>(lds[0])[i] = Vec<float, 4>{};
@@ -347,37 +409,47 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
     if (threadIdx.x == 0) flag = 0;
     __syncthreads();
     const Mover<S, BN, 256> mover(a, sq, kvh, threadIdx.x);
-    const float scale = a.scale * LOG2E;
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
     const uint32_t mine = min(me.keys, ke);
-    // The tiles that some row does not see whole come first, on a state of zeros: if a result is then not
-    // finite, they are taken again with care, so that a row is never touched by a value it does not see.
+    // The tiles that some row does not see whole come first, on a state of zeros, so that they can be taken again.
     const uint32_t seen = keys_of(a, sq, static_cast<uint32_t>(row0 / p.group));  // by every row of the tile
     const uint32_t full = max(kb, min(ke, seen) / BN * BN);                      // kb and pieces are multiples of BN
     const uint32_t parts = (ke - full + BN - 1) / BN, tiles = parts + (full - kb) / BN;
     auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
-    if (tiles) mover.go(start(0), lds[0], lds[0] + TILE);
-    for (uint32_t t = 0; t < tiles; ++t) {
-        char* tk = lds[t & 1];
-        meet();  // tile t is in LDS, and nobody reads tile t - 1 any more
+    auto arrive = [&](uint32_t t) {  // tile t is in LDS, and nobody reads tile t - 1 any more: t + 1 may come
+        meet();
         if (t + 1 < tiles) mover.go(start(t + 1), lds[~t & 1], lds[~t & 1] + TILE);
-        if (t >= parts) {
-            me_.template step<2, false, false>(tk, tk + TILE, start(t), mine, scale, lane);
-            continue;
+        return lds[t & 1];
+    };
+    if (tiles) mover.go(start(0), lds[0], lds[0] + TILE);
+    Found<DP / 32> found;
+    for (int pass = PLAIN; parts; ++pass) {
+        for (uint32_t t = 0; t < parts; ++t) {
+            char* tk = arrive(t);
+            if (pass != PLAIN) {
+                sift<T>(tk + TILE, TILE, pass, threadIdx.x, 256);
+                __syncthreads();
+            }
+            me_.template step<2, true>(tk, tk + TILE, start(t), mine, scale, lane);
         }
-        me_.template step<2, true, false>(tk, tk + TILE, start(t), mine, scale, lane);
-        if (t + 1 == parts) {
+        if (pass == PLAIN) {
             if (me_.odd()) flag = 1;
             meet();
-            if (flag) {
-                me_.clear();
-                for (uint32_t u = 0; u < parts; ++u) {
-                    meet();
-                    mover.go(start(u), tk, tk + TILE);
-                    meet();
-                    me_.template step<2, true, true>(tk, tk + TILE, start(u), mine, scale, lane);
-                }
-            }
+            if (!flag) break;
+            found.clear();
+        } else if (pass == FINITE) {
+            found.give(me_.o);
+            break;
+        } else {
+            found.take(me_.o, pass);
+            meet();
         }
+        me_.clear();
+        mover.go(start(0), lds[0], lds[0] + TILE);  // tile `parts` has landed, and is moved again
+    }
+    for (uint32_t t = parts; t < tiles; ++t) {
+        const char* tk = arrive(t);
+        me_.template step<2, false>(tk, tk + TILE, start(t), mine, scale, lane);
     }
     me_.join_halves();
     if (!me.live) return;
@@ -437,14 +509,14 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     if (kb >= ke && blockIdx.y > 0) return;  // the join does not read it
     Rows<T, DP> me_;
     me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
-             a.head_dim, h);
+             a.head_dim, a.scale, h);
     me_.clear();
     char* mem = lds + wave * 32768;
     if (a.head_dim != DP) {  // the padding of the heads is never moved to
         for (int i = lane; i < 32768 / 16; i += 64) reinterpret_cast<Vec<float, 4>*>(mem)[i] = Vec<float, 4>{};
     }
     const Mover<S, KN, 64> mover(a, sq, kvh, lane);
-    const float scale = a.scale * LOG2E;
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
     const uint32_t mine = min(me.keys, ke), seen = keys_of(a, sq, static_cast<uint32_t>(row0 / p.group));
     // tiles from the last to the first: of those that some row does not see whole (at most 2 in a row: a
     // tile of rows has at most 32 tokens) a wave has at most one, its first
@@ -464,14 +536,28 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
         else
             landed<0>();
         const uint32_t j0 = start(u);
-        const char* tk = buffer(u);
+        char* tk = buffer(u);
         if (j0 + KN <= min(seen, ke)) {
-            me_.template step<1, false, false>(tk, tk + TILE, j0, mine, scale, lane);
+            me_.template step<1, false>(tk, tk + TILE, j0, mine, scale, lane);
         } else {
-            me_.template step<1, true, false>(tk, tk + TILE, j0, mine, scale, lane);
-            if (__any(me_.odd())) {  // as above
+            Found<DP / 32> found;
+            for (int pass = PLAIN;; ++pass) {
+                me_.template step<1, true>(tk, tk + TILE, j0, mine, scale, lane);
+                if (pass == PLAIN) {
+                    if (!__any(me_.odd())) break;
+                    found.clear();
+                } else if (pass == FINITE) {
+                    found.give(me_.o);
+                    break;
+                } else {
+                    found.take(me_.o, pass);
+                }
                 me_.clear();
-                me_.template step<1, true, true>(tk, tk + TILE, j0, mine, scale, lane);
+                landed<63>();
+                mover.go(j0, tk, tk + TILE);
+                landed<0>();
+                sift<T>(tk + TILE, TILE, pass + 1, lane, 64);
+                landed<0>();
             }
         }
         if (u + NB < n) {
@@ -627,7 +713,7 @@ int check(const char* what, const bs_attention_args* a) {
         return refuse(w + ": heads must be in 1..1024 and a multiple of kv_heads");
     if (a->q_tokens > 0x7FFFFFFFu || a->k_tokens > 0x7FFFFFFFu) return refuse(w + ": q_tokens and k_tokens must be < 2^31");
     if (a->sequences == 0 || a->sequences > 0x7FFFFFFu) return refuse(w + ": sequences must be in 1..2^27");
-    if (!(std::fabs(a->scale) < INFINITY)) return refuse(w + ": scale must be finite");
+    if (!(std::fabs(a->scale) <= 1e30f)) return refuse(w + ": scale must be finite, at most 1e30");
     if (tiles_of(*a, 32) * a->kv_heads > 0x7FFFFFFFull || static_cast<uint64_t>(a->q_tokens) * a->heads > 0x7FFFFFFFull) return refuse(w + ": too many tiles for one launch");
     return BS_OK;
 }

@@ -104,7 +104,7 @@ typedef struct {
     uint32_t longest_q, longest_k;
     int32_t type;
     int32_t causal;
-    float scale; /* finite */
+    float scale; /* finite, at most 1e30 */
 } bs_attention_args;
 
 /* workspace: bs_attention_workspace bytes for the same args (pointers are not looked at), 16-byte

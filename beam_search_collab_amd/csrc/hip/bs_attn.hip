@@ -173,54 +173,57 @@ struct Rows {
             for (int r = 0; r < 16; ++r) is |= !(fabsf(o[d][r]) < INFINITY);
         return is;
     }
-    // KB x 32 keys from j0 on, in LDS.  Masked: only those below `mine` count.
-    template <int KB, bool Masked>
-    __device__ void step(const char* tk, const char* tv, uint32_t j0, uint32_t mine, float scale, int lane) {
-        const int l = lane & 31, h = lane >> 5;
-        // Operands are read a part ahead of their products: parts of 32 elements of the keys, then of 32
-        // elements of the values, the first of which comes in under the exponentials.
-        Vec<T, 8> k[2][2][KB];
-        auto read_keys = [&](int i) {
+    // What a step over KB x 32 keys holds besides.  Operands are read a part ahead of their products: parts of 32
+    // elements of the keys, then of 32 elements of the values, the first of which comes in under the exponentials.
+    template <int KB>
+    struct Work {
+        f32x16 z[KB];  // scores; register r of block b: key b * 32 + r % 4 + 8 (r / 4) + 4 h
+        Vec<T, 8> w[2 * KB], k[2][2][KB], v[2][2 * KB];
+    };
+    template <int KB>
+    __device__ static void read_keys(Work<KB>& x, const char* tk, int i, int lane) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
-                    k[i & 1][s][b] = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + l, i * 4 + s * 2 + h));
-        };
-        f32x16 z[KB];
-        read_keys(0);
+            for (int b = 0; b < KB; ++b)
+                x.k[i & 1][s][b] = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + (lane & 31), i * 4 + s * 2 + (lane >> 5)));
+    }
+    template <int KB>
+    __device__ static void read_values(Work<KB>& x, const char* tv, int d, int lane) {
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            if (i + 1 < DP / 32) read_keys(i + 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int b = 0; b < KB; ++b) z[b] = Mma<T>::go(k[i & 1][s][b], q[i * 2 + s], i + s ? z[b] : f32x16{});
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        auto value = [&](int d, int s) {  // 16 keys of 32 elements
+        for (int s = 0; s < 2 * KB; ++s) {
             // lanes 16g .. 16g + 15 read 4 keys x 16 elements and get an element's 4 keys each
-            const int key = s * 16 + h * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            const int key = s * 16 + (lane >> 5) * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
             const s16x4 lo = read_transposed(tv + place<S>(key, e >> 3) + (e & 7) * 2);
             const s16x4 hi = read_transposed(tv + place<S>(key + 8, e >> 3) + (e & 7) * 2);
-            return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-        };
-        Vec<T, 8> v[2][2 * KB];
-        auto read_values = [&](int d) {
+            x.v[d & 1][s] = __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+        }
+    }
+    // scores of the keys, whose first part has been read
+    template <int KB>
+    __device__ void scores(Work<KB>& x, const char* tk, int lane) const {
 #pragma unroll
-            for (int s = 0; s < 2 * KB; ++s) v[d & 1][s] = value(d, s);
-        };
-        read_values(0);
-        __builtin_amdgcn_sched_barrier(0);
-        // result register r of block b: key b * 32 + r % 4 + 8 (r / 4) + 4 h
+        for (int i = 0; i < DP / 32; ++i) {
+            if (i + 1 < DP / 32) read_keys(x, tk, i + 1, lane);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int b = 0; b < KB; ++b) x.z[b] = Mma<T>::go(x.k[i & 1][s][b], q[i * 2 + s], i + s ? x.z[b] : f32x16{});
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // weights of the scores.  Masked: only keys below `mine` count.
+    template <bool Masked, int KB>
+    __device__ void weights(Work<KB>& x, uint32_t j0, uint32_t mine, float scale, int lane) {
+        const int h = lane >> 5;
         float most = NONE;
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (Masked && j0 + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * h >= mine) z[b][r] = NONE;
-                most = fmaxf(most, z[b][r]);
+                if (Masked && j0 + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * h >= mine) x.z[b][r] = NONE;
+                most = fmaxf(most, x.z[b][r]);
             }
         const float2 two = halves(most);
         most = fmaxf(two.x, two.y) * scale;  // scale > 0
@@ -237,24 +240,41 @@ struct Rows {
         }
         const float base = top == NONE ? 0.0f : top;  // nothing visible yet: every weight is exp2(-inf) = 0
         float add = 0.0f;
-        Vec<T, 8> w[2 * KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(z[b][r], scale, -base));
+                const float e = __builtin_amdgcn_exp2f(fmaf(x.z[b][r], scale, -base));
                 add += e;
-                w[b * 2 + (r >> 3)][r & 7] = static_cast<T>(e);
+                x.w[b * 2 + (r >> 3)][r & 7] = static_cast<T>(e);
             }
         sum += add;
+    }
+    // the weighted values, whose first part has been read; `last` runs before the last part's products
+    template <int KB, typename F>
+    __device__ void results(Work<KB>& x, const char* tv, int lane, F last) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
             __builtin_amdgcn_sched_barrier(0);
-            if (d + 1 < DP / 32) read_values(d + 1);
+            if (d + 1 < DP / 32)
+                read_values(x, tv, d + 1, lane);
+            else
+                last();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(v[d & 1][s], w[s], o[d]);
+            for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(x.v[d & 1][s], x.w[s], o[d]);
         }
+    }
+    // all of it for the keys from j0 on, in LDS
+    template <int KB, bool Masked>
+    __device__ void step(const char* tk, const char* tv, uint32_t j0, uint32_t mine, float scale, int lane) {
+        Work<KB> x;
+        read_keys(x, tk, 0, lane);
+        scores(x, tk, lane);
+        read_values(x, tv, 0, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        weights<Masked>(x, j0, mine, scale, lane);
+        results(x, tv, lane, [] {});
     }
     __device__ void join_halves() {
         const float2 two = halves(sum);
@@ -333,27 +353,22 @@ struct Mover {
         kat = row * khop;
         vat = row * vhop;
     }
-    // keys j0 .. j0 + KEYS - 1; those past the sequence's end repeat its last one, and no row sees them
-    __device__ void go(uint32_t j0, char* tk, char* tv) const {
+    // rows j0 .. j0 + KEYS - 1; those past the sequence's end repeat its last one, and no row sees them
+    __device__ void go(const char* from, int64_t hop, int64_t at, uint32_t j0, char* to) const {
         const bool past = j0 + KEYS > nk;
 #pragma unroll
         for (int i = 0; i < MOVES; ++i) {
             const int r = i * N + row;
             const uint32_t c = (place<S>(r, slot) - r * S) >> 4;  // the chunk whose place this slot is
-            const char *kp, *vp;
-            if (past) {
-                const int64_t key = min(j0 + r, nk - 1);
-                kp = k + key * khop;
-                vp = v + key * vhop;
-            } else {
-                kp = k + static_cast<int64_t>(j0 + i * N) * khop + kat;
-                vp = v + static_cast<int64_t>(j0 + i * N) * vhop + vat;
-            }
-            if (c < chunks) {
-                __builtin_amdgcn_global_load_lds((global_ptr)(kp + c * 16), (lds_ptr)(tk + i * N * S + wave * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((global_ptr)(vp + c * 16), (lds_ptr)(tv + i * N * S + wave * 1024), 16, 0, 0);
-            }
+            const char* p = past ? from + static_cast<int64_t>(min(j0 + r, nk - 1)) * hop : from + static_cast<int64_t>(j0 + i * N) * hop + at;
+            if (c < chunks) __builtin_amdgcn_global_load_lds((global_ptr)(p + c * 16), (lds_ptr)(to + i * N * S + wave * 1024), 16, 0, 0);
         }
+    }
+    __device__ void keys(uint32_t j0, char* to) const { go(k, khop, kat, j0, to); }
+    __device__ void values(uint32_t j0, char* to) const { go(v, vhop, vat, j0, to); }
+    __device__ void both(uint32_t j0, char* to) const {  // the values after the keys
+        keys(j0, to);
+        values(j0, to + KEYS * S);
     }
 };
 
@@ -418,10 +433,10 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
     auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
     auto arrive = [&](uint32_t t) {  // tile t is in LDS, and nobody reads tile t - 1 any more: t + 1 may come
         meet();
-        if (t + 1 < tiles) mover.go(start(t + 1), lds[~t & 1], lds[~t & 1] + TILE);
+        if (t + 1 < tiles) mover.both(start(t + 1), lds[~t & 1]);
         return lds[t & 1];
     };
-    if (tiles) mover.go(start(0), lds[0], lds[0] + TILE);
+    if (tiles) mover.both(start(0), lds[0]);
     Found<DP / 32> found;
     for (int pass = PLAIN; parts; ++pass) {
         for (uint32_t t = 0; t < parts; ++t) {
@@ -445,7 +460,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
             meet();
         }
         me_.clear();
-        mover.go(start(0), lds[0], lds[0] + TILE);  // tile `parts` has landed, and is moved again
+        mover.both(start(0), lds[0]);  // tile `parts` has landed, and is moved again
     }
     for (uint32_t t = parts; t < tiles; ++t) {
         const char* tk = arrive(t);
@@ -528,7 +543,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     landed<0>();
 #pragma unroll
     for (int u = 0; u < NB; ++u)
-        if (static_cast<uint32_t>(u) < n) mover.go(start(u), buffer(u), buffer(u) + TILE);
+        if (static_cast<uint32_t>(u) < n) mover.both(start(u), buffer(u));
     for (uint32_t u = 0; u < n; ++u) {
         // the moves of tiles u + 1 .. u + NB - 1 may be on their way
         if (u + NB <= n)
@@ -554,7 +569,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
                 }
                 me_.clear();
                 landed<63>();
-                mover.go(j0, tk, tk + TILE);
+                mover.both(j0, tk);
                 landed<0>();
                 sift<T>(tk + TILE, TILE, pass + 1, lane, 64);
                 landed<0>();
@@ -562,7 +577,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
         }
         if (u + NB < n) {
             landed<63>();  // this tile's reads are done
-            mover.go(start(u + NB), buffer(u), buffer(u) + TILE);
+            mover.both(start(u + NB), buffer(u));
         }
     }
     me_.join_halves();

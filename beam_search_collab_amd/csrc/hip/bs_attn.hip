@@ -166,19 +166,21 @@ struct Rows {
         }
     }
     __device__ bool odd() const {  // some result is not finite
-        bool is = false;
+        uint32_t most = 0;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) is |= !(fabsf(o[d][r]) < INFINITY);
-        return is;
+            for (int r = 0; r < 16; ++r) most = max(most, __float_as_uint(o[d][r]) & 0x7FFFFFFFu);
+        return most >= 0x7F800000u;
     }
-    // What a step over KB x 32 keys holds besides.  Operands are read a part ahead of their products: parts of 32
-    // elements of the keys, then of 32 elements of the values, the first of which comes in under the exponentials.
+    // What a step over KB x 32 keys holds besides.  Operands are read AHEAD parts before their products: parts of
+    // 32 elements of the keys, then of 32 elements of the values, the first of which come in under the
+    // exponentials.  (Two ahead cost 16 registers more and spill at 128.)
+    static constexpr int PARTS = DP / 32, AHEAD = 1, HELD = 2;
     template <int KB>
     struct Work {
         f32x16 z[KB];  // scores; register r of block b: key b * 32 + r % 4 + 8 (r / 4) + 4 h
-        Vec<T, 8> w[2 * KB], k[2][2][KB], v[2][2 * KB];
+        Vec<T, 8> w[2 * KB], k[HELD][2][KB], v[HELD][2 * KB];
     };
     template <int KB>
     __device__ static void read_keys(Work<KB>& x, const char* tk, int i, int lane) {
@@ -186,7 +188,7 @@ struct Rows {
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int b = 0; b < KB; ++b)
-                x.k[i & 1][s][b] = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + (lane & 31), i * 4 + s * 2 + (lane >> 5)));
+                x.k[i % HELD][s][b] = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + (lane & 31), i * 4 + s * 2 + (lane >> 5)));
     }
     template <int KB>
     __device__ static void read_values(Work<KB>& x, const char* tv, int d, int lane) {
@@ -196,20 +198,31 @@ struct Rows {
             const int key = s * 16 + (lane >> 5) * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
             const s16x4 lo = read_transposed(tv + place<S>(key, e >> 3) + (e & 7) * 2);
             const s16x4 hi = read_transposed(tv + place<S>(key + 8, e >> 3) + (e & 7) * 2);
-            x.v[d & 1][s] = __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+            x.v[d % HELD][s] = __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
         }
     }
-    // scores of the keys, whose first part has been read
+    template <int KB>
+    __device__ static void first_keys(Work<KB>& x, const char* tk, int lane) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) read_keys(x, tk, i, lane);
+    }
+    template <int KB>
+    __device__ static void first_values(Work<KB>& x, const char* tv, int lane) {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) read_values(x, tv, d, lane);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // scores of the keys, whose first parts have been read
     template <int KB>
     __device__ void scores(Work<KB>& x, const char* tk, int lane) const {
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            if (i + 1 < DP / 32) read_keys(x, tk, i + 1, lane);
+        for (int i = 0; i < PARTS; ++i) {
+            if (i + AHEAD < PARTS) read_keys(x, tk, i + AHEAD, lane);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int b = 0; b < KB; ++b) x.z[b] = Mma<T>::go(x.k[i & 1][s][b], q[i * 2 + s], i + s ? x.z[b] : f32x16{});
+                for (int b = 0; b < KB; ++b) x.z[b] = Mma<T>::go(x.k[i % HELD][s][b], q[i * 2 + s], i + s ? x.z[b] : f32x16{});
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -217,16 +230,16 @@ struct Rows {
     template <bool Masked, int KB>
     __device__ void weights(Work<KB>& x, uint32_t j0, uint32_t mine, float scale, int lane) {
         const int h = lane >> 5;
-        float most = NONE;
+        float high[4] = {NONE, NONE, NONE, NONE};
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 if (Masked && j0 + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * h >= mine) x.z[b][r] = NONE;
-                most = fmaxf(most, x.z[b][r]);
+                high[r >> 2] = fmaxf(high[r >> 2], x.z[b][r]);
             }
-        const float2 two = halves(most);
-        most = fmaxf(two.x, two.y) * scale;  // scale > 0
+        const float2 two = halves(fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])));
+        const float most = fmaxf(two.x, two.y) * scale;  // scale > 0
         // The weights may stand against an older maximum while they stay below 2^8: sums and results lose
         // nothing by that, and the results are rescaled seldom.
         if (__any(most > top + 8.0f)) {
@@ -239,40 +252,37 @@ struct Rows {
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
         }
         const float base = top == NONE ? 0.0f : top;  // nothing visible yet: every weight is exp2(-inf) = 0
-        float add = 0.0f;
+        float add[4] = {};
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(x.z[b][r], scale, -base));
-                add += e;
+                add[r & 3] += e;
                 x.w[b * 2 + (r >> 3)][r & 7] = static_cast<T>(e);
             }
-        sum += add;
+        sum += (add[0] + add[1]) + (add[2] + add[3]);
     }
-    // the weighted values, whose first part has been read; `last` runs before the last part's products
+    // the weighted values, whose first parts have been read; `last` runs before the last part's products
     template <int KB, typename F>
     __device__ void results(Work<KB>& x, const char* tv, int lane, F last) {
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
+        for (int d = 0; d < PARTS; ++d) {
             __builtin_amdgcn_sched_barrier(0);
-            if (d + 1 < DP / 32)
-                read_values(x, tv, d + 1, lane);
-            else
-                last();
+            if (d + AHEAD < PARTS) read_values(x, tv, d + AHEAD, lane);
+            if (d == PARTS - 1) last();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(x.v[d & 1][s], x.w[s], o[d]);
+            for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(x.v[d % HELD][s], x.w[s], o[d]);
         }
     }
     // all of it for the keys from j0 on, in LDS
     template <int KB, bool Masked>
     __device__ void step(const char* tk, const char* tv, uint32_t j0, uint32_t mine, float scale, int lane) {
         Work<KB> x;
-        read_keys(x, tk, 0, lane);
+        first_keys(x, tk, lane);
         scores(x, tk, lane);
-        read_values(x, tv, 0, lane);
-        __builtin_amdgcn_sched_barrier(0);
+        first_values(x, tv, lane);
         weights<Masked>(x, j0, mine, scale, lane);
         results(x, tv, lane, [] {});
     }
@@ -387,6 +397,41 @@ __device__ inline Place place_of(const Params& p, const Sequence& sq, uint32_t k
     return x;
 }
 
+// a row's results: parts to the workspace, or the output
+template <typename T, int DP>
+__device__ inline void write_rows(const Params& p, const Sequence& sq, const Place& me, const Rows<T, DP>& r, int h) {
+    if (!me.live) return;
+    const bs_attention_args& a = p.a;
+    const int64_t at = static_cast<int64_t>(sq.q0 + me.tok) * a.heads + me.head;
+    if (p.splits > 1) {
+        const int64_t slot = static_cast<int64_t>(blockIdx.y) * a.q_tokens * a.heads + at;
+        if (h == 0) p.part_stat[slot] = make_float2(r.top, r.sum);
+        float* out = p.part_out + slot * a.head_dim;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t e = d * 32 + i * 8 + h * 4;
+                const f32x4 v = {r.o[d][i * 4], r.o[d][i * 4 + 1], r.o[d][i * 4 + 2], r.o[d][i * 4 + 3]};
+                if (e < a.head_dim) *reinterpret_cast<f32x4*>(out + e) = v;
+            }
+        return;
+    }
+    const float over = reciprocal_of(r.sum);
+    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(sq.q0 + me.tok) * a.out_stride + static_cast<int64_t>(me.head) * a.out_head_stride;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t e = d * 32 + i * 8 + h * 4;
+            Vec<T, 4> v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = static_cast<T>(r.o[d][i * 4 + j] * over);
+            if (e < a.head_dim) *reinterpret_cast<Vec<T, 4>*>(out + e) = v;
+        }
+    if (a.lse && h == 0) a.lse[at] = log_of(r.top, r.sum);
+}
+
 // Whole prompts.  Four waves of 32 rows share the tiles of 64 keys in LDS, two of them: the next tile's moves
 // run under a tile's products.  Two workgroups per compute unit: one's matrix instructions run under the
 // other's exponentials.
@@ -467,35 +512,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
         me_.template step<2, false>(tk, tk + TILE, start(t), mine, scale, lane);
     }
     me_.join_halves();
-    if (!me.live) return;
-    const int64_t at = static_cast<int64_t>(sq.q0 + me.tok) * a.heads + me.head;
-    if (p.splits > 1) {
-        const int64_t slot = static_cast<int64_t>(blockIdx.y) * a.q_tokens * a.heads + at;
-        if (h == 0) p.part_stat[slot] = make_float2(me_.top, me_.sum);
-        float* out = p.part_out + slot * a.head_dim;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t e = d * 32 + r * 8 + h * 4;
-                const f32x4 v = {me_.o[d][r * 4], me_.o[d][r * 4 + 1], me_.o[d][r * 4 + 2], me_.o[d][r * 4 + 3]};
-                if (e < a.head_dim) *reinterpret_cast<f32x4*>(out + e) = v;
-            }
-        return;
-    }
-    const float over = reciprocal_of(me_.sum);
-    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(sq.q0 + me.tok) * a.out_stride + static_cast<int64_t>(me.head) * a.out_head_stride;
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t e = d * 32 + r * 8 + h * 4;
-            Vec<T, 4> v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = static_cast<T>(me_.o[d][r * 4 + i] * over);
-            if (e < a.head_dim) *reinterpret_cast<Vec<T, 4>*>(out + e) = v;
-        }
-    if (a.lse && h == 0) a.lse[at] = log_of(me_.top, me_.sum);
+    write_rows<T, DP>(p, sq, me, me_, h);
 }
 
 // Few rows per sequence (single tokens): the keys' bytes bound the time.  A tile has at most 32 rows, and the

@@ -395,6 +395,45 @@ def test_attention_split_over_the_keys(gpu, nq, nk, heads, kv, dim, dtype):
         check_attention(q, k, v, nq, nk, True, dim ** -0.5, o, s)
 
 
+def attention_on_gpu(q, k, v, nq, nk, causal, scale):
+    """as attention_definition, a whole sequence and head at a time in 64 bits on the GPU"""
+    heads, kv = q.shape[1], k.shape[1]
+    o = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device="cuda")
+    size, total, spread = torch.zeros_like(o), torch.zeros_like(o), torch.zeros_like(lse)
+    a = b = 0
+    for m, n in zip(nq, nk):
+        for h in range(heads):
+            x, y, w = q[a:a + m, h].double(), k[b:b + n, h // (heads // kv)].double(), v[b:b + n, h // (heads // kv)].double()
+            hide = torch.ones(m, n, dtype=torch.bool, device="cuda").triu(n - m + 1) if causal else torch.zeros(m, n, dtype=torch.bool, device="cuda")
+            z = (x @ y.t().contiguous() * scale).masked_fill(hide, -math.inf)
+            t = torch.logsumexp(z, 1)
+            p = torch.exp(z - t[:, None])
+            o[a:a + m, h], lse[a:a + m, h] = p @ w, t
+            size[a:a + m, h], total[a:a + m, h] = p @ w.abs(), (~hide).double() @ w.abs()
+            spread[a:a + m, h] = (x.abs() @ y.abs().t().contiguous() * abs(scale)).masked_fill(hide, 0).amax(1)
+        a, b = a + m, b + n
+    return o, lse, size, total, spread
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv,dim", [([1500, 1100], [1500, 1100], 16, 8, 64), ([1290], [1290], 64, 16, 128), ([900, 40], [2000, 1300], 16, 16, 96),
+                                                ([1100], [1100], 64, 64, 32), ([640] * 40, [640] * 40, 2, 2, 72)])
+@pytest.mark.parametrize("dtype,causal", [(BF16, True), (F16, True), (BF16, False)])
+def test_attention_of_long_prompts(gpu, nq, nk, heads, kv, dim, dtype, causal):
+    q, k, v = rand(85, sum(nq), heads, dim, dtype=dtype), rand(86, sum(nk), kv, dim, dtype=dtype), rand(87, sum(nk), kv, dim, dtype=dtype)
+    out, lse = embed.attention(q, k, v, offsets(nq), offsets(nk), causal=causal, longest_q=max(nq), longest_k=max(nk), lse=True)
+    wo, wl, size, total, spread = attention_on_gpu(q, k, v, nq, nk, causal, dim ** -0.5)
+    d, count = (dim + 6) * E * spread + 4 * E * (spread + 1), max(nk)
+    near(out, wo, (U[dtype] + 4 * d + (count + 40) * E)[..., None] * size + 2.0 ** -24 * total * (dtype == F16) + U[dtype] * wo.abs() + TINY[dtype])
+    near(lse, wl, 2 * d + (count / 32 + 40) * E + 4 * E * wl.abs())
+    assert torch.equal(out, embed.attention(q, k, v, offsets(nq), offsets(nk), causal=causal, longest_q=max(nq), longest_k=max(nk)))
+    if causal:  # keys that a query does not see leave no trace, whatever they are
+        for t in (k, v):
+            t[-1] = math.nan
+        again = embed.attention(q, k, v, offsets(nq), offsets(nk), longest_q=max(nq), longest_k=max(nk))
+        assert torch.equal(again[:-1], out[:-1]) and torch.isnan(again[-1]).all()
+
+
 def test_attention_without_offsets_scales_and_repeats(gpu):
     q, k, v = rand(60, 90, 4, 64, dtype=BF16), rand(61, 90, 2, 64, dtype=BF16), rand(62, 90, 2, 64, dtype=BF16)
     a = embed.attention(q, k, v)

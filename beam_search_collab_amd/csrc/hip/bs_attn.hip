@@ -126,6 +126,14 @@ __device__ inline void meet() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// meets the workgroup's other waves with this wave's reads and writes of LDS done; moves stay on their way
+__device__ inline void settle() {
+    landed<63>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 __device__ inline uint32_t keys_of(const bs_attention_args& a, const Sequence& sq, uint32_t t) {  // visible keys of query t
     const int64_t e = a.causal ? min(static_cast<int64_t>(sq.nk), static_cast<int64_t>(sq.nk) - sq.nq + t + 1) : static_cast<int64_t>(sq.nk);
     return static_cast<uint32_t>(e < 0 ? 0 : e);
@@ -298,6 +306,11 @@ struct Rows {
 // finite.  The last pass gives the sums; NaN and infinities are added where their passes gave more than 0.
 enum { PLAIN = 0, NANS = 1, HIGH = 2, LOW = 3, FINITE = 4 };
 
+// the values past the end of a sequence, for which the moves repeat its last one: no weight of 0 meets NaN there
+template <int S>
+__device__ inline void blank(char* tv, uint32_t first, uint32_t rows, int thread, int threads) {
+    for (uint32_t i = first * (S / 16) + thread; i < rows * (S / 16); i += threads) reinterpret_cast<Vec<float, 4>*>(tv)[i] = Vec<float, 4>{};
+}
 // the values of a tile for a pass: 16 bytes at a time, by THREADS threads
 template <typename T>
 __device__ inline void sift(char* tv, int bytes, int pass, int thread, int threads) {
@@ -486,16 +499,20 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
     for (int pass = PLAIN; parts; ++pass) {
         for (uint32_t t = 0; t < parts; ++t) {
             char* tk = arrive(t);
-            if (pass != PLAIN) {
-                sift<T>(tk + TILE, TILE, pass, threadIdx.x, 256);
-                __syncthreads();
+            if (start(t) + BN > sq.nk || pass != PLAIN) {
+                if (start(t) + BN > sq.nk) blank<S>(tk + TILE, sq.nk - start(t), BN, threadIdx.x, 256);
+                settle();
+                if (pass != PLAIN) sift<T>(tk + TILE, TILE, pass, threadIdx.x, 256);
+                settle();
             }
             me_.template step<2, true>(tk, tk + TILE, start(t), mine, scale, lane);
         }
         if (pass == PLAIN) {
+            if (seen == all) break;  // all rows see the same keys
             if (me_.odd()) flag = 1;
-            meet();
+            settle();
             if (!flag) break;
+            meet();
             found.clear();
         } else if (pass == FINITE) {
             found.give(me_.o);
@@ -561,41 +578,53 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
 #pragma unroll
     for (int u = 0; u < NB; ++u)
         if (static_cast<uint32_t>(u) < n) mover.both(start(u), buffer(u));
-    for (uint32_t u = 0; u < n; ++u) {
-        // the moves of tiles u + 1 .. u + NB - 1 may be on their way
+    auto arrive = [&](uint32_t u) {  // the moves of tiles u + 1 .. u + NB - 1 may be on their way
         if (u + NB <= n)
             landed<(NB - 1) * MOVES>();
         else
             landed<0>();
-        const uint32_t j0 = start(u);
-        char* tk = buffer(u);
-        if (j0 + KN <= min(seen, ke)) {
-            me_.template step<1, false>(tk, tk + TILE, j0, mine, scale, lane);
-        } else {
-            Found<DP / 32> found;
-            for (int pass = PLAIN;; ++pass) {
-                me_.template step<1, true>(tk, tk + TILE, j0, mine, scale, lane);
-                if (pass == PLAIN) {
-                    if (!__any(me_.odd())) break;
-                    found.clear();
-                } else if (pass == FINITE) {
-                    found.give(me_.o);
-                    break;
-                } else {
-                    found.take(me_.o, pass);
-                }
-                me_.clear();
-                landed<63>();
-                mover.both(j0, tk);
-                landed<0>();
-                sift<T>(tk + TILE, TILE, pass + 1, lane, 64);
-                landed<0>();
-            }
-        }
+        return buffer(u);
+    };
+    auto follow = [&](uint32_t u) {
         if (u + NB < n) {
             landed<63>();  // this tile's reads are done
             mover.both(start(u + NB), buffer(u));
         }
+    };
+    uint32_t u = 0;
+    if (n && start(0) + KN > min(seen, ke)) {
+        char* tk = arrive(0);
+        const uint32_t j0 = start(0);
+        Found<DP / 32> found;
+        for (int pass = PLAIN;; ++pass) {
+            if (j0 + KN > sq.nk) blank<S>(tk + TILE, sq.nk - j0, KN, lane, 64);
+            landed<63>();
+            if (pass != PLAIN) {
+                sift<T>(tk + TILE, TILE, pass, lane, 64);
+                landed<63>();
+            }
+            me_.template step<1, true>(tk, tk + TILE, j0, mine, scale, lane);
+            if (pass == PLAIN) {
+                if (seen == all || !__any(me_.odd())) break;  // all rows see the same keys, or nothing is there to touch them
+                found.clear();
+            } else if (pass == FINITE) {
+                found.give(me_.o);
+                break;
+            } else {
+                found.take(me_.o, pass);
+            }
+            me_.clear();
+            landed<63>();
+            mover.both(j0, tk);
+            landed<0>();
+        }
+        follow(0);
+        u = 1;
+    }
+    for (; u < n; ++u) {
+        const char* tk = arrive(u);
+        me_.template step<1, false>(tk, tk + TILE, start(u), mine, scale, lane);
+        follow(u);
     }
     me_.join_halves();
     // joins the waves: every wave's results against the largest of their maxima, then a sum in wave order

@@ -181,14 +181,14 @@ struct Rows {
             for (int r = 0; r < 16; ++r) most = max(most, __float_as_uint(o[d][r]) & 0x7FFFFFFFu);
         return most >= 0x7F800000u;
     }
-    // What a step over KB x 32 keys holds besides.  Operands are read AHEAD parts before their products: parts of
-    // 32 elements of the keys, then of 32 elements of the values, the first of which come in under the
-    // exponentials.  (Two ahead cost 16 registers more and spill at 128.)
-    static constexpr int PARTS = DP / 32, AHEAD = 1, HELD = 2;
+    // What a step over KB x 32 keys holds besides.  Operands are read a part ahead of their products: parts of 32
+    // elements of the keys, then of 16 of the values, the first of which comes in under the exponentials.  (Two
+    // ahead cost 16 registers more and spill at 128.)
+    static constexpr int PARTS = DP / 32;
     template <int KB>
     struct Work {
         f32x16 z[KB];  // scores; register r of block b: key b * 32 + r % 4 + 8 (r / 4) + 4 h
-        Vec<T, 8> w[2 * KB], k[HELD][2][KB], v[HELD][2 * KB];
+        Vec<T, 8> w[2 * KB], k[2][2][KB], v[2][PARTS];
     };
     template <int KB>
     __device__ static void read_keys(Work<KB>& x, const char* tk, int i, int lane) {
@@ -196,41 +196,30 @@ struct Rows {
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int b = 0; b < KB; ++b)
-                x.k[i % HELD][s][b] = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + (lane & 31), i * 4 + s * 2 + (lane >> 5)));
+                x.k[i & 1][s][b] = *reinterpret_cast<const Vec<T, 8>*>(tk + place<S>(b * 32 + (lane & 31), i * 4 + s * 2 + (lane >> 5)));
     }
     template <int KB>
-    __device__ static void read_values(Work<KB>& x, const char* tv, int d, int lane) {
+    __device__ static void read_values(Work<KB>& x, const char* tv, int s, int lane) {
 #pragma unroll
-        for (int s = 0; s < 2 * KB; ++s) {
+        for (int d = 0; d < PARTS; ++d) {
             // lanes 16g .. 16g + 15 read 4 keys x 16 elements and get an element's 4 keys each
             const int key = s * 16 + (lane >> 5) * 4 + ((lane & 15) >> 2), e = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
             const s16x4 lo = read_transposed(tv + place<S>(key, e >> 3) + (e & 7) * 2);
             const s16x4 hi = read_transposed(tv + place<S>(key + 8, e >> 3) + (e & 7) * 2);
-            x.v[d % HELD][s] = __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+            x.v[s & 1][d] = __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
         }
     }
-    template <int KB>
-    __device__ static void first_keys(Work<KB>& x, const char* tk, int lane) {
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) read_keys(x, tk, i, lane);
-    }
-    template <int KB>
-    __device__ static void first_values(Work<KB>& x, const char* tv, int lane) {
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d) read_values(x, tv, d, lane);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    // scores of the keys, whose first parts have been read
+    // scores of the keys, whose first part has been read
     template <int KB>
     __device__ void scores(Work<KB>& x, const char* tk, int lane) const {
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
-            if (i + AHEAD < PARTS) read_keys(x, tk, i + AHEAD, lane);
+            if (i + 1 < PARTS) read_keys(x, tk, i + 1, lane);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int b = 0; b < KB; ++b) x.z[b] = Mma<T>::go(x.k[i % HELD][s][b], q[i * 2 + s], i + s ? x.z[b] : f32x16{});
+                for (int b = 0; b < KB; ++b) x.z[b] = Mma<T>::go(x.k[i & 1][s][b], q[i * 2 + s], i + s ? x.z[b] : f32x16{});
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -271,28 +260,29 @@ struct Rows {
             }
         sum += (add[0] + add[1]) + (add[2] + add[3]);
     }
-    // the weighted values, whose first parts have been read; `last` runs before the last part's products
-    template <int KB, typename F>
-    __device__ void results(Work<KB>& x, const char* tv, int lane, F last) {
+    // the weighted values, whose first part has been read: products that follow each other are of different
+    // elements, for one that waits for its predecessor's result takes twice as long
+    template <int KB>
+    __device__ void results(Work<KB>& x, const char* tv, int lane) {
 #pragma unroll
-        for (int d = 0; d < PARTS; ++d) {
+        for (int s = 0; s < 2 * KB; ++s) {
             __builtin_amdgcn_sched_barrier(0);
-            if (d + AHEAD < PARTS) read_values(x, tv, d + AHEAD, lane);
-            if (d == PARTS - 1) last();
+            if (s + 1 < 2 * KB) read_values(x, tv, s + 1, lane);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int s = 0; s < 2 * KB; ++s) o[d] = Mma<T>::go(x.v[d % HELD][s], x.w[s], o[d]);
+            for (int d = 0; d < PARTS; ++d) o[d] = Mma<T>::go(x.v[s & 1][d], x.w[s], o[d]);
         }
     }
     // all of it for the keys from j0 on, in LDS
     template <int KB, bool Masked>
     __device__ void step(const char* tk, const char* tv, uint32_t j0, uint32_t mine, float scale, int lane) {
         Work<KB> x;
-        first_keys(x, tk, lane);
+        read_keys(x, tk, 0, lane);
         scores(x, tk, lane);
-        first_values(x, tv, lane);
+        read_values(x, tv, 0, lane);
+        __builtin_amdgcn_sched_barrier(0);
         weights<Masked>(x, j0, mine, scale, lane);
-        results(x, tv, lane, [] {});
+        results(x, tv, lane);
     }
     __device__ void join_halves() {
         const float2 two = halves(sum);

@@ -59,7 +59,7 @@ __device__ inline Sequence sequence(const bs_attention_args& a, uint32_t s) {
         r.k0 = min(b, a.k_tokens);
         r.nk = min(e, a.k_tokens) - min(r.k0, min(e, a.k_tokens));
     }
-    return r;
+    return Sequence{uniform(r.q0), uniform(r.nq), uniform(r.k0), uniform(r.nk)};
 }
 
 // The tiles of all sequences are counted without a list of them: sequence s gets the tile numbers from
@@ -77,7 +77,7 @@ __device__ inline uint32_t find(const int32_t* off, uint32_t n, uint64_t tile, u
         lo += (k > 0 ? k - 1 : 0) * step;
         hi = min(lo + step, hi);
     }
-    return lo;
+    return uniform(lo);
 }
 
 // the last sequence that starts at or before the token
@@ -89,7 +89,7 @@ __device__ inline uint32_t holder(const int32_t* off, uint32_t n, uint32_t tok) 
         lo += (k > 0 ? k - 1 : 0) * step;
         hi = min(lo + step, hi);
     }
-    return lo;
+    return uniform(lo);
 }
 
 // chunk c of 16 bytes in row r of an LDS tile of S bytes per row (64, 128 or 256).  16 rows read at one
@@ -106,9 +106,6 @@ __device__ inline s16x4 read_transposed(const char* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
         reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p)));
 }
-
-typedef __attribute__((address_space(1))) const void* global_ptr;
-typedef __attribute__((address_space(3))) void* lds_ptr;
 
 // waits until all but the wave's N youngest moves to LDS are done, and its reads of LDS
 template <int N>
@@ -353,35 +350,46 @@ template <int S, int KEYS, int THREADS>
 struct Mover {
     static constexpr int CH = S / 16, N = THREADS / CH, MOVES = KEYS / N;  // rows of a move; moves of each kind
     const char *k, *v;
-    int64_t khop, vhop, kat, vat;  // bytes between rows; to this thread's row of a move
-    uint32_t nk;
-    int row, slot, wave;
-    uint32_t chunks;
+    int64_t khop, vhop;   // bytes between rows
+    uint32_t kat, vat;    // this thread's row of a move, if rows lie within 32 bits (near)
+    uint32_t nk, chunks, first;
+    int row, wave;
 
     __device__ Mover(const bs_attention_args& a, const Sequence& sq, uint32_t kvh, int thread)
-        : khop(a.k_stride * 2), vhop(a.v_stride * 2), nk(sq.nk), row(thread / CH), slot(thread % CH),
-          wave(__builtin_amdgcn_readfirstlane(thread >> 6)), chunks(a.head_dim / 8) {
+        : khop(a.k_stride * 2), vhop(a.v_stride * 2), nk(sq.nk), chunks(a.head_dim / 8), row(thread / CH),
+          wave(uniform(static_cast<uint32_t>(thread >> 6))) {
         k = static_cast<const char*>(a.k) + static_cast<int64_t>(sq.k0) * khop + static_cast<int64_t>(kvh) * a.k_head_stride * 2;
         v = static_cast<const char*>(a.v) + static_cast<int64_t>(sq.k0) * vhop + static_cast<int64_t>(kvh) * a.v_head_stride * 2;
-        kat = row * khop;
-        vat = row * vhop;
+        kat = row * static_cast<uint32_t>(khop);
+        vat = row * static_cast<uint32_t>(vhop);
+        first = (place<S>(row, thread % CH) - row * S) >> 4;
     }
-    // rows j0 .. j0 + KEYS - 1; those past the sequence's end repeat its last one, and no row sees them
-    __device__ void go(const char* from, int64_t hop, int64_t at, uint32_t j0, char* to) const {
-        const bool past = j0 + KEYS > nk;
+    // the chunk whose place this thread's slot is in move i
+    __device__ uint32_t chunk(int i) const { return first ^ static_cast<uint32_t>((place<S>(i * N, 0) - i * N * S) >> 4); }
+    // rows j0 .. j0 + KEYS - 1 of the sequence, near
+    __device__ void near(const char* from, int64_t hop, uint32_t at, uint32_t j0, char* to) const {
+        const char* p = from + static_cast<int64_t>(j0) * hop;
+#pragma unroll
+        for (int i = 0; i < MOVES; ++i)
+            if (chunk(i) < chunks) move16(p + i * (N * hop), at + chunk(i) * 16, to + i * N * S + wave * 1024);
+    }
+    // any rows; those past the sequence's end repeat its last one, and no row sees them
+    __device__ void any(const char* from, int64_t hop, uint32_t j0, char* to) const {
 #pragma unroll
         for (int i = 0; i < MOVES; ++i) {
-            const int r = i * N + row;
-            const uint32_t c = (place<S>(r, slot) - r * S) >> 4;  // the chunk whose place this slot is
-            const char* p = past ? from + static_cast<int64_t>(min(j0 + r, nk - 1)) * hop : from + static_cast<int64_t>(j0 + i * N) * hop + at;
-            if (c < chunks) __builtin_amdgcn_global_load_lds((global_ptr)(p + c * 16), (lds_ptr)(to + i * N * S + wave * 1024), 16, 0, 0);
+            const char* p = from + static_cast<int64_t>(min(j0 + i * N + row, nk - 1)) * hop;
+            if (chunk(i) < chunks)
+                __builtin_amdgcn_global_load_lds((global_ptr)(p + chunk(i) * 16), (lds_ptr)(to + i * N * S + wave * 1024), 16, 0, 0);
         }
     }
-    __device__ void keys(uint32_t j0, char* to) const { go(k, khop, kat, j0, to); }
-    __device__ void values(uint32_t j0, char* to) const { go(v, vhop, vat, j0, to); }
-    __device__ void both(uint32_t j0, char* to) const {  // the values after the keys
-        keys(j0, to);
-        values(j0, to + KEYS * S);
+    // the values lie after the keys
+    __device__ void near(uint32_t j0, char* to) const {
+        near(k, khop, kat, j0, to);
+        near(v, vhop, vat, j0, to + KEYS * S);
+    }
+    __device__ void any(uint32_t j0, char* to) const {
+        any(k, khop, j0, to);
+        any(v, vhop, j0, to + KEYS * S);
     }
 };
 
@@ -479,16 +487,13 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
     const uint32_t full = max(kb, min(ke, seen) / BN * BN);                      // kb and pieces are multiples of BN
     const uint32_t parts = (ke - full + BN - 1) / BN, tiles = parts + (full - kb) / BN;
     auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
-    auto arrive = [&](uint32_t t) {  // tile t is in LDS, and nobody reads tile t - 1 any more: t + 1 may come
-        meet();
-        if (t + 1 < tiles) mover.both(start(t + 1), lds[~t & 1]);
-        return lds[t & 1];
-    };
-    if (tiles) mover.both(start(0), lds[0]);
+    if (tiles) mover.any(start(0), lds[0]);
     Found<DP / 32> found;
     for (int pass = PLAIN; parts; ++pass) {
         for (uint32_t t = 0; t < parts; ++t) {
-            char* tk = arrive(t);
+            char* tk = lds[t & 1];
+            meet();  // tile t is in LDS, and nobody reads tile t - 1 any more
+            if (t + 1 < tiles) mover.any(start(t + 1), lds[~t & 1]);
             if (start(t) + BN > sq.nk || pass != PLAIN) {
                 if (start(t) + BN > sq.nk) blank<S>(tk + TILE, sq.nk - start(t), BN, threadIdx.x, 256);
                 settle();
@@ -501,7 +506,7 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
             if (seen == all) break;  // all rows see the same keys
             if (me_.odd()) flag = 1;
             settle();
-            if (!flag) break;
+            if (!uniform(static_cast<uint32_t>(flag))) break;
             meet();
             found.clear();
         } else if (pass == FINITE) {
@@ -512,11 +517,13 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
             meet();
         }
         me_.clear();
-        mover.both(start(0), lds[0]);  // tile `parts` has landed, and is moved again
+        mover.any(start(0), lds[0]);  // tile `parts` has landed, and is moved again
     }
     for (uint32_t t = parts; t < tiles; ++t) {
-        const char* tk = arrive(t);
-        me_.template step<2, false>(tk, tk + TILE, start(t), mine, scale, lane);
+        const char* tk = lds[t & 1];
+        meet();
+        if (t + 1 < tiles) mover.near(kb + (t + 1 - parts) * BN, lds[~t & 1]);
+        me_.template step<2, false>(tk, tk + TILE, 0, 0, scale, lane);
     }
     me_.join_halves();
     write_rows<T, DP>(p, sq, me, me_, h);
@@ -527,7 +534,8 @@ __global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
 // their results are joined at the end.
 constexpr int FEW_WAVES = 2;
 
-template <typename T, int DP>
+// Near: 16 rows of keys lie within 32 bits of each other, of values too
+template <typename T, int DP, bool Near>
 __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params p) {
     constexpr int ROWS = 32, KN = 32, S = ROW<DP>, TILE = KN * S, NB = 32768 / (2 * TILE);  // NB tiles of a wave in LDS
     constexpr int W = FEW_WAVES;
@@ -567,7 +575,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     landed<0>();
 #pragma unroll
     for (int u = 0; u < NB; ++u)
-        if (static_cast<uint32_t>(u) < n) mover.both(start(u), buffer(u));
+        if (static_cast<uint32_t>(u) < n) mover.any(start(u), buffer(u));
     auto arrive = [&](uint32_t u) {  // the moves of tiles u + 1 .. u + NB - 1 may be on their way
         if (u + NB <= n)
             landed<(NB - 1) * MOVES>();
@@ -578,7 +586,10 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     auto follow = [&](uint32_t u) {
         if (u + NB < n) {
             landed<63>();  // this tile's reads are done
-            mover.both(start(u + NB), buffer(u));
+            if (Near)  // whole: only a wave's first tile may pass the end
+                mover.near(start(u + NB), buffer(u));
+            else
+                mover.any(start(u + NB), buffer(u));
         }
     };
     uint32_t u = 0;
@@ -605,7 +616,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
             }
             me_.clear();
             landed<63>();
-            mover.both(j0, tk);
+            mover.any(j0, tk);
             landed<0>();
         }
         follow(0);
@@ -719,8 +730,13 @@ uint64_t tiles_of(const bs_attention_args& a, uint32_t rows) {
     return t / rows + a.sequences;
 }
 
+// whether rows of 16 tokens lie within 32 bits of each other
+bool near_of(const bs_attention_args& a) { return a.k_stride < (1 << 22) && a.v_stride < (1 << 22); }
+
 // Few rows: sequences of two tiles of 32 rows at most, by the longest one where it is given, else by their mean.
+// (Rows too far apart for the other kernel are taken like few ones.)
 bool few_of(const bs_attention_args& a) {
+    if (!near_of(a)) return true;
     const uint64_t group = a.heads / a.kv_heads;
     const uint64_t tokens = a.longest_q ? a.longest_q : (a.q_tokens + a.sequences - 1) / a.sequences;
     return tokens * group <= 64;
@@ -769,19 +785,22 @@ int check(const char* what, const bs_attention_args* a) {
     return BS_OK;
 }
 
+template <typename T, int DP, bool Near>
+void start_few(const Params& p, hipStream_t s) {
+    constexpr int LDS = FEW_WAVES * 32768;
+    auto* k = attention_few_kernel<T, DP, Near>;
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    (void)once;
+    k<<<dim3(static_cast<uint32_t>(tiles_of(p.a, 32) * p.a.kv_heads), p.splits), FEW_WAVES * 64, LDS, s>>>(p);
+}
 template <typename T, int DP>
 void start(const Params& p, hipStream_t s) {
-    const bool few = few_of(p.a);
-    const dim3 grid(static_cast<uint32_t>(tiles_of(p.a, few ? 32 : 128) * p.a.kv_heads), p.splits);
-    if (few) {
-        constexpr int LDS = FEW_WAVES * 32768;
-        auto* k = attention_few_kernel<T, DP>;
-        static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-        (void)once;
-        k<<<grid, FEW_WAVES * 64, LDS, s>>>(p);
-    } else {
-        attention_kernel<T, DP><<<grid, 256, 0, s>>>(p);
-    }
+    if (!near_of(p.a))
+        start_few<T, DP, false>(p, s);
+    else if (few_of(p.a))
+        start_few<T, DP, true>(p, s);
+    else
+        attention_kernel<T, DP><<<dim3(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits), 256, 0, s>>>(p);
 }
 
 template <typename T>

@@ -87,9 +87,6 @@ __device__ inline void finish(const Params& p, uint32_t row, uint32_t col, float
     }
 }
 
-typedef __attribute__((address_space(1))) const void* global_ptr;
-typedef __attribute__((address_space(3))) void* lds_ptr;
-
 // Meets the workgroup's other waves once all but this wave's N youngest moves to LDS are done.  Products
 // written before it stay before it, and with them the waits for the LDS reads that feed them; reads that
 // are still on their way at the meeting are of a step that nobody overwrites yet.
@@ -434,12 +431,10 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
     };
     const uint64_t xhop = static_cast<uint64_t>(p.xs) * 2, whop = static_cast<uint64_t>(p.ws) * 2;
     auto move_x = [&](const Source& f, int slot, int g, int i) {
-        __builtin_amdgcn_global_load_lds((global_ptr)(f.x + (i * 128 + g * 64) * xhop + vx),
-                                         (lds_ptr)(buf + slot * STEP + (i * 128 + g * 64 + rows8) * 64), 16, 0, 0);
+        move16(f.x + (i * 128 + g * 64) * xhop, vx, buf + slot * STEP + (i * 128 + g * 64 + rows8) * 64);
     };
     auto move_w = [&](const Source& f, int slot, int g, int i) {
-        __builtin_amdgcn_global_load_lds((global_ptr)(f.w + (i * 128 + g * 32) * whop + vw),
-                                         (lds_ptr)(buf + slot * STEP + (256 + i * 128 + g * 32 + rows8w) * 64), 16, 0, 0);
+        move16(f.w + (i * 128 + g * 32) * whop, vw, buf + slot * STEP + (256 + i * 128 + g * 32 + rows8w) * 64);
     };
     Vec<T, 8> fx[4][4], fw[2][4];
     // a lane's place in a row of LDS: rows of operands differ by multiples of 32, so the swizzle is the lane's

@@ -37,6 +37,18 @@ struct Params {
     float* parts;
 };
 
+constexpr float LOG2E = 1.4426950408889634f;
+
+// z (1 + erf(z / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun's handbook: with x = |z| / sqrt 2,
+// t = 1 / (1 + p x), erfc(x) = t (a1 + t (a2 + .. )) exp(-x^2), off by 1.5e-7 at most, so by 1.3 units of 2^-24
+// |z| here.  The library's erff took 30 of 102 us at 8191 x 1024 -> 4096.
+__device__ inline float gelu(float z) {
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+    const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float rest = 0.5f * q * __builtin_amdgcn_exp2f(-x * x * LOG2E);  // erfc(x) / 2
+    return z * (z < 0.0f ? rest : 1.0f - rest);
+}
+
 // one branch for all values: the branches are the call's, not the lanes'
 template <int N>
 __device__ inline void activate(float (&z)[N], int act) {
@@ -45,17 +57,17 @@ __device__ inline void activate(float (&z)[N], int act) {
         for (int j = 0; j < N; ++j) z[j] = z[j] < 0.0f ? 0.0f : z[j];
     } else if (act == BS_ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = 0.5f * z[j] * (1.0f + erff(z[j] * 0.70710678118654752f));
+        for (int j = 0; j < N; ++j) z[j] = gelu(z[j]);
     } else if (act == BS_ACT_GELU_TANH) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
             const float u = 0.79788456080286536f * fmaf(0.044715f * z[j] * z[j], z[j], z[j]);
-            z[j] = z[j] / (1.0f + __expf(-2.0f * u));
+            z[j] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.0f * LOG2E * u));
         }
     } else if (act == BS_ACT_SILU) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = z[j] / (1.0f + __expf(-z[j]));
+        for (int j = 0; j < N; ++j) z[j] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * z[j]));
     }
 }
 

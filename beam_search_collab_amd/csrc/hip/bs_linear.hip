@@ -71,9 +71,9 @@ __device__ inline void activate(float (&z)[N], int act) {
     }
 }
 
-// N adjacent columns of one row: those from `first` on, and inside
+// N adjacent columns of one row, those inside
 template <typename T, typename O, int N>
-__device__ inline void finish(const Params& p, uint32_t row, uint32_t col, float (&z)[N], int first = 0) {
+__device__ inline void finish(const Params& p, uint32_t row, uint32_t col, float (&z)[N]) {
     const int n = static_cast<int>(p.cols - col);
     if (p.bias) {
         const Vec<T, N> b = load_some<T, N>(static_cast<const T*>(p.bias) + col, n);
@@ -89,14 +89,7 @@ __device__ inline void finish(const Params& p, uint32_t row, uint32_t col, float
     Vec<O, N> o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = static_cast<O>(z[j]);
-    O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.os + col;
-    if (first <= 0 && n >= N) {
-        store_any<O, N>(out, o);
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j >= first && j < n) out[j] = o[j];
-    }
+    store_some<O, N>(static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.os + col, o, n);
 }
 
 // Meets the workgroup's other waves once all but this wave's N youngest moves to LDS are done.  Products
@@ -532,8 +525,20 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
             from.w += 128;
             slot ^= 1;
         }
-        // results: 16 rows at a time through the wave's 4 KB, then 8 adjacent columns a lane
+        // results: 16 rows at a time through the wave's 4 KB, then 8 adjacent columns a lane, the same for all rows:
+        // bias once, residuals 16 rows ahead
         const uint32_t ms = min(m0, p.rows - 256), ns = min(n0, p.cols - 256);
+        const uint32_t col = ns + wn + (lane & 7) * 8, top = ms + wm + (lane >> 3);
+        Vec<T, 8> bias = {};
+        if (p.bias) bias = load_any<T, 8>(static_cast<const T*>(p.bias) + col);
+        Vec<O, 8> res[2] = {};
+        auto residual = [&](int g, int k) {
+            return load_any<O, 8>(static_cast<const O*>(p.residual) + static_cast<int64_t>(top + g * 16 + k * 8) * p.rs + col);
+        };
+        if (p.residual) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) res[k] = residual(0, k);
+        }
         auto put = [&](auto J, int half) {
             constexpr int j = decltype(J)::value;
             if ((l >> 4) == half) {
@@ -554,6 +559,11 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
                 case 2: put(std::integral_constant<int, 2>(), half); break;
                 default: put(std::integral_constant<int, 3>(), half); break;
             }
+            Vec<O, 8> soon[2] = {};
+            if (p.residual && g < 7) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) soon[k] = residual(g + 1, k);
+            }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -562,10 +572,24 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
                 const f32x4 z1 = *reinterpret_cast<const f32x4*>(turn + rr * 64 + ((cc + 1) ^ rr) * 4);
                 float z[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[e] = z0[e], z[4 + e] = z1[e];
-                const uint32_t row = ms + wm + g * 16 + rr, col = ns + wn + cc * 4;
-                if (row >= m0 && col + 8 > n0) finish<T, O>(p, row, col, z, col < n0 ? static_cast<int>(n0 - col) : 0);
+                for (int e = 0; e < 8; ++e) z[e] = (e < 4 ? z0[e] : z1[e - 4]) + static_cast<float>(bias[e]);
+                activate(z, p.act);
+                Vec<O, 8> o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = static_cast<O>(z[e] + static_cast<float>(res[k][e]));
+                const uint32_t row = top + g * 16 + k * 8;
+                if (row < m0) continue;
+                O* out = static_cast<O*>(p.out) + static_cast<int64_t>(row) * p.os + col;
+                if (col >= n0) {
+                    store_any<O, 8>(out, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (col + e >= n0) out[e] = o[e];
+                }
             }
+            res[0] = soon[0];
+            res[1] = soon[1];
             __builtin_amdgcn_wave_barrier();
         }
         if (next >= end) break;

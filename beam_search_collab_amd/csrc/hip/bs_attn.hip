@@ -67,29 +67,31 @@ __device__ inline Sequence sequence(const bs_attention_args& a, uint32_t s) {
 __device__ inline uint64_t first_tile(const int32_t* off, uint32_t s, uint32_t group, uint32_t rows) {
     return static_cast<uint64_t>(max(off[s], 0)) * group / rows + s;
 }
-// the last sequence whose first tile is <= tile: 64 candidates a step, the same for all lanes
-__device__ inline uint32_t find(const int32_t* off, uint32_t n, uint64_t tile, uint32_t group, uint32_t rows) {
+// The last of n ascending values that `below` holds for (the first one if for none), the same for all lanes: 256
+// candidates a step, so one round of loads for up to 256 sequences.
+template <typename F>
+__device__ inline uint32_t last_below(uint32_t n, F below) {
     uint32_t lo = 0, hi = n;
     while (hi - lo > 1) {
-        const uint32_t step = (hi - lo + 63) / 64, at = lo + (threadIdx.x & 63) * step;
-        const bool below = at < hi && first_tile(off, at, group, rows) <= tile;
-        const int k = __popcll(__ballot(below));
+        const uint32_t step = (hi - lo + 255) / 256, at = lo + (threadIdx.x & 63) * step;
+        int k = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x = at + i * 64 * step;
+            k += __popcll(__ballot(x < hi && below(x)));
+        }
         lo += (k > 0 ? k - 1 : 0) * step;
         hi = min(lo + step, hi);
     }
     return uniform(lo);
 }
-
+// the sequence that a tile number belongs to
+__device__ inline uint32_t find(const int32_t* off, uint32_t n, uint64_t tile, uint32_t group, uint32_t rows) {
+    return last_below(n, [&](uint32_t s) { return first_tile(off, s, group, rows) <= tile; });
+}
 // the last sequence that starts at or before the token
 __device__ inline uint32_t holder(const int32_t* off, uint32_t n, uint32_t tok) {
-    uint32_t lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const uint32_t step = (hi - lo + 63) / 64, at = lo + (threadIdx.x & 63) * step;
-        const int k = __popcll(__ballot(at < hi && static_cast<uint32_t>(max(off[at], 0)) <= tok));
-        lo += (k > 0 ? k - 1 : 0) * step;
-        hi = min(lo + step, hi);
-    }
-    return uniform(lo);
+    return last_below(n, [&](uint32_t s) { return static_cast<uint32_t>(max(off[s], 0)) <= tok; });
 }
 
 // chunk c of 16 bytes in row r of an LDS tile of S bytes per row (64, 128 or 256).  16 rows read at one
@@ -223,13 +225,13 @@ struct Rows {
     // weights of the scores.  Masked: only keys below `mine` count.
     template <bool Masked, int KB>
     __device__ void weights(Work<KB>& x, uint32_t j0, uint32_t mine, float scale, int lane) {
-        const int h = lane >> 5;
+        const uint32_t from = j0 + (lane >> 5) * 4;  // of this half's keys
         float high[4] = {NONE, NONE, NONE, NONE};
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (Masked && j0 + b * 32 + (r & 3) + 8 * (r >> 2) + 4 * h >= mine) x.z[b][r] = NONE;
+                if (Masked && from + (b * 32 + (r & 3) + 8 * (r >> 2)) >= mine) x.z[b][r] = NONE;
                 high[r >> 2] = fmaxf(high[r >> 2], x.z[b][r]);
             }
         const float2 two = halves(fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])));
@@ -444,10 +446,10 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 }
 
 // Whole prompts.  Four waves of 32 rows share the tiles of 64 keys in LDS, two of them: the next tile's moves
-// run under a tile's products.  Two workgroups per compute unit: one's matrix instructions run under the
-// other's exponentials.
+// run under a tile's products.  Two workgroups per compute unit (three for heads up to 64): one's matrix
+// instructions run under the other's exponentials.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attention_kernel(Params p) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params p) {
     constexpr int ROWS = 128, S = ROW<DP>, TILE = BN * S;
     __shared__ __attribute__((aligned(16))) char lds[2][2 * TILE];
     __shared__ int flag;

@@ -41,11 +41,11 @@ constexpr float LOG2E = 1.4426950408889634f;
 
 // z (1 + erf(z / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun's handbook: with x = |z| / sqrt 2,
 // t = 1 / (1 + p x), erfc(x) = t (a1 + t (a2 + .. )) exp(-x^2), off by 1.5e-7 at most, so by 1.3 units of 2^-24
-// |z| here.  The library's erff took 30 of 102 us at 8191 x 1024 -> 4096.
+// |z| here; the halves and roots are in the constants.  8191 x 1024 -> 4096: 92 us, 102 us with the library's erff.
 __device__ inline float gelu(float z) {
-    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
-    const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float rest = 0.5f * q * __builtin_amdgcn_exp2f(-x * x * LOG2E);  // erfc(x) / 2
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, fabsf(z), 1.0f));
+    const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
+    const float rest = q * __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E));  // erfc(x) / 2
     return z * (z < 0.0f ? rest : 1.0f - rest);
 }
 

@@ -736,9 +736,7 @@ uint64_t tiles_of(const bs_attention_args& a, uint32_t rows) {
 bool near_of(const bs_attention_args& a) { return a.k_stride < (1 << 22) && a.v_stride < (1 << 22); }
 
 // Few rows: sequences of two tiles of 32 rows at most, by the longest one where it is given, else by their mean.
-// (Rows too far apart for the other kernel are taken like few ones.)
 bool few_of(const bs_attention_args& a) {
-    if (!near_of(a)) return true;
     const uint64_t group = a.heads / a.kv_heads;
     const uint64_t tokens = a.longest_q ? a.longest_q : (a.q_tokens + a.sequences - 1) / a.sequences;
     return tokens * group <= 64;
@@ -755,7 +753,7 @@ void split(const bs_attention_args& a, uint32_t& splits, uint32_t& piece) {
         want = std::max<uint64_t>(keys / (6 * CUS), 256);
     } else {
         const uint64_t groups = tiles_of(a, 128) * a.kv_heads;
-        want = groups >= 2 * CUS ? longest : std::max<uint64_t>(longest * groups / (4 * CUS), 256);
+        want = groups >= 2 * CUS ? longest : std::max<uint64_t>(longest * groups / (2 * CUS), 256);
     }
     piece = static_cast<uint32_t>(std::min<uint64_t>((want + 127) / 128 * 128, (static_cast<uint64_t>(longest) + 127) / 128 * 128));
     if (piece == 0) piece = 128;
@@ -788,37 +786,29 @@ int check(const char* what, const bs_attention_args* a) {
 }
 
 template <typename T, int DP, bool Near>
-void start_few(const Params& p, hipStream_t s) {
+int start_few(const Params& p, hipStream_t s) {
     constexpr int LDS = FEW_WAVES * 32768;
     auto* k = attention_few_kernel<T, DP, Near>;
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    (void)once;
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), LDS, done)) return rc;
     k<<<dim3(static_cast<uint32_t>(tiles_of(p.a, 32) * p.a.kv_heads), p.splits), FEW_WAVES * 64, LDS, s>>>(p);
+    return BS_OK;
 }
 template <typename T, int DP>
-void start(const Params& p, hipStream_t s) {
-    if (!near_of(p.a))
-        start_few<T, DP, false>(p, s);
-    else if (few_of(p.a))
-        start_few<T, DP, true>(p, s);
-    else
-        attention_kernel<T, DP><<<dim3(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits), 256, 0, s>>>(p);
+int start(const Params& p, hipStream_t s) {
+    if (!near_of(p.a)) return start_few<T, DP, false>(p, s);  // rows too far apart for the other kernel's moves
+    if (few_of(p.a)) return start_few<T, DP, true>(p, s);
+    attention_kernel<T, DP><<<dim3(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits), 256, 0, s>>>(p);
+    return BS_OK;
 }
 
 template <typename T>
-void launch(const Params& p, hipStream_t s) {
-    if (p.a.head_dim <= 32)
-        start<T, 32>(p, s);
-    else if (p.a.head_dim <= 64)
-        start<T, 64>(p, s);
-    else if (p.a.head_dim <= 96)
-        start<T, 96>(p, s);
-    else
-        start<T, 128>(p, s);
-    if (p.splits > 1) {
-        const uint64_t rows = static_cast<uint64_t>(p.a.q_tokens) * p.a.heads;
-        join_kernel<T><<<static_cast<uint32_t>(rows), 256, 0, s>>>(p);
-    }
+int launch(const Params& p, hipStream_t s) {
+    const uint32_t d = p.a.head_dim;
+    const int rc = d <= 32 ? start<T, 32>(p, s) : d <= 64 ? start<T, 64>(p, s) : d <= 96 ? start<T, 96>(p, s) : start<T, 128>(p, s);
+    if (rc) return rc;
+    if (p.splits > 1) join_kernel<T><<<p.a.q_tokens * p.a.heads, 256, 0, s>>>(p);
+    return launched("bs_attention");
 }
 
 }  // namespace
@@ -855,8 +845,7 @@ extern "C" int bs_attention(const bs_attention_args* args, void* workspace, uint
         p.part_out = static_cast<float*>(workspace);
         p.part_stat = reinterpret_cast<float2*>(p.part_out + static_cast<uint64_t>(p.splits) * a.q_tokens * a.heads * a.head_dim);
     }
-    a.type == BS_F16 ? launch<f16>(p, static_cast<hipStream_t>(stream)) : launch<bf16>(p, static_cast<hipStream_t>(stream));
-    return launched("bs_attention");
+    return a.type == BS_F16 ? launch<f16>(p, static_cast<hipStream_t>(stream)) : launch<bf16>(p, static_cast<hipStream_t>(stream));
 } catch (...) {
     return bs_internal_exception();
 }

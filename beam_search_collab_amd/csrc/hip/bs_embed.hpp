@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 void bs_internal_set_error(const std::string& msg);
@@ -27,6 +28,18 @@ inline int launched(const char* what) {
     const hipError_t e = hipGetLastError();
     if (e == hipSuccess) return BS_OK;
     bs_internal_set_error(std::string(what) + " launch failed: " + hipGetErrorString(e));
+    return BS_EHIP;
+}
+// Lets a kernel use more than 64 KB of dynamic LDS: once per device and kernel (`done`: a bit per device)
+inline int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1))) {
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == hipSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    if (e == hipSuccess) return BS_OK;
+    bs_internal_set_error(std::string("hipFuncSetAttribute failed: ") + hipGetErrorString(e));
     return BS_EHIP;
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

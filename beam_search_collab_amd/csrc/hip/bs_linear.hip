@@ -600,29 +600,6 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
     __builtin_amdgcn_s_waitcnt(0);  // moves into this workgroup's LDS end before it does
 }
 
-template <typename T, typename O, typename C, bool Direct>
-void start(const Params& p, hipStream_t s) {
-    const uint32_t tiles = (p.cols + C::BN - 1) / C::BN * ((p.rows + C::BM - 1) / C::BM);
-    auto* k = linear_kernel<T, O, C, Direct>;
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-    (void)once;
-    k<<<dim3(tiles, p.splits), C::THREADS, C::LDS, s>>>(p);
-    if (p.splits > 1) {
-        const uint64_t quads = static_cast<uint64_t>(p.rows) * ((p.cols + 3) / 4);
-        linear_join_kernel<T, O><<<static_cast<uint32_t>((quads + 255) / 256), 256, 0, s>>>(p);
-    }
-}
-
-template <typename T, typename O>
-void start_big(const Params& p, hipStream_t s) {
-    constexpr int LDS = 160 * 1024;
-    auto* k = linear_big_kernel<T, O>;
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    (void)once;
-    const uint32_t tiles = (p.cols + 255) / 256 * ((p.rows + 255) / 256);
-    k<<<tiles < CUS ? (tiles + 7) / 8 * 8 : CUS, 512, LDS, s>>>(p);
-}
-
 constexpr uint32_t FEW = 32;  // rows up to which the weight is streamed
 
 uint64_t tiles_of(uint64_t rows, uint32_t cols, uint32_t size) { return (rows + size - 1) / size * ((cols + size - 1) / size); }
@@ -638,29 +615,48 @@ uint32_t splits_of(uint64_t rows, uint32_t inner, uint32_t cols) {
     return (steps + piece - 1) / piece;
 }
 
+template <typename T, typename O, typename C, bool Direct>
+int start(const Params& p, hipStream_t s) {
+    auto* k = linear_kernel<T, O, C, Direct>;
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), C::LDS, done)) return rc;
+    const uint32_t tiles = (p.cols + C::BN - 1) / C::BN * ((p.rows + C::BM - 1) / C::BM);
+    k<<<dim3(tiles, p.splits), C::THREADS, C::LDS, s>>>(p);
+    if (p.splits > 1) {
+        const uint64_t quads = static_cast<uint64_t>(p.rows) * ((p.cols + 3) / 4);
+        linear_join_kernel<T, O><<<static_cast<uint32_t>((quads + 255) / 256), 256, 0, s>>>(p);
+    }
+    return BS_OK;
+}
+template <typename T, typename O>
+int start_big(const Params& p, hipStream_t s) {
+    constexpr int LDS = 160 * 1024;
+    auto* k = linear_big_kernel<T, O>;
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), LDS, done)) return rc;
+    const uint32_t tiles = (p.cols + 255) / 256 * ((p.rows + 255) / 256);
+    k<<<tiles < CUS ? (tiles + 7) / 8 * 8 : CUS, 512, LDS, s>>>(p);
+    return BS_OK;
+}
 template <typename T, typename O, int MT>
-void start_few(const Params& p, hipStream_t s) {
+int start_few(const Params& p, hipStream_t s) {
     // 32 columns a workgroup, half the reads of x, where that leaves a workgroup for every compute unit
     if (p.cols >= 32 * CUS)
         linear_few_kernel<T, O, MT, 2><<<(p.cols + 31) / 32, 512, 0, s>>>(p);
     else
         linear_few_kernel<T, O, MT, 1><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
+    return BS_OK;
 }
 
 template <typename T, typename O>
-void launch(const Params& p, hipStream_t s) {
-    if (p.rows <= FEW) {
-        p.rows <= 16 ? start_few<T, O, 1>(p, s) : start_few<T, O, 2>(p, s);
-        return;
-    }
+int launch(const Params& p, hipStream_t s) {
+    if (p.rows <= FEW) return p.rows <= 16 ? start_few<T, O, 1>(p, s) : start_few<T, O, 2>(p, s);
     const bool direct = aligned16(p.x) && aligned16(p.w) && p.xs % 8 == 0 && p.ws % 8 == 0;
     if (tiles_of(p.rows, p.cols, 256) >= CUS && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 &&
         p.xs < (1 << 22) && p.ws < (1 << 22))
-        start_big<T, O>(p, s);
-    else if (tiles_of(p.rows, p.cols, 128) >= CUS)
-        direct ? start<T, O, Mid, true>(p, s) : start<T, O, Mid, false>(p, s);
-    else
-        direct ? start<T, O, Small, true>(p, s) : start<T, O, Small, false>(p, s);
+        return start_big<T, O>(p, s);
+    if (tiles_of(p.rows, p.cols, 128) >= CUS) return direct ? start<T, O, Mid, true>(p, s) : start<T, O, Mid, false>(p, s);
+    return direct ? start<T, O, Small, true>(p, s) : start<T, O, Small, false>(p, s);
 }
 
 int check(const char* what, uint64_t rows, uint32_t inner, uint32_t cols) {
@@ -705,11 +701,9 @@ extern "C" int bs_linear(const void* x, int64_t x_stride, const void* w, int64_t
     const Params p{x, w, bias, residual, out, x_stride, w_stride, residual_stride, out_stride, static_cast<uint32_t>(rows), inner, cols, activation,
                    splits, static_cast<float*>(workspace)};
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (type == BS_F16)
-        out_type == BS_F32 ? launch<f16, float>(p, s) : launch<f16, f16>(p, s);
-    else
-        out_type == BS_F32 ? launch<bf16, float>(p, s) : launch<bf16, bf16>(p, s);
-    return launched("bs_linear");
+    const int rc = type == BS_F16 ? (out_type == BS_F32 ? launch<f16, float>(p, s) : launch<f16, f16>(p, s))
+                                  : (out_type == BS_F32 ? launch<bf16, float>(p, s) : launch<bf16, bf16>(p, s));
+    return rc ? rc : launched("bs_linear");
 } catch (...) {
     return bs_internal_exception();
 }

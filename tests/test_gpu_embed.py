@@ -513,6 +513,16 @@ def test_attention_past_32_bit_offsets(gpu):
     v.copy_(rand(79, 4, 1, 64))
     q = rand(80, 4, 2, 64, dtype=BF16)
     assert torch.equal(embed.attention(q, k, v), embed.attention(q, k.contiguous(), v.contiguous()))
+    # long ones, split over the keys, and with many queries
+    stride = (1 << 22) + 8
+    k = buf.as_strided((700, 1, 64), (stride, 64, 1))
+    v = buf.as_strided((700, 1, 64), (stride, 64, 1), 128)
+    k.copy_(rand(82, 700, 1, 64))
+    v.copy_(rand(83, 700, 1, 64))
+    for n in (1, 200):
+        q = rand(84, n, 2, 64, dtype=BF16)
+        got, lse = embed.attention(q, k, v, offsets([n]), offsets([700]), lse=True)
+        check_attention(q, k.contiguous(), v.contiguous(), [n], [700], True, 0.125, got, lse)
     x = buf.as_strided((4, 512), (1 << 30, 1))
     x.copy_(rand(81, 4, 512))
     assert torch.equal(embed.layer_norm(x), embed.layer_norm(x.contiguous()))

@@ -75,6 +75,11 @@ def _rows(what: str, name: str, t: torch.Tensor) -> Tuple[int, int, int]:
     return n, m, s
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """a contiguous tensor of x's shape and type (empty_like is the faster call, and keeps x's order)"""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _vector(what: str, name: str, t: torch.Tensor, n: int, *types):
     if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         _fail(f"{what}: {name} must be {n} contiguous elements")
@@ -118,7 +123,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
             wt = bias.dtype
         _vector(what, "bias", bias, m, *((type_, torch.float32) if weight is None else (wt,)))
     if out is None:
-        y, ys = x.new_empty(x.shape), m
+        y, ys = _like(x), m
     else:
         y = out
         if y.shape != x.shape or y.dtype != type_:
@@ -158,11 +163,11 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
         if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
             _fail(f"{what}: {name} must be {n} contiguous float32 values")
     wt = torch.float32 if weight is None else weight.dtype
-    dx = x.new_empty(x.shape)
+    dx = _like(x)
     dw = db = ws = None
     size = 0
     if params:
-        dw = x.new_empty((m,), dtype=wt)
+        dw = x.new_empty((m,), dtype=wt) if weight is None else torch.empty_like(weight)
         db = torch.empty_like(dw)
         size = _norm_workspace(n, m, code)
         ws = x.new_empty((size,), dtype=torch.uint8)

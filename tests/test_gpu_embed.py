@@ -591,3 +591,15 @@ def test_python_refusals(gpu):
     ]:
         with pytest.raises(ValueError, match=text):
             call()
+
+
+def test_example_embeds_searches_and_tunes(gpu):
+    """examples/embed_and_search.py: the vectors go through index and search; tuning raises the cosine"""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "embed_and_search.py")
+    spec = importlib.util.spec_from_file_location("embed_and_search", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    recall, own, before, after = m.main(["--passages", "1500", "--queries", "32", "--dim", "100"])
+    assert recall >= 0.9 and own > 0.5 and after > before

@@ -34,9 +34,21 @@ constexpr int BN = 64;  // keys of a tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 constexpr float NONE = -INFINITY;
 
+// n / d for n < 2^31 and one d: floor(n m / 2^(31 + s)) with s = ceil(log2 d), m = ceil(2^(31 + s) / d) < 2^32.  (m d -
+// 2^(31 + s) < d <= 2^s, so the quotient is off by less than n / 2^31 / d and never reaches the next integer.)
+struct Divisor {
+    uint32_t m, s;
+    Divisor(uint32_t d = 1) : m(0), s(0) {
+        while ((1ull << s) < d) ++s;
+        m = static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d);
+    }
+    __device__ uint32_t quotient(uint32_t n) const { return __umulhi(n << 1, m) >> s; }
+};
+
 struct Params {
     bs_attention_args a;
     uint32_t group;    // heads per key/value head
+    Divisor by_group, by_kv;
     uint32_t splits;   // pieces of the keys; > 1: parts go to the workspace
     uint32_t piece;    // keys of a piece, a multiple of BN
     float* part_out;   // splits x q_tokens x heads x head_dim: sums of p v, unscaled
@@ -400,12 +412,12 @@ struct Place {  // of a row: its query token in the sequence, its head, the keys
     bool live;
 };
 // row of a sequence's (token, head of the group) pairs; past the end the last one, not live
-__device__ inline Place place_of(const Params& p, const Sequence& sq, uint32_t kvh, uint64_t row, uint64_t rows) {
+__device__ inline Place place_of(const Params& p, const Sequence& sq, uint32_t kvh, uint32_t row, uint32_t rows) {
     Place x;
     x.live = row < rows;
-    const uint64_t r = x.live ? row : rows - 1;
-    x.tok = static_cast<uint32_t>(r / p.group);
-    x.head = kvh * p.group + static_cast<uint32_t>(r - static_cast<uint64_t>(x.tok) * p.group);
+    const uint32_t r = x.live ? row : rows - 1;
+    x.tok = p.by_group.quotient(r);
+    x.head = kvh * p.group + (r - x.tok * p.group);
     x.keys = keys_of(p.a, sq, x.tok);
     return x;
 }
@@ -455,41 +467,40 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     __shared__ int flag;
     const bs_attention_args& a = p.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+    const uint32_t tile = p.by_kv.quotient(blockIdx.x), kvh = blockIdx.x - tile * a.kv_heads;
     const uint32_t seq = a.q_offsets ? find(a.q_offsets, a.sequences, tile, p.group, ROWS) : 0;
     const uint64_t first = a.q_offsets ? first_tile(a.q_offsets, seq, p.group, ROWS) : 0;
     const Sequence sq = sequence(a, seq);
-    const uint64_t rows = static_cast<uint64_t>(sq.nq) * p.group;
+    const uint32_t rows = sq.nq * p.group;  // < 2^31, as q_tokens x heads
     if (tile < first || (tile - first) * ROWS >= rows) return;
     // the tiles that see most keys start first
-    const uint64_t row0 = ((rows - 1) / ROWS - (tile - first)) * ROWS;
-    const Place me = place_of(p, sq, kvh, row0 + wave * 32 + l, rows);
-    const uint64_t last_row = min(rows, row0 + ROWS) - 1;
-    const uint32_t all = keys_of(a, sq, static_cast<uint32_t>(last_row / p.group));  // of the tile's last row: the most
+    const uint32_t row0 = ((rows - 1) / ROWS - static_cast<uint32_t>(tile - first)) * ROWS;
+    const uint32_t all = keys_of(a, sq, p.by_group.quotient(min(rows, row0 + ROWS) - 1));  // of the tile's last row: the most
     uint32_t kb = 0, ke = all;
     if (p.splits > 1) {
         kb = min(all, blockIdx.y * p.piece);
         if (blockIdx.y + 1 < p.splits) ke = min(all, kb + p.piece);
         if (kb >= ke && blockIdx.y > 0) return;  // the join does not read it
     }
-    Rows<T, DP> me_;
-    me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
-             a.head_dim, a.scale, h);
-    me_.clear();
+    // The tiles that some row does not see whole come first, on a state of zeros, so that they can be taken again.
+    const uint32_t seen = keys_of(a, sq, p.by_group.quotient(row0));  // by every row of the tile
+    const uint32_t full = max(kb, min(ke, seen) / BN * BN);          // kb and pieces are multiples of BN
+    const uint32_t parts = (ke - full + BN - 1) / BN, tiles = parts + (full - kb) / BN;
+    auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
     if (a.head_dim != DP) {  // the padding of the heads is never moved to
         for (int i = threadIdx.x; i < 2 * 2 * TILE / 16; i += 256) reinterpret_cast<Vec<float, 4>*>(lds[0])[i] = Vec<float, 4>{};
     }
     if (threadIdx.x == 0) flag = 0;
-    __syncthreads();
+    settle();
     const Mover<S, BN, 256> mover(a, sq, kvh, threadIdx.x);
+    if (tiles) mover.any(start(0), lds[0]);
+    const Place me = place_of(p, sq, kvh, row0 + wave * 32 + l, rows);
+    Rows<T, DP> me_;
+    me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
+             a.head_dim, a.scale, h);
+    me_.clear();
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
     const uint32_t mine = min(me.keys, ke);
-    // The tiles that some row does not see whole come first, on a state of zeros, so that they can be taken again.
-    const uint32_t seen = keys_of(a, sq, static_cast<uint32_t>(row0 / p.group));  // by every row of the tile
-    const uint32_t full = max(kb, min(ke, seen) / BN * BN);                      // kb and pieces are multiples of BN
-    const uint32_t parts = (ke - full + BN - 1) / BN, tiles = parts + (full - kb) / BN;
-    auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
-    if (tiles) mover.any(start(0), lds[0]);
     Found<DP / 32> found;
     for (int pass = PLAIN; parts; ++pass) {
         for (uint32_t t = 0; t < parts; ++t) {
@@ -544,16 +555,16 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const bs_attention_args& a = p.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
-    const uint32_t kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads;
+    const uint32_t tile = p.by_kv.quotient(blockIdx.x), kvh = blockIdx.x - tile * a.kv_heads;
     const uint32_t seq = a.q_offsets ? find(a.q_offsets, a.sequences, tile, p.group, ROWS) : 0;
     const uint64_t first = a.q_offsets ? first_tile(a.q_offsets, seq, p.group, ROWS) : 0;
     const Sequence sq = sequence(a, seq);
-    const uint64_t rows = static_cast<uint64_t>(sq.nq) * p.group;
+    const uint32_t rows = sq.nq * p.group;  // < 2^31, as q_tokens x heads
     if (tile < first || (tile - first) * ROWS >= rows) return;
-    const uint64_t row0 = (tile - first) * ROWS;
+    const uint32_t row0 = static_cast<uint32_t>(tile - first) * ROWS;
     const Place me = place_of(p, sq, kvh, row0 + l, rows);
-    const uint32_t here = static_cast<uint32_t>(min(rows - row0, static_cast<uint64_t>(ROWS)));  // rows of the tile
-    const uint32_t all = keys_of(a, sq, static_cast<uint32_t>((row0 + here - 1) / p.group));
+    const uint32_t here = min(rows - row0, static_cast<uint32_t>(ROWS));  // rows of the tile
+    const uint32_t all = keys_of(a, sq, p.by_group.quotient(row0 + here - 1));
     const uint32_t kb = min(all, blockIdx.y * p.piece), ke = blockIdx.y + 1 < p.splits ? min(all, kb + p.piece) : all;
     if (kb >= ke && blockIdx.y > 0) return;  // the join does not read it
     Rows<T, DP> me_;
@@ -566,7 +577,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     }
     const Mover<S, KN, 64> mover(a, sq, kvh, lane);
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
-    const uint32_t mine = min(me.keys, ke), seen = keys_of(a, sq, static_cast<uint32_t>(row0 / p.group));
+    const uint32_t mine = min(me.keys, ke), seen = keys_of(a, sq, p.by_group.quotient(row0));
     // tiles from the last to the first: of those that some row does not see whole (at most 2 in a row: a
     // tile of rows has at most 32 tokens) a wave has at most one, its first
     const uint32_t tiles = (ke - kb + KN - 1) / KN, n = tiles > static_cast<uint32_t>(wave) ? (tiles - wave + W - 1) / W : 0;
@@ -686,7 +697,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     const bs_attention_args& a = p.a;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint64_t at = blockIdx.x, rows = static_cast<uint64_t>(a.q_tokens) * a.heads;
-    const uint32_t tok = static_cast<uint32_t>(at / a.heads), head = static_cast<uint32_t>(at % a.heads);
+    const uint32_t tok = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
     const uint32_t seq = a.q_offsets ? holder(a.q_offsets, a.sequences, tok) : 0;
     const Sequence sq = sequence(a, seq);
     if (tok < sq.q0 || tok - sq.q0 >= sq.nq) return;
@@ -837,6 +848,8 @@ extern "C" int bs_attention(const bs_attention_args* args, void* workspace, uint
     Params p{};
     p.a = a;
     p.group = a.heads / a.kv_heads;
+    p.by_group = Divisor(p.group);
+    p.by_kv = Divisor(a.kv_heads);
     split(a, p.splits, p.piece);
     if (p.splits > 1) {
         const uint64_t need = workspace_of(a);

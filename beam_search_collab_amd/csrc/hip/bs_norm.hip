@@ -1,7 +1,7 @@
 // Layer norm and its gradients (include/bs_embed.h).
 //
 // Both directions read each row once and keep it in registers: a row belongs to W wavefronts
-// (1, 4 or 16 for up to 1024, 4096, 16384 features), a lane to the same columns of every row, so
+// (1, 4 or 8 for up to 1024, 8192, 16384 features), a lane to the same 16 or 32 columns of every row, so
 // weights are loaded once per wavefront and the gradients of the weights grow in registers.
 #include "bs_embed.hpp"
 
@@ -15,7 +15,7 @@ template <typename T, int NV, int W>
 struct Cols {
     static constexpr int N = VN<T>;
     static constexpr int E = N * NV;                    // elements per lane
-    static constexpr int THREADS = W == 16 ? 1024 : 256;
+    static constexpr int THREADS = W == 1 ? 256 : 64 * W;
     static constexpr int ROWS = W == 1 ? 4 : 1;         // rows per workgroup at a time
     __device__ static int lane() { return W == 1 ? (threadIdx.x & 63) : threadIdx.x; }
     __device__ static int col(int i) { return (i * 64 * W + lane()) * N; }
@@ -221,8 +221,18 @@ __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, ui
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t c = blockIdx.x * 64 + lane, all = 2u * cols;
     float s = 0.0f;
-    if (c < all)
-        for (uint32_t i = wave; i < n; i += 16) s += parts[static_cast<size_t>(i) * all + c];
+    if (c < all) {
+        constexpr int U = 16;  // loads in flight; the sum stays in order
+        uint32_t i = wave;
+        for (; i + 16 * (U - 1) < n; i += 16 * U) {
+            float v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = parts[static_cast<size_t>(i + 16 * u) * all + c];
+#pragma unroll
+            for (int u = 0; u < U; ++u) s += v[u];
+        }
+        for (; i < n; i += 16) s += parts[static_cast<size_t>(i) * all + c];
+    }
     join[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && c < all) {
@@ -234,7 +244,7 @@ __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, ui
     }
 }
 
-int waves(uint32_t cols) { return cols <= 1024 ? 1 : cols <= 4096 ? 4 : 16; }
+int waves(uint32_t cols) { return cols <= 1024 ? 1 : cols <= 8192 ? 4 : 8; }
 
 // workgroups of a backward call
 uint32_t backward_groups(uint64_t rows, uint32_t cols) {
@@ -256,7 +266,7 @@ struct Forward {
     template <typename T, typename WT, int NV, int W>
     void go() const {
         using C = Cols<T, NV, W>;
-        const uint64_t want = (rows + C::ROWS - 1) / C::ROWS, most = CUS * (W == 16 ? 2 : 8);
+        const uint64_t want = (rows + C::ROWS - 1) / C::ROWS, most = CUS * (W == 8 ? 4 : 8);
         norm_kernel<T, WT, NV, W><<<static_cast<uint32_t>(want < most ? want : most), C::THREADS, 0, s>>>(
             static_cast<const T*>(x), xs, static_cast<const WT*>(weight), static_cast<const WT*>(bias), eps, static_cast<T*>(y), ys,
             mean, rstd, rows, cols);
@@ -282,15 +292,15 @@ struct Backward {
 
 template <typename T, typename WT, typename F>
 void by_cols(const F& f, uint32_t cols) {
-    constexpr int most = 16 / VN<T>;  // 16 elements per lane
+    constexpr int half = 8 / VN<T>, one = 16 / VN<T>, two = 32 / VN<T>;  // 8, 16, 32 elements per lane
     const int w = waves(cols);
-    const uint32_t nv = (cols + 64 * w * VN<T> - 1) / (64 * w * VN<T>);
-    if (w == 16)
-        f.template go<T, WT, most, 16>();
+    const uint32_t each = (cols + 64 * w - 1) / (64 * w);
+    if (w == 8)
+        f.template go<T, WT, two, 8>();
     else if (w == 4)
-        nv <= most / 2 ? f.template go<T, WT, most / 2, 4>() : f.template go<T, WT, most, 4>();
+        each <= 8 ? f.template go<T, WT, half, 4>() : each <= 16 ? f.template go<T, WT, one, 4>() : f.template go<T, WT, two, 4>();
     else
-        nv <= most / 2 ? f.template go<T, WT, most / 2, 1>() : f.template go<T, WT, most, 1>();
+        each <= 8 ? f.template go<T, WT, half, 1>() : f.template go<T, WT, one, 1>();
 }
 template <typename F>
 void by_type(const F& f, int type, int wtype, uint32_t cols) {

@@ -1,8 +1,13 @@
 // Layer norm and its gradients (include/bs_embed.h).
 //
-// Both directions read each row once and keep it in registers: a row belongs to W wavefronts
-// (1, 4 or 8 for up to 1024, 8192, 16384 features), a lane to the same 16 or 32 columns of every row, so
-// weights are loaded once per wavefront and the gradients of the weights grow in registers.
+//   y  = (x - mean) rstd w + b,  rstd = 1 / sqrt(var + eps),  xh = (x - mean) rstd
+//   dx = rstd (dy w - avg(dy w) - xh avg(dy w xh)),  dw = sum of dy xh and db = sum of dy over the rows
+//
+// Both directions read each row once and keep it in registers: a row belongs to W wavefronts, a lane to the
+// same 8, 16 or 32 columns of every row, so weights are loaded once per wavefront and the gradients of the
+// weights grow in registers.  Memory bounds both: 65536 x 1024 in bf16 takes 47 us forward (5.7 TB/s; a copy
+// reaches 5.1), 32768 x 4096 takes 147 us backward with 4-byte weights (5.5 TB/s).  Short calls are bounded by
+// the latency of their dependent steps: 24 x 768 takes 4.0 us, 1000 x 960 in f32 backward 7.0 + 6.2 us.
 #include "bs_embed.hpp"
 
 namespace {
@@ -214,7 +219,8 @@ __global__ __launch_bounds__((Cols<T, NV, W>::THREADS)) void norm_backward_kerne
     }
 }
 
-// sums of the workgroups' parts, in order: a workgroup takes 64 columns, wave i the parts i, i + 16, ..
+// Sums of the workgroups' parts, in order: a workgroup takes 64 columns, wave i the parts i, i + 16, ..  A wave's loads
+// wait for memory, so 16 are on their way at a time: 1024 parts of 2 x 4096 take 6.9 us, 18 with one at a time.
 template <typename WT>
 __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, uint32_t n, int cols, WT* dweight, WT* dbias) {
     __shared__ float join[16][64];
@@ -244,13 +250,13 @@ __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, ui
     }
 }
 
-int waves(uint32_t cols) { return cols <= 1024 ? 1 : cols <= 8192 ? 4 : 8; }
-
-// workgroups of a backward call
+// Workgroups of a backward call.  Each writes its sums once, so that fewer are better until loads run short of
+// waves: in us at 256 / 512 / 1024 workgroups, 65536 x 768: 107 / 65 / 59; 30000 x 2048: 171 / 95 / 74; 32768 x 4096:
+// 240 / 148 / 164; 16384 x 8192: 196 / 161 / 171; 8192 x 16384: 159 / 173 / 200.
 uint32_t backward_groups(uint64_t rows, uint32_t cols) {
     const uint32_t per = cols <= 1024 ? 4 : 1;
     const uint64_t want = (rows + per - 1) / per;
-    const uint64_t most = cols <= 4096 ? 1024 : 512;
+    const uint64_t most = CUS * (cols <= 2048 ? 4 : cols <= 8192 ? 2 : 1);
     return static_cast<uint32_t>(want < most ? want : most);
 }
 
@@ -263,9 +269,28 @@ struct Forward {
     uint64_t rows;
     int cols;
     hipStream_t s;
+    // Few waves meet seldom: 30000 x 2048 takes 43 us with two waves a row and 59 with four, 60000 x 1024 45 with one
+    // and 101 with four, 16000 x 8192 97 with four (32 columns a lane) and 109 with eight (16).
+    template <typename T, typename WT>
+    void pick() const {
+        if (cols <= 512)
+            go<T, WT, 8 / VN<T>, 1>();
+        else if (cols <= 1024)
+            go<T, WT, 16 / VN<T>, 1>();
+        else if (cols <= 2048)
+            go<T, WT, 16 / VN<T>, 2>();
+        else if (cols <= 4096)
+            go<T, WT, 32 / VN<T>, 2>();
+        else if (cols <= 8192)
+            go<T, WT, 32 / VN<T>, 4>();
+        else
+            go<T, WT, 32 / VN<T>, 8>();
+    }
     template <typename T, typename WT, int NV, int W>
     void go() const {
         using C = Cols<T, NV, W>;
+        // weights are loaded once per workgroup, so they stay for many rows; 2 / 4 / 8 / 16 per compute unit:
+        // 65536 x 768: 57 / 39 / 40 / 42 us, 32768 x 4096: 144 / 103 / 104 / 104, 8192 x 16384: 129 / 131 / 139 / 147
         const uint64_t want = (rows + C::ROWS - 1) / C::ROWS, most = CUS * (W == 8 ? 4 : 8);
         norm_kernel<T, WT, NV, W><<<static_cast<uint32_t>(want < most ? want : most), C::THREADS, 0, s>>>(
             static_cast<const T*>(x), xs, static_cast<const WT*>(weight), static_cast<const WT*>(bias), eps, static_cast<T*>(y), ys,
@@ -282,6 +307,25 @@ struct Backward {
     uint64_t rows;
     int cols;
     hipStream_t s;
+    // A lane holds five values per column here, so a row has more waves than forward: 60000 x 1024 takes 78 us with one
+    // wave a row and 98 with four, 30000 x 2048 74 with four and 75 with two, 16000 x 3000 61 and 65, 16000 x 8192 156
+    // with four and 154 with eight.  8 columns a lane where they are enough: 60000 x 512 37 us, with 16 39; 60000 x 2048
+    // 139 and 143.
+    template <typename T, typename WT>
+    void pick() const {
+        if (cols <= 512)
+            go<T, WT, 8 / VN<T>, 1>();
+        else if (cols <= 1024)
+            go<T, WT, 16 / VN<T>, 1>();
+        else if (cols <= 2048)
+            go<T, WT, 8 / VN<T>, 4>();
+        else if (cols <= 4096)
+            go<T, WT, 16 / VN<T>, 4>();
+        else if (cols <= 8192)
+            go<T, WT, 32 / VN<T>, 4>();
+        else
+            go<T, WT, 32 / VN<T>, 8>();
+    }
     template <typename T, typename WT, int NV, int W>
     void go() const {
         norm_backward_kernel<T, WT, NV, W><<<groups, Cols<T, NV, W>::THREADS, 0, s>>>(
@@ -290,26 +334,14 @@ struct Backward {
     }
 };
 
-template <typename T, typename WT, typename F>
-void by_cols(const F& f, uint32_t cols) {
-    constexpr int half = 8 / VN<T>, one = 16 / VN<T>, two = 32 / VN<T>;  // 8, 16, 32 elements per lane
-    const int w = waves(cols);
-    const uint32_t each = (cols + 64 * w - 1) / (64 * w);
-    if (w == 8)
-        f.template go<T, WT, two, 8>();
-    else if (w == 4)
-        each <= 8 ? f.template go<T, WT, half, 4>() : each <= 16 ? f.template go<T, WT, one, 4>() : f.template go<T, WT, two, 4>();
-    else
-        each <= 8 ? f.template go<T, WT, half, 1>() : f.template go<T, WT, one, 1>();
-}
 template <typename F>
-void by_type(const F& f, int type, int wtype, uint32_t cols) {
+void by_type(const F& f, int type, int wtype) {
     if (type == BS_F32)
-        by_cols<float, float>(f, cols);
+        f.template pick<float, float>();
     else if (type == BS_F16)
-        wtype == BS_F32 ? by_cols<f16, float>(f, cols) : by_cols<f16, f16>(f, cols);
+        wtype == BS_F32 ? f.template pick<f16, float>() : f.template pick<f16, f16>();
     else
-        wtype == BS_F32 ? by_cols<bf16, float>(f, cols) : by_cols<bf16, bf16>(f, cols);
+        wtype == BS_F32 ? f.template pick<bf16, float>() : f.template pick<bf16, bf16>();
 }
 
 int check(const char* what, uint64_t rows, uint32_t cols, int type, int wtype) {
@@ -333,7 +365,7 @@ extern "C" int bs_layer_norm(const void* x, int64_t x_stride, const void* weight
     if (x_stride < cols || y_stride < cols) return refuse("bs_layer_norm: rows overlap (stride < cols)");
     by_type(Forward{x, weight, bias, x_stride, y_stride, eps, y, mean, rstd, rows, static_cast<int>(cols),
                     static_cast<hipStream_t>(stream)},
-            type, wtype, cols);
+            type, wtype);
     return launched("bs_layer_norm");
 } catch (...) {
     return bs_internal_exception();
@@ -369,7 +401,7 @@ extern "C" int bs_layer_norm_backward(const void* dy, int64_t dy_stride, const v
     if (groups && (dx || dweight))
         by_type(Backward{dy, x, weight, dy_stride, x_stride, dx_stride, mean, rstd, dx, parts, groups, rows,
                          static_cast<int>(cols), s},
-                type, wtype, cols);
+                type, wtype);
     if (dweight) {  // also without rows: the sums are then 0
         const uint32_t blocks = (2 * cols + 63) / 64;
         if (wtype == BS_F32)

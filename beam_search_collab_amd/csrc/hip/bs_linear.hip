@@ -326,7 +326,8 @@ struct Mma16<bf16> {
 
 // Few rows: the weight is read once, from memory to registers, and bounds the time.  A workgroup has NT x 16 of
 // its rows, its eight waves a contiguous piece each of the inner dimension, so that 16 columns are enough work
-// for a compute unit and nothing is joined across workgroups; x (MT x 16 rows) comes from the L2.
+// for a compute unit and nothing is joined across workgroups; x (MT x 16 rows) comes from the L2.  17 x 4096 -> 4096
+// in bf16: 10.6 us among other calls, 3.2 TB/s; 1 x 1024 -> 128 4.2 us, a chain of four loads and a launch.
 template <typename T, typename O, int MT, int NT>
 __global__ __launch_bounds__(512) void linear_few_kernel(Params p) {
     __shared__ f32x4 join[8][NT * MT][64];
@@ -387,6 +388,9 @@ __global__ __launch_bounds__(512) void linear_few_kernel(Params p) {
     if (row < p.rows && col < p.cols) finish<T, O>(p, row, col, z);
 }
 
+// Mid: four steps of 32 in LDS cover the way from memory; 2048 x 4096 -> 4096 takes 81 us (850 TFLOP/s).  Operands in
+// 64-byte rows cost twice the requests of the 128-byte rows below and bound it.
+// Small: 1024 x 1024 -> 1024 takes 8 us, the latency of its 16 steps.
 using Mid = Tile<128, 128, 2, 2, 32, 4, 2>;
 using Small = Tile<64, 64, 2, 2, 64, 4, 2>;
 
@@ -403,6 +407,11 @@ using Small = Tile<64, 64, 2, 2, 64, 4, 2>;
 // A workgroup per CU goes through its tiles without a break: the moves of the next tile's first steps are
 // under way while a tile's results are written.  A tile that would pass an edge is shifted back inside and
 // does not write what its neighbour writes.
+//
+// 16384 x 4096 -> 4096 with bias and residual takes 474 us (1160 TFLOP/s; the library reaches 1348 without either at
+// 8192 x 8192 x 8192), the matrix pipe busy for 0.59 of the time at 1.83 GHz: the meetings bound it, four a step.
+// Inner steps of 32 took 625 us, reads and moves in a row before the products 562, moves later in the phase 583.
+// 8191 x 1024 -> 4096 with gelu takes 84 us: 8 us of epilogue after every 16 steps, which nothing overlaps.
 template <typename T, typename O>
 __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -600,17 +609,22 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
     __builtin_amdgcn_s_waitcnt(0);  // moves into this workgroup's LDS end before it does
 }
 
-constexpr uint32_t FEW = 32;  // rows up to which the weight is streamed
+// Rows up to which the weight is streamed: 17 x 4096 -> 4096 12 us, 40 with the tiles of 64; 48 and 64 rows would take
+// 18.3 and 20.7, against 15.0 and 14.8.
+constexpr uint32_t FEW = 32;
 
 uint64_t tiles_of(uint64_t rows, uint32_t cols, uint32_t size) { return (rows + size - 1) / size * ((cols + size - 1) / size); }
 
-// Pieces of the inner dimension for tiles of 64: where they leave compute units idle, pieces of 512 elements
-// at least.
+// Pieces of the inner dimension for tiles of 64, where they leave compute units idle: three at least, of 1024 elements
+// at least, to be worth the second launch.  With and without: 64 x 8192 -> 1024 12.2 and 31.6 us, 64 x 4096 -> 4096 12.2
+// and 17.7, but two pieces of 512 x 2048 -> 768 12.0 and 10.8, of 700 x 4096 -> 1000 18.5 and 18.1.  (Pieces of 512
+// elements: 14.5 us for the first, 14.3 for the second.)  Where rows cannot be 16-byte aligned a step takes twice the
+// time and two are enough: 64 x 2500 -> 1024 16.4 and 25.0.
 uint32_t splits_of(uint64_t rows, uint32_t inner, uint32_t cols) {
     if (rows <= FEW) return 1;
     const uint64_t tiles = tiles_of(rows, cols, 64);
-    if (tiles >= CUS || inner < 1024) return 1;
-    const uint32_t want = static_cast<uint32_t>(std::min<uint64_t>(2 * CUS / tiles, inner / 512));
+    const uint32_t want = static_cast<uint32_t>(std::min<uint64_t>(2 * CUS / tiles, inner / 1024));
+    if (want < (inner % 8 ? 2 : 3)) return 1;
     const uint32_t steps = (inner + 63) / 64, piece = (steps + want - 1) / want;
     return (steps + piece - 1) / piece;
 }
@@ -640,7 +654,8 @@ int start_big(const Params& p, hipStream_t s) {
 }
 template <typename T, typename O, int MT>
 int start_few(const Params& p, hipStream_t s) {
-    // 32 columns a workgroup, half the reads of x, where that leaves a workgroup for every compute unit
+    // 32 columns a workgroup, half the reads of x, where that leaves a workgroup for every compute unit:
+    // 17 x 8192 -> 8192 takes 35 us instead of 46
     if (p.cols >= 32 * CUS)
         linear_few_kernel<T, O, MT, 2><<<(p.cols + 31) / 32, 512, 0, s>>>(p);
     else
@@ -652,9 +667,14 @@ template <typename T, typename O>
 int launch(const Params& p, hipStream_t s) {
     if (p.rows <= FEW) return p.rows <= 16 ? start_few<T, O, 1>(p, s) : start_few<T, O, 2>(p, s);
     const bool direct = aligned16(p.x) && aligned16(p.w) && p.xs % 8 == 0 && p.ws % 8 == 0;
-    if (tiles_of(p.rows, p.cols, 256) >= CUS && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 &&
+    // Tiles of 256 where they fill the compute units' rounds to 0.55 at least.  Big and Mid: 4096 x 4096 -> 4096 (1.0)
+    // 113 and 163 us, -> 3584 (0.88) 102 and 149, 3000 x 1024 -> 4096 (0.75) 33.6 and 38, 2304 x 4096 -> 4096 (0.56) 88
+    // and 110, but 4096 x 1024 -> 4352 (0.53) 62 and 55, 2048 x 4096 -> 4096 (0.5) 86 and 81.
+    const uint64_t large = tiles_of(p.rows, p.cols, 256), rounds = (large + CUS - 1) / CUS;
+    if (large * 20 >= rounds * CUS * 11 && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 &&
         p.xs < (1 << 22) && p.ws < (1 << 22))
         return start_big<T, O>(p, s);
+    // Mid and Small: 2048 x 4096 -> 2048 (256 tiles of 128) 42 and 53 us, 1024 x 4096 -> 2048 (128) 38 and 28
     if (tiles_of(p.rows, p.cols, 128) >= CUS) return direct ? start<T, O, Mid, true>(p, s) : start<T, O, Mid, false>(p, s);
     return direct ? start<T, O, Small, true>(p, s) : start<T, O, Small, false>(p, s);
 }

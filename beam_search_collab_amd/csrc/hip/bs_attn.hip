@@ -459,7 +459,14 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 
 // Whole prompts.  Four waves of 32 rows share the tiles of 64 keys in LDS, two of them: the next tile's moves
 // run under a tile's products.  Two workgroups per compute unit (three for heads up to 64): one's matrix
-// instructions run under the other's exponentials.
+// instructions run under the other's exponentials.  (Three for heads of 64: passages below 90 to 83 us; four spill: 144.)
+//
+// Two causal documents of 8192 and 7500 tokens, 32 heads of 128, 8 key/value heads, bf16: 985 us (980 TFLOP/s), the
+// vector and matrix pipes half busy each (0.49, 0.46): a wave's exponentials and its products do not overlap, only two
+// waves' do.  96 passages of 37..512 tokens, 16 heads of 64: 74 us, bound by vector instructions (200 beside 16 matrix
+// instructions a tile, 500 in tiles with masks) and 12 us of latency per workgroup.  Other orders that were slower for
+// the documents: two groups of waves half a step apart, meeting between their phases (1244 against 1175), moves between
+// the products and exponentials instead of before them (1246 against 1142).
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params p) {
     constexpr int ROWS = 128, S = ROW<DP>, TILE = BN * S;
@@ -544,10 +551,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
 
 // Few rows per sequence (single tokens): the keys' bytes bound the time.  A tile has at most 32 rows, and the
 // FEW_WAVES waves of a workgroup take turns at its tiles of 32 keys, through LDS of their own, without meeting;
-// their results are joined at the end.
+// their results are joined at the end.  16 tokens over 16 sequences of 1.4k..16k keys, 8 heads of 128: 135 us, 4.7 TB/s
+// (a copy reaches 5.1), and 5 us for the join of the pieces; four waves, of which fewer fit: 155 against 146 then.
 constexpr int FEW_WAVES = 2;
 
-// Near: 16 rows of keys lie within 32 bits of each other, of values too
+// Near: rows of keys that a move takes lie within 32 bits of each other, of values too
 template <typename T, int DP, bool Near>
 __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params p) {
     constexpr int ROWS = 32, KN = 32, S = ROW<DP>, TILE = KN * S, NB = 32768 / (2 * TILE);  // NB tiles of a wave in LDS
@@ -689,7 +697,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     }
 }
 
-// Joins the pieces of a row (query token, head): a workgroup each.  First the maximum of all pieces and the sum
+// Joins the pieces of a row (query token, head): a workgroup each, since single tokens have few rows and many pieces (one
+// token over 16384 keys: 21 us in all, 63 with a wave that walked them; long inputs pay about 1 ns a row).  First the maximum of all pieces and the sum
 // against it, a piece per lane; then the results, the pieces in four contiguous runs, one per wave.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
@@ -743,33 +752,45 @@ uint64_t tiles_of(const bs_attention_args& a, uint32_t rows) {
     return t / rows + a.sequences;
 }
 
-// whether rows of 16 tokens lie within 32 bits of each other
+// Whether the rows of a move lie within 32 bits of each other, so that its addresses are a scalar and an offset per lane
+// (documents above: 1118 us, 1173 with 64 bits per lane).  Rows farther apart go to the few rows' kernel, which has both.
 bool near_of(const bs_attention_args& a) { return a.k_stride < (1 << 22) && a.v_stride < (1 << 22); }
 
-// Few rows: sequences of two tiles of 32 rows at most, by the longest one where it is given, else by their mean.
+// Single tokens of groups up to 8, by the longest sequence where it is given, else by the mean.  Against whole prompts'
+// kernel: 16 tokens over 1.4k..16k keys of 8 heads of 128, groups of 4: 141 and 162 us, of 16 heads of 64: 147 and 210;
+// but two tokens each over 4096 keys, groups of 4: 38 and 36, eight 68 and 40; one token over 16384 keys, group of 32:
+// 16.7 and 15.4.
 bool few_of(const bs_attention_args& a) {
-    const uint64_t group = a.heads / a.kv_heads;
     const uint64_t tokens = a.longest_q ? a.longest_q : (a.q_tokens + a.sequences - 1) / a.sequences;
-    return tokens * group <= 64;
+    return tokens <= 1 && a.heads / a.kv_heads <= 8;
 }
 
 // Pieces of the keys, multiples of the keys that a workgroup takes at a time.  The last one takes what is left,
 // should a sequence be longer than longest_k said.
 void split(const bs_attention_args& a, uint32_t& splits, uint32_t& piece) {
     const uint32_t longest = a.longest_k ? std::min(a.longest_k, a.k_tokens) : a.k_tokens;
+    const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * a.heads;
     uint64_t want;
     if (few_of(a)) {
-        // about six workgroups per compute unit, so that sequences of different lengths even out
-        const uint64_t keys = static_cast<uint64_t>(a.k_tokens) * a.kv_heads * std::max<uint64_t>(1, (tiles_of(a, 32) - a.sequences) / a.sequences);
-        want = std::max<uint64_t>(keys / (6 * CUS), 256);
+        // About six workgroups per compute unit, so that sequences of different lengths even out: 16 tokens over 1.4k..16k
+        // keys take 141 us, with two 161, with twelve 140.  Pieces of 256 keys at least (one token over 16384 keys 20.2 us,
+        // 25.9 with 128, 21.4 with 512), of 512 where there is a workgroup for every compute unit without (64 over 1024
+        // keys, 4 heads of 64: 20.8, with 256 24.5).
+        const uint64_t keys = static_cast<uint64_t>(a.k_tokens) * a.kv_heads;
+        const uint64_t least = static_cast<uint64_t>(a.sequences) * a.kv_heads >= CUS ? 512 : 256;
+        want = std::max<uint64_t>(keys / (6 * CUS), least);
     } else {
+        // Two workgroups per compute unit, where the keys are long enough for the joining of the rows: about 1 ns a row,
+        // 15 to 25 ns saved a key.  With and without: 200 tokens over 4096 keys, 32 heads 40 and 101 us, 768 over 8192 136
+        // and 204; 900 over 900 62 and 26, 1024 over 1024, 16 heads 33 and 20.
         const uint64_t groups = tiles_of(a, 128) * a.kv_heads;
-        want = groups >= 2 * CUS ? longest : std::max<uint64_t>(longest * groups / (2 * CUS), 256);
+        const bool whole = groups >= 2 * CUS || static_cast<uint64_t>(longest) * 16 <= rows + 8192;
+        want = whole ? longest : std::max<uint64_t>(longest * groups / (2 * CUS), 256);
     }
     piece = static_cast<uint32_t>(std::min<uint64_t>((want + 127) / 128 * 128, (static_cast<uint64_t>(longest) + 127) / 128 * 128));
     if (piece == 0) piece = 128;
     // at most 256 MB of parts: with many sequences the pieces are for their different lengths alone
-    const uint64_t row = static_cast<uint64_t>(a.q_tokens) * a.heads * (a.head_dim + 2) * sizeof(float);
+    const uint64_t row = rows * (a.head_dim + 2) * sizeof(float);
     const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(65535, (1ull << 28) / std::max<uint64_t>(row, 1)));
     if ((longest + piece - 1) / piece > most) piece = static_cast<uint32_t>((longest + most - 1) / most + 127) / 128 * 128;
     splits = std::max(1u, (longest + piece - 1) / piece);
@@ -792,7 +813,8 @@ int check(const char* what, const bs_attention_args* a) {
     if (a->q_tokens > 0x7FFFFFFFu || a->k_tokens > 0x7FFFFFFFu) return refuse(w + ": q_tokens and k_tokens must be < 2^31");
     if (a->sequences == 0 || a->sequences > 0x7FFFFFFu) return refuse(w + ": sequences must be in 1..2^27");
     if (!(std::fabs(a->scale) <= 1e30f)) return refuse(w + ": scale must be finite, at most 1e30");
-    if (tiles_of(*a, 32) * a->kv_heads > 0x7FFFFFFFull || static_cast<uint64_t>(a->q_tokens) * a->heads > 0x7FFFFFFFull) return refuse(w + ": too many tiles for one launch");
+    // threads of a launch are counted in 32 bits
+    if (tiles_of(*a, 32) * a->kv_heads * 256 > 0xFFFFFFFFull || static_cast<uint64_t>(a->q_tokens) * a->heads > 0x7FFFFFFFull) return refuse(w + ": too many tiles for one launch");
     return BS_OK;
 }
 

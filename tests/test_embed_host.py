@@ -98,6 +98,7 @@ def attention_args(**change):
     (dict(q_tokens=1 << 31), "must be < 2^31"),
     (dict(sequences=0), "sequences must be"),
     (dict(sequences=2), "need q_offsets"),
+    (dict(sequences=1 << 24), "too many tiles"),
     (dict(scale=float("inf")), "scale must be finite"),
     (dict(scale=float("nan")), "scale must be finite"),
     (dict(k=None), "must be given"),

@@ -157,6 +157,10 @@ __device__ inline float2 halves(float v) {
     return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// The maximum that keeps NaN: three operands an instruction, and none of them is multiplied by 1 first, as fmaxf has it
+// done to quiet NaN.
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 template <int DP>
 constexpr int ROW = DP <= 32 ? 64 : DP <= 64 ? 128 : 256;  // bytes of a key or value in LDS
 
@@ -237,22 +241,31 @@ struct Rows {
     // weights of the scores.  Masked: only keys below `mine` count.
     template <bool Masked, int KB>
     __device__ void weights(Work<KB>& x, uint32_t j0, uint32_t mine, float scale, int lane) {
-        const uint32_t from = j0 + (lane >> 5) * 4;  // of this half's keys
+        // Keys that this lane's row sees: register r of block b has key b * 32 + r % 4 + 8 (r / 4) + 4 h.  Opaque, and the
+        // scores after it, so that a comparison with a constant and a selection per score are all that is left of it.
+        int left = static_cast<int>(min(mine, j0 + 64u) - min(mine, j0)) - (lane >> 5) * 4;
+        if (Masked) asm volatile("" : "+v"(left));
         float high[4] = {NONE, NONE, NONE, NONE};
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                if (Masked && from + (b * 32 + (r & 3) + 8 * (r >> 2)) >= mine) x.z[b][r] = NONE;
-                high[r >> 2] = fmaxf(high[r >> 2], x.z[b][r]);
+                if (Masked) {
+                    float z = b * 32 + (r & 3) + 8 * (r >> 2) >= left ? NONE : x.z[b][r];
+                    asm volatile("" : "+v"(z));
+                    x.z[b][r] = z;
+                }
+                high[r >> 2] = larger(high[r >> 2], x.z[b][r]);
             }
-        const float2 two = halves(fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])));
-        const float most = fmaxf(two.x, two.y) * scale;  // scale > 0
+        const float2 two = halves(larger(larger(high[0], high[1]), larger(high[2], high[3])));
+        const float most = larger(two.x, two.y) * scale;  // scale > 0; NaN if some score is, as the row's sum will be
         // The weights may stand against an older maximum while they stay below 2^8: sums and results lose
-        // nothing by that, and the results are rescaled seldom.
-        if (__any(most > top + 8.0f)) {
-            const float now = fmaxf(top, most), fade = __builtin_amdgcn_exp2f(top - (now == NONE ? 0.0f : now));
-            top = now;
+        // nothing by that, and the results are rescaled seldom.  A row's own scores alone decide about it, so that no
+        // other row's keys show in its bits.
+        const bool grows = most > top + 8.0f;
+        if (__any(grows)) {
+            const float fade = grows ? __builtin_amdgcn_exp2f(top - most) : 1.0f;
+            top = grows ? most : top;
             sum *= fade;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
@@ -470,6 +483,10 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params p) {
     constexpr int ROWS = 128, S = ROW<DP>, TILE = BN * S;
+    // blocks of 32 keys at a time in the tiles that some row does not see whole: one where heads are short, for its code
+    // is short too and half of a short prompt's tiles are such (passages: 74 us, 80 with two); two for heads of 128
+    // (documents: 989 us, 1001 with one)
+    constexpr int KB = DP <= 64 ? 1 : 2;
     __shared__ __attribute__((aligned(16))) char lds[2][2 * TILE];
     __shared__ int flag;
     const bs_attention_args& a = p.a;
@@ -508,6 +525,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     me_.clear();
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
     const uint32_t mine = min(me.keys, ke);
+    // keys up to which this wave's last row sees; a wave past the last row has nothing to do but its moves
+    const uint32_t wave0 = row0 + wave * 32;
+    const uint32_t reach = wave0 < rows ? min(ke, keys_of(a, sq, p.by_group.quotient(min(rows, wave0 + 32) - 1))) : 0;
     Found<DP / 32> found;
     for (int pass = PLAIN; parts; ++pass) {
         for (uint32_t t = 0; t < parts; ++t) {
@@ -520,7 +540,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
                 if (pass != PLAIN) sift<T>(tk + TILE, TILE, pass, threadIdx.x, 256);
                 settle();
             }
-            me_.template step<2, true>(tk, tk + TILE, start(t), mine, scale, lane);
+#pragma unroll 1
+            for (int b = 0; b < BN; b += KB * 32)
+                if (reach > start(t) + b) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, start(t) + b, mine, scale, lane);
         }
         if (pass == PLAIN) {
             if (seen == all) break;  // all rows see the same keys
@@ -543,7 +565,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
         const char* tk = lds[t & 1];
         meet();
         if (t + 1 < tiles) mover.near(kb + (t + 1 - parts) * BN, lds[~t & 1]);
-        me_.template step<2, false>(tk, tk + TILE, 0, 0, scale, lane);
+        if (reach) {
+            // a loop of one turn: as a block of its own the step is scheduled apart from the moves (documents: 989 us, 1004
+            // in one block with them)
+#pragma unroll 1
+            for (int b = 0; b < BN; b += 64) me_.template step<2, false>(tk + b * S, tk + TILE + b * S, 0, 0, scale, lane);
+        }
     }
     me_.join_halves();
     write_rows<T, DP>(p, sq, me, me_, h);

@@ -491,6 +491,17 @@ def test_attention_never_touches_what_a_query_does_not_see(gpu, bad, nq, nk, hea
         which.copy_(was)
 
 
+@pytest.mark.parametrize("nq,nk,heads,kv,dim", [([300], [300], 4, 1, 64), ([7, 90], [7, 200], 2, 2, 128), ([33], [33], 1, 1, 32)])
+@pytest.mark.parametrize("bad", [40.0, -40.0, math.inf, math.nan])
+def test_attention_rows_show_no_other_rows_keys(gpu, nq, nk, heads, kv, dim, bad):
+    """bit for bit, also where the last query's scores grow so much that its results are rescaled"""
+    q, k, v = rand(91, sum(nq), heads, dim, dtype=BF16), rand(92, sum(nk), kv, dim, dtype=BF16), rand(93, sum(nk), kv, dim, dtype=BF16)
+    out = embed.attention(q, k, v, offsets(nq), offsets(nk), causal=True)
+    k[-1] *= bad
+    again = embed.attention(q, k, v, offsets(nq), offsets(nk), causal=True)
+    assert torch.equal(again[:-1], out[:-1]) and not torch.equal(again[-1], out[-1])
+
+
 def test_attention_of_extreme_scores(gpu):
     """scores far apart, one key with all the weight, and keys that score minus infinity"""
     q, k, v = (rand(75 + i, 80, 1, 64, dtype=BF16) for i in range(3))

@@ -388,9 +388,12 @@ __global__ __launch_bounds__(512) void linear_few_kernel(Params p) {
     if (row < p.rows && col < p.cols) finish<T, O>(p, row, col, z);
 }
 
-// Mid: four steps of 32 in LDS cover the way from memory; 2048 x 4096 -> 4096 takes 81 us (850 TFLOP/s).  Operands in
-// 64-byte rows cost twice the requests of the 128-byte rows below and bound it.
+// Tall: one workgroup of 8 waves per compute unit, three steps of 64; 2048 x 4096 -> 4096 takes 73 us (945 TFLOP/s).  The
+// wait for the oldest step at every meeting bounds it.  Four waves of 128 x 64 take 76 us, tiles of 128 x 256 74.
+// Mid: two workgroups per compute unit, four steps of 32; the same takes 90 us: operands in 64-byte rows cost twice
+// the requests.  Steps of 64, which leave one workgroup of 128 x 128 per compute unit, take 96.
 // Small: 1024 x 1024 -> 1024 takes 8 us, the latency of its 16 steps.
+using Tall = Tile<256, 128, 4, 2, 64, 3, 1>;
 using Mid = Tile<128, 128, 2, 2, 32, 4, 2>;
 using Small = Tile<64, 64, 2, 2, 64, 4, 2>;
 
@@ -613,7 +616,8 @@ __global__ __launch_bounds__(512, 2) void linear_big_kernel(Params p) {
 // 18.3 and 20.7, against 15.0 and 14.8.
 constexpr uint32_t FEW = 32;
 
-uint64_t tiles_of(uint64_t rows, uint32_t cols, uint32_t size) { return (rows + size - 1) / size * ((cols + size - 1) / size); }
+uint64_t tiles_of(uint64_t rows, uint32_t cols, uint32_t high, uint32_t wide) { return (rows + high - 1) / high * ((cols + wide - 1) / wide); }
+uint64_t tiles_of(uint64_t rows, uint32_t cols, uint32_t size) { return tiles_of(rows, cols, size, size); }
 
 // Pieces of the inner dimension for tiles of 64, where they leave compute units idle: three at least, of 1024 elements
 // at least, to be worth the second launch.  With and without: 64 x 8192 -> 1024 12.2 and 31.6 us, 64 x 4096 -> 4096 12.2
@@ -670,10 +674,13 @@ int launch(const Params& p, hipStream_t s) {
     // Tiles of 256 where they fill the compute units' rounds to 0.55 at least.  Big and Mid: 4096 x 4096 -> 4096 (1.0)
     // 113 and 163 us, -> 3584 (0.88) 102 and 149, 3000 x 1024 -> 4096 (0.75) 33.6 and 38, 2304 x 4096 -> 4096 (0.56) 88
     // and 110, but 4096 x 1024 -> 4352 (0.53) 62 and 55, 2048 x 4096 -> 4096 (0.5) 86 and 81.
-    const uint64_t large = tiles_of(p.rows, p.cols, 256), rounds = (large + CUS - 1) / CUS;
-    if (large * 20 >= rounds * CUS * 11 && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 &&
+    auto fill = [](uint64_t tiles) { return static_cast<float>(tiles) / static_cast<float>((tiles + CUS - 1) / CUS * CUS); };
+    if (fill(tiles_of(p.rows, p.cols, 256)) >= 0.55f && direct && p.rows >= 256 && p.cols >= 256 && p.inner % 64 == 0 && p.inner >= 128 &&
         p.xs < (1 << 22) && p.ws < (1 << 22))
         return start_big<T, O>(p, s);
+    // Tall and Mid: 2048 x 4096 -> 4096 (1.0) 73 and 90 us, 8192 x 1024 -> 1024 (1.0) 24 and 27, 3000 x 2048 -> 2048 (0.75)
+    // 35 and 40, but 2048 x 1024 -> 2048 (0.5) 20 and 16
+    if (fill(tiles_of(p.rows, p.cols, 256, 128)) >= 0.75f && direct) return start<T, O, Tall, true>(p, s);
     // Mid and Small: 2048 x 4096 -> 2048 (256 tiles of 128) 42 and 53 us, 1024 x 4096 -> 2048 (128) 38 and 28
     if (tiles_of(p.rows, p.cols, 128) >= CUS) return direct ? start<T, O, Mid, true>(p, s) : start<T, O, Mid, false>(p, s);
     return direct ? start<T, O, Small, true>(p, s) : start<T, O, Small, false>(p, s);

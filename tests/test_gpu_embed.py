@@ -255,6 +255,16 @@ def test_linear_of_many_tiles(gpu, rows, inner, cols, dtype):
     assert torch.equal(wide[:, 3:cols + 3], want) and (wide[:, :3] == 7).all() and (wide[:, cols + 3:] == 7).all()
 
 
+@pytest.mark.parametrize("rows,inner,cols", [(2048, 200, 4001), (2047, 64, 4096), (8000, 1032, 900), (16300, 72, 384), (2048, 8, 4096)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_linear_of_half_as_many_tiles(gpu, rows, inner, cols, dtype):
+    x, w = rand(48, rows, inner, dtype=dtype), rand(49, cols, inner, dtype=dtype, std=inner ** -0.5)
+    b, r = rand(50, cols, dtype=dtype), rand(51, rows, cols, dtype=dtype)
+    got = embed.linear(x, w, b, activation="gelu", residual=r)
+    check_linear(x, w, b, "gelu", r, got)
+    assert torch.equal(got, embed.linear(x, w, b, activation="gelu", residual=r))
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("rows,inner,cols", [(4, 128, 64), (300, 256, 384), (600, 100, 130)])
 def test_linear_activations(gpu, act, rows, inner, cols):

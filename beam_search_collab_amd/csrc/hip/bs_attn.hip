@@ -475,9 +475,9 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 // instructions run under the other's exponentials.  (Three for heads of 64: passages below 90 to 83 us; four spill: 144.)
 //
 // Two causal documents of 8192 and 7500 tokens, 32 heads of 128, 8 key/value heads, bf16: 985 us (980 TFLOP/s), the
-// vector and matrix pipes half busy each (0.49, 0.46): a wave's exponentials and its products do not overlap, only two
-// waves' do.  96 passages of 37..512 tokens, 16 heads of 64: 74 us, bound by vector instructions (200 beside 16 matrix
-// instructions a tile, 500 in tiles with masks) and 12 us of latency per workgroup.  Other orders that were slower for
+// vector and matrix pipes half busy each (0.49, 0.47): a wave's exponentials and its products do not overlap, only two
+// waves' do.  96 passages of 37..512 tokens, 16 heads of 64: 68 us, bound by vector instructions (170 beside 16 matrix
+// instructions a tile, 270 with masks) and the latency of each workgroup's first loads.  Other orders that were slower for
 // the documents: two groups of waves half a step apart, meeting between their phases (1244 against 1175), moves between
 // the products and exponentials instead of before them (1246 against 1142).
 template <typename T, int DP>
@@ -725,8 +725,9 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
 }
 
 // Joins the pieces of a row (query token, head): a workgroup each, since single tokens have few rows and many pieces (one
-// token over 16384 keys: 21 us in all, 63 with a wave that walked them; long inputs pay about 1 ns a row).  First the maximum of all pieces and the sum
-// against it, a piece per lane; then the results, the pieces in four contiguous runs, one per wave.
+// token over 16384 keys: 21 us in all, 63 with a wave that walked them; long inputs pay about 1 ns a row).  First the
+// maximum of all pieces and the sum against it, a piece per lane; then the results, the pieces in four contiguous runs,
+// one per wave.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
     __shared__ float2 half[4][64];

@@ -724,17 +724,18 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     }
 }
 
-// Joins the pieces of a row (query token, head): a workgroup each, since single tokens have few rows and many pieces (one
-// token over 16384 keys: 21 us in all, 63 with a wave that walked them; long inputs pay about 1 ns a row).  First the
-// maximum of all pieces and the sum against it, a piece per lane; then the results, the pieces in four contiguous runs,
-// one per wave.
-template <typename T>
+// Joins the pieces of a row (query token, head), W waves a row.  First the maximum of all pieces and the sum against it, a
+// piece per lane; then the results, the pieces in W contiguous runs, one per wave.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void join_kernel(Params p) {
+    static_assert(W == 1 || W == 4, "a workgroup has four waves");
     __shared__ float2 half[4][64];
     const bs_attention_args& a = p.a;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t at = blockIdx.x, rows = static_cast<uint64_t>(a.q_tokens) * a.heads;
-    const uint32_t tok = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+    const int lane = threadIdx.x & 63, wave = static_cast<int>(uniform(threadIdx.x >> 6)), part = W == 1 ? 0 : wave;
+    const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * a.heads;
+    const uint32_t at = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;  // < 2^31 + 4
+    if (at >= rows) return;
+    const uint32_t tok = at / a.heads, head = at % a.heads;
     const uint32_t seq = a.q_offsets ? holder(a.q_offsets, a.sequences, tok) : 0;
     const Sequence sq = sequence(a, seq);
     if (tok < sq.q0 || tok - sq.q0 >= sq.nq) return;
@@ -750,7 +751,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
         sum += st.y * __builtin_amdgcn_exp2f(st.x - base);
     }
     sum = wave_sum(sum);
-    const uint32_t d = lane * 2, run = (n + 3) / 4, begin = wave * run, end = min(begin + run, n);
+    const uint32_t d = lane * 2, run = (n + W - 1) / W, begin = part * run, end = min(begin + run, n);
     float2 o = make_float2(0.0f, 0.0f);
     if (d < a.head_dim) {
 #pragma unroll 4
@@ -762,11 +763,13 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
             o.y = fmaf(v.y, gain, o.y);
         }
     }
-    half[wave][lane] = o;
-    __syncthreads();
-    if (wave) return;
+    if (W > 1) {
+        half[wave][lane] = o;
+        __syncthreads();
+        if (wave) return;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) o.x += half[w][lane].x, o.y += half[w][lane].y;
+        for (int w = 1; w < W; ++w) o.x += half[w][lane].x, o.y += half[w][lane].y;
+    }
     const float over = reciprocal_of(sum);
     if (d < a.head_dim) {
         T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tok) * a.out_stride + static_cast<int64_t>(head) * a.out_head_stride;
@@ -808,9 +811,9 @@ void split(const bs_attention_args& a, uint32_t& splits, uint32_t& piece) {
         const uint64_t least = static_cast<uint64_t>(a.sequences) * a.kv_heads >= CUS ? 512 : 256;
         want = std::max<uint64_t>(keys / (6 * CUS), least);
     } else {
-        // Two workgroups per compute unit, where the keys are long enough for the joining of the rows: about 1 ns a row,
-        // 15 to 25 ns saved a key.  With and without: 200 tokens over 4096 keys, 32 heads 40 and 101 us, 768 over 8192 136
-        // and 204; 900 over 900 62 and 26, 1024 over 1024, 16 heads 33 and 20.
+        // Two workgroups per compute unit, where the keys are long enough for the parts of the rows to be written and joined.
+        // With and without: 200 tokens over 4096 keys, 32 heads of 128 35 and 101 us, 768 over 8192 117 and 204; 900 over 900
+        // 34 and 25, 600 over 1200 34 and 31, 1024 over 1024, 16 heads of 64 26 and 20.
         const uint64_t groups = tiles_of(a, 128) * a.kv_heads;
         const bool whole = groups >= 2 * CUS || static_cast<uint64_t>(longest) * 16 <= rows + 8192;
         want = whole ? longest : std::max<uint64_t>(longest * groups / (2 * CUS), 256);
@@ -868,7 +871,16 @@ int launch(const Params& p, hipStream_t s) {
     const uint32_t d = p.a.head_dim;
     const int rc = d <= 32 ? start<T, 32>(p, s) : d <= 64 ? start<T, 64>(p, s) : d <= 96 ? start<T, 96>(p, s) : start<T, 128>(p, s);
     if (rc) return rc;
-    if (p.splits > 1) join_kernel<T><<<p.a.q_tokens * p.a.heads, 256, 0, s>>>(p);
+    if (p.splits > 1) {
+        // Four waves a row where rows are few and their latency counts, one where there are many.  One and four: 1000 tokens
+        // over 4096 keys, 16 heads of 64 38 and 54 us, 768 over 8192, 32 heads of 128 117 and 137, 8 x 8 over 4096 (2048
+        // rows) 38.5 and 39.2; but 40 over 8192 (1280 rows) 26.4 and 25.5, one token over 16384 24.0 and 20.3.
+        const uint32_t rows = p.a.q_tokens * p.a.heads;
+        if (rows >= 8 * CUS)
+            join_kernel<T, 1><<<(rows + 3) / 4, 256, 0, s>>>(p);
+        else
+            join_kernel<T, 4><<<rows, 256, 0, s>>>(p);
+    }
     return launched("bs_attention");
 }
 

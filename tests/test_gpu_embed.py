@@ -426,6 +426,18 @@ def attention_on_gpu(q, k, v, nq, nk, causal, scale):
     return o, lse, size, total, spread
 
 
+@pytest.mark.parametrize("nq,nk,heads,kv,dim", [([800], [5000], 8, 2, 64), ([701], [2800], 3, 1, 72), ([1, 300, 0, 400], [900, 3000, 40, 2500], 4, 4, 128)])
+@pytest.mark.parametrize("dtype,causal", [(BF16, True), (F16, False)])
+def test_attention_of_many_rows_split_over_the_keys(gpu, nq, nk, heads, kv, dim, dtype, causal):
+    q, k, v = rand(95, sum(nq), heads, dim, dtype=dtype), rand(96, sum(nk), kv, dim, dtype=dtype), rand(97, sum(nk), kv, dim, dtype=dtype)
+    out, lse = embed.attention(q, k, v, offsets(nq), offsets(nk), causal=causal, longest_q=max(nq), longest_k=max(nk), lse=True)
+    wo, wl, size, total, spread = attention_on_gpu(q, k, v, nq, nk, causal, dim ** -0.5)
+    d, count = (dim + 6) * E * spread + 4 * E * (spread + 1), max(nk)
+    near(out, wo, (U[dtype] + 4 * d + (count + 40) * E)[..., None] * size + 2.0 ** -24 * total * (dtype == F16) + U[dtype] * wo.abs() + TINY[dtype])
+    near(lse, wl, 2 * d + (count / 32 + 40) * E + 4 * E * wl.abs())
+    assert torch.equal(out, embed.attention(q, k, v, offsets(nq), offsets(nk), causal=causal, longest_q=max(nq), longest_k=max(nk)))
+
+
 @pytest.mark.parametrize("nq,nk,heads,kv,dim", [([1500, 1100], [1500, 1100], 16, 8, 64), ([1290], [1290], 64, 16, 128), ([900, 40], [2000, 1300], 16, 16, 96),
                                                 ([1100], [1100], 64, 64, 32), ([640] * 40, [640] * 40, 2, 2, 72)])
 @pytest.mark.parametrize("dtype,causal", [(BF16, True), (F16, True), (BF16, False)])

@@ -4,6 +4,7 @@ Tolerances are the sums of the roundings an operator makes, worst case:  U is th
 output type, E = 2^-24 that of the float32 arithmetic; a float32 sum of n terms is off by at most n E
 times the sum of the magnitudes (n: the longest chain of additions).
 """
+import gc
 import math
 
 import numpy as np
@@ -18,6 +19,17 @@ E = 2.0 ** -24
 U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}  # below the normal range
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_given_back():
+    """tests of other files look at the device's free memory"""
+    yield
+    if torch.cuda.is_available():
+        gc.collect()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
 
 
 def rand(seed, *shape, dtype=F32, std=1.0):

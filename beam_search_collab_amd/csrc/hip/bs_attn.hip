@@ -320,7 +320,8 @@ struct Rows {
 // finite.  The last pass gives the sums; NaN and infinities are added where their passes gave more than 0.
 enum { PLAIN = 0, NANS = 1, HIGH = 2, LOW = 3, FINITE = 4 };
 
-// the values past the end of a sequence, for which the moves repeat its last one: no weight of 0 meets NaN there
+// the values of keys that no row of the tile sees -- later ones of the sequence, and what lies past its end, for which the
+// moves repeat its last one: no weight of 0 meets NaN there
 template <int S>
 __device__ inline void blank(char* tv, uint32_t first, uint32_t rows, int thread, int threads) {
     for (uint32_t i = first * (S / 16) + thread; i < rows * (S / 16); i += threads) reinterpret_cast<Vec<float, 4>*>(tv)[i] = Vec<float, 4>{};
@@ -534,8 +535,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
             char* tk = lds[t & 1];
             meet();  // tile t is in LDS, and nobody reads tile t - 1 any more
             if (t + 1 < tiles) mover.any(start(t + 1), lds[~t & 1]);
-            if (start(t) + BN > sq.nk || pass != PLAIN) {
-                if (start(t) + BN > sq.nk) blank<S>(tk + TILE, sq.nk - start(t), BN, threadIdx.x, 256);
+            if (start(t) + BN > all || pass != PLAIN) {
+                if (start(t) + BN > all) blank<S>(tk + TILE, all - start(t), BN, threadIdx.x, 256);  // start(t) < ke <= all
                 settle();
                 if (pass != PLAIN) sift<T>(tk + TILE, TILE, pass, threadIdx.x, 256);
                 settle();
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
                 if (reach > start(t) + b) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, start(t) + b, mine, scale, lane);
         }
         if (pass == PLAIN) {
-            if (seen == all) break;  // all rows see the same keys
+            if (seen == all) break;  // all rows see the same keys, and the others' values are blank
             if (me_.odd()) flag = 1;
             settle();
             if (!uniform(static_cast<uint32_t>(flag))) break;
@@ -646,7 +647,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
         const uint32_t j0 = start(0);
         Found<DP / 32> found;
         for (int pass = PLAIN;; ++pass) {
-            if (j0 + KN > sq.nk) blank<S>(tk + TILE, sq.nk - j0, KN, lane, 64);
+            if (j0 + KN > all) blank<S>(tk + TILE, all - j0, KN, lane, 64);  // j0 < ke <= all
             landed<63>();
             if (pass != PLAIN) {
                 sift<T>(tk + TILE, TILE, pass, lane, 64);
@@ -654,7 +655,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
             }
             me_.template step<1, true>(tk, tk + TILE, j0, mine, scale, lane);
             if (pass == PLAIN) {
-                if (seen == all || !__any(me_.odd())) break;  // all rows see the same keys, or nothing is there to touch them
+                // all rows see the same keys, and the others' values are blank; or nothing is there to touch them
+                if (seen == all || !__any(me_.odd())) break;
                 found.clear();
             } else if (pass == FINITE) {
                 found.give(me_.o);

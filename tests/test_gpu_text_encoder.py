@@ -648,3 +648,44 @@ def test_example_embeds_searches_and_tunes(gpu):
     spec.loader.exec_module(m)
     recall, own, before, after = m.main(["--passages", "1500", "--queries", "32", "--dim", "100"])
     assert recall >= 0.9 and own > 0.5 and after > before
+
+
+# ---------------------------------------------------------------- keys and values that nobody of a tile sees
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("nq,nk,heads,kv", [([5], [5], 128, 1), ([3, 4], [70, 40], 256, 1), ([6, 2], [6, 90], 200, 1), ([4], [130], 256, 2),
+                                            ([2], [700], 1024, 1)])
+def test_attention_of_large_groups_never_touches_what_a_query_does_not_see(gpu, bad, nq, nk, heads, kv):
+    """a tile of rows belongs to one token here, so that all its rows see the same keys, and others lie in its last tile of keys"""
+    q, k, v = (rand(110 + i, sum(n), h, 32, dtype=BF16) for i, (n, h) in enumerate(((nq, heads), (nk, kv), (nk, kv))))
+    good = embed.attention(q, k, v, offsets(nq), offsets(nk), lse=True)
+    ends_q, ends_k = np.cumsum(nq), np.cumsum(nk)
+    for hidden in range(1, min(nq)):  # the last keys of every sequence, which its last `hidden` queries see in part
+        rows = torch.ones(sum(nq), dtype=torch.bool, device="cuda")
+        for a, b in zip(ends_q, ends_k):
+            rows[a - hidden:a] = False
+        for which in (k, v):
+            was = which.clone()
+            for b in ends_k:
+                which[b - hidden:b] = bad
+            got = embed.attention(q, k, v, offsets(nq), offsets(nk), lse=True)
+            for a, b in zip(got, good):
+                assert torch.equal(a[rows], b[rows])
+            if which is v:
+                assert not torch.isfinite(got[0][~rows]).any()
+            which.copy_(was)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_of_rows_far_apart_never_touches_what_a_query_does_not_see(gpu, bad):
+    """32 heads of a group over values whose rows lie 2^22 elements apart: a tile of 32 rows belongs to one token"""
+    tokens, stride = 40, 1 << 22
+    q, k = rand(113, 4, 32, 64, dtype=BF16), rand(114, tokens, 1, 64, dtype=BF16)
+    v = torch.empty(tokens * stride, dtype=BF16, device="cuda").as_strided((tokens, 1, 64), (stride, 64, 1))
+    v.copy_(rand(115, tokens, 1, 64))
+    good, lse = embed.attention(q, k, v, offsets([4]), offsets([tokens]), lse=True)
+    check_attention(q, k, v.contiguous(), [4], [tokens], True, 0.125, good, lse)
+    for hidden in (1, 2, 3):
+        v[tokens - hidden] = bad
+        got = embed.attention(q, k, v, offsets([4]), offsets([tokens]))
+        assert torch.equal(got[:4 - hidden], good[:4 - hidden]) and not torch.isfinite(got[4 - hidden:]).any()

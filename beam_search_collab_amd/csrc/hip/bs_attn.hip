@@ -171,6 +171,12 @@ struct Rows {
     Vec<T, 8> q[DP / 16];
     f32x16 o[DP / 32];
     float top, sum;  // what the weights are taken against, in units of log2, and their sum over this half's keys
+    // The weights are rounded to the values' type for their product (the sum takes them as they are), since two 16-bit
+    // products a score, of a weight's upper and lower bits, would double the matrix work.  float16 has nothing below 2^-24,
+    // where many small weights beside a large one would be lost: there the largest weight stands at 2^7, and may grow to
+    // 2^11 before the row is rescaled.  (Its largest value is 2^16; 2^4 are left for scores so large that float32 has them
+    // in steps of up to 8.)  A weight is then off by 2^-32 of the row's largest at most.
+    static constexpr float ROOM = std::is_same<T, f16>::value ? 7.0f : 0.0f, LAG = std::is_same<T, f16>::value ? 4.0f : 8.0f;
 
     __device__ void clear() {
         top = NONE;
@@ -259,13 +265,13 @@ struct Rows {
             }
         const float2 two = halves(larger(larger(high[0], high[1]), larger(high[2], high[3])));
         const float most = larger(two.x, two.y) * scale;  // scale > 0; NaN if some score is, as the row's sum will be
-        // The weights may stand against an older maximum while they stay below 2^8: sums and results lose
+        // The weights may stand against an older maximum while they stay below 2^(ROOM + LAG): sums and results lose
         // nothing by that, and the results are rescaled seldom.  A row's own scores alone decide about it, so that no
         // other row's keys show in its bits.
-        const bool grows = most > top + 8.0f;
+        const bool grows = most - top > ROOM + LAG;
         if (__any(grows)) {
-            const float fade = grows ? __builtin_amdgcn_exp2f(top - most) : 1.0f;
-            top = grows ? most : top;
+            const float now = most - ROOM, fade = grows ? __builtin_amdgcn_exp2f(top - now) : 1.0f;
+            top = grows ? now : top;
             sum *= fade;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)

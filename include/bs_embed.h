@@ -19,7 +19,8 @@
  *   - inputs are not written; outputs must not overlap inputs or the workspace, except where
  *     an entry says so.
  *   - sums, row statistics, softmax maxima and sums are float32; results are rounded once, to
- *     the nearest value of their type.  Two calls on the same inputs give the same bits.
+ *     the nearest value of their type (attention rounds its weights too, see there).  Two calls
+ *     on the same inputs give the same bits.
  */
 #ifndef BS_EMBED_H
 #define BS_EMBED_H
@@ -79,6 +80,10 @@ int bs_linear_workspace(uint64_t rows, uint32_t inner, uint32_t cols, uint64_t* 
  *   for j < nk, and if causal, j <= i + nk - nq (the last query sees the last key).
  *   out = sum_j p_j v_j,  p = softmax over the visible keys of scale * (q . k_j)
  *   lse (float32, q_tokens x heads, or NULL) = log of the sum of exp(scale * (q . k_j))
+ * The weights exp(..) are rounded to `type` for their product with the values; their sum, which
+ * divides it, and lse take them as they are.  So out is off by up to 2^-9 (BS_BF16) or 2^-12
+ * (BS_F16) of sum_j p_j |v_j| besides its own rounding, and in BS_F16 by 2^-32 of
+ * max_j p_j sum_j |v_j|.
  * A query that sees no key gets out 0 and lse -infinity.  Keys and values that a query does not
  * see never touch its result, NaN and infinities included.  Tokens outside every sequence are
  * neither read nor written.  Offsets are read on the device, and ones that are not ascending or

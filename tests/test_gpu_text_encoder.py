@@ -689,3 +689,35 @@ def test_attention_of_rows_far_apart_never_touches_what_a_query_does_not_see(gpu
         v[tokens - hidden] = bad
         got = embed.attention(q, k, v, offsets([4]), offsets([tokens]))
         assert torch.equal(got[:4 - hidden], good[:4 - hidden]) and not torch.isfinite(got[4 - hidden:]).any()
+
+
+# ---------------------------------------------------------------- float16 weights far below the largest
+
+def check_float16_weights(q, k, v, nq, nk, causal, scale, out):
+    """as check_attention, but for the weights: those under float16's normal range are off by 2^-32 of the row's largest"""
+    dim = q.shape[2]
+    wo, _, size, total, spread, count = attention_definition(q, k, v, nq, nk, causal, scale)
+    d = (dim + 6) * E * spread + 4 * E * (spread + 1)
+    near(out, wo, (U[F16] + 4 * d + (count + 40) * E)[..., None] * size + 2.0 ** -32 * total + U[F16] * wo.abs() + TINY[F16])
+
+
+@pytest.mark.parametrize("where", ["first", "last", "middle"])
+@pytest.mark.parametrize("below", [14.6, 20.375, 23.6, 26.0, 28.3])
+@pytest.mark.parametrize("nq,nk", [(1, 3000), (24, 3000), (200, 500), (1, 40)])
+def test_attention_of_many_small_weights(gpu, nq, nk, below, where):
+    """one key has 2^below times the weight of every other; the others' values are large"""
+    k, v = torch.zeros(nk, 1, 8, dtype=F16), torch.full((nk, 1, 8), 512.0, dtype=F16)
+    v[:, 0, 1::2] = rand(120, nk, 4, dtype=F16, std=300.0).cpu()
+    k[:, 0, 0] = -below
+    heavy = {"first": 0, "last": nk - 1, "middle": nk // 2 + 3}[where]
+    k[heavy], v[heavy] = 0.0, 0.0
+    k, v, q = k.cuda(), v.cuda(), torch.ones(nq, 2, 8, dtype=F16, device="cuda")
+    out = embed.attention(q, k, v, offsets([nq]), offsets([nk]), causal=False, scale=math.log(2.0))
+    check_float16_weights(q, k, v, [nq], [nk], False, math.log(2.0), out)
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv,dim,std", [([200], [200], 4, 2, 64, 1.0), ([1, 1], [3000, 700], 8, 2, 128, 2.0), ([70, 33], [300, 33], 2, 1, 32, 3.0)])
+def test_attention_of_float16_weights(gpu, nq, nk, heads, kv, dim, std):
+    q, k, v = rand(121, sum(nq), heads, dim, dtype=F16, std=std), rand(122, sum(nk), kv, dim, dtype=F16), rand(123, sum(nk), kv, dim, dtype=F16)
+    out = embed.attention(q, k, v, offsets(nq), offsets(nk))
+    check_float16_weights(q, k, v, nq, nk, True, dim ** -0.5, out)

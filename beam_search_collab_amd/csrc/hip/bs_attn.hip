@@ -174,13 +174,19 @@ struct Rows {
     // The weights are rounded to the values' type for their product (the sum takes them as they are), since two 16-bit
     // products a score, of a weight's upper and lower bits, would double the matrix work.  float16 has nothing below 2^-24,
     // where many small weights beside a large one would be lost: there the largest weight stands at 2^7, and may grow to
-    // 2^11 before the row is rescaled.  (Its largest value is 2^16; 2^4 are left for scores so large that float32 has them
-    // in steps of up to 8.)  A weight is then off by 2^-32 of the row's largest at most.
+    // 2^11 before the row is rescaled.  (Its largest value is 2^16; the rest is for scores so large that float32 has them
+    // in steps of up to 4.)  A weight is then off by 2^-32 of the row's largest at most.
+    // A weight is exp2(score * scale - top) with one rounding, so scores and the top, which is rounded, may differ by half a
+    // step of the top.  Where steps are 8 and more that could be any weight: rows so `far` have their scores rounded alike and
+    // the top taken off first, in the branch that rescales (in one of its own: documents 1124 us instead of 1006).
+    bool far;  // some row of the wave is
+    __device__ static bool is_far(float top) { return fabsf(top) >= 0x1p26f && fabsf(top) < INFINITY; }
     static constexpr float ROOM = std::is_same<T, f16>::value ? 7.0f : 0.0f, LAG = std::is_same<T, f16>::value ? 4.0f : 8.0f;
 
     __device__ void clear() {
         top = NONE;
         sum = 0.0f;
+        far = false;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
     }
@@ -269,7 +275,8 @@ struct Rows {
         // nothing by that, and the results are rescaled seldom.  A row's own scores alone decide about it, so that no
         // other row's keys show in its bits.
         const bool grows = most - top > ROOM + LAG;
-        if (__any(grows)) {
+        float base = top;
+        if (__any(grows) || far) {
             const float now = most - ROOM, fade = grows ? __builtin_amdgcn_exp2f(top - now) : 1.0f;
             top = grows ? now : top;
             sum *= fade;
@@ -277,8 +284,18 @@ struct Rows {
             for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[d][r] *= fade;
+            far = __any(is_far(top));
+            base = top;
+            if (far) {
+                const float by = is_far(top) ? scale : 1.0f, off = is_far(top) ? top : 0.0f, back = 1.0f / by;
+                base = is_far(top) ? 0.0f : top;
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x.z[b][r] = (x.z[b][r] * by - off) * back;
+            }
         }
-        const float base = top == NONE ? 0.0f : top;  // nothing visible yet: every weight is exp2(-inf) = 0
+        base = base == NONE ? 0.0f : base;  // nothing visible yet: every weight is exp2(-inf) = 0
         float add[4] = {};
 #pragma unroll
         for (int b = 0; b < KB; ++b)

@@ -721,3 +721,27 @@ def test_attention_of_float16_weights(gpu, nq, nk, heads, kv, dim, std):
     q, k, v = rand(121, sum(nq), heads, dim, dtype=F16, std=std), rand(122, sum(nk), kv, dim, dtype=F16), rand(123, sum(nk), kv, dim, dtype=F16)
     out = embed.attention(q, k, v, offsets(nq), offsets(nk))
     check_float16_weights(q, k, v, nq, nk, True, dim ** -0.5, out)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("nq,nk", [(1, 1), (1, 70), (3, 3), (40, 130), (1, 2000)])
+@pytest.mark.parametrize("dtype,a,b", [(t, a, b) for t in (F16, BF16) for a, b in ((3 * 2.0 ** 9, 5 * 2.0 ** 8), (7 * 2.0 ** 9, 11 * 2.0 ** 10), (13 * 2.0 ** 11, 11 * 2.0 ** 11),
+                                                                                  (3 * 2.0 ** 14, 5 * 2.0 ** 13))]
+                         + [(BF16, 3 * 2.0 ** 20, 19 * 2.0 ** 19), (BF16, 3 * 2.0 ** 40, 37 * 2.0 ** 41)])
+def test_attention_of_huge_scores(gpu, dtype, a, b, nq, nk, sign):
+    """scores so large that float32 has them in steps of one and more: equal ones have equal weights all the same, and what
+    lies below them has none"""
+    dim = 16
+    q, k = torch.full((nq, 2, dim), a, dtype=dtype, device="cuda"), torch.full((nk, 1, dim), sign * b, dtype=dtype, device="cuda")
+    v = rand(124, nk, 1, dim, dtype=dtype)
+    even = torch.arange(nk, device="cuda") % 2 == 0
+    for some in (False, True):
+        if some:  # every other key scores less by 2^-7 of it and more
+            k[~even] *= 1 - sign * 2.0 ** -5
+        out, lse = embed.attention(q, k, v, offsets([nq]), offsets([nk]), causal=False, scale=1.0, lse=True)
+        use = v[even].double() if some else v.double()
+        want, size = use.mean(0), use.abs().mean(0)
+        tol = (U[dtype] + (nk + 40) * E) * size + U[dtype] * want.abs() + TINY[dtype]
+        near(out, want.expand(nq, 2, dim), tol.expand(nq, 2, dim))
+        top = torch.full((nq, 2), sign * dim * a * b, dtype=torch.float64) + math.log(len(use))
+        near(lse, top, 8 * E * top.abs() + (nk / 32 + 40) * E)

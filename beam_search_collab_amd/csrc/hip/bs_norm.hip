@@ -61,11 +61,27 @@ __device__ inline void store_cols(S* p, int cols, const float (&in)[Cols<T, NV, 
     }
 }
 
-// mean and sum of squared differences over the row, from the parts of its waves.  A wave takes
-// its own mean first (two passes over registers), so nothing cancels however far the mean lies
-// from zero; parts are joined as  M2 = sum(M2_w + n_w (mean_w - mean)^2).
+// The sums of two values over the wave at the price of one: the lower half of the lanes adds up the first, the upper half the
+// second, as the first exchange leaves them.
+__device__ inline void both_sums(float& a, float& b) {
+    const bool low = (threadIdx.x & 63) < 32;
+    float v = (low ? a : b) + __shfl_xor(low ? b : a, 32);
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) v += __shfl_xor(v, m);
+    a = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 0));
+    b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 32));
+}
+
+// Statistics of a row, whose values become their differences from a mean of the wave's own columns.  That mean is off by
+// the roundings of a sum of large values where the row lies far from zero; the mean c of the differences corrects it:
+// mean = m + c, M2 = sum of d^2 - n c^2.  So neither the variance nor what is normalised, d - off, loses more than the
+// roundings of differences, however far the mean lies from zero.  (At 1000 +- 0.001 and 512 columns the first mean alone is
+// off by 0.05 deviations.)  Waves' parts are joined about the first one's mean, M2 = sum(M2_w + n_w (mean_w - mean)^2).
+struct Stats {
+    float mean, off, m2;
+};
 template <typename T, int NV, int W>
-__device__ inline void row_stats(const float (&x)[Cols<T, NV, W>::E], int cols, float2* part, float& mean, float& m2) {
+__device__ inline Stats row_stats(int cols, float4* part, float (&x)[Cols<T, NV, W>::E]) {
     using C = Cols<T, NV, W>;
     const int wave = W == 1 ? 0 : threadIdx.x >> 6;
     float s = 0.0f;
@@ -73,31 +89,42 @@ __device__ inline void row_stats(const float (&x)[Cols<T, NV, W>::E], int cols, 
     for (int i = 0; i < C::E; ++i) s += x[i];  // 0 past the row
     s = wave_sum(s);
     const int mine = C::held(wave, cols);
-    mean = mine > 0 ? s / static_cast<float>(mine) : 0.0f;
-    float q = 0.0f;
+    const float over = mine > 0 ? 1.0f / static_cast<float>(mine) : 0.0f, m = s * over;  // the same for all rows
+    float q = 0.0f, e = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = C::col(i);
 #pragma unroll
         for (int j = 0; j < C::N; ++j) {
-            const float d = c + j < cols ? x[i * C::N + j] - mean : 0.0f;
+            const float d = c + j < cols ? x[i * C::N + j] - m : 0.0f;
+            x[i * C::N + j] = d;
+            e += d;
             q = fmaf(d, d, q);
         }
     }
-    m2 = wave_sum(q);
+    both_sums(e, q);
+    const bool fine = fabsf(e) < INFINITY;  // else m, which is not finite either, is the mean
+    const float c = fine ? e * over : 0.0f, m2 = fine ? fmaf(-e, c, q) : q;
+    Stats r{m + c, c, m2 < 0.0f ? 0.0f : m2};
     if (W > 1) {
-        if ((threadIdx.x & 63) == 0) part[wave] = make_float2(s, m2);
+        if ((threadIdx.x & 63) == 0) part[wave] = make_float4(m, c, r.m2, 0.0f);
         __syncthreads();
-        float total = 0.0f;
-        for (int w = 0; w < W; ++w) total += part[w].x;
-        mean = total / static_cast<float>(cols);
-        m2 = 0.0f;
+        const float m0 = part[0].x;
+        float t = 0.0f;
+        for (int w = 0; w < W; ++w) t = fmaf(static_cast<float>(C::held(w, cols)), (part[w].x - m0) + part[w].y, t);
+        t /= static_cast<float>(cols);
+        r = Stats{m0 + t, t - (m - m0), 0.0f};
         for (int w = 0; w < W; ++w) {
-            const int n = C::held(w, cols);
-            const float d = n > 0 ? part[w].x / static_cast<float>(n) - mean : 0.0f;
-            m2 += fmaf(static_cast<float>(n) * d, d, part[w].y);
+            const int k = C::held(w, cols);
+            const float d = k > 0 ? ((part[w].x - m0) + part[w].y) - t : 0.0f;
+            r.m2 += fmaf(static_cast<float>(k) * d, d, part[w].z);
+        }
+        if (!(fabsf(t) < INFINITY)) {  // some wave's mean is not finite
+            r.mean = 0.0f;
+            for (int w = 0; w < W; ++w) r.mean += C::held(w, cols) > 0 ? part[w].x : 0.0f;
         }
     }
+    return r;
 }
 
 template <typename T, typename WT, int NV, int W>
@@ -105,7 +132,7 @@ __global__ __launch_bounds__((Cols<T, NV, W>::THREADS)) void norm_kernel(const T
                                                                         float eps, T* y, int64_t ys, float* mean_out,
                                                                         float* rstd_out, uint64_t rows, int cols) {
     using C = Cols<T, NV, W>;
-    __shared__ float2 part[2][W];
+    __shared__ float4 part[2][W];
     float w[C::E], b[C::E], v[C::E];
     if (weight) {
         load_cols<T, NV, W>(weight, cols, w);
@@ -123,14 +150,13 @@ __global__ __launch_bounds__((Cols<T, NV, W>::THREADS)) void norm_kernel(const T
     int turn = 0;
     for (uint64_t r = static_cast<uint64_t>(blockIdx.x) * C::ROWS + (C::ROWS > 1 ? threadIdx.x >> 6 : 0); r < rows; r += step, turn ^= 1) {
         load_cols<T, NV, W>(x + static_cast<int64_t>(r) * xs, cols, v);
-        float mean, m2;
-        row_stats<T, NV, W>(v, cols, part[turn], mean, m2);
-        const float rstd = 1.0f / sqrtf(m2 / static_cast<float>(cols) + eps);
+        const Stats st = row_stats<T, NV, W>(cols, part[turn], v);
+        const float rstd = 1.0f / sqrtf(st.m2 / static_cast<float>(cols) + eps);
 #pragma unroll
-        for (int i = 0; i < C::E; ++i) v[i] = fmaf((v[i] - mean) * rstd, w[i], b[i]);
+        for (int i = 0; i < C::E; ++i) v[i] = fmaf(fmaf(v[i], rstd, -st.off * rstd), w[i], b[i]);
         store_cols<T, NV, W>(y + static_cast<int64_t>(r) * ys, cols, v);
         if (C::lane() == 0) {
-            if (mean_out) mean_out[r] = mean;
+            if (mean_out) mean_out[r] = st.mean;
             if (rstd_out) rstd_out[r] = rstd;
         }
     }
@@ -290,8 +316,10 @@ struct Forward {
     void go() const {
         using C = Cols<T, NV, W>;
         // weights are loaded once per workgroup, so they stay for many rows; 2 / 4 / 8 / 16 per compute unit:
-        // 65536 x 768: 57 / 39 / 40 / 42 us, 32768 x 4096: 144 / 103 / 104 / 104, 8192 x 16384: 129 / 131 / 139 / 147
-        const uint64_t want = (rows + C::ROWS - 1) / C::ROWS, most = CUS * (W == 8 ? 4 : 8);
+        // 65536 x 768: 57 / 39 / 40 / 42 us, 32768 x 4096: 144 / 103 / 104 / 104, 8192 x 16384: 129 / 131 / 139 / 147.
+        // Six where six fit at a time (by registers, 16 columns of 16 bits a lane), so that all have the same number of rows:
+        // 65536 x 1024 47.3 us, with four 47.6, with eight 51.2; 65536 x 768 in another run 39.8, with eight 43.1
+        const uint64_t want = (rows + C::ROWS - 1) / C::ROWS, most = CUS * (W == 8 ? 4 : W == 1 && C::E == 16 && sizeof(T) == 2 ? 6 : 8);
         norm_kernel<T, WT, NV, W><<<static_cast<uint32_t>(want < most ? want : most), C::THREADS, 0, s>>>(
             static_cast<const T*>(x), xs, static_cast<const WT*>(weight), static_cast<const WT*>(bias), eps, static_cast<T*>(y), ys,
             mean, rstd, rows, cols);

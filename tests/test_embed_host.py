@@ -144,3 +144,23 @@ def test_python_refuses_tensors_off_the_gpu():
         embed.linear(x.float(), x.float())
     with pytest.raises(ValueError, match="x must be"):
         embed.layer_norm(x.double())
+
+
+def test_the_check_of_norms_far_from_zero_rejects_mistakes():
+    """planted in a norm in 32 bits on the CPU, at the inputs of the GPU's test"""
+    import torch
+    from test_gpu_text_encoder import FAR, check_norm_far, far_rows
+    for mean, std in FAR:
+        x = far_rows(130, 5, 960, mean, std)
+        m = x.double().mean(1)
+        c = (x.double() - m[:, None]).float()
+        r = (1 / torch.sqrt(c.double().square().mean(1) + 1e-5)).float()
+        y = c * r[:, None]
+        check_norm_far(x, None, None, 1e-5, y, m.float(), r)
+        cancelled = (1 / torch.sqrt((x.square().mean(1) - x.mean(1).square()).clamp_min(0) + 1e-5))
+        shifted = m.float() + 20 * 2.0 ** -24 * abs(mean)  # as a sum of 20 roundings may be
+        for wrong in ((0 * y, m.float(), r), (-y, m.float(), r), (y * 1.001, m.float(), r), (y, m.float(), r * 1.001), (y, m.float(), 0 * r),
+                      (c * cancelled[:, None], m.float(), cancelled), ((x - shifted[:, None]) * r[:, None], m.float(), r),
+                      (y, shifted, r)):
+            with pytest.raises(AssertionError):
+                check_norm_far(x, None, None, 1e-5, *wrong)

@@ -745,3 +745,56 @@ def test_attention_of_huge_scores(gpu, dtype, a, b, nq, nk, sign):
         near(out, want.expand(nq, 2, dim), tol.expand(nq, 2, dim))
         top = torch.full((nq, 2), sign * dim * a * b, dtype=torch.float64) + math.log(len(use))
         near(lse, top, 8 * E * top.abs() + (nk / 32 + 40) * E)
+
+
+# ---------------------------------------------------------------- layer norm far from zero
+
+FAR = [(1000.0, 1e-3), (100.0, 0.05), (-1e4, 1.0), (3e5, 0.5)]  # mean and spread
+
+
+def check_norm_far(x, w, b, eps, y, mean, rstd):
+    """for a mean that is corrected by the mean of the differences from it, as check_norm is for one that is not.  The first
+    mean is off by 40 additions' roundings, `off`; all that follows is computed on differences, of at most dev + off"""
+    wy, wm, wr = norm_definition(x, w, b, eps)
+    xd = x.double()
+    off = 40 * E * xd.abs().amax(-1)
+    dev = (xd - wm[..., None]).abs().amax(-1)
+    tm = 80 * E * (dev + off)  # 41 additions of differences, 12 roundings where the waves' means (2 dev + 3 off apart) are joined
+    near(mean, wm, tm + E * wm.abs())
+    # the variance: 64 roundings of squares up to var + 3 off^2; the root halves their part
+    rel = 36 * E * (1 + 3 * (off * wr) ** 2) + (tm * wr) ** 2
+    near(rstd, wr, rel * wr)
+    ww = 1.0 if w is None else w.double().abs()
+    tol = ww * ((tm * wr)[..., None] + (rel + 6 * E)[..., None] * (xd - wm[..., None]).abs() * wr[..., None])
+    if b is not None:
+        tol = tol + 2 * E * b.double().abs()
+    near(y, wy, tol + (U[y.dtype] + 2 * E) * wy.abs() + TINY[y.dtype])
+
+
+def far_rows(seed, rows, cols, mean, std, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    offset = torch.randn(cols, generator=g) * std  # features that differ in their means, and so do the waves' columns
+    return (torch.randn(rows, cols, generator=g) * std + offset + mean).to(dtype)
+
+
+@pytest.mark.parametrize("mean,std", FAR)
+@pytest.mark.parametrize("cols", [1, 64, 512, 960, 1100, 2048, 4100, 16384])
+def test_layer_norm_far_from_zero(gpu, mean, std, cols):
+    x, w, b = far_rows(130, 5, cols, mean, std).cuda(), rand(131, cols), rand(132, cols)
+    for eps in (1e-5, 1e-12 if cols > 1 else 1e-5):
+        y, m, r = embed.layer_norm(x, w, b, eps=eps, stats=True)
+        check_norm_far(x, w, b, eps, y, m, r)
+
+
+@pytest.mark.parametrize("cols", [100, 1000, 3000, 10000])
+def test_layer_norm_of_constant_and_not_finite_rows(gpu, cols):
+    """a constant row has variance 0 whatever the roundings of its sum; statistics of rows that are not finite stay what
+    they are by definition"""
+    x = torch.full((5, cols), 0.1, device="cuda") * torch.tensor([1.0, 1e4, -3e-5, 7.7, 1e-30], device="cuda")[:, None]
+    y, mean, rstd = embed.layer_norm(x, eps=1e-10, stats=True)
+    check_norm_far(x, None, None, 1e-10, y, mean, rstd)
+    x = rand(133, 5, cols)
+    x[0, cols - 1], x[1, 0], x[2, cols // 2] = math.inf, -math.inf, math.nan
+    y, mean, rstd = embed.layer_norm(x, stats=True)
+    assert mean[0] == math.inf and mean[1] == -math.inf and torch.isnan(mean[2]) and torch.isnan(rstd[:3]).all()
+    assert torch.isnan(y[:3]).all() and torch.isfinite(y[3:]).all()

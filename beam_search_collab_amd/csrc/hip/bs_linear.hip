@@ -690,7 +690,9 @@ int check(const char* what, uint64_t rows, uint32_t inner, uint32_t cols) {
     const std::string w = what;
     if (rows > 0x7FFFFFFFull) return refuse(w + ": rows must be < 2^31");
     if (inner == 0 || inner > (1u << 24) || cols == 0 || cols > (1u << 24)) return refuse(w + ": inner and cols must be in 1..2^24");
-    if (((rows + 63) >> 6) * ((cols + 63) >> 6) > 0x7FFFFFFFull) return refuse(w + ": rows x cols is too large for one launch");
+    // A grid of 2^32 threads is cut short without an error.  Tiles of 256 x 128 by 512 threads and of 128 x 128 by 256 have the
+    // most; smaller ones run where those are few.
+    if ((rows + 255) / 256 * 512 * ((cols + 127) / 128) > 0xFFFFFFFFull) return refuse(w + ": rows x cols is too large for one launch");
     return BS_OK;
 }
 

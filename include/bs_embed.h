@@ -63,8 +63,8 @@ int bs_layer_norm_backward_workspace(uint64_t rows, uint32_t cols, int type, uin
 
 /* out = act(x w^T + bias) + residual:  x rows x inner, w cols x inner, bias cols, all of `type`
  * (BS_F16 or BS_BF16); residual and out rows x cols of out_type (`type` or BS_F32).  bias and
- * residual may be NULL; residual may be out itself with its stride.  rows < 2^31, inner and
- * cols 1..2^24, strides < 2^24.  Products are summed in float32.  workspace:
+ * residual may be NULL; residual may be out itself with its stride.  rows x ceil(cols / 128) up
+ * to 2^31 - 256, inner and cols 1..2^24, strides < 2^24.  Products are summed in float32.  workspace:
  * bs_linear_workspace bytes (0 where the call does not split the inner dimension), 16-byte
  * aligned. */
 int bs_linear(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* bias, const void* residual,

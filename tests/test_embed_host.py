@@ -164,3 +164,17 @@ def test_the_check_of_norms_far_from_zero_rejects_mistakes():
                       (y, shifted, r)):
             with pytest.raises(AssertionError):
                 check_norm_far(x, None, None, 1e-5, *wrong)
+
+
+@pytest.mark.parametrize("rows,inner,cols", [((1 << 31) - 1, 1, 1), ((1 << 31) - 255, 8, 128), ((1 << 30) + 1, 1, 129), (1 << 26, 1, 1 << 13)])
+def test_linear_refuses_launches_of_2_to_the_32_threads(rows, inner, cols):
+    """a grid of 2^32 threads is cut short without an error"""
+    n = C.c_uint64(0)
+    refused(_lib.hip().bs_linear_workspace(rows, inner, cols, C.byref(n)), "too large for one launch")
+    refused(_lib.hip().bs_linear(PTR, inner, PTR, inner, None, None, 0, PTR, cols, rows, inner, cols, 2, 2, 0, None, 0, None), "too large for one launch")
+
+
+def test_linear_takes_as_many_rows_as_a_launch_has():
+    n = C.c_uint64(1)
+    for rows, cols in (((1 << 31) - 256, 1), ((1 << 30) - 256, 256), (32, 1 << 24)):
+        assert _lib.hip().bs_linear_workspace(rows, 8, cols, C.byref(n)) == 0

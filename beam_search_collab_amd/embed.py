@@ -10,6 +10,8 @@ They take and return torch tensors on the GPU and run on torch's current stream,
 result can go to GPUGraph.search_device on the same stream without a copy or a wait.  Every call goes
 through libbs_hip.so (include/bs_embed.h); wrong arguments raise ValueError.  The features of a row are
 contiguous, rows may lie any distance apart (slices of a wider tensor are taken as they are).
+Autograd does not see the calls: tensors that require a gradient are refused while it records, and taken
+under torch.no_grad(); layer_norm_backward is called by hand or from a torch.autograd.Function.
 Workspaces and results come from torch's allocator, so the calls can be captured in a torch.cuda.graph.
 """
 from __future__ import annotations
@@ -32,6 +34,8 @@ __all__ = ["attention", "layer_norm", "layer_norm_backward", "linear", "ACTIVATI
 
 # the current stream's handle: torch.cuda.current_stream() makes an object for it (2.9 us a call against 0.1)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_device = torch._C._cuda_getDevice  # as torch.cuda.current_device, without its look at whether CUDA is initialised
+_recording = torch.is_grad_enabled
 
 
 def _fail(message):
@@ -39,15 +43,22 @@ def _fail(message):
 
 
 def _gpu(what: str, x: torch.Tensor, *tensors) -> int:
-    """the GPU that all tensors given are on, which must be the current one"""
+    """the GPU that all tensors given are on, which must be the current one; no gradient may be wanted of them"""
     dev = x.get_device()
+    grad = _recording()
+    lost = grad and x.requires_grad
+    for t in tensors:
+        if t is not None:
+            if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+                _fail(f"{what}: every argument must be a tensor on {x.device if dev >= 0 else 'a GPU'}, got {getattr(t, 'device', type(t))}")
+            if grad and t.requires_grad:
+                lost = True
+    if lost:
+        _fail(f"{what}: a tensor requires a gradient, which autograd would not get: call it under torch.no_grad() or with detached tensors")
     if dev < 0:
         _fail(f"{what}: the tensors must be on a GPU")
-    for t in tensors:
-        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != dev):
-            _fail(f"{what}: every argument must be a tensor on {x.device}, got {getattr(t, 'device', type(t))}")
-    if dev != torch.cuda.current_device():
-        _fail(f"{what}: the tensors are on {x.device}, the current device is {torch.cuda.current_device()}")
+    if dev != _device():
+        _fail(f"{what}: the tensors are on {x.device}, the current device is cuda:{_device()}")
     return dev
 
 

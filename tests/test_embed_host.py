@@ -178,3 +178,25 @@ def test_linear_takes_as_many_rows_as_a_launch_has():
     n = C.c_uint64(1)
     for rows, cols in (((1 << 31) - 256, 1), ((1 << 30) - 256, 256), (32, 1 << 24)):
         assert _lib.hip().bs_linear_workspace(rows, 8, cols, C.byref(n)) == 0
+
+
+def test_python_refuses_to_lose_a_gradient():
+    """autograd does not see these calls: a result without a gradient, from tensors that want one, would be a silent loss"""
+    import torch
+    from beam_search_collab_amd import embed
+    x, w, s = torch.zeros(4, 32, dtype=torch.bfloat16), torch.zeros(32, 32, dtype=torch.bfloat16), torch.zeros(4)
+    h = x[:, None]
+
+    def wants(t):
+        return t.detach().clone().requires_grad_()
+    calls = [lambda: embed.layer_norm(wants(x)), lambda: embed.layer_norm(x, wants(w[0])), lambda: embed.layer_norm(x, None, wants(w[0])),
+             lambda: embed.linear(x, wants(w)), lambda: embed.linear(x, w, wants(w[0])), lambda: embed.linear(x, w, residual=wants(x)),
+             lambda: embed.attention(wants(h), h, h), lambda: embed.attention(h, h, wants(h)),
+             lambda: embed.layer_norm_backward(x, x, s, s, wants(w[0])), lambda: embed.layer_norm_backward(wants(x), x, s, s)]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):  # goes on to the next check
+            call()
+        with torch.inference_mode(), pytest.raises(ValueError, match="on a GPU"):
+            call()

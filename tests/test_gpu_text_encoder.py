@@ -798,3 +798,16 @@ def test_layer_norm_of_constant_and_not_finite_rows(gpu, cols):
     y, mean, rstd = embed.layer_norm(x, stats=True)
     assert mean[0] == math.inf and mean[1] == -math.inf and torch.isnan(mean[2]) and torch.isnan(rstd[:3]).all()
     assert torch.isnan(y[:3]).all() and torch.isfinite(y[3:]).all()
+
+
+def test_tensors_that_require_a_gradient(gpu):
+    """refused while autograd records, else as others"""
+    x, w = rand(140, 5, 64, dtype=BF16), rand(141, 64, 64, dtype=BF16)
+    p = torch.nn.Parameter(w.clone())
+    for call in (lambda w: embed.layer_norm(x, w[0]), lambda w: embed.linear(x, w),
+                 lambda w: embed.attention(x[:, None], w[:5, None], x[:, None])):
+        with pytest.raises(ValueError, match="gradient"):
+            call(p)
+        with torch.no_grad():
+            assert torch.equal(call(p), call(w))
+        assert torch.equal(call(p.detach()), call(w))

@@ -811,3 +811,51 @@ def test_tensors_that_require_a_gradient(gpu):
         with torch.no_grad():
             assert torch.equal(call(p), call(w))
         assert torch.equal(call(p.detach()), call(w))
+
+
+# ---------------------------------------------------------------- on both sides of the rules that choose a kernel
+
+@pytest.mark.parametrize("rows,inner,cols", [
+    (256, 128, 36096), (256, 128, 35840), (256, 136, 36096), (256, 64, 36096),  # 141 and 140 tiles of 256; steps of 64 that are not whole, or one
+    (512, 72, 12288), (256, 72, 24448), (250, 200, 24449),  # 192 and 191 tiles of 256 x 128
+    (512, 96, 8192), (384, 96, 10880), (385, 100, 8191),  # 256 and 255 of 128; rows of x that are not 16-byte aligned
+    (64, 4096, 10880), (64, 4096, 10944), (33, 3071, 700), (33, 2047, 700), (40, 2049, 16384),  # pieces of the inner dimension
+    (32, 300, 8192), (32, 300, 8191), (16, 300, 8192), (17, 300, 100)])  # columns and rows of a workgroup of few rows
+def test_linear_on_both_sides_of_the_rules(gpu, rows, inner, cols):
+    x, w = rand(150, rows, inner, dtype=BF16), rand(151, cols, inner, dtype=BF16, std=inner ** -0.5)
+    b, r = rand(152, cols, dtype=BF16), rand(153, rows, cols, dtype=BF16)
+    got = embed.linear(x, w, b, activation="silu", residual=r)
+    check_linear(x, w, b, "silu", r, got)
+    assert torch.equal(got, embed.linear(x, w, b, activation="silu", residual=r))
+
+
+@pytest.mark.parametrize("rows,cols", [(8200, 96), (8193, 512), (6150, 1000), (6145, 520), (2060, 1100), (2049, 8192), (1030, 8193)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_of_more_rows_than_workgroups(gpu, rows, cols, dtype):
+    x, w, b, dy = (rand(154, rows, cols) * 1.5 + 0.7).to(dtype), rand(155, cols), rand(156, cols), rand(157, rows, cols, dtype=dtype)
+    y, mean, rstd = embed.layer_norm(x, w, b, stats=True)
+    check_norm(x, w, b, 1e-5, y, mean, rstd)
+    check_norm_far(x, w, b, 1e-5, y, mean, rstd)
+    check_backward(dy, x, mean, rstd, w, *embed.layer_norm_backward(dy, x, mean, rstd, w))
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv,dim", [([1] * 3, [300, 5, 900], 8, 1, 64), ([1] * 3, [300, 5, 900], 9, 1, 64), ([2, 1], [300, 500], 8, 1, 64),
+                                                ([100], [537], 4, 4, 64), ([100], [538], 4, 4, 64), ([256], [4000], 8, 8, 32), ([255], [4000], 8, 8, 32)])
+def test_attention_on_both_sides_of_the_rules(gpu, nq, nk, heads, kv, dim):
+    q, k, v = rand(160, sum(nq), heads, dim, dtype=BF16), rand(161, sum(nk), kv, dim, dtype=BF16), rand(162, sum(nk), kv, dim, dtype=BF16)
+    for causal in (True, False):
+        out, lse = embed.attention(q, k, v, offsets(nq), offsets(nk), causal=causal, longest_q=max(nq), longest_k=max(nk), lse=True)
+        wo, wl, size, total, spread = attention_on_gpu(q, k, v, nq, nk, causal, dim ** -0.5)
+        d, count = (dim + 6) * E * spread + 4 * E * (spread + 1), max(nk)
+        near(out, wo, (U[BF16] + 4 * d + (count + 40) * E)[..., None] * size + U[BF16] * wo.abs() + TINY[BF16])
+        near(lse, wl, 2 * d + (count / 32 + 40) * E + 4 * E * wl.abs())
+
+
+@pytest.mark.parametrize("stride", [(1 << 22) - 8, 1 << 22])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_attention_of_rows_farther_apart_than_a_move_reaches(gpu, stride, tokens):
+    q, k = rand(163, tokens, 4, 64, dtype=BF16), rand(164, 150, 2, 64, dtype=BF16)
+    v = torch.empty(150 * stride, dtype=BF16, device="cuda").as_strided((150, 2, 64), (stride, 64, 1))
+    v.copy_(rand(165, 150, 2, 64))
+    out, lse = embed.attention(q, k, v, offsets([tokens]), offsets([150]), lse=True)
+    check_attention(q, k, v.contiguous(), [tokens], [150], True, 0.125, out, lse)

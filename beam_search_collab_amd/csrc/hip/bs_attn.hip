@@ -176,9 +176,9 @@ struct Rows {
     // where many small weights beside a large one would be lost: there the largest weight stands at 2^7, and may grow to
     // 2^11 before the row is rescaled.  (Its largest value is 2^16; the rest is for scores so large that float32 has them
     // in steps of up to 4.)  A weight is then off by 2^-32 of the row's largest at most.
-    // A weight is exp2(score * scale - top) with one rounding, so scores and the top, which is rounded, may differ by half a
-    // step of the top.  Where steps are 8 and more that could be any weight: rows so `far` have their scores rounded alike and
-    // the top taken off first, in the branch that rescales (in one of its own: documents 1124 us instead of 1006).
+    // A weight is exp2(score * scale - top) with one rounding, while the top is rounded too: where float32 has steps of 8 and
+    // more, the largest weight could be anything up to 2^4 and more off.  Rows so `far` have scores and top rounded alike
+    // and subtracted first, in the branch that rescales (in a branch of its own: documents 1124 us instead of 1006).
     bool far;  // some row of the wave is
     __device__ static bool is_far(float top) { return fabsf(top) >= 0x1p26f && fabsf(top) < INFINITY; }
     static constexpr float ROOM = std::is_same<T, f16>::value ? 7.0f : 0.0f, LAG = std::is_same<T, f16>::value ? 4.0f : 8.0f;
@@ -498,10 +498,11 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 // run under a tile's products.  Two workgroups per compute unit (three for heads up to 64): one's matrix
 // instructions run under the other's exponentials.  (Three for heads of 64: passages below 90 to 83 us; four spill: 144.)
 //
-// Two causal documents of 8192 and 7500 tokens, 32 heads of 128, 8 key/value heads, bf16: 985 us (980 TFLOP/s), the
-// vector and matrix pipes half busy each (0.49, 0.47): a wave's exponentials and its products do not overlap, only two
-// waves' do.  96 passages of 37..512 tokens, 16 heads of 64: 68 us, bound by vector instructions (170 beside 16 matrix
-// instructions a tile, 270 with masks) and the latency of each workgroup's first loads.  Other orders that were slower for
+// Two causal documents of 8192 and 7500 tokens, 32 heads of 128, 8 key/value heads, bf16: 973 us (992 TFLOP/s), the
+// vector and matrix pipes half busy each (0.50, 0.47): a wave's exponentials and its products do not overlap, only two
+// waves' do.  96 passages of 37..512 tokens, 16 heads of 64: 69 us, the vector pipe busy for 0.43 of the time (170
+// instructions beside 16 matrix instructions a tile, 270 with masks) and waves waiting for 0.40 of theirs, on the four
+// dependent rounds of loads with which each of the 3864 short workgroups starts.  Other orders that were slower for
 // the documents: two groups of waves half a step apart, meeting between their phases (1244 against 1175), moves between
 // the products and exponentials instead of before them (1246 against 1142).
 template <typename T, int DP>

@@ -246,7 +246,8 @@ __global__ __launch_bounds__((Cols<T, NV, W>::THREADS)) void norm_backward_kerne
 }
 
 // Sums of the workgroups' parts, in order: a workgroup takes 64 columns, wave i the parts i, i + 16, ..  A wave's loads
-// wait for memory, so 16 are on their way at a time: 1024 parts of 2 x 4096 take 6.9 us, 18 with one at a time.
+// wait for memory, so 16 are on their way at a time: 1024 parts of 2 x 4096 take 6.9 us, 18 with one at a time.  What is left of
+// n past a multiple of 256 is loaded one at a time, so fewer parts can take longer: 250 of 2 x 960 6.4 us.
 template <typename WT>
 __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* parts, uint32_t n, int cols, WT* dweight, WT* dbias) {
     __shared__ float join[16][64];

@@ -256,7 +256,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: Opti
     before it one key less.  scale: head_dim ** -0.5 if None.  longest_q, longest_k: the longest
     sequences, if known (they choose how the work is split, not the result).  lse: returns (out,
     lse), lse (tokens, heads) float32 the log of the sum of the exponentials.  A query that sees no key
-    gets 0 and -inf.  out: where to write the result."""
+    gets 0 and -inf.  out: where to write the result.  Tokens past the last offset are in no sequence:
+    their rows of the result and of lse are not written and hold what was in that memory before."""
     what = "attention"
     type_ = q.dtype
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:

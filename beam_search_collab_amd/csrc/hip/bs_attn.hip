@@ -340,8 +340,10 @@ struct Rows {
 // A weight of 0 times NaN or an infinity is NaN, so a row would be touched by values that it does not see.  Where
 // the tiles that some row does not see whole give a result that is not finite, they are taken five times:
 // as they are, with 1 for every NaN (+infinity, -infinity) and 0 for the rest, and with 0 for what is not
-// finite.  The last pass gives the sums; NaN and infinities are added where their passes gave more than 0.
+// finite.  The last pass gives the sums; NaN and infinities are added where their passes gave more than 0.  Those passes take
+// every key that is seen about alike, for its weight may be too small for its type.
 enum { PLAIN = 0, NANS = 1, HIGH = 2, LOW = 3, FINITE = 4 };
+__device__ inline float scale_of(int pass, float scale) { return pass == PLAIN || pass == FINITE ? scale : 0x1p-126f; }
 
 // the values of keys that no row of the tile sees -- later ones of the sequence, and what lies past its end, for which the
 // moves repeat its last one: no weight of 0 meets NaN there
@@ -567,7 +569,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
             }
 #pragma unroll 1
             for (int b = 0; b < BN; b += KB * 32)
-                if (reach > start(t) + b) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, start(t) + b, mine, scale, lane);
+                if (reach > start(t) + b) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, start(t) + b, mine, scale_of(pass, scale), lane);
         }
         if (pass == PLAIN) {
             if (seen == all) break;  // all rows see the same keys, and the others' values are blank
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
                 sift<T>(tk + TILE, TILE, pass, lane, 64);
                 landed<63>();
             }
-            me_.template step<1, true>(tk, tk + TILE, j0, mine, scale, lane);
+            me_.template step<1, true>(tk, tk + TILE, j0, mine, scale_of(pass, scale), lane);
             if (pass == PLAIN) {
                 // all rows see the same keys, and the others' values are blank; or nothing is there to touch them
                 if (seen == all || !__any(me_.odd())) break;

@@ -859,3 +859,19 @@ def test_attention_of_rows_farther_apart_than_a_move_reaches(gpu, stride, tokens
     v.copy_(rand(165, 150, 2, 64))
     out, lse = embed.attention(q, k, v, offsets([tokens]), offsets([150]), lse=True)
     check_attention(q, k, v.contiguous(), [tokens], [150], True, 0.125, out, lse)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype,below", [(F16, 20.0), (F16, 45.0), (F16, 110.0), (BF16, 45.0), (BF16, 160.0)])
+@pytest.mark.parametrize("nq,nk,heads,kv", [(40, 40, 2, 1), (5, 30, 2, 2), (3, 150, 4, 1)])
+def test_attention_shows_values_that_a_query_sees_however_small_their_weight(gpu, bad, dtype, below, nq, nk, heads, kv):
+    """a weight is more than 0 for every key that is seen; 2^-below here"""
+    k = torch.zeros(nk, kv, 32, dtype=dtype, device="cuda")
+    hidden = 2  # the last queries only see it
+    k[nk - hidden, :, 0] = -below
+    v = rand(170, nk, kv, 32, dtype=dtype)
+    q = torch.ones(nq, heads, 32, dtype=dtype, device="cuda")
+    good = embed.attention(q, k, v, offsets([nq]), offsets([nk]), scale=math.log(2.0))
+    v[nk - hidden] = bad
+    got = embed.attention(q, k, v, offsets([nq]), offsets([nk]), scale=math.log(2.0))
+    assert torch.equal(got[:nq - hidden], good[:nq - hidden]) and not torch.isfinite(got[nq - hidden:]).any()

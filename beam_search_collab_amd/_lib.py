@@ -65,6 +65,18 @@ class AttentionArgs(C.Structure):
     )
 
 
+class HeadNormRotaryArgs(C.Structure):
+    """bs_head_norm_rotary_args (include/bs_embed.h)."""
+    _fields_ = (
+        [(n, vp) for n in ("q", "k", "q_grad", "k_grad", "q_out", "k_out", "q_weight", "k_weight", "q_weight_grad",
+                           "k_weight_grad", "positions", "frequencies")]
+        + [(n + e, i64) for n in ("q", "k", "q_grad", "k_grad", "q_out", "k_out") for e in ("_stride", "_head_stride")]
+        + [(n, u32) for n in ("tokens", "heads", "kv_heads", "head_dim", "rotary")]
+        + [(n, i32) for n in ("interleaved", "norm", "type", "wtype")]
+        + [("eps", f32), ("magnitude", f32)]
+    )
+
+
 # name -> (restype, argtypes)
 HIP_API = {
     "bs_index_create": (C.c_int, [vp, vp, u64, u32, u32, P(vp)]),
@@ -107,6 +119,9 @@ EMBED_API = {
     "bs_linear_workspace": (C.c_int, [u64, u32, u32, P(u64)]),
     "bs_attention": (C.c_int, [P(AttentionArgs), vp, u64, vp]),
     "bs_attention_workspace": (C.c_int, [P(AttentionArgs), P(u64)]),
+    "bs_head_norm_rotary": (C.c_int, [P(HeadNormRotaryArgs), vp]),
+    "bs_head_norm_rotary_backward": (C.c_int, [P(HeadNormRotaryArgs), vp, u64, vp]),
+    "bs_head_norm_rotary_backward_workspace": (C.c_int, [P(HeadNormRotaryArgs), P(u64)]),
 }
 
 HOST_API = {

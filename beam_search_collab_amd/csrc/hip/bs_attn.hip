@@ -34,17 +34,6 @@ constexpr int BN = 64;  // keys of a tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 constexpr float NONE = -INFINITY;
 
-// n / d for n < 2^31 and one d: floor(n m / 2^(31 + s)) with s = ceil(log2 d), m = ceil(2^(31 + s) / d) < 2^32.  (m d -
-// 2^(31 + s) < d <= 2^s, so the quotient is off by less than n / 2^31 / d and never reaches the next integer.)
-struct Divisor {
-    uint32_t m, s;
-    Divisor(uint32_t d = 1) : m(0), s(0) {
-        while ((1ull << s) < d) ++s;
-        m = static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d);
-    }
-    __device__ uint32_t quotient(uint32_t n) const { return __umulhi(n << 1, m) >> s; }
-};
-
 struct Params {
     bs_attention_args a;
     uint32_t group;    // heads per key/value head

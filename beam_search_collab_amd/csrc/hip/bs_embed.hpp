@@ -101,6 +101,17 @@ __device__ inline void move16(const char* base, uint32_t offset, void* to) {
     __builtin_amdgcn_global_load_lds((global_ptr)(reinterpret_cast<const char*>(b) + offset), (lds_ptr)to, 16, 0, 0);
 }
 
+// n / d for n < 2^31 and one d: floor(n m / 2^(31 + s)) with s = ceil(log2 d), m = ceil(2^(31 + s) / d) < 2^32.  (m d -
+// 2^(31 + s) < d <= 2^s, so the quotient is off by less than n / 2^31 / d and never reaches the next integer.)
+struct Divisor {
+    uint32_t m, s;
+    Divisor(uint32_t d = 1) : m(0), s(0) {
+        while ((1ull << s) < d) ++s;
+        m = static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d);
+    }
+    __device__ uint32_t quotient(uint32_t n) const { return __umulhi(n << 1, m) >> s; }
+};
+
 // sum over the 64 lanes, the same bits in every lane
 __device__ inline float wave_sum(float v) {
 #pragma unroll

@@ -5,18 +5,21 @@
     z = embed.linear(y, w, b, activation="gelu", residual=None)
     o = embed.attention(q, k, v, offsets, causal=True)
     dx, dweight, dbias = embed.layer_norm_backward(dy, x, mean, rstd, weight)
+    q, k = embed.head_norm_rotary(q, k, positions, frequencies, q_weight, k_weight)
+    dq, dk, dq_weight, dk_weight = embed.head_norm_rotary_backward(dq, dk, q, k, positions, frequencies, q_weight, k_weight)
 
 They take and return torch tensors on the GPU and run on torch's current stream, so that a float32
 result can go to GPUGraph.search_device on the same stream without a copy or a wait.  Every call goes
 through libbs_hip.so (include/bs_embed.h); wrong arguments raise ValueError.  The features of a row are
 contiguous, rows may lie any distance apart (slices of a wider tensor are taken as they are).
 Autograd does not see the calls: tensors that require a gradient are refused while it records, and taken
-under torch.no_grad(); layer_norm_backward is called by hand or from a torch.autograd.Function.
+under torch.no_grad(); the *_backward calls are made by hand or from a torch.autograd.Function.
 Workspaces and results come from torch's allocator, so the calls can be captured in a torch.cuda.graph.
 """
 from __future__ import annotations
 
 import ctypes as C
+import math
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -27,9 +30,11 @@ from .search import BeamSearchError, _check
 
 _HALF = (torch.float16, torch.bfloat16)
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+LAYOUTS = {"half": 0, "interleaved": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
-__all__ = ["attention", "layer_norm", "layer_norm_backward", "linear", "ACTIVATIONS", "BeamSearchError"]
+__all__ = ["attention", "head_norm_rotary", "head_norm_rotary_backward", "layer_norm", "layer_norm_backward", "linear",
+           "rotary_frequencies", "ACTIVATIONS", "LAYOUTS", "BeamSearchError"]
 
 
 # the current stream's handle: torch.cuda.current_stream() makes an object for it (2.9 us a call against 0.1)
@@ -315,4 +320,157 @@ def _attention_workspace(tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, 
     a.longest_q, a.longest_k, a.type, a.causal, a.scale = longest_q, longest_k, code, causal, 1.0
     b = C.c_uint64(0)
     _check(_lib.hip().bs_attention_workspace(C.byref(a), C.byref(b)), "bs_attention_workspace")
+    return b.value
+
+
+def rotary_frequencies(rotary: int, base: float = 10000.0, stretch: float = 1.0, trained: Optional[int] = None, low: float = 1.0,
+                       high: float = 32.0, device="cuda") -> torch.Tensor:
+    """Radians per position of the pairs of head_norm_rotary, float64: base ** (-2 i / rotary) for pair i.  stretch: for
+    contexts that many times as long as those the model was trained on, all frequencies divided by it; with trained (the
+    length it was trained on, in tokens) only those that make fewer than `low` turns over that length are, those that make
+    more than `high` stay, and between them the two are mixed in proportion."""
+    what = "rotary_frequencies"
+    if rotary < 0 or rotary % 2:
+        _fail(f"{what}: rotary must be even and not negative")
+    if not (base > 0 and stretch > 0 and math.isfinite(base) and math.isfinite(stretch)):
+        _fail(f"{what}: base and stretch must be positive")
+    f = base ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / max(rotary, 1))
+    if trained is None:
+        f = f / stretch
+    else:
+        if not high > low:
+            _fail(f"{what}: high must be above low")
+        keep = ((trained * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f * keep + f / stretch * (1 - keep)
+    return f.to(device)
+
+
+def _heads(what: str, name: str, t: torch.Tensor, shape, type_) -> Tuple[int, int]:
+    """the distances of tokens and of heads of `t`"""
+    if t.dim() != 3 or t.dtype != type_ or (shape is not None and t.shape != shape):
+        _fail(f"{what}: {name} must be {'tokens x heads x head_dim' if shape is None else tuple(shape)} of {type_}")
+    s, h, e = t.stride()
+    if e != 1 and t.shape[2] > 1:
+        _fail(f"{what}: the elements of a head of {name} must be contiguous")
+    return s, h
+
+
+def _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude):
+    type_ = q.dtype
+    code = TYPES.get(type_)
+    if code is None:
+        _fail(f"{what}: q must be a float32, float16 or bfloat16 tensor")
+    a = _lib.HeadNormRotaryArgs()
+    a.q_stride, a.q_head_stride = _heads(what, "q", q, None, type_)
+    tokens, heads, dim = q.shape
+    a.q = q.data_ptr()
+    a.tokens, a.heads, a.head_dim, a.type = tokens, heads, dim, code
+    if k is not None:
+        a.k_stride, a.k_head_stride = _heads(what, "k", k, (tokens, k.shape[1] if k.dim() == 3 else 0, dim), type_)
+        a.k, a.kv_heads = k.data_ptr(), k.shape[1]
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous():
+            _fail(f"{what}: positions must be {tokens} contiguous int32 values")
+        a.positions = positions.data_ptr()
+    if frequencies is not None:
+        if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+            _fail(f"{what}: frequencies must be contiguous float64 values")
+        a.frequencies, a.rotary = frequencies.data_ptr(), 2 * frequencies.shape[0]
+        if a.rotary > dim:
+            _fail(f"{what}: frequencies must be at most head_dim / 2")
+    if eps is None:
+        if q_weight is not None or k_weight is not None:
+            _fail(f"{what}: weights belong to the norm: eps must be given with them")
+    else:
+        a.norm, a.eps = 1, eps
+        first = q_weight if q_weight is not None else k_weight
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None:
+                _vector(what, name, w, dim, *((type_, torch.float32) if w is first else (first.dtype,)))
+        if first is not None:
+            a.wtype = TYPES[first.dtype]
+        if q_weight is not None:
+            a.q_weight = q_weight.data_ptr()
+        if k_weight is not None:
+            if k is None:
+                _fail(f"{what}: k_weight without k")
+            a.k_weight = k_weight.data_ptr()
+    if layout not in LAYOUTS:
+        _fail(f"{what}: unknown layout {layout!r}")
+    a.interleaved, a.magnitude = LAYOUTS[layout], magnitude
+    return a
+
+
+def _rotary_out(what, a, x, name, out):
+    o = x.new_empty(x.shape) if out is None else out
+    s, h = _heads(what, name, o, x.shape, x.dtype)
+    return o, o.data_ptr(), s, h
+
+
+def head_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                     frequencies: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                     k_weight: Optional[torch.Tensor] = None, eps: Optional[float] = 1e-6, layout: str = "half",
+                     magnitude: float = 1.0, out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None):
+    """Every head of q (tokens, heads, head_dim) and k (tokens, kv_heads, head_dim; or None) divided by the root of its
+    mean square (+ eps), times q_weight or k_weight (head_dim; of q's type or float32; None: 1), and its first elements
+    turned by the token's position: pair i by positions * frequencies[i], times magnitude.  float32, float16 or bfloat16;
+    head_dim even, up to 256.  eps None: no norm.  positions: int32 (None: 0, 1, ..).  frequencies: float64, one per pair
+    (rotary_frequencies), so 2 len(frequencies) elements of a head are turned (None: none).  layout: "half" pairs element i
+    with i + len(frequencies), "interleaved" 2 i with 2 i + 1.  out: where to write (may be (q, k)).  Returns (q, k)."""
+    what = "head_norm_rotary"
+    outs = (None, None) if out is None else out
+    dev = _gpu(what, q, k, positions, frequencies, q_weight, k_weight, *outs)
+    a = _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude)
+    y, a.q_out, a.q_out_stride, a.q_out_head_stride = _rotary_out(what, a, q, "out[0]", outs[0])
+    z = None
+    if k is not None:
+        z, a.k_out, a.k_out_stride, a.k_out_head_stride = _rotary_out(what, a, k, "out[1]", outs[1])
+    rc = _lib.hip().bs_head_norm_rotary(C.byref(a), _raw_stream(dev))
+    if rc:
+        _check(rc, what)
+    return y, z
+
+
+def head_norm_rotary_backward(dq: torch.Tensor, dk: Optional[torch.Tensor], q: torch.Tensor, k: Optional[torch.Tensor] = None,
+                              positions: Optional[torch.Tensor] = None, frequencies: Optional[torch.Tensor] = None,
+                              q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                              eps: Optional[float] = 1e-6, layout: str = "half", magnitude: float = 1.0, params: bool = True):
+    """Gradients (dq, dk, dq_weight, dk_weight) of head_norm_rotary for the gradients dq and dk of its results; the weights'
+    are of the weights' type (float32 without any), None if params is False or eps is None.  The sums over tokens and
+    heads have a fixed order."""
+    what = "head_norm_rotary_backward"
+    dev = _gpu(what, q, k, dq, dk, positions, frequencies, q_weight, k_weight)
+    a = _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude)
+    if (k is None) != (dk is None):
+        _fail(f"{what}: k and dk must be given together")
+    a.q_grad_stride, a.q_grad_head_stride = _heads(what, "dq", dq, q.shape, q.dtype)
+    a.q_grad = dq.data_ptr()
+    gq, a.q_out, a.q_out_stride, a.q_out_head_stride = _rotary_out(what, a, q, "dq", None)
+    gk = dwq = dwk = ws = None
+    if k is not None:
+        a.k_grad_stride, a.k_grad_head_stride = _heads(what, "dk", dk, k.shape, q.dtype)
+        a.k_grad = dk.data_ptr()
+        gk, a.k_out, a.k_out_stride, a.k_out_head_stride = _rotary_out(what, a, k, "dk", None)
+    size = 0
+    if params and eps is not None:
+        wt = q.dtype if a.wtype == a.type else torch.float32
+        dwq = q.new_empty((a.head_dim,), dtype=wt)
+        a.q_weight_grad = dwq.data_ptr()
+        if k is not None:
+            dwk = torch.empty_like(dwq)
+            a.k_weight_grad = dwk.data_ptr()
+        size = _rotary_workspace(a.tokens, a.heads, a.kv_heads, a.head_dim, a.rotary, a.type)
+        ws = q.new_empty((size,), dtype=torch.uint8)
+    rc = _lib.hip().bs_head_norm_rotary_backward(C.byref(a), ws.data_ptr() if size else None, size, _raw_stream(dev))
+    if rc:
+        _check(rc, what)
+    return gq, gk, dwq, dwk
+
+
+@lru_cache(maxsize=1024)
+def _rotary_workspace(tokens, heads, kv_heads, dim, rotary, code) -> int:
+    a = _lib.HeadNormRotaryArgs()
+    a.tokens, a.heads, a.kv_heads, a.head_dim, a.rotary, a.type, a.wtype, a.norm = tokens, heads, kv_heads, dim, rotary, code, code, 1
+    b = C.c_uint64(0)
+    _check(_lib.hip().bs_head_norm_rotary_backward_workspace(C.byref(a), C.byref(b)), "bs_head_norm_rotary_backward_workspace")
     return b.value

@@ -117,6 +117,57 @@ typedef struct {
 int bs_attention(const bs_attention_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
 int bs_attention_workspace(const bs_attention_args* args, uint64_t* bytes);
 
+/* Norm of every head of queries and keys and the rotation by their positions, in one pass.
+ * q: tokens x heads x head_dim, k: tokens x kv_heads x head_dim (kv_heads 0: none), `type`
+ * BS_F32, BS_F16 or BS_BF16.  With n = x / sqrt(mean(x^2) + eps) * weight over a head's elements
+ * (x itself without `norm`; weight q_weight or k_weight, head_dim each of wtype, NULL: 1), the
+ * first `rotary` elements are turned in pairs i = 0 .. rotary / 2 - 1 and the others are n:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin),  angle = position * frequencies[i]
+ * where a pair is (i, i + rotary / 2), or (2 i, 2 i + 1) if `interleaved`.  Angles are reduced in
+ * float64, so far positions lose nothing; squares are summed in float32.  Elements of a head
+ * are contiguous; *_out may be the call's own q and k (or q_grad and k_grad) with their strides. */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* q_grad; /* of the results; backward alone */
+    const void* k_grad;
+    void* q_out; /* the results; backward: the gradients of q and k */
+    void* k_out;
+    const void* q_weight; /* head_dim, or NULL */
+    const void* k_weight;
+    void* q_weight_grad; /* backward alone, may be NULL */
+    void* k_weight_grad;
+    const int32_t* positions;  /* tokens, any values, or NULL: 0, 1, .. */
+    const double* frequencies; /* rotary / 2, radians per position */
+    int64_t q_stride, q_head_stride;
+    int64_t k_stride, k_head_stride;
+    int64_t q_grad_stride, q_grad_head_stride;
+    int64_t k_grad_stride, k_grad_head_stride;
+    int64_t q_out_stride, q_out_head_stride;
+    int64_t k_out_stride, k_out_head_stride;
+    uint32_t tokens;          /* < 2^31 */
+    uint32_t heads, kv_heads; /* 1..1024, 0..1024 */
+    uint32_t head_dim;        /* even, 2..256 */
+    uint32_t rotary;          /* even, 0..head_dim */
+    int32_t interleaved;
+    int32_t norm;
+    int32_t type;
+    int32_t wtype; /* of weights and their gradients: type or BS_F32 */
+    float eps;
+    float magnitude;
+} bs_head_norm_rotary_args;
+
+int bs_head_norm_rotary(const bs_head_norm_rotary_args* args, void* stream);
+
+/* Its gradients from q, k and the gradients of the results.  With d the gradients turned back
+ * (times magnitude) and r = 1 / sqrt(mean(x^2) + eps):
+ *   q_out, k_out: r * (d weight - x r^2 mean(d weight x))  (d without `norm`; q and k are not read)
+ *   q_weight_grad, k_weight_grad: the sums of d x r over tokens and heads, in a fixed order
+ * workspace: bs_head_norm_rotary_backward_workspace bytes, 16-byte aligned; not needed without
+ * weight gradients. */
+int bs_head_norm_rotary_backward(const bs_head_norm_rotary_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+int bs_head_norm_rotary_backward_workspace(const bs_head_norm_rotary_args* args, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -356,55 +356,57 @@ def _heads(what: str, name: str, t: torch.Tensor, shape, type_) -> Tuple[int, in
 
 
 def _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude):
+    """(pointers of q, k, weights, positions and frequencies; strides of q and k; the sizes and choices; the weights' type)"""
     type_ = q.dtype
     code = TYPES.get(type_)
     if code is None:
         _fail(f"{what}: q must be a float32, float16 or bfloat16 tensor")
-    a = _lib.HeadNormRotaryArgs()
-    a.q_stride, a.q_head_stride = _heads(what, "q", q, None, type_)
+    strides = _heads(what, "q", q, None, type_)
     tokens, heads, dim = q.shape
-    a.q = q.data_ptr()
-    a.tokens, a.heads, a.head_dim, a.type = tokens, heads, dim, code
+    kv = rotary = norm = 0
+    kp = pp = fp = wq = wk = None
+    wt = torch.float32
     if k is not None:
-        a.k_stride, a.k_head_stride = _heads(what, "k", k, (tokens, k.shape[1] if k.dim() == 3 else 0, dim), type_)
-        a.k, a.kv_heads = k.data_ptr(), k.shape[1]
+        kv = k.shape[1] if k.dim() == 3 else 0
+        strides += _heads(what, "k", k, (tokens, kv, dim), type_)
+        kp = k.data_ptr()
+    else:
+        strides += (0, 0)
     if positions is not None:
-        if positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous():
+        if positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] != tokens or not positions.is_contiguous():
             _fail(f"{what}: positions must be {tokens} contiguous int32 values")
-        a.positions = positions.data_ptr()
+        pp = positions.data_ptr()
     if frequencies is not None:
         if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
             _fail(f"{what}: frequencies must be contiguous float64 values")
-        a.frequencies, a.rotary = frequencies.data_ptr(), 2 * frequencies.shape[0]
-        if a.rotary > dim:
+        fp, rotary = frequencies.data_ptr(), 2 * frequencies.shape[0]
+        if rotary > dim:
             _fail(f"{what}: frequencies must be at most head_dim / 2")
     if eps is None:
+        eps = 0.0
         if q_weight is not None or k_weight is not None:
             _fail(f"{what}: weights belong to the norm: eps must be given with them")
     else:
-        a.norm, a.eps = 1, eps
-        first = q_weight if q_weight is not None else k_weight
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None:
-                _vector(what, name, w, dim, *((type_, torch.float32) if w is first else (first.dtype,)))
-        if first is not None:
-            a.wtype = TYPES[first.dtype]
+        norm = 1
         if q_weight is not None:
-            a.q_weight = q_weight.data_ptr()
+            _vector(what, "q_weight", q_weight, dim, type_, torch.float32)
+            wq, wt = q_weight.data_ptr(), q_weight.dtype
         if k_weight is not None:
             if k is None:
                 _fail(f"{what}: k_weight without k")
-            a.k_weight = k_weight.data_ptr()
-    if layout not in LAYOUTS:
+            _vector(what, "k_weight", k_weight, dim, *((type_, torch.float32) if wq is None else (wt,)))
+            wk, wt = k_weight.data_ptr(), k_weight.dtype
+    inter = LAYOUTS.get(layout)
+    if inter is None:
         _fail(f"{what}: unknown layout {layout!r}")
-    a.interleaved, a.magnitude = LAYOUTS[layout], magnitude
-    return a
+    return (q.data_ptr(), kp, wq, wk, pp, fp), strides, (tokens, heads, kv, dim, rotary, inter, norm, code, TYPES[wt], eps, magnitude), wt
 
 
-def _rotary_out(what, a, x, name, out):
-    o = x.new_empty(x.shape) if out is None else out
-    s, h = _heads(what, name, o, x.shape, x.dtype)
-    return o, o.data_ptr(), s, h
+def _rotary_out(what, x, name, out):
+    if out is None:
+        o = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+        return o, (o.shape[1] * o.shape[2], o.shape[2])
+    return out, _heads(what, name, out, x.shape, x.dtype)
 
 
 def head_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
@@ -420,11 +422,13 @@ def head_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, position
     what = "head_norm_rotary"
     outs = (None, None) if out is None else out
     dev = _gpu(what, q, k, positions, frequencies, q_weight, k_weight, *outs)
-    a = _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude)
-    y, a.q_out, a.q_out_stride, a.q_out_head_stride = _rotary_out(what, a, q, "out[0]", outs[0])
-    z = None
+    (qp, kp, wq, wk, pp, fp), strides, sizes, _ = _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude)
+    y, ys = _rotary_out(what, q, "out[0]", outs[0])
+    z, zp, zs = None, None, (0, 0)
     if k is not None:
-        z, a.k_out, a.k_out_stride, a.k_out_head_stride = _rotary_out(what, a, k, "out[1]", outs[1])
+        z, zs = _rotary_out(what, k, "out[1]", outs[1])
+        zp = z.data_ptr()
+    a = _lib.HeadNormRotaryArgs(qp, kp, None, None, y.data_ptr(), zp, wq, wk, None, None, pp, fp, *strides, 0, 0, 0, 0, *ys, *zs, *sizes)
     rc = _lib.hip().bs_head_norm_rotary(C.byref(a), _raw_stream(dev))
     if rc:
         _check(rc, what)
@@ -440,31 +444,34 @@ def head_norm_rotary_backward(dq: torch.Tensor, dk: Optional[torch.Tensor], q: t
     heads have a fixed order."""
     what = "head_norm_rotary_backward"
     dev = _gpu(what, q, k, dq, dk, positions, frequencies, q_weight, k_weight)
-    a = _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude)
+    (qp, kp, wq, wk, pp, fp), strides, sizes, wt = _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, layout, magnitude)
     if (k is None) != (dk is None):
         _fail(f"{what}: k and dk must be given together")
-    a.q_grad_stride, a.q_grad_head_stride = _heads(what, "dq", dq, q.shape, q.dtype)
-    a.q_grad = dq.data_ptr()
-    gq, a.q_out, a.q_out_stride, a.q_out_head_stride = _rotary_out(what, a, q, "dq", None)
-    gk = dwq = dwk = ws = None
+    gs = _heads(what, "dq", dq, q.shape, q.dtype)
+    y, ys = _rotary_out(what, q, "dq", None)
+    z = dkp = zp = dwq = dwk = ws = None
+    zs = (0, 0)
     if k is not None:
-        a.k_grad_stride, a.k_grad_head_stride = _heads(what, "dk", dk, k.shape, q.dtype)
-        a.k_grad = dk.data_ptr()
-        gk, a.k_out, a.k_out_stride, a.k_out_head_stride = _rotary_out(what, a, k, "dk", None)
+        gs += _heads(what, "dk", dk, k.shape, q.dtype)
+        z, zs = _rotary_out(what, k, "dk", None)
+        dkp, zp = dk.data_ptr(), z.data_ptr()
+    else:
+        gs += (0, 0)
     size = 0
     if params and eps is not None:
-        wt = q.dtype if a.wtype == a.type else torch.float32
-        dwq = q.new_empty((a.head_dim,), dtype=wt)
-        a.q_weight_grad = dwq.data_ptr()
+        dim = q.shape[2]
+        both = q.new_empty((2 if k is not None else 1, dim), dtype=wt)
+        dwq = both[0]
         if k is not None:
-            dwk = torch.empty_like(dwq)
-            a.k_weight_grad = dwk.data_ptr()
-        size = _rotary_workspace(a.tokens, a.heads, a.kv_heads, a.head_dim, a.rotary, a.type)
+            dwk = both[1]
+        size = _rotary_workspace(*sizes[:5], sizes[7])
         ws = q.new_empty((size,), dtype=torch.uint8)
+    a = _lib.HeadNormRotaryArgs(qp, kp, dq.data_ptr(), dkp, y.data_ptr(), zp, wq, wk, None if dwq is None else dwq.data_ptr(),
+                                None if dwk is None else dwk.data_ptr(), pp, fp, *strides, *gs, *ys, *zs, *sizes)
     rc = _lib.hip().bs_head_norm_rotary_backward(C.byref(a), ws.data_ptr() if size else None, size, _raw_stream(dev))
     if rc:
         _check(rc, what)
-    return gq, gk, dwq, dwk
+    return y, z, dwq, dwk
 
 
 @lru_cache(maxsize=1024)

@@ -119,6 +119,9 @@ EMBED_API = {
     "bs_linear_workspace": (C.c_int, [u64, u32, u32, P(u64)]),
     "bs_attention": (C.c_int, [P(AttentionArgs), vp, u64, vp]),
     "bs_attention_workspace": (C.c_int, [P(AttentionArgs), P(u64)]),
+    "bs_gated": (C.c_int, [vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, u64, u32, u32, C.c_int, C.c_int, vp]),
+    "bs_gated_backward": (C.c_int, [vp, i64] * 6 + [vp, vp, vp, u64, u32, u32, C.c_int, C.c_int, vp, u64, vp]),
+    "bs_gated_backward_workspace": (C.c_int, [u64, u32, u32, P(u64)]),
     "bs_head_norm_rotary": (C.c_int, [P(HeadNormRotaryArgs), vp]),
     "bs_head_norm_rotary_backward": (C.c_int, [P(HeadNormRotaryArgs), vp, u64, vp]),
     "bs_head_norm_rotary_backward_workspace": (C.c_int, [P(HeadNormRotaryArgs), P(u64)]),

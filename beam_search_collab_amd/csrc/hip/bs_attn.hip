@@ -6,7 +6,7 @@
 // one row of the tile and its scores stay in its registers -- maximum, sum and rescaling are per lane
 // (plus one exchange between the wave's halves), and the weights are the second operand of O^T = V^T P^T
 // as they stand, once V's keys are taken in the order in which the result of the first product has them.
-#include "bs_embed.hpp"
+#include "bs_product.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -15,23 +15,8 @@
 namespace {
 using namespace bse;
 
-template <typename T>
-struct Mma;
-template <>
-struct Mma<f16> {
-    __device__ static f32x16 go(Vec<f16, 8> a, Vec<f16, 8> b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-    }
-};
-template <>
-struct Mma<bf16> {
-    __device__ static f32x16 go(Vec<bf16, 8> a, Vec<bf16, 8> b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-    }
-};
-
 constexpr int BN = 64;  // keys of a tile
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
+constexpr float LN2 = 0.69314718055994531f;
 constexpr float NONE = -INFINITY;
 
 struct Params {
@@ -93,21 +78,6 @@ __device__ inline uint32_t find(const int32_t* off, uint32_t n, uint64_t tile, u
 // the last sequence that starts at or before the token
 __device__ inline uint32_t holder(const int32_t* off, uint32_t n, uint32_t tok) {
     return last_below(n, [&](uint32_t s) { return static_cast<uint32_t>(max(off[s], 0)) <= tok; });
-}
-
-// chunk c of 16 bytes in row r of an LDS tile of S bytes per row (64, 128 or 256).  16 rows read at one
-// chunk (a quarter wave's operand of K) lie in 16 different chunks of the 256 bytes that all banks span,
-// and the 4 rows x 64 bytes of a transposed read of V in 4 different quarters of them.
-template <int S>
-__device__ inline int place(int r, int c) {
-    const int f = S == 256 ? ((r & 3) << 2 | ((r >> 2) & 3)) : S == 128 ? (((r >> 1) & 1) << 2 | ((r >> 2) & 3)) : ((r >> 2) & 3);
-    return r * S + ((c ^ f) << 4);
-}
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-__device__ inline s16x4 read_transposed(const char* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
-        reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p)));
 }
 
 // waits until all but the wave's N youngest moves to LDS are done, and its reads of LDS

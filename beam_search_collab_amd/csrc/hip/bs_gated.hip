@@ -1,0 +1,640 @@
+// Gated products and their gradients (include/bs_embed.h).
+//
+//   h  = act(g) u,  g = x wg^T,  u = x wu^T
+//   dg = dh u act'(g),  du = dh act(g):  rows of d = (dg | du), in the workspace
+//   dx = dg wg + du wu,  dwg = dg^T x,  dwu = du^T x
+//
+// Three kinds of products, all of an operand X, whose rows are the result's rows, and an operand W, whose rows are its
+// columns:
+//   GATED    X = x (rows x inner), W = 32 rows of wg, 32 of wu, and so on, so that a wave has g and u of the same results
+//   INPUT    X = d (rows x 2 cols), W = the columns of wg over those of wu
+//   WEIGHTS  X = the columns of d, W = the columns of x: the inner dimension is the rows
+// Where an operand's rows are columns in memory, its tile lies in LDS as in memory, an inner element per row, and is read
+// by transposing LDS reads.
+#include "bs_product.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+namespace {
+using namespace bse;
+
+enum { GATED = 0, INPUT = 1, WEIGHTS = 2 };
+
+struct Params {
+    const void *x, *wg, *wu;
+    int64_t xs, wgs, wus;
+    void *h, *gate, *up;  // GATED; gate and up may be null
+    int64_t hs;
+    const void *dh, *g, *u;
+    int64_t dhs, gs, us;
+    void *dx, *dwg, *dwu;
+    char* d;      // rows_up x 2 cols, rows past the last are 0
+    char* tail;   // the last rows % 64 rows of x, then zeros: 64 x inner
+    float* parts; // splits x the result
+    uint32_t rows, inner, cols;
+    int act;
+    uint32_t splits;
+};
+
+// ------------------------------------------------------------------------------------------------ d
+
+// 1 / (1 + e) and e / (1 + e) for e = 2^v, neither by a difference
+__device__ inline void halves_of_one(float v, float& s, float& rest) {
+    const float e = __builtin_amdgcn_exp2f(fminf(v, 126.0f));
+    s = __builtin_amdgcn_rcpf(1.0f + e);
+    rest = e * s;
+}
+// an activation and its slope
+__device__ inline void act_and_slope(float z, int act, float& a, float& slope) {
+    if (act == BS_ACT_RELU) {
+        a = z < 0.0f ? 0.0f : z;
+        slope = z > 0.0f ? 1.0f : 0.0f;
+    } else if (act == BS_ACT_GELU) {  // P = (1 + erf(z / sqrt 2)) / 2: slope P + z exp(-z^2 / 2) / sqrt(2 pi)
+        const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E)), part = gelu_part(z, e);
+        a = z * part;
+        slope = fmaf(z * 0.3989422804014327f, e, part);
+    } else if (act == BS_ACT_GELU_TANH) {  // z s, s = 1 / (1 + exp(-2 v)): slope s + z s (1 - s) 2 v'
+        const float q = z * z;
+        float s, rest;
+        halves_of_one(-2.0f * LOG2E * 0.79788456080286536f * fmaf(0.044715f * q, z, z), s, rest);
+        a = z * s;
+        const float bend = s * rest;
+        slope = bend == 0.0f ? s : fmaf(z * bend, 1.59576912160573072f * fmaf(3.0f * 0.044715f, q, 1.0f), s);
+    } else if (act == BS_ACT_SILU) {  // z s, s = 1 / (1 + exp(-z)): slope s + z s (1 - s)
+        float s, rest;
+        halves_of_one(-LOG2E * z, s, rest);
+        a = z * s;
+        slope = fmaf(z * rest, s, s);
+    } else {
+        a = z;
+        slope = 1.0f;
+    }
+}
+
+// d, 8 columns a thread; the rows past the last are 0 and so are those of x's tail.  dg and du are rounded to the inputs' type
+// for their products, as every operand of a matrix product is: off by half a unit each, at random, which gives a sum of n of
+// them the error that the same sum of rounded inputs has.
+template <typename T>
+__global__ __launch_bounds__(256) void gated_slopes_kernel(Params p, uint32_t rows_up, uint32_t tail_rows) {
+    const uint32_t across = (p.cols + 7) / 8, wide = (p.inner + 7) / 8;
+    const uint64_t all = static_cast<uint64_t>(rows_up) * across, more = static_cast<uint64_t>(tail_rows) * wide;
+    T* d = reinterpret_cast<T*>(p.d);
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < all + more; i += static_cast<uint64_t>(gridDim.x) * 256) {
+        if (i >= all) {
+            const uint32_t r = static_cast<uint32_t>((i - all) / wide), c = static_cast<uint32_t>((i - all) % wide) * 8, row = rows_up - tail_rows + r;
+            const int n = static_cast<int>(p.inner - c);
+            Vec<T, 8> v = {};
+            if (row < p.rows) v = load_some<T, 8>(static_cast<const T*>(p.x) + static_cast<int64_t>(row) * p.xs + c, n);
+            store_some<T, 8>(reinterpret_cast<T*>(p.tail) + static_cast<size_t>(r) * p.inner + c, v, n);
+            continue;
+        }
+        const uint32_t row = static_cast<uint32_t>(i / across), c = static_cast<uint32_t>(i % across) * 8;
+        const int n = static_cast<int>(p.cols - c);
+        Vec<T, 8> dg = {}, du = {};
+        if (row < p.rows) {
+            const Vec<T, 8> h = load_some<T, 8>(static_cast<const T*>(p.dh) + static_cast<int64_t>(row) * p.dhs + c, n);
+            const Vec<T, 8> g = load_some<T, 8>(static_cast<const T*>(p.g) + static_cast<int64_t>(row) * p.gs + c, n);
+            const Vec<T, 8> u = load_some<T, 8>(static_cast<const T*>(p.u) + static_cast<int64_t>(row) * p.us + c, n);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float a, slope;
+                act_and_slope(static_cast<float>(g[j]), p.act, a, slope);
+                dg[j] = static_cast<T>(static_cast<float>(h[j]) * static_cast<float>(u[j]) * slope);
+                du[j] = static_cast<T>(static_cast<float>(h[j]) * a);
+            }
+        }
+        store_some<T, 8>(d + static_cast<size_t>(row) * 2 * p.cols + c, dg, n);
+        store_some<T, 8>(d + static_cast<size_t>(row) * 2 * p.cols + p.cols + c, du, n);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ results
+
+// the sizes of a product: rows and columns of its result, inner elements
+template <int FORM>
+__device__ __host__ inline uint32_t rows_of(const Params& p) { return FORM == WEIGHTS ? 2 * p.cols : p.rows; }
+template <int FORM>
+__device__ __host__ inline uint32_t cols_of(const Params& p) { return FORM == GATED ? p.cols : p.inner; }
+template <int FORM>
+__device__ __host__ inline uint32_t inner_of(const Params& p) { return FORM == GATED ? p.inner : FORM == INPUT ? 2 * p.cols : p.rows; }
+
+// N adjacent results of a row, those inside
+template <typename T, int FORM, int N>
+__device__ inline void write(const Params& p, uint32_t row, uint32_t col, const float (&z)[N]) {
+    T* to = FORM == INPUT ? static_cast<T*>(p.dx) + static_cast<size_t>(row) * p.inner
+                          : row < p.cols ? static_cast<T*>(p.dwg) + static_cast<size_t>(row) * p.inner : static_cast<T*>(p.dwu) + static_cast<size_t>(row - p.cols) * p.inner;
+    Vec<T, N> o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = static_cast<T>(z[j]);
+    store_some<T, N>(to + col, o, static_cast<int>(p.inner - col));
+}
+template <typename T, int N>
+__device__ inline void write_gated(const Params& p, uint32_t row, uint32_t col, float (&g)[N], const float (&u)[N]) {
+    const int n = static_cast<int>(p.cols - col);
+    Vec<T, N> o;
+    if (p.gate) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = static_cast<T>(g[j]);
+        store_some<T, N>(static_cast<T*>(p.gate) + static_cast<size_t>(row) * p.cols + col, o, n);
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = static_cast<T>(u[j]);
+        store_some<T, N>(static_cast<T*>(p.up) + static_cast<size_t>(row) * p.cols + col, o, n);
+    }
+    activate(g, p.act);
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = static_cast<T>(g[j] * u[j]);
+    store_some<T, N>(static_cast<T*>(p.h) + static_cast<int64_t>(row) * p.hs + col, o, n);
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+
+// 8 inner elements of a lane's row of an operand whose inner elements are rows of S bytes in LDS: lanes 16 g .. 16 g + 15 read
+// 4 rows x 16 columns and get a column's 4 rows each
+template <typename T, int S>
+__device__ inline Vec<T, 8> read_across(const char* tile, int inner, int column, int lane) {
+    const int k = inner + (lane >> 5) * 8 + ((lane & 15) >> 2), e = column + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    const s16x4 lo = read_transposed(tile + place<S>(k, e >> 3) + (e & 7) * 2);
+    const s16x4 hi = read_transposed(tile + place<S>(k + 4, e >> 3) + (e & 7) * 2);
+    return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+}
+
+// Tiles of any size and alignment.  Direct: operands are 16-byte aligned, whole steps go from memory to LDS without registers.
+template <typename T, int FORM, typename C, bool Direct>
+__global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_kernel(Params p) {
+    constexpr bool XT = FORM == WEIGHTS, WT = FORM != GATED;  // the operand's rows are columns in memory
+    constexpr int OUT = FORM == GATED ? C::BN / 2 : C::BN;    // columns of the result in a tile
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    T* buf = reinterpret_cast<T*>(lds);
+    const uint32_t rows = rows_of<FORM>(p), cols = cols_of<FORM>(p), inner = inner_of<FORM>(p);
+    // Workgroup b runs on XCD b mod 8: each XCD takes a contiguous run of tiles, 8 tile rows high, so that
+    // the tiles in flight on it share operands in its L2.
+    const uint32_t mt = (rows + C::BM - 1) / C::BM, nt = (cols + OUT - 1) / OUT, total = mt * nt;
+    const uint32_t xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+    const uint32_t id = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
+    const uint32_t band = id / (8 * nt), high = mt - band * 8 < 8 ? mt - band * 8 : 8, in = id - band * 8 * nt;
+    const uint32_t m0 = (band * 8 + in % high) * C::BM, n0 = in / high * OUT;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
+    const int wm = wave / C::WN * C::TM * 32, wn = wave % C::WN * C::TN * 32;
+    constexpr int XMOVES = C::BM * C::BK / 8 / C::THREADS;
+
+    // A thread's moves: 16 bytes each, to LDS positions that are linear over the workgroup.  Of an operand that lies in LDS as
+    // rows of the result: row `line` of it, inner elements `at` on; of one that lies there as rows of inner elements: inner
+    // element `line`, results `at` on.
+    auto spot = [&](int i, int& line, int& at) {
+        const int k = i * C::THREADS + static_cast<int>(threadIdx.x);
+        if (i < XMOVES ? XT : WT) {
+            const int w = i < XMOVES ? C::BM : C::BN, j = i < XMOVES ? k : k - C::BM * C::BK / 8;
+            line = j / (w / 8);
+            const int c = j % (w / 8);
+            at = (w == 64 ? (place<128>(line, c) - line * 128) : w == 128 ? (place<256>(line, c) - line * 256) : (place<512>(line, c) - line * 512)) / 2;
+        } else {
+            line = (k / C::CH) - (i < XMOVES ? 0 : C::BM);
+            at = C::swizzle(k / C::CH, k % C::CH) * 8;
+        }
+    };
+    // where the 8 elements of a move come from, at inner element k0 of the product, and how many of them there are
+    auto source = [&](int i, uint32_t k0, int& n) -> const T* {
+        int line, at;
+        spot(i, line, at);
+        if (i < XMOVES) {
+            if (XT) {
+                const uint32_t k = k0 + line, m = m0 + at;
+                n = k < inner && m < rows ? static_cast<int>(rows - m) : 0;
+                return reinterpret_cast<const T*>(p.d) + static_cast<size_t>(k) * 2 * p.cols + m;
+            }
+            const uint32_t m = min(m0 + line, rows - 1), k = k0 + at;  // rows past the end repeat the last one: their products are not stored
+            n = static_cast<int>(inner) - static_cast<int>(k);
+            return FORM == GATED ? static_cast<const T*>(p.x) + static_cast<int64_t>(m) * p.xs + k : reinterpret_cast<const T*>(p.d) + static_cast<size_t>(m) * 2 * p.cols + k;
+        }
+        if (WT) {
+            const uint32_t k = k0 + line, c = n0 + at;
+            n = k < inner && c < cols ? static_cast<int>(cols - c) : 0;
+            if (FORM == WEIGHTS) return static_cast<const T*>(p.x) + static_cast<int64_t>(k) * p.xs + c;
+            return k < p.cols ? static_cast<const T*>(p.wg) + static_cast<int64_t>(k) * p.wgs + c : static_cast<const T*>(p.wu) + static_cast<int64_t>(k - p.cols) * p.wus + c;
+        }
+        const uint32_t c = min(n0 + (line >> 6) * 32 + (line & 31), cols - 1), k = k0 + at;
+        n = static_cast<int>(inner) - static_cast<int>(k);
+        return line & 32 ? static_cast<const T*>(p.wu) + static_cast<int64_t>(c) * p.wus + k : static_cast<const T*>(p.wg) + static_cast<int64_t>(c) * p.wgs + k;
+    };
+    // this workgroup's piece: whole steps [begin, whole), and for the last piece what is left after them
+    const uint32_t allsteps = (inner + C::BK - 1) / C::BK, piece = (allsteps + p.splits - 1) / p.splits;
+    const uint32_t begin = blockIdx.y * piece, steps = min(begin + piece, allsteps), whole = min(steps, inner / C::BK);
+    auto fetch = [&](uint32_t t, Vec<T, 8> (&v)[C::MOVES]) {
+#pragma unroll
+        for (int i = 0; i < C::MOVES; ++i) {
+            int n;
+            const T* from = source(i, t * C::BK, n);
+            v[i] = n > 0 ? load_some<T, 8>(from, n) : Vec<T, 8>{};
+        }
+    };
+    auto put = [&](int slot, const Vec<T, 8> (&v)[C::MOVES]) {
+#pragma unroll
+        for (int i = 0; i < C::MOVES; ++i) *reinterpret_cast<Vec<T, 8>*>(buf + slot * C::STEP + (i * C::THREADS + threadIdx.x) * 8) = v[i];
+    };
+    f32x16 acc[C::TN][C::TM] = {};
+    struct Parts {
+        Vec<T, 8> a[C::TN], b[C::TM];
+    };
+    auto read = [&](int slot, int s, Parts& f) {  // 16 inner elements
+        const T* tx = buf + slot * C::STEP;
+        const T* tw = tx + C::BM * C::BK;
+#pragma unroll
+        for (int i = 0; i < C::TN; ++i)
+            f.a[i] = WT ? read_across<T, C::BN * 2>(reinterpret_cast<const char*>(tw), s * 16, wn + i * 32, lane)
+                        : *reinterpret_cast<const Vec<T, 8>*>(tw + C::place(wn + i * 32 + l, s * 2 + h));
+#pragma unroll
+        for (int j = 0; j < C::TM; ++j)
+            f.b[j] = XT ? read_across<T, C::BM * 2>(reinterpret_cast<const char*>(tx), s * 16, wm + j * 32, lane)
+                        : *reinterpret_cast<const Vec<T, 8>*>(tx + C::place(wm + j * 32 + l, s * 2 + h));
+    };
+    auto product = [&](const Parts& f, int from_, int to) {
+#pragma unroll
+        for (int i = from_; i < to; ++i)
+#pragma unroll
+            for (int j = 0; j < C::TM; ++j) acc[i][j] = Mma<T>::go(f.a[i], f.b[j], acc[i][j]);
+    };
+    auto multiply = [&](int slot) {
+        Parts f;
+#pragma unroll
+        for (int s = 0; s < C::BK / 16; ++s) {
+            read(slot, s, f);
+            product(f, 0, C::TN);
+        }
+    };
+    if (Direct) {
+        // whole steps: no inner element is past the end; results past it repeat the last 8, and are not stored
+        const T* from[C::MOVES];
+#pragma unroll
+        for (int i = 0; i < C::MOVES; ++i) {
+            int line, at, n;
+            spot(i, line, at);
+            from[i] = source(i, 0, n);
+            if (i < XMOVES) {
+                if (XT) from[i] = reinterpret_cast<const T*>(p.d) + static_cast<size_t>(line) * 2 * p.cols + min(m0 + at, rows - 8);
+            } else if (WT) {
+                const uint32_t c = min(n0 + at, cols - 8);
+                from[i] = FORM == WEIGHTS ? static_cast<const T*>(p.x) + static_cast<int64_t>(line) * p.xs + c : static_cast<const T*>(p.wg) + static_cast<int64_t>(line) * p.wgs + c;
+            }
+        }
+        auto move = [&](uint32_t t, int slot) {
+            const size_t k = static_cast<size_t>(t) * C::BK;
+            // elements from step 0 to step t of an operand
+            const int64_t xhop = XT ? static_cast<int64_t>(k) * 2 * p.cols : static_cast<int64_t>(k);
+            int64_t whop = static_cast<int64_t>(k);
+            if (FORM == WEIGHTS) whop *= p.xs;
+            if (FORM == INPUT)  // cols is a multiple of the step; strides of both weights are alike
+                whop = k < p.cols ? whop * p.wgs : (static_cast<const T*>(p.wu) - static_cast<const T*>(p.wg)) + (whop - p.cols) * p.wgs;
+#pragma unroll
+            for (int i = 0; i < C::MOVES; ++i)
+                __builtin_amdgcn_global_load_lds((global_ptr)(from[i] + (i < XMOVES ? xhop : whop)),
+                                                 (lds_ptr)(buf + slot * C::STEP + (i * C::THREADS + wave * 64) * 8), 16, 0, 0);
+        };
+        // At meeting t steps t and t + 1 are in LDS and nobody reads step t - 1 any more, whose place step
+        // t + NS - 1 gets.  Operands are read one part (16 inner elements) ahead of their products, across the
+        // meeting too.  A move past the last step repeats the last one, so that every wait counts the same.
+        const uint32_t last = whole ? whole - 1 : 0;
+        if (whole > begin) {
+            Parts f[2];
+#pragma unroll
+            for (int i = 0; i < C::NS - 1; ++i) move(min(begin + i, last), i);
+            meet<(C::NS - 2) * C::MOVES>();
+            read(0, 0, f[0]);
+            int slot = 0;
+            for (uint32_t t = begin; t < whole; ++t) {
+                meet<(C::NS - 3) * C::MOVES>();
+                move(min(t + C::NS - 1, last), slot == 0 ? C::NS - 1 : slot - 1);
+                const int next = slot == C::NS - 1 ? 0 : slot + 1;
+#pragma unroll
+                for (int s = 0; s < C::BK / 16; ++s) {
+                    product(f[s & 1], 0, C::TN / 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (s + 1 < C::BK / 16)
+                        read(slot, s + 1, f[(s + 1) & 1]);
+                    else
+                        read(next, 0, f[(s + 1) & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    product(f[s & 1], C::TN / 2, C::TN);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                slot = next;
+            }
+        }
+        meet<0>();
+        __syncthreads();
+        if (steps > whole) {
+            Vec<T, 8> v[C::MOVES];
+            fetch(whole, v);
+            put(0, v);
+            __syncthreads();
+            multiply(0);
+            __syncthreads();
+        }
+    } else {
+        Vec<T, 8> v[C::MOVES];
+        if (steps > begin) {
+            fetch(begin, v);
+            put(begin & 1, v);
+        }
+        for (uint32_t t = begin; t < steps; ++t) {
+            __syncthreads();
+            if (t + 1 < steps) fetch(t + 1, v);
+            multiply(t & 1);
+            if (t + 1 < steps) put(~t & 1, v);
+        }
+        __syncthreads();
+    }
+    // a wave turns 32 rows of its results at a time: a lane then has 8 adjacent columns (GATED: of both products)
+    static_assert(FORM != GATED || C::TN == 2, "a wave has 32 columns of both products");
+    constexpr int W = C::TN * 32, PITCH = W + 4, LANES = FORM == GATED ? 4 : W / 8;
+    float* turn = reinterpret_cast<float*>(lds + wave * C::JOIN);
+    auto spread = [&](auto J) {
+        constexpr int j = decltype(J)::value;
+        if constexpr (j < C::TM) {
+#pragma unroll
+            for (int i = 0; i < C::TN; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f32x4*>(turn + l * PITCH + i * 32 + q * 8 + h * 4) =
+                        f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+        }
+    };
+    static_assert(C::TM <= 2, "cases below");
+#pragma unroll 1
+    for (int j = 0; j < C::TM; ++j) {  // not unrolled: the epilogue's code stays in the instruction cache
+        if (j == 0)
+            spread(std::integral_constant<int, 0>());
+        else
+            spread(std::integral_constant<int, 1>());
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int k = 0; k < 32 * LANES / 64; ++k) {
+            const int r = k * (64 / LANES) + lane / LANES, c = lane % LANES * 8;
+            const uint32_t row = m0 + wm + j * 32 + r, col = n0 + (FORM == GATED ? wn / 2 : wn) + c;
+            float z[8], u[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const f32x4 z4 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + c + e);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) z[e + x] = z4[x];
+                if (FORM == GATED) {
+                    const f32x4 u4 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + 32 + c + e);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) u[e + x] = u4[x];
+                }
+            }
+            if (row >= rows || col >= cols) continue;
+            if constexpr (FORM == GATED) {
+                write_gated<T, 8>(p, row, col, z, u);
+            } else if (p.splits > 1) {
+                float* part = p.parts + (static_cast<size_t>(blockIdx.y) * rows + row) * cols + col;
+                store_some<float, 4>(part, f32x4{z[0], z[1], z[2], z[3]}, static_cast<int>(cols - col));
+                if (cols - col > 4) store_some<float, 4>(part + 4, f32x4{z[4], z[5], z[6], z[7]}, static_cast<int>(cols - col) - 4);
+            } else {
+                write<T, FORM, 8>(p, row, col, z);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// the pieces' sums in order: a thread takes four adjacent columns of a row
+template <typename T, int FORM>
+__global__ __launch_bounds__(256) void gated_join_kernel(Params p) {
+    const uint32_t rows = rows_of<FORM>(p), cols = cols_of<FORM>(p), across = (cols + 3) / 4;
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const uint32_t row = static_cast<uint32_t>(at / across), col = static_cast<uint32_t>(at % across) * 4;
+    if (row >= rows) return;
+    const int n = static_cast<int>(cols - col);
+    const float* part = p.parts + static_cast<size_t>(row) * cols + col;
+    f32x4 s = load_some<float, 4>(part, n);
+    for (uint32_t i = 1; i < p.splits; ++i) s += load_some<float, 4>(part + static_cast<size_t>(i) * rows * cols, n);
+    const float z[4] = {s[0], s[1], s[2], s[3]};
+    write<T, FORM, 4>(p, row, col, z);
+}
+
+// Few rows: both weights are read once, from memory to registers, and bound the time.  A workgroup has 16 rows of each, its
+// eight waves a contiguous piece each of the inner dimension; x (MT x 16 rows) comes from the L2.
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void gated_few_kernel(Params p) {
+    __shared__ f32x4 join[8][2 * MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const uint32_t n0 = blockIdx.x * 16;
+    // rows past the end repeat the last one: their products are not stored
+    const uint32_t n = min(n0 + l, p.cols - 1);
+    const T *wp[2] = {static_cast<const T*>(p.wg) + static_cast<int64_t>(n) * p.wgs + g * 8, static_cast<const T*>(p.wu) + static_cast<int64_t>(n) * p.wus + g * 8}, *xp[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xp[i] = static_cast<const T*>(p.x) + static_cast<int64_t>(min(static_cast<uint32_t>(i * 16 + l), p.rows - 1)) * p.xs + g * 8;
+    f32x4 acc[2][MT] = {};
+    const uint32_t steps = (p.inner + 31) / 32, piece = (steps + 7) / 8, begin = wave * piece;
+    const uint32_t end = min(begin + piece, steps), whole = min(end, p.inner / 32);
+    constexpr int U = 8;  // steps in flight
+    uint32_t t = begin;
+    for (; t + U <= whole; t += U) {
+        Vec<T, 8> a[U][2], b[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) a[u][i] = load_any<T, 8>(wp[i] + (t + u) * 32);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) b[u][i] = load_any<T, 8>(xp[i] + (t + u) * 32);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) acc[i][j] = Mma16<T>::go(a[u][i], b[u][j], acc[i][j]);
+    }
+    for (; t < end; ++t) {
+        const int left = static_cast<int>(p.inner - t * 32) - g * 8;
+        Vec<T, 8> a[2], b[MT];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) a[i] = left > 0 ? load_some<T, 8>(wp[i] + t * 32, left) : Vec<T, 8>{};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) b[i] = left > 0 ? load_some<T, 8>(xp[i] + t * 32, left) : Vec<T, 8>{};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] = Mma16<T>::go(a[i], b[j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) join[wave][i * MT + j][lane] = acc[i][j];
+    __syncthreads();
+    if (wave >= MT) return;
+    // wave j: rows 16 j + l, columns 4 g to + 3; the waves' sums in order
+    f32x4 s = join[0][wave][lane], r = join[0][MT + wave][lane];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += join[k][wave][lane], r += join[k][MT + wave][lane];
+    const uint32_t row = wave * 16 + l, col = n0 + g * 4;
+    float z[4] = {s[0], s[1], s[2], s[3]};
+    const float u[4] = {r[0], r[1], r[2], r[3]};
+    if (row < p.rows && col < p.cols) write_gated<T, 4>(p, row, col, z, u);
+}
+
+using Mid = Tile<128, 128, 2, 2, 32, 4, 2>;
+using Small = Tile<64, 64, 2, 2, 64, 4, 2>;
+using Flat = Tile<64, 128, 2, 2, 64, 3, 2>;  // of GATED, whose waves have 64 rows of W
+
+constexpr uint32_t FEW = 32;
+
+uint64_t tiles_of(uint64_t rows, uint64_t cols, uint32_t high, uint32_t wide) { return (rows + high - 1) / high * ((cols + wide - 1) / wide); }
+
+// pieces of the inner dimension for tiles of 64, where they leave compute units idle
+uint32_t splits_of(uint64_t rows, uint64_t inner, uint64_t cols) {
+    const uint64_t tiles = tiles_of(rows, cols, 64, 64);
+    const uint64_t want = std::min<uint64_t>(2 * CUS / tiles, inner / 1024);
+    if (want < 2) return 1;
+    const uint64_t steps = (inner + 63) / 64, piece = (steps + want - 1) / want;
+    return static_cast<uint32_t>((steps + piece - 1) / piece);
+}
+
+template <typename T, int FORM, typename C, bool Direct>
+int start(const Params& p, hipStream_t s) {
+    auto* k = gated_kernel<T, FORM, C, Direct>;
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), C::LDS, done)) return rc;
+    k<<<dim3(static_cast<uint32_t>(tiles_of(rows_of<FORM>(p), cols_of<FORM>(p), C::BM, FORM == GATED ? C::BN / 2 : C::BN)), p.splits), C::THREADS, C::LDS, s>>>(p);
+    if constexpr (FORM != GATED) {
+        if (p.splits > 1) {
+            const uint64_t quads = static_cast<uint64_t>(rows_of<FORM>(p)) * ((cols_of<FORM>(p) + 3) / 4);
+            gated_join_kernel<T, FORM><<<static_cast<uint32_t>((quads + 255) / 256), 256, 0, s>>>(p);
+        }
+    }
+    return BS_OK;
+}
+
+bool rows16(const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; }
+
+template <typename T>
+int launch_forward(Params p, hipStream_t s) {
+    if (p.rows <= FEW) {
+        if (p.rows <= 16)
+            gated_few_kernel<T, 1><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
+        else
+            gated_few_kernel<T, 2><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
+        return BS_OK;
+    }
+    const bool direct = rows16(p.x, p.xs) && rows16(p.wg, p.wgs) && rows16(p.wu, p.wus);
+    if (tiles_of(p.rows, p.cols, 128, 64) >= CUS) return direct ? start<T, GATED, Mid, true>(p, s) : start<T, GATED, Mid, false>(p, s);
+    return direct ? start<T, GATED, Flat, true>(p, s) : start<T, GATED, Flat, false>(p, s);
+}
+template <typename T, int FORM>
+int launch_gradient(Params p, hipStream_t s) {
+    const uint64_t rows = rows_of<FORM>(p), cols = cols_of<FORM>(p);
+    // of INPUT: a step lies in one weight
+    const bool direct = p.cols % 64 == 0 && p.inner % 8 == 0 && (FORM == WEIGHTS ? rows16(p.x, p.xs) : rows16(p.wg, p.wgs) && rows16(p.wu, p.wus) && p.wgs == p.wus);
+    p.splits = splits_of(rows, inner_of<FORM>(p), cols);
+    if (p.splits == 1 && tiles_of(rows, cols, 128, 128) >= CUS) return direct ? start<T, FORM, Mid, true>(p, s) : start<T, FORM, Mid, false>(p, s);
+    return direct ? start<T, FORM, Small, true>(p, s) : start<T, FORM, Small, false>(p, s);
+}
+template <typename T>
+int launch_backward(const Params& p, hipStream_t s) {
+    const uint64_t quads = static_cast<uint64_t>((p.rows + 63) / 64 * 64) * ((p.cols + 7) / 8);
+    const uint32_t rows_up = (p.rows + 63) / 64 * 64;
+    gated_slopes_kernel<T><<<static_cast<uint32_t>(std::min<uint64_t>((quads + 255) / 256, 1u << 22)), 256, 0, s>>>(p, rows_up, 0);
+    if (p.dx)
+        if (const int rc = launch_gradient<T, INPUT>(p, s)) return rc;
+    if (p.dwg)
+        if (const int rc = launch_gradient<T, WEIGHTS>(p, s)) return rc;
+    return BS_OK;
+}
+
+int check(const std::string& what, uint64_t rows, uint32_t inner, uint32_t cols) {
+    if (rows > 0x7FFFFFFFull) return refuse(what + ": rows must be < 2^31");
+    if (inner == 0 || inner > (1u << 24) || cols == 0 || cols > (1u << 23)) return refuse(what + ": inner must be in 1..2^24, cols in 1..2^23");
+    // A grid of 2^32 threads is cut short without an error.  Tiles of 64 x 64 results by 256 threads are the most.
+    if (tiles_of(rows, std::max(inner, cols), 64, 64) * 256 > 0xFFFFFFFFull || tiles_of(2 * static_cast<uint64_t>(cols), inner, 64, 64) * 256 > 0xFFFFFFFFull)
+        return refuse(what + ": the sizes are too large for one launch");
+    return BS_OK;
+}
+int check_rows(const std::string& what, const char* name, const void* p, int64_t stride, uint32_t row) {
+    if (!p) return refuse(what + ": " + name + " must be given");
+    if (stride < row) return refuse(what + ": rows of " + name + " overlap (a stride is shorter than its row)");
+    if (stride >= (1 << 24)) return refuse(what + ": strides must be < 2^24");
+    return BS_OK;
+}
+
+// the workspace of the gradients: d, then the pieces' sums of the one product and, in the same place, of the other
+uint64_t up16(uint64_t n) { return (n + 15) / 16 * 16; }
+uint64_t d_bytes(uint64_t rows, uint32_t cols) { return up16((rows + 63) / 64 * 64 * 2 * cols * 2); }
+uint64_t parts_bytes(uint64_t rows, uint32_t inner, uint32_t cols) {
+    const uint64_t a = splits_of(rows, 2ull * cols, inner), b = splits_of(2ull * cols, rows, inner);
+    return std::max(a > 1 ? a * rows * inner * 4 : 0, b > 1 ? b * 2 * cols * inner * 4 : 0);
+}
+
+}  // namespace
+
+extern "C" int bs_gated(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, void* out,
+                        int64_t out_stride, void* gate, void* up, uint64_t rows, uint32_t inner, uint32_t cols, int type, int activation, void* stream) try {
+    const std::string what = "bs_gated";
+    if (const int rc = check(what, rows, inner, cols)) return rc;
+    if (type != BS_F16 && type != BS_BF16) return refuse(what + ": type must be BS_F16 or BS_BF16");
+    if (activation < BS_ACT_NONE || activation > BS_ACT_SILU) return refuse(what + ": unknown activation " + std::to_string(activation));
+    if (!gate != !up) return refuse(what + ": gate and up must be given together");
+    if (rows == 0) return BS_OK;
+    if (const int rc = check_rows(what, "x", x, x_stride, inner)) return rc;
+    if (const int rc = check_rows(what, "w_gate", w_gate, w_gate_stride, inner)) return rc;
+    if (const int rc = check_rows(what, "w_up", w_up, w_up_stride, inner)) return rc;
+    if (const int rc = check_rows(what, "out", out, out_stride, cols)) return rc;
+    Params p{};
+    p.x = x, p.wg = w_gate, p.wu = w_up, p.h = out, p.gate = gate, p.up = up;
+    p.xs = x_stride, p.wgs = w_gate_stride, p.wus = w_up_stride, p.hs = out_stride;
+    p.rows = static_cast<uint32_t>(rows), p.inner = inner, p.cols = cols, p.act = activation, p.splits = 1;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int rc = type == BS_F16 ? launch_forward<f16>(p, s) : launch_forward<bf16>(p, s);
+    return rc ? rc : launched("bs_gated");
+} catch (...) {
+    return bs_internal_exception();
+}
+
+extern "C" int bs_gated_backward_workspace(uint64_t rows, uint32_t inner, uint32_t cols, uint64_t* bytes) try {
+    if (!bytes) return refuse("bs_gated_backward_workspace: bytes is null");
+    if (const int rc = check("bs_gated_backward_workspace", rows, inner, cols)) return rc;
+    *bytes = rows ? d_bytes(rows, cols) + parts_bytes(rows, inner, cols) : 0;
+    return BS_OK;
+} catch (...) {
+    return bs_internal_exception();
+}
+
+extern "C" int bs_gated_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride,
+                                 const void* w_up, int64_t w_up_stride, const void* gate, int64_t gate_stride, const void* up, int64_t up_stride,
+                                 void* dx, void* dw_gate, void* dw_up, uint64_t rows, uint32_t inner, uint32_t cols, int type, int activation,
+                                 void* workspace, uint64_t workspace_bytes, void* stream) try {
+    const std::string what = "bs_gated_backward";
+    if (const int rc = check(what, rows, inner, cols)) return rc;
+    if (type != BS_F16 && type != BS_BF16) return refuse(what + ": type must be BS_F16 or BS_BF16");
+    if (activation < BS_ACT_NONE || activation > BS_ACT_SILU) return refuse(what + ": unknown activation " + std::to_string(activation));
+    if (!dw_gate != !dw_up) return refuse(what + ": dw_gate and dw_up must be given together");
+    if (!dx && !dw_gate) return BS_OK;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    Params p{};
+    p.x = x, p.wg = w_gate, p.wu = w_up, p.dh = dh, p.g = gate, p.u = up, p.dx = dx, p.dwg = dw_gate, p.dwu = dw_up;
+    p.xs = x_stride, p.wgs = w_gate_stride, p.wus = w_up_stride, p.dhs = dh_stride, p.gs = gate_stride, p.us = up_stride;
+    p.rows = static_cast<uint32_t>(rows), p.inner = inner, p.cols = cols, p.act = activation, p.splits = 1;
+    if (rows) {
+        if (const int rc = check_rows(what, "dh", dh, dh_stride, cols)) return rc;
+        if (const int rc = check_rows(what, "x", x, x_stride, inner)) return rc;
+        if (const int rc = check_rows(what, "w_gate", w_gate, w_gate_stride, inner)) return rc;
+        if (const int rc = check_rows(what, "w_up", w_up, w_up_stride, inner)) return rc;
+        if (const int rc = check_rows(what, "gate", gate, gate_stride, cols)) return rc;
+        if (const int rc = check_rows(what, "up", up, up_stride, cols)) return rc;
+        const uint64_t need = d_bytes(rows, cols) + parts_bytes(rows, inner, cols);
+        if (!workspace || workspace_bytes < need) return refuse(what + ": the workspace must hold " + std::to_string(need) + " bytes");
+        if (!aligned16(workspace)) return refuse(what + ": the workspace must be 16-byte aligned");
+        p.d = static_cast<char*>(workspace);
+        p.parts = reinterpret_cast<float*>(p.d + d_bytes(rows, cols));
+        const int rc = type == BS_F16 ? launch_backward<f16>(p, s) : launch_backward<bf16>(p, s);
+        return rc ? rc : launched("bs_gated_backward");
+    }
+    if (!dw_gate) return BS_OK;
+    // no rows: the weights' gradients are 0, the sums of no pieces' steps
+    const int rc = type == BS_F16 ? start<f16, WEIGHTS, Small, false>(p, s) : start<bf16, WEIGHTS, Small, false>(p, s);
+    return rc ? rc : launched("bs_gated_backward");
+} catch (...) {
+    return bs_internal_exception();
+}

@@ -5,6 +5,8 @@
     z = embed.linear(y, w, b, activation="gelu", residual=None)
     o = embed.attention(q, k, v, offsets, causal=True)
     dx, dweight, dbias = embed.layer_norm_backward(dy, x, mean, rstd, weight)
+    h, gate, up = embed.gated(x, w_gate, w_up, activation="silu", save=True)
+    dx, dw_gate, dw_up = embed.gated_backward(dh, x, w_gate, w_up, gate, up, activation="silu")
     q, k = embed.head_norm_rotary(q, k, positions, frequencies, q_weight, k_weight)
     dq, dk, dq_weight, dk_weight = embed.head_norm_rotary_backward(dq, dk, q, k, positions, frequencies, q_weight, k_weight)
 
@@ -33,7 +35,7 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 LAYOUTS = {"half": 0, "interleaved": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
-__all__ = ["attention", "head_norm_rotary", "head_norm_rotary_backward", "layer_norm", "layer_norm_backward", "linear",
+__all__ = ["attention", "gated", "gated_backward", "head_norm_rotary", "head_norm_rotary_backward", "layer_norm", "layer_norm_backward", "linear",
            "rotary_frequencies", "ACTIVATIONS", "LAYOUTS", "BeamSearchError"]
 
 
@@ -481,3 +483,82 @@ def _rotary_workspace(tokens, heads, kv_heads, dim, rotary, code) -> int:
     b = C.c_uint64(0)
     _check(_lib.hip().bs_head_norm_rotary_backward_workspace(C.byref(a), C.byref(b)), "bs_head_norm_rotary_backward_workspace")
     return b.value
+
+
+def _gated_sizes(what, x, w_gate, w_up, activation):
+    """the type's and the activation's code; rows, inner, cols; strides of x, w_gate and w_up"""
+    type_ = x.dtype
+    if type_ not in _HALF:
+        _fail(f"{what}: x must be a float16 or bfloat16 tensor")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        _fail(f"{what}: unknown activation {activation!r}")
+    n, inner, xs = _rows(what, "x", x)
+    if w_gate.dim() != 2 or w_gate.dtype != type_ or w_up.shape != w_gate.shape or w_up.dtype != type_:
+        _fail(f"{what}: w_gate and w_up must be cols x inner, both of x's type")
+    cols, k, gs = _rows(what, "w_gate", w_gate)
+    if k != inner:
+        _fail(f"{what}: x has {inner} features, w_gate and w_up {k}")
+    return TYPES[type_], act, n, inner, cols, xs, gs, _rows(what, "w_up", w_up)[2]
+
+
+def gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu", save: bool = False,
+          out: Optional[torch.Tensor] = None):
+    """activation(x w_gate^T) * (x w_up^T).  x (..., inner), w_gate and w_up (cols, inner; for instance the halves of one
+    weight) of one type, float16 or bfloat16; the result (..., cols) of that type.  activation: none, relu, gelu, gelu_tanh
+    or silu.  save: returns (result, x w_gate^T, x w_up^T), as gated_backward takes them.  out: where to write the result."""
+    what = "gated"
+    dev = _gpu(what, x, w_gate, w_up, out)
+    code, act, n, inner, cols, xs, gs, us = _gated_sizes(what, x, w_gate, w_up, activation)
+    shape = (n, cols) if x.dim() == 2 else (*x.shape[:-1], cols)
+    if out is None:
+        y, ys = x.new_empty(shape), cols
+    else:
+        y = out
+        if y.shape != shape or y.dtype != x.dtype:
+            _fail(f"{what}: out must be {tuple(shape)} of {x.dtype}")
+        ys = _rows(what, "out", y)[2]
+    gate = up = None
+    if save:
+        gate, up = x.new_empty(shape), x.new_empty(shape)
+    rc = _lib.hip().bs_gated(x.data_ptr(), xs, w_gate.data_ptr(), gs, w_up.data_ptr(), us, y.data_ptr(), ys,
+                             gate.data_ptr() if save else None, up.data_ptr() if save else None, n, inner, cols, code, act,
+                             _raw_stream(dev))
+    if rc:
+        _check(rc, what)
+    return (y, gate, up) if save else y
+
+
+def gated_backward(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
+                   up: torch.Tensor, activation: str = "silu", params: bool = True):
+    """Gradients (dx, dw_gate, dw_up) of gated for the gradient dh of its result and the gate and up that it saved, all of x's
+    type; the weights' are None if params is False.  The sums over the rows have a fixed order."""
+    what = "gated_backward"
+    dev = _gpu(what, x, dh, w_gate, w_up, gate, up)
+    code, act, n, inner, cols, xs, gs, us = _gated_sizes(what, x, w_gate, w_up, activation)
+    shape = (n, cols) if x.dim() == 2 else (*x.shape[:-1], cols)
+    strides = []
+    for name, t in (("dh", dh), ("gate", gate), ("up", up)):
+        if t.shape != shape or t.dtype != x.dtype:
+            _fail(f"{what}: {name} must be {tuple(shape)} of {x.dtype}")
+        strides.append(_rows(what, name, t)[2])
+    dx = _like(x)
+    dwg = dwu = None
+    if params:
+        dwg, dwu = _like(w_gate), _like(w_up)
+    size = _gated_workspace(n, inner, cols)
+    ws = x.new_empty((size,), dtype=torch.uint8)
+    rc = _lib.hip().bs_gated_backward(dh.data_ptr(), strides[0], x.data_ptr(), xs, w_gate.data_ptr(), gs, w_up.data_ptr(), us,
+                                      gate.data_ptr(), strides[1], up.data_ptr(), strides[2], dx.data_ptr(),
+                                      dwg.data_ptr() if params else None, dwu.data_ptr() if params else None, n, inner, cols, code,
+                                      act, ws.data_ptr() if size else None, size, _raw_stream(dev))
+    if rc:
+        _check(rc, what)
+    return dx, dwg, dwu
+
+
+@lru_cache(maxsize=4096)
+def _gated_workspace(rows: int, inner: int, cols: int) -> int:
+    n = C.c_uint64(0)
+    _check(_lib.hip().bs_gated_backward_workspace(rows, inner, cols, C.byref(n)), "bs_gated_backward_workspace")
+    return n.value

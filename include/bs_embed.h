@@ -168,6 +168,26 @@ int bs_head_norm_rotary(const bs_head_norm_rotary_args* args, void* stream);
 int bs_head_norm_rotary_backward(const bs_head_norm_rotary_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
 int bs_head_norm_rotary_backward_workspace(const bs_head_norm_rotary_args* args, uint64_t* bytes);
 
+/* Gated products:  out = act(x w_gate^T) * (x w_up^T),  x rows x inner, w_gate and w_up cols x
+ * inner, out rows x cols, all of `type` (BS_F16 or BS_BF16); inner 1..2^24, cols 1..2^23, strides <
+ * 2^24.  gate and up (rows x cols each, contiguous, or both NULL): x w_gate^T and x w_up^T, as the
+ * gradients take them.  Products are summed and multiplied in float32. */
+int bs_gated(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate_stride, const void* w_up, int64_t w_up_stride,
+             void* out, int64_t out_stride, void* gate, void* up, uint64_t rows, uint32_t inner, uint32_t cols, int type,
+             int activation, void* stream);
+
+/* Its gradients from dh, the gradient of out, and the saved gate and up:
+ *   dgate = dh up act'(gate),  dup = dh act(gate), both rounded to `type` for their products
+ *   dx = dgate w_gate + dup w_up,  dw_gate = dgate^T x,  dw_up = dup^T x
+ * (relu's slope at 0 is 0).  dx (rows x inner) may be NULL, dw_gate and dw_up (cols x inner) too,
+ * both or neither; all contiguous.  The sums over the rows have a fixed order.  workspace:
+ * bs_gated_backward_workspace bytes, 16-byte aligned. */
+int bs_gated_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride, const void* w_gate,
+                      int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, const void* gate, int64_t gate_stride,
+                      const void* up, int64_t up_stride, void* dx, void* dw_gate, void* dw_up, uint64_t rows, uint32_t inner,
+                      uint32_t cols, int type, int activation, void* workspace, uint64_t workspace_bytes, void* stream);
+int bs_gated_backward_workspace(uint64_t rows, uint32_t inner, uint32_t cols, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,3 +72,45 @@ def test_rotary_frequencies():
     for bad in (dict(rotary=7), dict(rotary=-2), dict(rotary=8, base=0.0), dict(rotary=8, stretch=0.0), dict(rotary=8, trained=10, low=3.0, high=3.0)):
         with pytest.raises(ValueError):
             embed.rotary_frequencies(device="cpu", **bad)
+
+
+GATED = [
+    (dict(type=0), "type must be"), (dict(act=5), "unknown activation"), (dict(act=-1), "unknown activation"), (dict(inner=0), "inner must be"),
+    (dict(cols=(1 << 23) + 1), "cols in 1..2^23"), (dict(rows=1 << 31), "rows must be"), (dict(rows=(1 << 31) - 1, cols=128), "too large for one launch"),
+    (dict(x=None), "x must be given"), (dict(wg=None), "w_gate must be given"), (dict(wu=None), "w_up must be given"),
+    (dict(xs=31), "rows of x overlap"), (dict(wus=31), "rows of w_up overlap"), (dict(wgs=1 << 24), "strides must be"),
+]
+
+
+@pytest.mark.parametrize("change,text", GATED + [(dict(out=None), "out must be given"), (dict(os=47), "rows of out overlap"), (dict(gate=PTR), "together")])
+def test_gated_refuses(change, text):
+    a = dict(x=PTR, xs=32, wg=PTR, wgs=32, wu=PTR, wus=32, out=PTR, os=48, gate=None, up=None, rows=4, inner=32, cols=48, type=2, act=4, stream=None) | change
+    refused(_lib.hip().bs_gated(*a.values()), text)
+
+
+@pytest.mark.parametrize("change,text", GATED + [
+    (dict(dh=None), "dh must be given"), (dict(gate=None), "gate must be given"), (dict(us=47), "rows of up overlap"), (dict(dwg=None), "together"),
+    (dict(ws=None), "the workspace must hold"), (dict(size=100), "the workspace must hold"), (dict(ws=PTR + 8), "16-byte aligned")])
+def test_gated_backward_refuses(change, text):
+    a = dict(dh=PTR, dhs=48, x=PTR, xs=32, wg=PTR, wgs=32, wu=PTR, wus=32, gate=PTR, gs=48, up=PTR, us=48, dx=PTR, dwg=PTR, dwu=PTR, rows=4, inner=32,
+             cols=48, type=2, act=4, ws=PTR, size=1 << 30, stream=None) | change
+    refused(_lib.hip().bs_gated_backward(*a.values()), text)
+
+
+def test_gated_workspaces_and_empty_calls():
+    n = C.c_uint64(1)
+    hip = _lib.hip()
+    assert hip.bs_gated_backward_workspace(0, 32, 48, C.byref(n)) == 0 and n.value == 0
+    assert hip.bs_gated_backward_workspace(70, 32, 48, C.byref(n)) == 0 and n.value >= 128 * 96 * 2
+    refused(hip.bs_gated_backward_workspace(4, 4, 4, None), "bytes is null")
+    assert hip.bs_gated(None, 0, None, 0, None, 0, None, 0, None, None, 0, 32, 48, 2, 4, None) == 0
+    assert hip.bs_gated_backward(*[None, 0] * 6, None, None, None, 0, 32, 48, 2, 4, None, 0, None) == 0
+
+
+def test_python_refuses_tensors_off_the_gpu():
+    import torch
+    from beam_search_collab_amd import embed
+    x = torch.zeros(4, 32, dtype=torch.bfloat16)
+    for call in (lambda: embed.gated(x, x, x), lambda: embed.gated_backward(x, x, x, x, x, x), lambda: embed.head_norm_rotary(x[:, None])):
+        with pytest.raises(ValueError, match="on a GPU"):
+            call()

@@ -275,3 +275,201 @@ def test_head_norm_rotary_refusals(gpu):
     ]:
         with pytest.raises(ValueError, match=text):
             call()
+
+
+# ---------------------------------------------------------------- gated products
+
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+
+
+def act_and_slope(z, act):
+    f = torch.nn.functional
+    z = z.detach().requires_grad_()
+    with torch.enable_grad():
+        y = {"none": lambda t: t * 1.0, "relu": f.relu, "gelu": f.gelu, "gelu_tanh": lambda t: f.gelu(t, approximate="tanh"), "silu": f.silu}[act](z)
+        slope, = torch.autograd.grad(y.sum(), z)
+    return y.detach(), slope
+
+
+def check_gated(x, wg, wu, act, h, gate=None, up=None):
+    k = x.shape[-1]
+    xd = x.double()
+    (g, eg), (u, eu) = (((xd @ w.double().t().contiguous()), (k + 4) * E * (xd.abs() @ w.double().abs().t().contiguous())) for w in (wg, wu))
+    a, _ = act_and_slope(g, act)
+    ea = 1.2 * eg  # no activation is steeper than 1.13
+    if act != "none":
+        ea = ea + 16 * E * g.abs() + 2 * E * g * g  # erf, exp: a few units, exp's argument rounded
+    tol = ea * u.abs() + a.abs() * eu + ea * eu + 2 * E * (a * u).abs()
+    near(h, a * u, tol + U[h.dtype] * (a * u).abs() + TINY[h.dtype])
+    for got, want, e in ((gate, g, eg), (up, u, eu)):
+        if got is not None:
+            near(got, want, e + U[h.dtype] * want.abs() + TINY[h.dtype])
+
+
+def check_gated_backward(dh, x, wg, wu, gate, up, act, dx, dwg, dwu):
+    t = x.dtype
+    dh, x, wg, wu, g, u = (y.double() for y in (dh, x, wg, wu, gate, up))
+    a, slope = act_and_slope(g, act)
+    dg, du = dh * u * slope, dh * a
+    # the slope and the activation in float32: their parts are at most 1.13 and |g|; then the rounding to the type
+    eg = (dh * u).abs() * 32 * E + (U[t] + 2 * E) * dg.abs() + TINY[t]
+    eu = dh.abs() * 16 * E * g.abs() * (act != "none") + (U[t] + 2 * E) * du.abs() + TINY[t]
+    n = 2 * g.shape[1] + 8
+    want = dg @ wg + du @ wu
+    tol = eg @ wg.abs() + eu @ wu.abs() + n * E * (dg.abs() @ wg.abs() + du.abs() @ wu.abs()) * 1.01
+    near(dx, want, tol + U[t] * want.abs() + TINY[t])
+    for got, d, e in ((dwg, dg, eg), (dwu, du, eu)):
+        if got is not None:
+            want = d.t().contiguous() @ x
+            tol = e.t().contiguous() @ x.abs() + (len(x) + 8) * E * (d.abs().t().contiguous() @ x.abs()) * 1.01
+            near(got, want, tol + U[t] * want.abs() + TINY[t])
+
+
+GATED = [(1, 1, 1), (1, 1024, 128), (2, 100, 3), (5, 63, 65), (16, 64, 128), (17, 4096, 256), (31, 200, 96), (32, 256, 512), (33, 257, 131),
+         (64, 1024, 64), (65, 72, 1000), (100, 1000, 300), (127, 128, 127), (128, 128, 128), (129, 192, 257), (200, 1088, 128), (255, 64, 255),
+         (256, 512, 256), (257, 520, 264), (300, 768, 2048), (1000, 96, 777), (513, 1024, 1024), (1111, 333, 222), (0, 64, 32), (29, 72, 4109)]
+
+
+def gated_case(seed, rows, inner, cols, dtype):
+    return rand(seed, rows, inner, dtype=dtype), rand(seed + 1, cols, inner, dtype=dtype, std=inner ** -0.5), rand(seed + 2, cols, inner, dtype=dtype, std=inner ** -0.5)
+
+
+@pytest.mark.parametrize("rows,inner,cols", GATED)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gated(gpu, rows, inner, cols, dtype):
+    x, wg, wu = gated_case(200, rows, inner, cols, dtype)
+    act = ACTS[(rows + cols) % 5]
+    h, gate, up = embed.gated(x, wg, wu, activation=act, save=True)
+    check_gated(x, wg, wu, act, h, gate, up)
+    assert torch.equal(h, embed.gated(x, wg, wu, activation=act))
+
+
+@pytest.mark.parametrize("rows,inner,cols", GATED)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gated_backward(gpu, rows, inner, cols, dtype):
+    x, wg, wu = gated_case(210, rows, inner, cols, dtype)
+    act = ACTS[(rows + cols + 1) % 5]
+    gate, up, dh = rand(214, rows, cols, dtype=dtype, std=1.5), rand(215, rows, cols, dtype=dtype), rand(216, rows, cols, dtype=dtype, std=0.3)
+    got = embed.gated_backward(dh, x, wg, wu, gate, up, activation=act)
+    assert [g.shape for g in got] == [x.shape, wg.shape, wu.shape]
+    check_gated_backward(dh, x, wg, wu, gate, up, act, *got)
+    assert all(torch.equal(a, b) for a, b in zip(got, embed.gated_backward(dh, x, wg, wu, gate, up, activation=act)))
+    only = embed.gated_backward(dh, x, wg, wu, gate, up, activation=act, params=False)
+    assert torch.equal(only[0], got[0]) and only[1] is None and only[2] is None
+
+
+@pytest.mark.parametrize("rows,inner,cols", [(4096, 128, 2048), (4111, 192, 2112), (300, 320, 16500), (8200, 256, 1001), (8000, 72, 512), (2000, 2048, 768)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gated_of_many_tiles(gpu, rows, inner, cols, dtype):
+    """more tiles than compute units, shifted ones at the edges"""
+    x, wg, wu = gated_case(220, rows, inner, cols, dtype)
+    h, gate, up = embed.gated(x, wg, wu, save=True)
+    check_gated(x, wg, wu, "silu", h, gate, up)
+    wide = torch.full((rows, cols + 9), 7.0, dtype=dtype, device="cuda")
+    embed.gated(x, wg, wu, out=wide[:, 3:cols + 3])
+    assert torch.equal(wide[:, 3:cols + 3], h) and (wide[:, :3] == 7).all() and (wide[:, cols + 3:] == 7).all()
+    dh = rand(223, rows, cols, dtype=dtype, std=0.3)
+    got = embed.gated_backward(dh, x, wg, wu, gate, up)
+    check_gated_backward(dh, x, wg, wu, gate, up, "silu", *got)
+    assert all(torch.equal(a, b) for a, b in zip(got, embed.gated_backward(dh, x, wg, wu, gate, up)))
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_gated_activations_far_from_zero(gpu, act):
+    """slopes where exponentials overflow, vanish or cancel"""
+    z = torch.cat([torch.linspace(-12, 12, 200), torch.tensor([-3e4, -200.0, -90.0, -40.0, 0.0, 40.0, 90.0, 200.0, 3e4, -1e-3, 1e-3, 60.0])])
+    for dtype in (F16, BF16):
+        gate = z.to(dtype).cuda()[:, None].repeat(1, 64)
+        up, dh, x = rand(230, len(z), 64, dtype=dtype), rand(231, len(z), 64, dtype=dtype, std=0.1), rand(232, len(z), 64, dtype=dtype)
+        wg, wu = (torch.eye(64, dtype=dtype, device="cuda") for _ in range(2))
+        dx, _, _ = embed.gated_backward(dh, x, wg, 0 * wu, gate, up, activation=act)
+        check_gated_backward(dh, x, wg, 0 * wu, gate, up, act, dx, None, None)
+        dx, _, _ = embed.gated_backward(dh, x, 0 * wg, wu, gate, up, activation=act)
+        check_gated_backward(dh, x, 0 * wg, wu, gate, up, act, dx, None, None)
+
+
+@pytest.mark.parametrize("rows,inner,cols", [(3, 64, 40), (20, 1000, 320), (130, 96, 140), (520, 512, 512)])
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_gated_of_slices(gpu, rows, inner, cols, shift):
+    """operands inside wider tensors, at any element; the weights are halves of one"""
+    x = rand(240, rows, inner + 24, dtype=F16)[:, shift:shift + inner]
+    both = rand(241, 2 * cols, inner + 16, dtype=F16, std=inner ** -0.5)[:, shift:shift + inner]
+    wg, wu = both[:cols], both[cols:]
+    cut = [rand(242 + i, rows, cols + 16, dtype=F16)[:, shift:shift + cols] for i in range(3)]
+    plain = [t.contiguous() for t in (x, wg, wu, *cut)]
+    h = embed.gated(x, wg, wu, activation="gelu")
+    assert torch.equal(h, embed.gated(*plain[:3], activation="gelu")) or shift  # another kernel may take them
+    check_gated(x, wg, wu, "gelu", h)
+    got = embed.gated_backward(cut[0], x, wg, wu, cut[1], cut[2], activation="gelu")
+    check_gated_backward(cut[0], x, wg, wu, cut[1], cut[2], "gelu", *got)
+    assert all(t.is_contiguous() for t in got)
+
+
+def test_gated_leading_dimensions_and_not_finite(gpu):
+    x, wg, wu = rand(250, 2, 3, 70, dtype=BF16), rand(251, 50, 70, dtype=BF16), rand(252, 50, 70, dtype=BF16)
+    h, gate, up = embed.gated(x, wg, wu, save=True)
+    assert h.shape == gate.shape == (2, 3, 50)
+    dx, dwg, _ = embed.gated_backward(h, x, wg, wu, gate, up)
+    assert dx.shape == x.shape and dwg.shape == wg.shape
+    for rows in (6, 200, 700):
+        x, wg, wu = gated_case(253, rows, 320, 256, BF16)
+        gate, up, dh = (rand(256 + i, rows, 256, dtype=BF16) for i in range(3))
+        x[3, 299] = math.nan
+        h = embed.gated(x, wg, wu)
+        rest = torch.arange(rows, device="cuda") != 3
+        assert torch.isnan(h[3]).all() and torch.isfinite(h[rest]).all()
+        dh[rows - 1, 5] = math.inf  # of the last row, whose successors do not exist
+        dx, dwg, dwu = embed.gated_backward(dh, x, wg, wu, gate, up)
+        assert torch.isfinite(dx[:-1]).all() and not torch.isfinite(dx[-1]).any()
+        one = torch.arange(256, device="cuda") != 5
+        keep = torch.arange(320, device="cuda") != 299
+        assert torch.isfinite(dwg[one][:, keep]).all() and torch.isnan(dwg[:, 299]).all() and not torch.isfinite(dwg[5]).any()
+        x[3, 299], dh[rows - 1, 5], x[rows - 1, 7] = 0.0, 0.0, math.inf
+        _, dwg, _ = embed.gated_backward(dh, x, wg, wu, gate, up)
+        want = torch.where(dh[-1] * up[-1] == 0, math.nan, math.inf)  # 0 times infinity
+        assert torch.equal(torch.isnan(dwg[:, 7]), torch.isnan(want)) and not torch.isfinite(dwg[:, 7]).any()
+        assert torch.isfinite(dwg[:, torch.arange(320, device="cuda") != 7]).all()
+
+
+def test_gated_backward_against_differences(gpu):
+    """directional derivatives of the definition in 64 bits; the gradients' own error is that of the types"""
+    rows, inner, cols, h = 40, 24, 56, 1e-6
+    x, wg, wu = gated_case(260, rows, inner, cols, F16)
+    dh = rand(263, rows, cols, dtype=F16)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        _, gate, up = embed.gated(x, wg, wu, activation=act, save=True)
+        got = embed.gated_backward(dh, x, wg, wu, gate, up, activation=act)
+
+        def loss(x, wg, wu):
+            return (act_and_slope(x @ wg.t(), act)[0] * (x @ wu.t()) * dh.double()).sum().item()
+        for t in range(3):
+            for i, g in enumerate(got):
+                d = rand(270 + t, *g.shape).double()
+                args = [y.double() for y in (x, wg, wu)]
+                up_, down = list(args), list(args)
+                up_[i], down[i] = args[i] + h * d, args[i] - h * d
+                slope = (loss(*up_) - loss(*down)) / (2 * h)
+                # saved values, d and the result are rounded: 5 roundings, none of which moves a term by more than 2^-11 (the
+                # second derivatives of the activations are below 1.13)
+                assert abs(slope - (g.double() * d).sum().item()) <= 8 * 2.0 ** -11 * (g.double() * d).abs().sum().item()
+
+
+def test_gated_refusals(gpu):
+    x, w = rand(1, 4, 64, dtype=BF16), rand(2, 32, 64, dtype=BF16)
+    h = rand(3, 4, 32, dtype=BF16)
+    for call, text in [
+        (lambda: embed.gated(x.float(), w, w), "x must be"),
+        (lambda: embed.gated(x, w[:, :32], w[:, :32]), "x has 64 features"),
+        (lambda: embed.gated(x, w, w[:31]), "both of x's type"),
+        (lambda: embed.gated(x, w.half(), w), "both of x's type"),
+        (lambda: embed.gated(x, w, w, activation="tanh"), "unknown activation"),
+        (lambda: embed.gated(x, w, w, out=h.float()), "out must be"),
+        (lambda: embed.gated(x, w.cpu(), w), "must be a tensor on"),
+        (lambda: embed.gated(x, torch.nn.Parameter(w), w), "gradient"),
+        (lambda: embed.gated_backward(h[:3], x, w, w, h, h), "dh must be"),
+        (lambda: embed.gated_backward(h, x, w, w, h, h.float()), "up must be"),
+        (lambda: embed.gated_backward(h, x, w, w, h[:, :31], h), "gate must be"),
+        (lambda: embed.gated_backward(h, x, w, w, h.t().contiguous().t(), h), "features of gate"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            call()

@@ -65,6 +65,12 @@ class AttentionArgs(C.Structure):
     )
 
 
+class AttentionPrefix(C.Structure):
+    """bs_attention_prefix (include/bs_embed.h)."""
+    _fields_ = [("k", vp), ("v", vp), ("k_stride", i64), ("k_head_stride", i64), ("v_stride", i64), ("v_head_stride", i64),
+                ("tokens", u32)]
+
+
 class HeadNormRotaryArgs(C.Structure):
     """bs_head_norm_rotary_args (include/bs_embed.h)."""
     _fields_ = (
@@ -119,6 +125,8 @@ EMBED_API = {
     "bs_linear_workspace": (C.c_int, [u64, u32, u32, P(u64)]),
     "bs_attention": (C.c_int, [P(AttentionArgs), vp, u64, vp]),
     "bs_attention_workspace": (C.c_int, [P(AttentionArgs), P(u64)]),
+    "bs_attention_shared_prefix": (C.c_int, [P(AttentionArgs), P(AttentionPrefix), vp, u64, vp]),
+    "bs_attention_shared_prefix_workspace": (C.c_int, [P(AttentionArgs), P(AttentionPrefix), P(u64)]),
     "bs_gated": (C.c_int, [vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, u64, u32, u32, C.c_int, C.c_int, vp]),
     "bs_gated_backward": (C.c_int, [vp, i64] * 6 + [vp, vp, vp, u64, u32, u32, C.c_int, C.c_int, vp, u64, vp]),
     "bs_gated_backward_workspace": (C.c_int, [u64, u32, u32, P(u64)]),

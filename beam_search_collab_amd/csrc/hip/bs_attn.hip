@@ -23,10 +23,12 @@ struct Params {
     bs_attention_args a;
     uint32_t group;    // heads per key/value head
     Divisor by_group, by_kv;
-    uint32_t splits;   // pieces of the keys; > 1: parts go to the workspace
+    uint32_t splits;   // pieces of the keys
     uint32_t piece;    // keys of a piece, a multiple of BN
-    float* part_out;   // splits x q_tokens x heads x head_dim: sums of p v, unscaled
-    float2* part_stat; // splits x q_tokens x heads: maximum (in units of log2) and sum
+    uint32_t before;   // parts of a row that another launch writes, in front of these
+    float* part_out;   // null, or where parts go: (before + splits) x q_tokens x heads x head_dim, sums of p v, unscaled
+    float2* part_stat; // as many x q_tokens x heads: maximum (in units of log2) and sum
+    bs_attention_prefix prefix; // keys that every row sees besides its sequence's
 };
 
 struct Sequence {
@@ -367,11 +369,13 @@ struct Mover {
     uint32_t nk, chunks, first;
     int row, wave;
 
-    __device__ Mover(const bs_attention_args& a, const Sequence& sq, uint32_t kvh, int thread)
-        : khop(a.k_stride * 2), vhop(a.v_stride * 2), nk(sq.nk), chunks(a.head_dim / 8), row(thread / CH),
+    // `a`: the call's arguments, or the prefix
+    template <typename A>
+    __device__ Mover(const A& a, uint32_t k0, uint32_t nk_, uint32_t head_dim, uint32_t kvh, int thread)
+        : khop(a.k_stride * 2), vhop(a.v_stride * 2), nk(nk_), chunks(head_dim / 8), row(thread / CH),
           wave(uniform(static_cast<uint32_t>(thread >> 6))) {
-        k = static_cast<const char*>(a.k) + static_cast<int64_t>(sq.k0) * khop + static_cast<int64_t>(kvh) * a.k_head_stride * 2;
-        v = static_cast<const char*>(a.v) + static_cast<int64_t>(sq.k0) * vhop + static_cast<int64_t>(kvh) * a.v_head_stride * 2;
+        k = static_cast<const char*>(a.k) + static_cast<int64_t>(k0) * khop + static_cast<int64_t>(kvh) * a.k_head_stride * 2;
+        v = static_cast<const char*>(a.v) + static_cast<int64_t>(k0) * vhop + static_cast<int64_t>(kvh) * a.v_head_stride * 2;
         kat = row * static_cast<uint32_t>(khop);
         vat = row * static_cast<uint32_t>(vhop);
         first = (place<S>(row, thread % CH) - row * S) >> 4;
@@ -426,8 +430,8 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
     if (!me.live) return;
     const bs_attention_args& a = p.a;
     const int64_t at = static_cast<int64_t>(sq.q0 + me.tok) * a.heads + me.head;
-    if (p.splits > 1) {
-        const int64_t slot = static_cast<int64_t>(blockIdx.y) * a.q_tokens * a.heads + at;
+    if (p.part_out) {
+        const int64_t slot = static_cast<int64_t>(p.before + blockIdx.y) * a.q_tokens * a.heads + at;
         if (h == 0) p.part_stat[slot] = make_float2(r.top, r.sum);
         float* out = p.part_out + slot * a.head_dim;
 #pragma unroll
@@ -466,7 +470,9 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 // dependent rounds of loads with which each of the 3864 short workgroups starts.  Other orders that were slower for
 // the documents: two groups of waves half a step apart, meeting between their phases (1244 against 1175), moves between
 // the products and exponentials instead of before them (1246 against 1142).
-template <typename T, int DP>
+//
+// Prefix: behind the sequence's own keys the tiles of the prefix, which every row sees, the last of them in part.
+template <typename T, int DP, bool Prefix>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params p) {
     constexpr int ROWS = 128, S = ROW<DP>, TILE = BN * S;
     // blocks of 32 keys at a time in the tiles that some row does not see whole: one where heads are short, for its code
@@ -502,8 +508,19 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     }
     if (threadIdx.x == 0) flag = 0;
     settle();
-    const Mover<S, BN, 256> mover(a, sq, kvh, threadIdx.x);
-    if (tiles) mover.any(start(0), lds[0]);
+    const Mover<S, BN, 256> mover(a, sq.k0, sq.nk, a.head_dim, kvh, threadIdx.x);
+    const uint32_t shared = Prefix ? p.prefix.tokens : 0, shared_whole = shared / BN, shared_tiles = (shared + BN - 1) / BN;
+    auto bring = [&](uint32_t u, char* to) {  // tile u of the prefix
+        const Mover<S, BN, 256> front(p.prefix, 0, shared, a.head_dim, kvh, threadIdx.x);
+        if (u < shared_whole)
+            front.near(u * BN, to);
+        else if (u < shared_tiles)
+            front.any(u * BN, to);
+    };
+    if (tiles)
+        mover.any(start(0), lds[0]);
+    else if (Prefix)
+        bring(0, lds[0]);
     const Place me = place_of(p, sq, kvh, row0 + wave * 32 + l, rows);
     Rows<T, DP> me_;
     me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
@@ -519,7 +536,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
         for (uint32_t t = 0; t < parts; ++t) {
             char* tk = lds[t & 1];
             meet();  // tile t is in LDS, and nobody reads tile t - 1 any more
-            if (t + 1 < tiles) mover.any(start(t + 1), lds[~t & 1]);
+            if (t + 1 < tiles)
+                mover.any(start(t + 1), lds[~t & 1]);
+            else if (Prefix)
+                bring(t + 1 - tiles, lds[~t & 1]);
             if (start(t) + BN > all || pass != PLAIN) {
                 if (start(t) + BN > all) blank<S>(tk + TILE, all - start(t), BN, threadIdx.x, 256);  // start(t) < ke <= all
                 settle();
@@ -550,12 +570,34 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     for (uint32_t t = parts; t < tiles; ++t) {
         const char* tk = lds[t & 1];
         meet();
-        if (t + 1 < tiles) mover.near(kb + (t + 1 - parts) * BN, lds[~t & 1]);
+        if (t + 1 < tiles)
+            mover.near(kb + (t + 1 - parts) * BN, lds[~t & 1]);
+        else if (Prefix)
+            bring(t + 1 - tiles, lds[~t & 1]);
         if (reach) {
             // a loop of one turn: as a block of its own the step is scheduled apart from the moves (documents: 989 us, 1004
             // in one block with them)
 #pragma unroll 1
             for (int b = 0; b < BN; b += 64) me_.template step<2, false>(tk + b * S, tk + TILE + b * S, 0, 0, scale, lane);
+        }
+    }
+    if constexpr (Prefix) {
+        for (uint32_t u = 0; u < shared_tiles; ++u) {
+            char* tk = lds[(tiles + u) & 1];
+            meet();
+            bring(u + 1, lds[~(tiles + u) & 1]);
+            if (u < shared_whole) {
+                if (wave0 < rows) {
+#pragma unroll 1
+                    for (int b = 0; b < BN; b += 64) me_.template step<2, false>(tk + b * S, tk + TILE + b * S, 0, 0, scale, lane);
+                }
+            } else {
+                blank<S>(tk + TILE, shared - u * BN, BN, threadIdx.x, 256);
+                settle();
+#pragma unroll 1
+                for (int b = 0; b < BN; b += KB * 32)
+                    if (wave0 < rows && u * BN + b < shared) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, u * BN + b, shared, scale, lane);
+            }
         }
     }
     me_.join_halves();
@@ -596,7 +638,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     if (a.head_dim != DP) {  // the padding of the heads is never moved to
         for (int i = lane; i < 32768 / 16; i += 64) reinterpret_cast<Vec<float, 4>*>(mem)[i] = Vec<float, 4>{};
     }
-    const Mover<S, KN, 64> mover(a, sq, kvh, lane);
+    const Mover<S, KN, 64> mover(a, sq.k0, sq.nk, a.head_dim, kvh, lane);
     const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * LOG2E;
     const uint32_t mine = min(me.keys, ke), seen = keys_of(a, sq, p.by_group.quotient(row0));
     // tiles from the last to the first: of those that some row does not see whole (at most 2 in a row: a
@@ -697,8 +739,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
         }
         const Place x = place_of(p, sq, kvh, row0 + r, rows);
         const int64_t at = static_cast<int64_t>(sq.q0 + x.tok) * a.heads + x.head;
-        if (p.splits > 1) {
-            const int64_t slot = static_cast<int64_t>(blockIdx.y) * a.q_tokens * a.heads + at;
+        if (p.part_out) {
+            const int64_t slot = static_cast<int64_t>(p.before + blockIdx.y) * a.q_tokens * a.heads + at;
             *reinterpret_cast<f32x4*>(p.part_out + slot * a.head_dim + e) = v;
             if (e == 0) p.part_stat[slot] = make_float2(t, sum);
         } else {
@@ -727,7 +769,7 @@ __global__ __launch_bounds__(256) void join_kernel(Params p) {
     const Sequence sq = sequence(a, seq);
     if (tok < sq.q0 || tok - sq.q0 >= sq.nq) return;
     const uint32_t keys = keys_of(a, sq, tok - sq.q0);
-    const uint32_t n = max(1u, min(p.splits, (keys + p.piece - 1) / p.piece));
+    const uint32_t n = p.before + max(1u, min(p.splits, (keys + p.piece - 1) / p.piece));
     float top = NONE, sum = 0.0f;
     for (uint32_t s = lane; s < n; s += 64) top = fmaxf(top, p.part_stat[s * rows + at].x);
 #pragma unroll
@@ -849,26 +891,113 @@ template <typename T, int DP>
 int start(const Params& p, hipStream_t s) {
     if (!near_of(p.a)) return start_few<T, DP, false>(p, s);  // rows too far apart for the other kernel's moves
     if (few_of(p.a)) return start_few<T, DP, true>(p, s);
-    attention_kernel<T, DP><<<dim3(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits), 256, 0, s>>>(p);
+    attention_kernel<T, DP, false><<<dim3(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits), 256, 0, s>>>(p);
+    return BS_OK;
+}
+template <typename T, int DP>
+int start_along(const Params& p, hipStream_t s) {
+    attention_kernel<T, DP, true><<<static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), 256, 0, s>>>(p);
     return BS_OK;
 }
 
 template <typename T>
-int launch(const Params& p, hipStream_t s) {
+int start_any(const Params& p, hipStream_t s) {
     const uint32_t d = p.a.head_dim;
-    const int rc = d <= 32 ? start<T, 32>(p, s) : d <= 64 ? start<T, 64>(p, s) : d <= 96 ? start<T, 96>(p, s) : start<T, 128>(p, s);
-    if (rc) return rc;
-    if (p.splits > 1) {
-        // Four waves a row where rows are few and their latency counts, one where there are many.  One and four: 1000 tokens
-        // over 4096 keys, 16 heads of 64 38 and 54 us, 768 over 8192, 32 heads of 128 117 and 137, 8 x 8 over 4096 (2048
-        // rows) 38.5 and 39.2; but 40 over 8192 (1280 rows) 26.4 and 25.5, one token over 16384 24.0 and 20.3.
-        const uint32_t rows = p.a.q_tokens * p.a.heads;
-        if (rows >= 8 * CUS)
-            join_kernel<T, 1><<<(rows + 3) / 4, 256, 0, s>>>(p);
-        else
-            join_kernel<T, 4><<<rows, 256, 0, s>>>(p);
-    }
+    return d <= 32 ? start<T, 32>(p, s) : d <= 64 ? start<T, 64>(p, s) : d <= 96 ? start<T, 96>(p, s) : start<T, 128>(p, s);
+}
+template <typename T>
+void join(const Params& p, hipStream_t s) {
+    // Four waves a row where rows are few and their latency counts, one where there are many.  One and four: 1000 tokens
+    // over 4096 keys, 16 heads of 64 38 and 54 us, 768 over 8192, 32 heads of 128 117 and 137, 8 x 8 over 4096 (2048
+    // rows) 38.5 and 39.2; but 40 over 8192 (1280 rows) 26.4 and 25.5, one token over 16384 24.0 and 20.3.
+    const uint32_t rows = p.a.q_tokens * p.a.heads;
+    if (rows >= 8 * CUS)
+        join_kernel<T, 1><<<(rows + 3) / 4, 256, 0, s>>>(p);
+    else
+        join_kernel<T, 4><<<rows, 256, 0, s>>>(p);
+}
+template <typename T>
+int launch(const Params& p, hipStream_t s) {
+    if (const int rc = start_any<T>(p, s)) return rc;
+    if (p.splits > 1) join<T>(p, s);
     return launched("bs_attention");
+}
+
+// ------------------------------------------------------------------------------------------------ a shared prefix
+
+// the rows of all sequences over the prefix: one sequence, whose queries see all of it
+bs_attention_args over_prefix(const bs_attention_args& a, const bs_attention_prefix& f) {
+    bs_attention_args b = a;
+    b.k = f.k, b.v = f.v, b.k_stride = f.k_stride, b.k_head_stride = f.k_head_stride, b.v_stride = f.v_stride, b.v_head_stride = f.v_head_stride;
+    b.q_offsets = b.k_offsets = nullptr;
+    b.sequences = 1;
+    b.k_tokens = f.tokens;
+    b.longest_q = b.longest_k = 0;
+    b.causal = 0;
+    return b;
+}
+// Whether the sequences' tiles go along the prefix, each for itself, instead of the rows of all sequences at once apart from
+// their own keys.
+bool along_of(const bs_attention_args& a) {
+    const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * (a.heads / a.kv_heads);
+    return rows / a.sequences >= 64 && tiles_of(a, 128) * a.kv_heads >= 2 * CUS;
+}
+struct Apart {
+    Params front, own;
+    uint64_t bytes;
+};
+Apart apart(const bs_attention_args& a, const bs_attention_prefix& f) {
+    Apart x{};
+    x.front.a = over_prefix(a, f);
+    x.own.a = a;
+    split(x.front.a, x.front.splits, x.front.piece);
+    split(x.own.a, x.own.splits, x.own.piece);
+    x.own.before = x.front.splits;
+    for (Params* p : {&x.front, &x.own}) {
+        p->group = a.heads / a.kv_heads;
+        p->by_group = Divisor(p->group);
+        p->by_kv = Divisor(a.kv_heads);
+    }
+    x.bytes = static_cast<uint64_t>(x.front.splits + x.own.splits) * a.q_tokens * a.heads * (a.head_dim + 2) * sizeof(float);
+    return x;
+}
+template <typename T>
+int launch_prefix(const Params& p, void* workspace, hipStream_t s) {
+    const uint32_t d = p.a.head_dim;
+    if (along_of(p.a)) {
+        const int rc = d <= 32 ? start_along<T, 32>(p, s) : d <= 64 ? start_along<T, 64>(p, s) : d <= 96 ? start_along<T, 96>(p, s) : start_along<T, 128>(p, s);
+        return rc ? rc : launched("bs_attention_shared_prefix");
+    }
+    Apart x = apart(p.a, p.prefix);
+    for (Params* q : {&x.front, &x.own}) {
+        q->part_out = static_cast<float*>(workspace);
+        q->part_stat = reinterpret_cast<float2*>(q->part_out + static_cast<uint64_t>(x.front.splits + x.own.splits) * p.a.q_tokens * p.a.heads * d);
+        if (const int rc = start_any<T>(*q, s)) return rc;
+    }
+    join<T>(x.own, s);
+    return launched("bs_attention_shared_prefix");
+}
+
+int check_rows(const std::string& what, const bs_attention_args& a) {
+    if (a.sequences > 1 && (!a.q_offsets || !a.k_offsets)) return refuse(what + ": several sequences need q_offsets and k_offsets");
+    return BS_OK;
+}
+bool stride_ok(const bs_attention_args& a, const void* p, int64_t s, int64_t hs, uint32_t heads, uint32_t tokens) {
+    return aligned16(p) && (tokens <= 1 || (s >= a.head_dim && s % 8 == 0)) && (heads <= 1 || (hs >= a.head_dim && hs % 8 == 0));
+}
+int check_pointers(const std::string& what, const bs_attention_args& a) {
+    if (!a.q || !a.out || (a.k_tokens && (!a.k || !a.v))) return refuse(what + ": q, k, v and out must be given");
+    if (!stride_ok(a, a.q, a.q_stride, a.q_head_stride, a.heads, a.q_tokens) || !stride_ok(a, a.out, a.out_stride, a.out_head_stride, a.heads, a.q_tokens) ||
+        (a.k_tokens && (!stride_ok(a, a.k, a.k_stride, a.k_head_stride, a.kv_heads, a.k_tokens) || !stride_ok(a, a.v, a.v_stride, a.v_head_stride, a.kv_heads, a.k_tokens))))
+        return refuse(what + ": base addresses must be multiples of 16 bytes, strides multiples of 8 and >= head_dim");
+    return BS_OK;
+}
+int check_prefix(const std::string& what, const bs_attention_args* a, const bs_attention_prefix* f) {
+    if (const int rc = check(what.c_str(), a)) return rc;
+    if (!f) return refuse(what + ": prefix is null");
+    if (f->tokens > 0x7FFFFFFFu) return refuse(what + ": tokens of the prefix must be < 2^31");
+    const bs_attention_args b = over_prefix(*a, *f);
+    return check(what.c_str(), &b);
 }
 
 }  // namespace
@@ -885,15 +1014,9 @@ extern "C" int bs_attention_workspace(const bs_attention_args* args, uint64_t* b
 extern "C" int bs_attention(const bs_attention_args* args, void* workspace, uint64_t workspace_bytes, void* stream) try {
     if (const int rc = check("bs_attention", args)) return rc;
     const bs_attention_args& a = *args;
-    if (a.sequences > 1 && (!a.q_offsets || !a.k_offsets)) return refuse("bs_attention: several sequences need q_offsets and k_offsets");
+    if (const int rc = check_rows("bs_attention", a)) return rc;
     if (a.q_tokens == 0) return BS_OK;
-    if (!a.q || !a.out || (a.k_tokens && (!a.k || !a.v))) return refuse("bs_attention: q, k, v and out must be given");
-    auto stride_ok = [&](const void* p, int64_t s, int64_t hs, uint32_t heads, uint32_t tokens) {
-        return aligned16(p) && (tokens <= 1 || (s >= a.head_dim && s % 8 == 0)) && (heads <= 1 || (hs >= a.head_dim && hs % 8 == 0));
-    };
-    if (!stride_ok(a.q, a.q_stride, a.q_head_stride, a.heads, a.q_tokens) || !stride_ok(a.out, a.out_stride, a.out_head_stride, a.heads, a.q_tokens) ||
-        (a.k_tokens && (!stride_ok(a.k, a.k_stride, a.k_head_stride, a.kv_heads, a.k_tokens) || !stride_ok(a.v, a.v_stride, a.v_head_stride, a.kv_heads, a.k_tokens))))
-        return refuse("bs_attention: base addresses must be multiples of 16 bytes, strides multiples of 8 and >= head_dim");
+    if (const int rc = check_pointers("bs_attention", a)) return rc;
     Params p{};
     p.a = a;
     p.group = a.heads / a.kv_heads;
@@ -908,6 +1031,51 @@ extern "C" int bs_attention(const bs_attention_args* args, void* workspace, uint
         p.part_stat = reinterpret_cast<float2*>(p.part_out + static_cast<uint64_t>(p.splits) * a.q_tokens * a.heads * a.head_dim);
     }
     return a.type == BS_F16 ? launch<f16>(p, static_cast<hipStream_t>(stream)) : launch<bf16>(p, static_cast<hipStream_t>(stream));
+} catch (...) {
+    return bs_internal_exception();
+}
+
+extern "C" int bs_attention_shared_prefix_workspace(const bs_attention_args* args, const bs_attention_prefix* prefix, uint64_t* bytes) try {
+    const std::string what = "bs_attention_shared_prefix_workspace";
+    if (!bytes) return refuse(what + ": bytes is null");
+    if (const int rc = check_prefix(what, args, prefix)) return rc;
+    if (prefix->tokens == 0) {
+        *bytes = workspace_of(*args);
+        return BS_OK;
+    }
+    *bytes = along_of(*args) ? 0 : apart(*args, *prefix).bytes;
+    return BS_OK;
+} catch (...) {
+    return bs_internal_exception();
+}
+
+extern "C" int bs_attention_shared_prefix(const bs_attention_args* args, const bs_attention_prefix* prefix, void* workspace, uint64_t workspace_bytes,
+                                          void* stream) try {
+    const std::string what = "bs_attention_shared_prefix";
+    if (const int rc = check_prefix(what, args, prefix)) return rc;
+    const bs_attention_args& a = *args;
+    const bs_attention_prefix& f = *prefix;
+    if (f.tokens == 0) return bs_attention(args, workspace, workspace_bytes, stream);
+    if (const int rc = check_rows(what, a)) return rc;
+    if (a.q_tokens == 0) return BS_OK;
+    if (const int rc = check_pointers(what, a)) return rc;
+    if (!f.k || !f.v) return refuse(what + ": k and v of the prefix must be given");
+    if (!stride_ok(a, f.k, f.k_stride, f.k_head_stride, a.kv_heads, f.tokens) || !stride_ok(a, f.v, f.v_stride, f.v_head_stride, a.kv_heads, f.tokens))
+        return refuse(what + ": base addresses of the prefix must be multiples of 16 bytes, strides multiples of 8 and >= head_dim");
+    if (!near_of(a) || f.k_stride >= (1 << 22) || f.v_stride >= (1 << 22)) return refuse(what + ": strides of keys and values must be < 2^22");
+    Params p{};
+    p.a = a;
+    p.prefix = f;
+    p.group = a.heads / a.kv_heads;
+    p.by_group = Divisor(p.group);
+    p.by_kv = Divisor(a.kv_heads);
+    p.splits = 1;
+    if (!along_of(a)) {
+        const uint64_t need = apart(a, f).bytes;
+        if (!workspace || workspace_bytes < need) return refuse(what + ": the workspace must hold " + std::to_string(need) + " bytes");
+        if (!aligned16(workspace)) return refuse(what + ": the workspace must be 16-byte aligned");
+    }
+    return a.type == BS_F16 ? launch_prefix<f16>(p, workspace, static_cast<hipStream_t>(stream)) : launch_prefix<bf16>(p, workspace, static_cast<hipStream_t>(stream));
 } catch (...) {
     return bs_internal_exception();
 }

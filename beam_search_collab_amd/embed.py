@@ -5,6 +5,7 @@
     z = embed.linear(y, w, b, activation="gelu", residual=None)
     o = embed.attention(q, k, v, offsets, causal=True)
     dx, dweight, dbias = embed.layer_norm_backward(dy, x, mean, rstd, weight)
+    o = embed.attention_shared_prefix(q, k, v, prefix_k, prefix_v, offsets)
     h, gate, up = embed.gated(x, w_gate, w_up, activation="silu", save=True)
     dx, dw_gate, dw_up = embed.gated_backward(dh, x, w_gate, w_up, gate, up, activation="silu")
     q, k = embed.head_norm_rotary(q, k, positions, frequencies, q_weight, k_weight)
@@ -35,7 +36,7 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 LAYOUTS = {"half": 0, "interleaved": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
-__all__ = ["attention", "gated", "gated_backward", "head_norm_rotary", "head_norm_rotary_backward", "layer_norm", "layer_norm_backward", "linear",
+__all__ = ["attention", "attention_shared_prefix", "gated", "gated_backward", "head_norm_rotary", "head_norm_rotary_backward", "layer_norm", "layer_norm_backward", "linear",
            "rotary_frequencies", "ACTIVATIONS", "LAYOUTS", "BeamSearchError"]
 
 
@@ -253,25 +254,14 @@ def _offsets(what: str, name: str, t: torch.Tensor, n: int):
         _fail(f"{what}: {name} must be sequences + 1 contiguous int32 values")
 
 
-def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: Optional[torch.Tensor] = None,
-              k_offsets: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None,
-              longest_q: int = 0, longest_k: int = 0, lse: bool = False, out: Optional[torch.Tensor] = None):
-    """Attention of q (tokens, heads, head_dim) over k and v (tokens, kv_heads, head_dim), float16 or
-    bfloat16; head h reads key/value head h // (heads // kv_heads).  q_offsets, k_offsets (int32 on the
-    GPU, sequences + 1, from 0, ascending): the sequences packed in q and in k; k_offsets None: as
-    q_offsets; both None: one sequence.  causal: the last query of a sequence sees its last key, the one
-    before it one key less.  scale: head_dim ** -0.5 if None.  longest_q, longest_k: the longest
-    sequences, if known (they choose how the work is split, not the result).  lse: returns (out,
-    lse), lse (tokens, heads) float32 the log of the sum of the exponentials.  A query that sees no key
-    gets 0 and -inf.  out: where to write the result.  Tokens past the last offset are in no sequence:
-    their rows of the result and of lse are not written and hold what was in that memory before."""
-    what = "attention"
+def _attention_args(what, q, k, v, q_offsets, k_offsets, causal, scale, longest_q, longest_k, lse, out, *others):
+    """the GPU; the C call's arguments; its results (lse None unless asked for); the sizes that its workspace depends on"""
     type_ = q.dtype
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         _fail(f"{what}: q, k and v must be tokens x heads x head_dim")
     if type_ not in _HALF or k.dtype != type_ or v.dtype != type_:
         _fail(f"{what}: q, k and v must be of one type, float16 or bfloat16")
-    dev = _gpu(what, q, k, v, q_offsets, k_offsets, out)
+    dev = _gpu(what, q, k, v, q_offsets, k_offsets, out, *others)
     tq, heads, dim = q.shape
     tk, kv_heads, kdim = k.shape
     qt, qh, qe = q.stride()
@@ -307,7 +297,24 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: Opti
                            None if q_offsets is None else q_offsets.data_ptr(), None if k_offsets is None else k_offsets.data_ptr(),
                            qt, qh, kt, kh, vt, vh, ot, oh, tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, code,
                            1 if causal else 0, (dim ** -0.5 if dim else 0.0) if scale is None else scale)
-    size = _attention_workspace(tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, code, causal)
+    return dev, a, o, stat, (tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, code, causal)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: Optional[torch.Tensor] = None,
+              k_offsets: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None,
+              longest_q: int = 0, longest_k: int = 0, lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Attention of q (tokens, heads, head_dim) over k and v (tokens, kv_heads, head_dim), float16 or
+    bfloat16; head h reads key/value head h // (heads // kv_heads).  q_offsets, k_offsets (int32 on the
+    GPU, sequences + 1, from 0, ascending): the sequences packed in q and in k; k_offsets None: as
+    q_offsets; both None: one sequence.  causal: the last query of a sequence sees its last key, the one
+    before it one key less.  scale: head_dim ** -0.5 if None.  longest_q, longest_k: the longest
+    sequences, if known (they choose how the work is split, not the result).  lse: returns (out,
+    lse), lse (tokens, heads) float32 the log of the sum of the exponentials.  A query that sees no key
+    gets 0 and -inf.  out: where to write the result.  Tokens past the last offset are in no sequence:
+    their rows of the result and of lse are not written and hold what was in that memory before."""
+    what = "attention"
+    dev, a, o, stat, sizes = _attention_args(what, q, k, v, q_offsets, k_offsets, causal, scale, longest_q, longest_k, lse, out)
+    size = _attention_workspace(*sizes)
     space = q.new_empty((size,), dtype=torch.uint8) if size else None
     rc = _lib.hip().bs_attention(C.byref(a), space.data_ptr() if size else None, size, _raw_stream(dev))
     if rc:
@@ -562,3 +569,41 @@ def _gated_workspace(rows: int, inner: int, cols: int) -> int:
     n = C.c_uint64(0)
     _check(_lib.hip().bs_gated_backward_workspace(rows, inner, cols, C.byref(n)), "bs_gated_backward_workspace")
     return n.value
+
+
+def attention_shared_prefix(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
+                            q_offsets: Optional[torch.Tensor] = None, k_offsets: Optional[torch.Tensor] = None, causal: bool = True,
+                            scale: Optional[float] = None, longest_q: int = 0, longest_k: int = 0, lse: bool = False,
+                            out: Optional[torch.Tensor] = None):
+    """Attention of packed sequences that share their first keys (queries behind one instruction, chunks behind one
+    document): as attention, but every query sees all of prefix_k and prefix_v (tokens, kv_heads, head_dim) besides the keys
+    that it sees of its own sequence in k and v, in one softmax.  causal: concerns the sequence's own keys.  A sequence may
+    have no keys of its own."""
+    what = "attention_shared_prefix"
+    dev, a, o, stat, sizes = _attention_args(what, q, k, v, q_offsets, k_offsets, causal, scale, longest_q, longest_k, lse, out, prefix_k, prefix_v)
+    if prefix_k.dim() != 3 or prefix_v.shape != prefix_k.shape or prefix_k.shape[1:] != k.shape[1:]:
+        _fail(f"{what}: prefix_k and prefix_v must have one shape, tokens x kv_heads x head_dim as k has them")
+    if prefix_k.dtype != q.dtype or prefix_v.dtype != q.dtype:
+        _fail(f"{what}: prefix_k and prefix_v must be of q's type")
+    pt, ph, pe = prefix_k.stride()
+    vt, vh, ve = prefix_v.stride()
+    if prefix_k.shape[2] > 1 and not pe == ve == 1:
+        _fail(f"{what}: the elements of a head of prefix_k and prefix_v must be contiguous")
+    tokens = prefix_k.shape[0]
+    f = _lib.AttentionPrefix(prefix_k.data_ptr(), prefix_v.data_ptr(), pt, ph, vt, vh, tokens)
+    size = _prefix_workspace(tokens, *sizes)
+    space = q.new_empty((size,), dtype=torch.uint8) if size else None
+    rc = _lib.hip().bs_attention_shared_prefix(C.byref(a), C.byref(f), space.data_ptr() if size else None, size, _raw_stream(dev))
+    if rc:
+        _check(rc, what)
+    return (o, stat) if lse else o
+
+
+@lru_cache(maxsize=4096)
+def _prefix_workspace(tokens, tq, tk, n, heads, kv_heads, dim, longest_q, longest_k, code, causal) -> int:
+    a, f = _lib.AttentionArgs(), _lib.AttentionPrefix()
+    a.q_tokens, a.k_tokens, a.sequences, a.heads, a.kv_heads, a.head_dim = tq, tk, n, heads, kv_heads, dim
+    a.longest_q, a.longest_k, a.type, a.causal, a.scale, f.tokens = longest_q, longest_k, code, causal, 1.0, tokens
+    b = C.c_uint64(0)
+    _check(_lib.hip().bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), C.byref(b)), "bs_attention_shared_prefix_workspace")
+    return b.value

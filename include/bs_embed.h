@@ -188,6 +188,25 @@ int bs_gated_backward(const void* dh, int64_t dh_stride, const void* x, int64_t 
                       uint32_t cols, int type, int activation, void* workspace, uint64_t workspace_bytes, void* stream);
 int bs_gated_backward_workspace(uint64_t rows, uint32_t inner, uint32_t cols, uint64_t* bytes);
 
+/* Attention of sequences that share their first keys: as bs_attention, but every query sees the
+ * `tokens` keys of the prefix besides those that it sees of its own sequence, and the softmax is
+ * over both.  The prefix is read once for the rows of all sequences where sequences are short, and
+ * by each tile of rows where they fill tiles.  Its type, kv_heads and head_dim are args'; a prefix
+ * of 0 tokens is bs_attention.  A query's own keys may be none.  Strides of keys and values, the
+ * prefix's too, are < 2^22.  Queries outside every sequence may be read, not written.
+ * workspace: bs_attention_shared_prefix_workspace bytes for the same sizes, 16-byte aligned. */
+typedef struct {
+    const void* k;
+    const void* v;
+    int64_t k_stride, k_head_stride; /* aligned as those of bs_attention_args */
+    int64_t v_stride, v_head_stride;
+    uint32_t tokens; /* < 2^31 */
+} bs_attention_prefix;
+
+int bs_attention_shared_prefix(const bs_attention_args* args, const bs_attention_prefix* prefix, void* workspace,
+                               uint64_t workspace_bytes, void* stream);
+int bs_attention_shared_prefix_workspace(const bs_attention_args* args, const bs_attention_prefix* prefix, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

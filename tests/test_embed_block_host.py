@@ -5,7 +5,7 @@ import math
 import pytest
 
 from beam_search_collab_amd import _lib
-from test_embed_host import PTR, refused
+from test_embed_host import PTR, attention_args, refused
 
 
 def rotary_args(**change):
@@ -114,3 +114,40 @@ def test_python_refuses_tensors_off_the_gpu():
     for call in (lambda: embed.gated(x, x, x), lambda: embed.gated_backward(x, x, x, x, x, x), lambda: embed.head_norm_rotary(x[:, None])):
         with pytest.raises(ValueError, match="on a GPU"):
             call()
+
+
+def prefix_args(**change):
+    f = _lib.AttentionPrefix()
+    for n, x in (dict(k=PTR, v=PTR, k_stride=32, k_head_stride=32, v_stride=32, v_head_stride=32, tokens=9) | change).items():
+        setattr(f, n, x)
+    return f
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(tokens=1 << 31), "tokens of the prefix"), (dict(k=None), "prefix must be given"), (dict(v=None), "prefix must be given"),
+    (dict(k=PTR + 8), "multiples of 16 bytes"), (dict(v_stride=24), "multiples of 8"), (dict(k_stride=1 << 22), "must be < 2^22")])
+def test_attention_shared_prefix_refuses_prefixes(change, text):
+    refused(_lib.hip().bs_attention_shared_prefix(C.byref(attention_args()), C.byref(prefix_args(**change)), PTR, 1 << 30, None), text)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(type=0), "type must be"), (dict(head_dim=20), "head_dim must be"), (dict(heads=3, kv_heads=2), "multiple of kv_heads"), (dict(sequences=2), "need q_offsets"),
+    (dict(scale=math.nan), "scale must be finite"), (dict(k=None), "must be given"), (dict(q=PTR + 8), "multiples of 16 bytes"), (dict(v_stride=1 << 22), "must be < 2^22")])
+def test_attention_shared_prefix_refuses_arguments(change, text):
+    refused(_lib.hip().bs_attention_shared_prefix(C.byref(attention_args(**change)), C.byref(prefix_args()), PTR, 1 << 30, None), text)
+
+
+def test_attention_shared_prefix_asks_for_its_workspace():
+    hip, a, f, n = _lib.hip(), attention_args(), prefix_args(), C.c_uint64(0)
+    assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), C.byref(n)) == 0 and n.value > 0
+    refused(hip.bs_attention_shared_prefix(C.byref(a), C.byref(f), None, 0, None), "the workspace must hold")
+    refused(hip.bs_attention_shared_prefix(C.byref(a), C.byref(f), PTR, n.value - 1, None), "the workspace must hold")
+    refused(hip.bs_attention_shared_prefix(C.byref(a), C.byref(f), PTR + 4, n.value, None), "16-byte aligned")
+    refused(hip.bs_attention_shared_prefix(C.byref(a), None, PTR, n.value, None), "prefix is null")
+    refused(hip.bs_attention_shared_prefix(None, C.byref(f), PTR, n.value, None), "args is null")
+    refused(hip.bs_attention_shared_prefix_workspace(C.byref(a), None, C.byref(n)), "prefix is null")
+    refused(hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), None), "bytes is null")
+    assert hip.bs_attention_shared_prefix(C.byref(attention_args(q_tokens=0)), C.byref(f), None, 0, None) == 0
+    b = C.c_uint64(1)  # of no prefix: attention's
+    assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(prefix_args(tokens=0)), C.byref(n)) == 0
+    assert hip.bs_attention_workspace(C.byref(a), C.byref(b)) == 0 and b.value == n.value

@@ -473,3 +473,188 @@ def test_gated_refusals(gpu):
     ]:
         with pytest.raises(ValueError, match=text):
             call()
+
+
+# ---------------------------------------------------------------- attention behind a shared prefix
+
+def prefix_case(seed, nq, nk, prefix, heads, kv, dim, dtype, std=1.0):
+    return (rand(seed, sum(nq), heads, dim, dtype=dtype, std=std), rand(seed + 1, sum(nk), kv, dim, dtype=dtype), rand(seed + 2, sum(nk), kv, dim, dtype=dtype),
+            rand(seed + 3, prefix, kv, dim, dtype=dtype), rand(seed + 4, prefix, kv, dim, dtype=dtype))
+
+
+def check_prefix(q, k, v, pk, pv, nq, nk, causal, scale, out, lse):
+    """a sequence and a head at a time in 64 bits; tolerances as attention's, whose arithmetic it is: one more joining of parts"""
+    heads, kv, dim, t = q.shape[1], k.shape[1], q.shape[2], q.dtype
+    a = b = 0
+    p = len(pk)
+    for m, n in zip(nq, nk):
+        if not m:
+            b += n
+            continue
+        for h in range(heads):
+            g = h // (heads // kv)
+            x = q[a:a + m, h].double()
+            y, w = torch.cat([pk[:, g], k[b:b + n, g]]).double(), torch.cat([pv[:, g], v[b:b + n, g]]).double()
+            hide = torch.zeros(m, p + n, dtype=torch.bool, device="cuda")
+            if causal:
+                hide = torch.ones_like(hide).triu(p + n - m + 1)
+                hide[:, :p] = False
+            z = (x @ y.t().contiguous() * scale).masked_fill(hide, -math.inf)
+            s = torch.logsumexp(z, 1)
+            none = s == -math.inf
+            e = torch.exp(z - torch.where(none, 0.0, s)[:, None])
+            spread = (x.abs() @ y.abs().t().contiguous() * abs(scale)).masked_fill(hide, 0).amax(1) if p + n else torch.zeros(m, dtype=torch.float64, device="cuda")
+            count = p + n
+            d = (dim + 6) * E * spread + 4 * E * (spread + 1)
+            want, size, total = e @ w, e @ w.abs(), (~hide).double() @ w.abs()
+            tol = (U[t] + 4 * d + (count + 48) * E)[:, None] * size + 2.0 ** -24 * total * (t == F16) + U[t] * want.abs() + TINY[t]
+            near(out[a:a + m, h], want, tol)
+            if lse is not None:
+                near(lse[a:a + m, h], s, 2 * d + (count / 32 + 48) * E + 4 * E * torch.where(none, 0.0, s.abs()))
+        a, b = a + m, b + n
+
+
+def offsets(lengths):
+    import numpy as np
+    return torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32, device="cuda")
+
+
+def behind_prefix(seed, nq, nk, prefix, heads, kv, dim, dtype, causal=True, scale=None, hints=True):
+    q, k, v, pk, pv = prefix_case(seed, nq, nk, prefix, heads, kv, dim, dtype)
+    lo = dict(longest_q=max(nq), longest_k=max(nk)) if hints else {}
+    out, lse = embed.attention_shared_prefix(q, k, v, pk, pv, offsets(nq), offsets(nk), causal=causal, scale=scale, lse=True, **lo)
+    check_prefix(q, k, v, pk, pv, nq, nk, causal, dim ** -0.5 if scale is None else scale, out, lse)
+    again = embed.attention_shared_prefix(q, k, v, pk, pv, offsets(nq), offsets(nk), causal=causal, scale=scale, **lo)
+    assert torch.equal(again, out)
+    return q, k, v, pk, pv, out, lse
+
+
+PREFIX = [
+    ([1], [1], 1), ([1], [0], 3), ([2], [2], 64), ([24], [24], 100), ([1, 1, 1], [5, 700, 64], 65), ([7], [3], 63), ([5, 2], [0, 9], 33),
+    ([0, 3, 0, 4], [2, 3, 0, 4], 129), ([1, 40, 3, 130, 17], [1, 40, 3, 130, 17], 200), ([1] * 70, list(range(70)), 300), ([1] * 9, [0] * 9, 1000),
+    ([2] * 9, [300 - 31 * i for i in range(9)], 1), ([3], [3], 0), ([1, 2], [900, 40], 2500), ([1] * 40, [20] * 40, 5000)]
+
+
+@pytest.mark.parametrize("nq,nk,prefix", PREFIX, ids=[str(i) for i in range(len(PREFIX))])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(4, 2, 64, BF16), (3, 1, 128, F16), (2, 2, 32, BF16)])
+def test_attention_shared_prefix(gpu, nq, nk, prefix, causal, heads, kv, dim, dtype):
+    behind_prefix(300, nq, nk, prefix, heads, kv, dim, dtype, causal)
+
+
+MANY = [([130, 64, 1, 200, 0, 77] * 4, None, 150, 16, 16), ([300] * 8, None, 64, 16, 8), ([300] * 8, [0] * 8, 1, 16, 8), ([500, 400] * 4, [600, 100] * 4, 1023, 16, 4),
+        ([64] * 64, None, 65, 8, 8), ([100] * 40, [37] * 40, 500, 8, 8)]
+
+
+@pytest.mark.parametrize("nq,nk,prefix,heads,kv", MANY, ids=[str(i) for i in range(len(MANY))])
+@pytest.mark.parametrize("dim,dtype,causal", [(32, BF16, True), (64, F16, True), (72, BF16, False), (128, BF16, True)])
+def test_attention_shared_prefix_of_full_tiles(gpu, nq, nk, prefix, heads, kv, dim, dtype, causal):
+    behind_prefix(310, nq, nq if nk is None else nk, prefix, heads, kv, dim, dtype, causal)
+
+
+@pytest.mark.parametrize("dim", [8, 16, 24, 40, 48, 56, 72, 80, 88, 96, 104, 120])
+def test_attention_shared_prefix_head_sizes(gpu, dim):
+    behind_prefix(320, [70, 9], [70, 150], 77, 3, 3, dim, BF16)
+    behind_prefix(325, [260] * 12, [260] * 12, 77, 16, 16, dim, BF16)
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (5, 1), (8, 8), (12, 4), (16, 1), (40, 2), (64, 1)])
+def test_attention_shared_prefix_heads(gpu, heads, kv):
+    behind_prefix(330, [19, 1], [19, 77], 140, heads, kv, 64, F16)
+    behind_prefix(335, [1] * 5, [3, 0, 7, 200, 64], 140, heads, kv, 64, BF16, hints=False)
+
+
+def test_attention_shared_prefix_is_attention_over_both(gpu):
+    """one sequence: the prefix and its own keys in a row; without offsets; of no prefix"""
+    q, k, v, pk, pv = prefix_case(340, [90], [90], 200, 4, 2, 64, BF16)
+    out = embed.attention_shared_prefix(q, k, v, pk, pv)
+    check_prefix(q, k, v, pk, pv, [90], [90], True, 0.125, out, None)
+    whole = embed.attention(q, torch.cat([pk, k]), torch.cat([pv, v]), offsets([90]), offsets([290]))
+    assert (out.float() - whole.float()).abs().max() < 0.05
+    none = embed.attention_shared_prefix(q, k, v, pk[:0], pv[:0], lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(none, embed.attention(q, k, v, lse=True)))
+    for scale in (0.0, -0.3, 2.0):
+        behind_prefix(341, [90, 1], [90, 3], 200, 4, 2, 64, BF16, scale=scale)
+        behind_prefix(342, [300] * 8, [300] * 8, 70, 16, 8, 64, BF16, scale=scale)
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv", [([70, 20], [70, 20], 4, 2), ([1, 2], [900, 40], 4, 2), ([300] * 8, [300] * 8, 16, 8)])
+def test_attention_shared_prefix_of_slices(gpu, nq, nk, heads, kv):
+    """all operands as columns of wider tensors, the result inside another; tokens behind the last sequence"""
+    dim, more = 64, 5
+    q = rand(350, sum(nq) + more, heads * dim + 16, dtype=F16)[:, 8:8 + heads * dim].unflatten(1, (heads, dim))
+    own = rand(351, sum(nk) + more, 2 * kv * dim, dtype=F16)
+    k, v = own[:, :kv * dim].unflatten(1, (kv, dim)), own[:, kv * dim:].unflatten(1, (kv, dim))
+    own[sum(nk):] = math.nan
+    q[sum(nq):] = math.nan
+    front = rand(352, 300, 2 * kv * dim + 8, dtype=F16)
+    pk, pv = front[:, :kv * dim].unflatten(1, (kv, dim)), front[:, kv * dim:2 * kv * dim].unflatten(1, (kv, dim))
+    buf = torch.full((sum(nq) + more, heads, dim + 8), 7.0, dtype=F16, device="cuda")
+    got, lse = embed.attention_shared_prefix(q, k, v, pk, pv, offsets(nq), offsets(nk), out=buf[:, :, :dim], lse=True)
+    assert (buf[:, :, dim:] == 7).all() and (buf[sum(nq):] == 7).all()
+    want = embed.attention_shared_prefix(*(t.contiguous() for t in (q, k, v, pk, pv)), offsets(nq), offsets(nk))
+    assert torch.equal(buf[:sum(nq), :, :dim], want[:sum(nq)])
+    check_prefix(q, k, v, pk, pv, nq, nk, True, 0.125, want, lse)
+    pkt, pvt = pk.transpose(0, 1).contiguous().transpose(0, 1), pv.transpose(0, 1).contiguous().transpose(0, 1)  # heads before tokens
+    assert torch.equal(embed.attention_shared_prefix(q, k, v, pkt, pvt, offsets(nq), offsets(nk))[:sum(nq)], want[:sum(nq)])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 65000.0])
+@pytest.mark.parametrize("nq,nk,heads,kv", [([100, 30], [100, 30], 2, 1), ([3, 5], [80, 900], 2, 2), ([1, 4], [1300, 60], 8, 1), ([130] * 20, [130] * 20, 16, 16)])
+def test_attention_shared_prefix_never_touches_what_a_query_does_not_see(gpu, bad, nq, nk, heads, kv):
+    """the last key and value of every sequence hold `bad`: only the last query's result may change; those of the prefix: all"""
+    import numpy as np
+    q, k, v, pk, pv = prefix_case(360, nq, nk, 70, heads, kv, 64, BF16)
+
+    def run():
+        return embed.attention_shared_prefix(q, k, v, pk, pv, offsets(nq), offsets(nk), lse=True)
+    good = run()
+    last_q, last_k = (torch.tensor(np.cumsum(n) - 1, device="cuda") for n in (nq, nk))
+    keep = torch.ones(sum(nq), dtype=torch.bool, device="cuda")
+    keep[last_q] = False
+    for which in (k, v):
+        was = which.clone()
+        which[last_k] = bad
+        got = run()
+        for a, b in zip(got, good):
+            assert torch.equal(a[keep], b[keep])
+        if which is v and not math.isfinite(bad):
+            assert not torch.isfinite(got[0][last_q]).any()
+        which.copy_(was)
+    if not math.isfinite(bad):
+        for at in (69, 64, 3):
+            was = pv.clone()
+            pv[at, :, 5] = bad
+            got = run()[0]
+            assert (torch.isnan(got[..., 5]).all() if math.isnan(bad) else (got[..., 5] == bad).all())
+            rest = torch.arange(64, device="cuda") != 5
+            assert torch.equal(got[..., rest], good[0][..., rest])
+            pv.copy_(was)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("nq,nk,prefix,heads,kv", [([1] * 4, [50] * 4, 2000, 2, 1), ([300] * 8, [300] * 8, 130, 16, 8)])
+def test_attention_shared_prefix_of_scores_far_apart(gpu, sign, nq, nk, prefix, heads, kv):
+    """the prefix's keys score far more, or far less, than the own ones"""
+    q, k, v, pk, pv = prefix_case(370, nq, nk, prefix, heads, kv, 32, BF16)
+    q[..., 0] = 8.0
+    pk[..., 0] = sign * 30.0
+    out, lse = embed.attention_shared_prefix(q, k, v, pk, pv, offsets(nq), offsets(nk), scale=1.0, lse=True)
+    check_prefix(q, k, v, pk, pv, nq, nk, True, 1.0, out, lse)
+
+
+def test_attention_shared_prefix_refusals(gpu):
+    q, k = rand(3, 4, 2, 32, dtype=BF16), rand(4, 4, 1, 32, dtype=BF16)
+    p, off = rand(5, 9, 1, 32, dtype=BF16), offsets([4])
+    for call, text in [
+        (lambda: embed.attention_shared_prefix(q, k, k, p, p[:8], off), "one shape"),
+        (lambda: embed.attention_shared_prefix(q, k, k, p[..., :16], p[..., :16], off), "one shape"),
+        (lambda: embed.attention_shared_prefix(q, k, k, p.half(), p.half(), off), "q's type"),
+        (lambda: embed.attention_shared_prefix(q, k, k, rand(6, 9, 1, 64, dtype=BF16)[..., ::2], p, off), "contiguous"),
+        (lambda: embed.attention_shared_prefix(q, k, k, p.cpu(), p, off), "must be a tensor on"),
+        (lambda: embed.attention_shared_prefix(q, k, k, p, p, None, off), "k_offsets without"),
+        (lambda: embed.attention_shared_prefix(q, k, k, torch.nn.Parameter(p), p, off), "gradient"),
+        (lambda: embed.attention_shared_prefix(q, k, k, rand(6, 9, 1, 36, dtype=BF16)[..., 4:], p, off), "multiples of 16 bytes|one shape"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            call()

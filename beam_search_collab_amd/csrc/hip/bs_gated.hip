@@ -120,15 +120,18 @@ __device__ __host__ inline uint32_t cols_of(const Params& p) { return FORM == GA
 template <int FORM>
 __device__ __host__ inline uint32_t inner_of(const Params& p) { return FORM == GATED ? p.inner : FORM == INPUT ? 2 * p.cols : p.rows; }
 
-// N adjacent results of a row, those inside
+// a row of the result, and N adjacent ones of it, those inside
+template <typename T, int FORM>
+__device__ inline T* row_of(const Params& p, uint32_t row) {
+    if (FORM == INPUT) return static_cast<T*>(p.dx) + static_cast<size_t>(row) * p.inner;
+    return row < p.cols ? static_cast<T*>(p.dwg) + static_cast<size_t>(row) * p.inner : static_cast<T*>(p.dwu) + static_cast<size_t>(row - p.cols) * p.inner;
+}
 template <typename T, int FORM, int N>
 __device__ inline void write(const Params& p, uint32_t row, uint32_t col, const float (&z)[N]) {
-    T* to = FORM == INPUT ? static_cast<T*>(p.dx) + static_cast<size_t>(row) * p.inner
-                          : row < p.cols ? static_cast<T*>(p.dwg) + static_cast<size_t>(row) * p.inner : static_cast<T*>(p.dwu) + static_cast<size_t>(row - p.cols) * p.inner;
     Vec<T, N> o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = static_cast<T>(z[j]);
-    store_some<T, N>(to + col, o, static_cast<int>(p.inner - col));
+    store_some<T, N>(row_of<T, FORM>(p, row) + col, o, static_cast<int>(p.inner - col));
 }
 template <typename T, int N>
 __device__ inline void write_gated(const Params& p, uint32_t row, uint32_t col, float (&g)[N], const float (&u)[N]) {
@@ -476,6 +479,292 @@ __global__ __launch_bounds__(512) void gated_few_kernel(Params p) {
     if (row < p.rows && col < p.cols) write_gated<T, 4>(p, row, col, z, u);
 }
 
+// ------------------------------------------------------------------------------------------------ large tiles
+
+// Tiles of 256 rows of X x 256 rows of W by 8 waves of 128 x 64, inner steps of 64, two of them in LDS.  A step is four phases,
+// and the quarters of its operands (x0, x1: the first and second 64 rows of every wave; w0, w1: the first and second 32) are
+// read into registers a phase before their products, whereupon the moves of step t + 2 into that quarter start.
+//   phase 0: read w1(t)              products w0 x0
+//   phase 1: read x1(t)              products w1 x0    move x0, w0 (t + 2)
+//   phase 2:                         products w0 x1    move w1 (t + 2)
+//   phase 3: read x0, w0 (t + 1)     products w1 x1    move x1 (t + 2)
+// GATED: w0 is of wg and w1 of wu.  A quarter of an operand whose rows are columns in memory lies in LDS as 64 inner elements x
+// its 128 rows.  A workgroup goes through its tiles without a break: the moves of the next tile's first steps are under way
+// while a tile's results are written.  A tile that would pass an edge is shifted back inside and does not write what its
+// neighbour writes.
+//
+// The tiles run .. run + count - 1 of the product, 8 tile rows high; this workgroup's are those from `first` on, `stride` apart.
+template <typename T, int FORM>
+__device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint32_t first, uint32_t count, uint32_t stride) {
+    constexpr bool XT = FORM == WEIGHTS, WT = FORM != GATED;
+    constexpr uint32_t OUT = FORM == GATED ? 128 : 256;  // columns of the result in a tile
+    constexpr int STEP = 512 * 64;                       // elements: 256 rows of X, then 256 of W
+    if (first >= count) return;
+    T* buf = reinterpret_cast<T*>(lds);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
+    float* turn = reinterpret_cast<float*>(lds + 2 * STEP * 2) + wave * 1024;
+    const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+    auto swizzle = [](int r, int c) { return c ^ ((r >> 1) & 7); };
+    const uint32_t rows = rows_of<FORM>(p), cols = cols_of<FORM>(p);
+    const uint32_t steps = FORM == GATED ? p.inner / 64 : FORM == INPUT ? p.cols / 32 : (p.rows + 63) / 64;
+    const uint32_t mt = (rows + 255) / 256, nt = (cols + OUT - 1) / OUT;
+    auto origin = [&](uint32_t i, uint32_t& m, uint32_t& n) {
+        const uint32_t id = run + i, band = id / (8 * nt), high = min(mt - band * 8, 8u), in = id - band * 8 * nt;
+        m = (band * 8 + in % high) * 256;
+        n = in / high * OUT;
+    };
+
+    // bytes between the lines of an operand in memory, and this thread's part of a move: 64 lines of 64 inner elements, or 32
+    // inner elements of 128 rows, of which x's quarters have 64 of each 128 and w's 32 of each 64
+    const uint64_t xhop = FORM == GATED ? static_cast<uint64_t>(p.xs) * 2 : static_cast<uint64_t>(p.cols) * 4;
+    const uint64_t whop = FORM == WEIGHTS ? static_cast<uint64_t>(p.xs) * 2 : static_cast<uint64_t>(p.wgs) * 2;
+    const int r = threadIdx.x >> 3, c = swizzle(r, threadIdx.x & 7);
+    const int k = threadIdx.x >> 4, kc = (threadIdx.x & 15) ^ ((k & 3) << 2 | ((k >> 2) & 3));
+    const uint32_t vx = XT ? k * static_cast<uint32_t>(xhop) + ((kc >> 3) * 128 + (kc & 7) * 8) * 2 : r * static_cast<uint32_t>(xhop) + c * 16;
+    const uint32_t across = ((kc >> 2) * 64 + (kc & 3) * 8) * 2;
+    const uint32_t vw = WT ? k * static_cast<uint32_t>(whop) + across : r * static_cast<uint32_t>(whop) + c * 16;
+    const uint32_t vtail = k * p.inner * 2 + across;  // WEIGHTS: in x's tail
+    const int rows8 = wave * 8, rows8w = (rows8 & 31) + (rows8 >> 5) * 64;
+    struct Source {
+        const char *x, *w0, *w1;  // the tile's first lines at the step to be moved
+        uint64_t whop;
+        bool tail;
+    } from;
+    // the sources of step t of the tile at m, n
+    auto point = [&](uint32_t m, uint32_t n, uint32_t t) {
+        const uint64_t ms = min(m, rows - 256), ns = min(n, cols - OUT);
+        from.whop = whop;
+        from.tail = false;
+        if (FORM == GATED) {
+            from.x = static_cast<const char*>(p.x) + ms * xhop + t * 128ull;
+            from.w0 = static_cast<const char*>(p.wg) + ns * whop + t * 128ull;
+            from.w1 = static_cast<const char*>(p.wu) + ns * whop + t * 128ull;
+        } else if (FORM == INPUT) {
+            from.x = p.d + ms * xhop + t * 128ull;
+            const uint32_t at = t * 64;
+            from.w0 = (at < p.cols ? static_cast<const char*>(p.wg) + at * whop : static_cast<const char*>(p.wu) + (at - p.cols) * whop) + ns * 2;
+            from.w1 = from.w0 + 64;
+        } else {
+            from.x = p.d + t * 64ull * xhop + ms * 2;
+            from.tail = t * 64 + 64 > p.rows;
+            from.whop = from.tail ? p.inner * 2ull : whop;
+            from.w0 = (from.tail ? p.tail : static_cast<const char*>(p.x) + t * 64ull * whop) + ns * 2;
+            from.w1 = from.w0 + 64;
+        }
+    };
+    auto move_x = [&](int slot, int g, int i) {
+        if (XT)
+            move16(from.x + i * 32 * xhop + g * 128, vx, buf + slot * STEP + g * 8192 + i * 4096 + wave * 512);
+        else
+            move16(from.x + (i * 128 + g * 64) * xhop, vx, buf + slot * STEP + (i * 128 + g * 64 + rows8) * 64);
+    };
+    auto move_w = [&](int slot, int g, int i) {
+        const char* w = g ? from.w1 : from.w0;
+        if (WT)
+            move16(w + i * 32 * from.whop, FORM == WEIGHTS && from.tail ? vtail : vw, buf + slot * STEP + 256 * 64 + g * 8192 + i * 4096 + wave * 512);
+        else
+            move16(w + i * 64 * whop, vw, buf + slot * STEP + (256 + i * 128 + g * 32 + rows8w) * 64);
+    };
+    Vec<T, 8> fx[4][4], fw[2][4];
+    // a lane's places in LDS: of 16 inner elements in a row (rows of operands differ by multiples of 32, so the swizzle is the
+    // lane's), or of 4 inner elements and the next 4 in a column
+    int at[4], ax[2][2], aw[2];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) at[s] = l * 64 + swizzle(l, s * 2 + h) * 8;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int kk = h * 8 + ((lane & 15) >> 2) + half * 4, e = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ax[j][half] = place<256>(kk, ((wave >> 2) * 64 + j * 32 + e) >> 3) + (e & 7) * 2;
+        aw[half] = place<256>(kk, ((wave & 3) * 32 + e) >> 3) + (e & 7) * 2;
+    }
+    auto pair = [&](const T* base, int lo, int hi) {
+        const s16x4 a = read_transposed(reinterpret_cast<const char*>(base) + lo), b = read_transposed(reinterpret_cast<const char*>(base) + hi);
+        return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    };
+    auto read_x = [&](int slot, int j, int s) {
+        fx[j][s] = XT ? pair(buf + slot * STEP + (j >> 1) * 8192 + s * 2048, ax[j & 1][0], ax[j & 1][1])
+                      : *reinterpret_cast<const Vec<T, 8>*>(buf + slot * STEP + (wm + j * 32) * 64 + at[s]);
+    };
+    auto read_w = [&](int slot, int i, int s) {
+        fw[i][s] = WT ? pair(buf + slot * STEP + 256 * 64 + i * 8192 + s * 2048, aw[0], aw[1])
+                      : *reinterpret_cast<const Vec<T, 8>*>(buf + slot * STEP + (256 + wn + i * 32) * 64 + at[s]);
+    };
+    f32x16 acc[2][4];
+    // Eight matrix instructions; `between` puts the phase's reads and moves between them, one or two at a time:
+    // issued in a row they would keep the wave from its products until the memory pipes have taken them all.
+    auto product = [&](int i, int j, auto between) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            acc[i][j + (n & 1)] = Mma<T>::go(fw[i][n >> 1], fx[j + (n & 1)][n >> 1], acc[i][j + (n & 1)]);
+            __builtin_amdgcn_sched_barrier(0);
+            between(n);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    uint32_t m0, n0, id = first;
+    origin(id, m0, n0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        point(m0, n0, t);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) move_x(t, 0, i), move_w(t, 0, i);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) move_w(t, 1, i);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) move_x(t, 1, i);
+    }
+    meet<12>();
+    int slot = 0;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) read_x(0, 0, n), read_x(0, 1, n), read_w(0, 0, n);
+    while (true) {
+        const uint32_t next = id + stride;
+        uint32_t mn = m0, nn = n0;
+        if (next < count) origin(next, mn, nn);  // else the moves past the end repeat this tile's, unread
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
+        for (uint32_t t = 0; t < steps; ++t) {
+            if (t + 2 < steps)
+                point(m0, n0, t + 2);
+            else
+                point(mn, nn, t + 2 - steps);
+            // the moves in flight at a meeting, from the oldest: the quarter that the phase reads is the first of them
+            meet<10>();
+            product(0, 0, [&](int n) {
+                if (n < 4) read_w(slot, 1, n);
+            });
+            meet<8>();
+            product(1, 0, [&](int n) {
+                read_x(slot, 2 + (n & 1), n >> 1);
+                if (n & 1) (n & 2) ? move_w(slot, 0, n >> 2) : move_x(slot, 0, n >> 2);
+            });
+            meet<12>();
+            product(0, 2, [&](int n) {
+                if ((n & 3) == 1) move_w(slot, 1, n >> 2);
+            });
+            meet<10>();
+            product(1, 2, [&](int n) {
+                if (n < 4) {
+                    read_w(slot ^ 1, 0, n);
+                    read_x(slot ^ 1, 0, n);
+                } else {
+                    read_x(slot ^ 1, 1, n - 4);
+                    if (n & 1) move_x(slot, 1, (n - 4) >> 1);
+                }
+            });
+            slot ^= 1;
+        }
+        // results: 16 rows at a time through the wave's 4 KB, then 8 adjacent columns a lane (GATED: of both products)
+        const uint32_t ms = min(m0, rows - 256), ns = min(n0, cols - OUT);
+        auto put = [&](auto J, int half) {
+            constexpr int j = decltype(J)::value;
+            if ((l >> 4) == half) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<f32x4*>(turn + (l & 15) * 64 + ((i * 8 + q * 2 + h) ^ (l & 15)) * 4) =
+                            f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+            }
+        };
+        auto take = [&](int rr, int chunk, float (&z)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(turn + rr * 64 + ((chunk + e / 4) ^ rr) * 4);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) z[e + x] = v[x];
+            }
+        };
+        auto give = [&](T* row, uint32_t col, const float (&z)[8]) {  // those from n0 on
+            Vec<T, 8> o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(z[e]);
+            if (col >= n0) {
+                store_any<T, 8>(row + col, o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col + e >= n0) row[col + e] = o[e];
+            }
+        };
+#pragma unroll 1
+        for (int g = 0; g < 8; ++g) {  // not unrolled: the epilogue's code stays in the instruction cache
+            const int half = g & 1;
+            switch (g >> 1) {
+                case 0: put(std::integral_constant<int, 0>(), half); break;
+                case 1: put(std::integral_constant<int, 1>(), half); break;
+                case 2: put(std::integral_constant<int, 2>(), half); break;
+                default: put(std::integral_constant<int, 3>(), half); break;
+            }
+            __builtin_amdgcn_wave_barrier();
+            float z[8];
+            if constexpr (FORM == GATED) {
+                const int rr = lane >> 2, cc = (lane & 3) * 2;
+                const uint32_t row = ms + wm + g * 16 + rr, col = ns + wn / 2 + cc * 4;
+                float u[8];
+                take(rr, cc, z);
+                take(rr, 8 + cc, u);
+                if (row >= m0) {
+                    if (p.gate) {
+                        give(static_cast<T*>(p.gate) + static_cast<size_t>(row) * p.cols, col, z);
+                        give(static_cast<T*>(p.up) + static_cast<size_t>(row) * p.cols, col, u);
+                    }
+                    activate(z, p.act);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] *= u[e];
+                    give(static_cast<T*>(p.h) + static_cast<int64_t>(row) * p.hs, col, z);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int rr = q * 8 + (lane >> 3), cc = (lane & 7) * 2;
+                    const uint32_t row = ms + wm + g * 16 + rr, col = ns + wn + cc * 4;
+                    take(rr, cc, z);
+                    if (row >= m0) give(row_of<T, FORM>(p, row), col, z);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        if (next >= count) break;
+        id = next;
+        m0 = mn;
+        n0 = nn;
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // moves into this workgroup's LDS end before it does
+}
+
+// Workgroup b runs on XCD b mod 8: each XCD takes a contiguous run of tiles, so that the tiles in flight on it share operands
+// in its L2.
+struct Share {
+    uint32_t run, count;
+};
+__device__ inline Share share_of(uint32_t tiles) {
+    const uint32_t xcd = blockIdx.x & 7, q8 = tiles >> 3, r8 = tiles & 7;
+    return Share{xcd * q8 + (xcd < r8 ? xcd : r8), q8 + (xcd < r8 ? 1 : 0)};
+}
+template <typename T>
+__global__ __launch_bounds__(512, 2) void gated_big_kernel(Params p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const Share s = share_of((p.rows + 255) / 256 * ((p.cols + 127) / 128));
+    big_tiles<T, GATED>(p, lds, s.run, blockIdx.x >> 3, s.count, gridDim.x >> 3);
+}
+// Both products of the gradients in one launch, so that the tiles of both fill the compute units.
+template <typename T>
+__global__ __launch_bounds__(512, 2) void gated_big_backward_kernel(Params p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t nt = (p.inner + 255) / 256, stride = gridDim.x >> 3;
+    const Share a = share_of(p.dx ? (p.rows + 255) / 256 * nt : 0), b = share_of(p.dwg ? (2 * p.cols + 255) / 256 * nt : 0);
+    uint32_t first = blockIdx.x >> 3;
+    big_tiles<T, INPUT>(p, lds, a.run, first, a.count, stride);
+    __syncthreads();
+    if (first < a.count) first += (a.count - first + stride - 1) / stride * stride;
+    big_tiles<T, WEIGHTS>(p, lds, b.run, first - a.count, b.count, stride);
+}
+
 using Mid = Tile<128, 128, 2, 2, 32, 4, 2>;
 using Small = Tile<64, 64, 2, 2, 64, 4, 2>;
 using Flat = Tile<64, 128, 2, 2, 64, 3, 2>;  // of GATED, whose waves have 64 rows of W
@@ -511,6 +800,17 @@ int start(const Params& p, hipStream_t s) {
 bool rows16(const void* p, int64_t stride) { return aligned16(p) && stride % 8 == 0; }
 
 template <typename T>
+int start_big(const Params& p, bool backward, uint64_t tiles, hipStream_t s) {
+    constexpr int LDS = 160 * 1024;
+    auto* k = backward ? gated_big_backward_kernel<T> : gated_big_kernel<T>;
+    static std::atomic<uint64_t> done[2];
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), LDS, done[backward])) return rc;
+    k<<<tiles < CUS ? static_cast<uint32_t>(tiles + 7) / 8 * 8 : CUS, 512, LDS, s>>>(p);
+    return BS_OK;
+}
+float fill(uint64_t tiles) { return static_cast<float>(tiles) / static_cast<float>((tiles + CUS - 1) / CUS * CUS); }
+
+template <typename T>
 int launch_forward(Params p, hipStream_t s) {
     if (p.rows <= FEW) {
         if (p.rows <= 16)
@@ -520,6 +820,9 @@ int launch_forward(Params p, hipStream_t s) {
         return BS_OK;
     }
     const bool direct = rows16(p.x, p.xs) && rows16(p.wg, p.wgs) && rows16(p.wu, p.wus);
+    const uint64_t big = tiles_of(p.rows, p.cols, 256, 128);
+    if (direct && fill(big) >= 0.55f && p.rows >= 256 && p.cols >= 128 && p.inner % 64 == 0 && p.inner >= 128 && p.xs < (1 << 22) && p.wgs < (1 << 22) && p.wgs == p.wus)
+        return start_big<T>(p, false, big, s);
     if (tiles_of(p.rows, p.cols, 128, 64) >= CUS) return direct ? start<T, GATED, Mid, true>(p, s) : start<T, GATED, Mid, false>(p, s);
     return direct ? start<T, GATED, Flat, true>(p, s) : start<T, GATED, Flat, false>(p, s);
 }
@@ -532,11 +835,17 @@ int launch_gradient(Params p, hipStream_t s) {
     if (p.splits == 1 && tiles_of(rows, cols, 128, 128) >= CUS) return direct ? start<T, FORM, Mid, true>(p, s) : start<T, FORM, Mid, false>(p, s);
     return direct ? start<T, FORM, Small, true>(p, s) : start<T, FORM, Small, false>(p, s);
 }
+uint64_t big_backward(const Params& p) {
+    return (p.dx ? tiles_of(p.rows, p.inner, 256, 256) : 0) + (p.dwg ? tiles_of(2ull * p.cols, p.inner, 256, 256) : 0);
+}
 template <typename T>
 int launch_backward(const Params& p, hipStream_t s) {
-    const uint64_t quads = static_cast<uint64_t>((p.rows + 63) / 64 * 64) * ((p.cols + 7) / 8);
-    const uint32_t rows_up = (p.rows + 63) / 64 * 64;
-    gated_slopes_kernel<T><<<static_cast<uint32_t>(std::min<uint64_t>((quads + 255) / 256, 1u << 22)), 256, 0, s>>>(p, rows_up, 0);
+    const bool big = rows16(p.x, p.xs) && rows16(p.wg, p.wgs) && rows16(p.wu, p.wus) && p.wgs == p.wus && p.xs < (1 << 22) && p.wgs < (1 << 22) && p.cols < (1 << 21) &&
+                     p.rows >= 256 && p.cols >= 128 && p.cols % 64 == 0 && p.inner >= 256 && p.inner % 8 == 0 && fill(big_backward(p)) >= 0.55f;
+    const uint32_t rows_up = (p.rows + 63) / 64 * 64, tail_rows = big && p.rows % 64 ? 64 : 0;
+    const uint64_t chunks = static_cast<uint64_t>(rows_up) * ((p.cols + 7) / 8) + static_cast<uint64_t>(tail_rows) * ((p.inner + 7) / 8);
+    gated_slopes_kernel<T><<<static_cast<uint32_t>(std::min<uint64_t>((chunks + 255) / 256, 1u << 22)), 256, 0, s>>>(p, rows_up, tail_rows);
+    if (big) return start_big<T>(p, true, big_backward(p), s);
     if (p.dx)
         if (const int rc = launch_gradient<T, INPUT>(p, s)) return rc;
     if (p.dwg)
@@ -559,12 +868,12 @@ int check_rows(const std::string& what, const char* name, const void* p, int64_t
     return BS_OK;
 }
 
-// the workspace of the gradients: d, then the pieces' sums of the one product and, in the same place, of the other
+// the workspace of the gradients: d, then x's tail or the pieces' sums of the one product and, in the same place, of the other
 uint64_t up16(uint64_t n) { return (n + 15) / 16 * 16; }
 uint64_t d_bytes(uint64_t rows, uint32_t cols) { return up16((rows + 63) / 64 * 64 * 2 * cols * 2); }
 uint64_t parts_bytes(uint64_t rows, uint32_t inner, uint32_t cols) {
     const uint64_t a = splits_of(rows, 2ull * cols, inner), b = splits_of(2ull * cols, rows, inner);
-    return std::max(a > 1 ? a * rows * inner * 4 : 0, b > 1 ? b * 2 * cols * inner * 4 : 0);
+    return std::max<uint64_t>(128ull * inner, std::max(a > 1 ? a * rows * inner * 4 : 0, b > 1 ? b * 2 * cols * inner * 4 : 0));
 }
 
 }  // namespace
@@ -627,7 +936,8 @@ extern "C" int bs_gated_backward(const void* dh, int64_t dh_stride, const void* 
         if (!workspace || workspace_bytes < need) return refuse(what + ": the workspace must hold " + std::to_string(need) + " bytes");
         if (!aligned16(workspace)) return refuse(what + ": the workspace must be 16-byte aligned");
         p.d = static_cast<char*>(workspace);
-        p.parts = reinterpret_cast<float*>(p.d + d_bytes(rows, cols));
+        p.tail = p.d + d_bytes(rows, cols);
+        p.parts = reinterpret_cast<float*>(p.tail);
         const int rc = type == BS_F16 ? launch_backward<f16>(p, s) : launch_backward<bf16>(p, s);
         return rc ? rc : launched("bs_gated_backward");
     }

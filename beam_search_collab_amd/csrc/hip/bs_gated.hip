@@ -153,13 +153,18 @@ __device__ inline void write_gated(const Params& p, uint32_t row, uint32_t col, 
 
 // ------------------------------------------------------------------------------------------------ tiles
 
+// read_transposed for code that counts its moves to LDS by itself (meet): the compiler takes every transposing read for one that
+// may read what a move writes, and puts a wait for all moves before it, unless the read's pointer is known to have no alias
+__device__ __forceinline__ s16x4 read_landed(const char* __restrict p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
 // 8 inner elements of a lane's row of an operand whose inner elements are rows of S bytes in LDS: lanes 16 g .. 16 g + 15 read
 // 4 rows x 16 columns and get a column's 4 rows each
 template <typename T, int S>
 __device__ inline Vec<T, 8> read_across(const char* tile, int inner, int column, int lane) {
     const int k = inner + (lane >> 5) * 8 + ((lane & 15) >> 2), e = column + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    const s16x4 lo = read_transposed(tile + place<S>(k, e >> 3) + (e & 7) * 2);
-    const s16x4 hi = read_transposed(tile + place<S>(k + 4, e >> 3) + (e & 7) * 2);
+    const s16x4 lo = read_landed(tile + place<S>(k, e >> 3) + (e & 7) * 2);
+    const s16x4 hi = read_landed(tile + place<S>(k + 4, e >> 3) + (e & 7) * 2);
     return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
 }
 
@@ -488,8 +493,9 @@ __global__ __launch_bounds__(512) void gated_few_kernel(Params p) {
 //   phase 1: read x1(t)              products w1 x0    move x0, w0 (t + 2)
 //   phase 2:                         products w0 x1    move w1 (t + 2)
 //   phase 3: read x0, w0 (t + 1)     products w1 x1    move x1 (t + 2)
-// GATED: w0 is of wg and w1 of wu.  A quarter of an operand whose rows are columns in memory lies in LDS as 64 inner elements x
-// its 128 rows.  A workgroup goes through its tiles without a break: the moves of the next tile's first steps are under way
+// GATED: w0 is of wg and w1 of wu.  Where an operand's rows are columns in memory, its quarters are its first and second 128
+// rows, so that a line of a move is 256 bytes (of 64 bytes in w and 128 in x, as the waves' rows follow each other, the
+// weights' gradients of 8192 x 4096 -> 4096 took 726 us), and lie in LDS as 64 inner elements x 128 rows.  A workgroup goes through its tiles without a break: the moves of the next tile's first steps are under way
 // while a tile's results are written.  A tile that would pass an edge is shifted back inside and does not write what its
 // neighbour writes.
 //
@@ -515,15 +521,14 @@ __device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint3
     };
 
     // bytes between the lines of an operand in memory, and this thread's part of a move: 64 lines of 64 inner elements, or 32
-    // inner elements of 128 rows, of which x's quarters have 64 of each 128 and w's 32 of each 64
+    // inner elements of 128 rows of the operand
     const uint64_t xhop = FORM == GATED ? static_cast<uint64_t>(p.xs) * 2 : static_cast<uint64_t>(p.cols) * 4;
     const uint64_t whop = FORM == WEIGHTS ? static_cast<uint64_t>(p.xs) * 2 : static_cast<uint64_t>(p.wgs) * 2;
     const int r = threadIdx.x >> 3, c = swizzle(r, threadIdx.x & 7);
     const int k = threadIdx.x >> 4, kc = (threadIdx.x & 15) ^ ((k & 3) << 2 | ((k >> 2) & 3));
-    const uint32_t vx = XT ? k * static_cast<uint32_t>(xhop) + ((kc >> 3) * 128 + (kc & 7) * 8) * 2 : r * static_cast<uint32_t>(xhop) + c * 16;
-    const uint32_t across = ((kc >> 2) * 64 + (kc & 3) * 8) * 2;
-    const uint32_t vw = WT ? k * static_cast<uint32_t>(whop) + across : r * static_cast<uint32_t>(whop) + c * 16;
-    const uint32_t vtail = k * p.inner * 2 + across;  // WEIGHTS: in x's tail
+    const uint32_t vx = XT ? k * static_cast<uint32_t>(xhop) + kc * 16 : r * static_cast<uint32_t>(xhop) + c * 16;
+    const uint32_t vw = WT ? k * static_cast<uint32_t>(whop) + kc * 16 : r * static_cast<uint32_t>(whop) + c * 16;
+    const uint32_t vtail = k * p.inner * 2 + kc * 16;  // WEIGHTS: in x's tail
     const int rows8 = wave * 8, rows8w = (rows8 & 31) + (rows8 >> 5) * 64;
     struct Source {
         const char *x, *w0, *w1;  // the tile's first lines at the step to be moved
@@ -543,18 +548,18 @@ __device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint3
             from.x = p.d + ms * xhop + t * 128ull;
             const uint32_t at = t * 64;
             from.w0 = (at < p.cols ? static_cast<const char*>(p.wg) + at * whop : static_cast<const char*>(p.wu) + (at - p.cols) * whop) + ns * 2;
-            from.w1 = from.w0 + 64;
+            from.w1 = from.w0 + 256;
         } else {
             from.x = p.d + t * 64ull * xhop + ms * 2;
             from.tail = t * 64 + 64 > p.rows;
             from.whop = from.tail ? p.inner * 2ull : whop;
             from.w0 = (from.tail ? p.tail : static_cast<const char*>(p.x) + t * 64ull * whop) + ns * 2;
-            from.w1 = from.w0 + 64;
+            from.w1 = from.w0 + 256;
         }
     };
     auto move_x = [&](int slot, int g, int i) {
         if (XT)
-            move16(from.x + i * 32 * xhop + g * 128, vx, buf + slot * STEP + g * 8192 + i * 4096 + wave * 512);
+            move16(from.x + i * 32 * xhop + g * 256, vx, buf + slot * STEP + g * 8192 + i * 4096 + wave * 512);
         else
             move16(from.x + (i * 128 + g * 64) * xhop, vx, buf + slot * STEP + (i * 128 + g * 64 + rows8) * 64);
     };
@@ -579,7 +584,7 @@ __device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint3
         aw[half] = place<256>(kk, ((wave & 3) * 32 + e) >> 3) + (e & 7) * 2;
     }
     auto pair = [&](const T* base, int lo, int hi) {
-        const s16x4 a = read_transposed(reinterpret_cast<const char*>(base) + lo), b = read_transposed(reinterpret_cast<const char*>(base) + hi);
+        const s16x4 a = read_landed(reinterpret_cast<const char*>(base) + lo), b = read_landed(reinterpret_cast<const char*>(base) + hi);
         return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     };
     auto read_x = [&](int slot, int j, int s) {
@@ -722,7 +727,8 @@ __device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint3
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     const int rr = q * 8 + (lane >> 3), cc = (lane & 7) * 2;
-                    const uint32_t row = ms + wm + g * 16 + rr, col = ns + wn + cc * 4;
+                    const uint32_t row = ms + (XT ? (g >> 2) * 128 + (wave >> 2) * 64 + (g & 3) * 16 : wm + g * 16) + rr;
+                    const uint32_t col = ns + (cc >> 3) * 128 + (wave & 3) * 32 + (cc & 7) * 4;
                     take(rr, cc, z);
                     if (row >= m0) give(row_of<T, FORM>(p, row), col, z);
                 }

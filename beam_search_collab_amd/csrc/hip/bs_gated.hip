@@ -153,18 +153,13 @@ __device__ inline void write_gated(const Params& p, uint32_t row, uint32_t col, 
 
 // ------------------------------------------------------------------------------------------------ tiles
 
-// read_transposed for code that counts its moves to LDS by itself (meet): the compiler takes every transposing read for one that
-// may read what a move writes, and puts a wait for all moves before it, unless the read's pointer is known to have no alias
-__device__ __forceinline__ s16x4 read_landed(const char* __restrict p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-}
 // 8 inner elements of a lane's row of an operand whose inner elements are rows of S bytes in LDS: lanes 16 g .. 16 g + 15 read
 // 4 rows x 16 columns and get a column's 4 rows each
 template <typename T, int S>
 __device__ inline Vec<T, 8> read_across(const char* tile, int inner, int column, int lane) {
     const int k = inner + (lane >> 5) * 8 + ((lane & 15) >> 2), e = column + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    const s16x4 lo = read_landed(tile + place<S>(k, e >> 3) + (e & 7) * 2);
-    const s16x4 hi = read_landed(tile + place<S>(k + 4, e >> 3) + (e & 7) * 2);
+    const s16x4 lo = read_transposed(tile + place<S>(k, e >> 3) + (e & 7) * 2);
+    const s16x4 hi = read_transposed(tile + place<S>(k + 4, e >> 3) + (e & 7) * 2);
     return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
 }
 
@@ -584,7 +579,7 @@ __device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint3
         aw[half] = place<256>(kk, ((wave & 3) * 32 + e) >> 3) + (e & 7) * 2;
     }
     auto pair = [&](const T* base, int lo, int hi) {
-        const s16x4 a = read_landed(reinterpret_cast<const char*>(base) + lo), b = read_landed(reinterpret_cast<const char*>(base) + hi);
+        const s16x4 a = read_transposed(reinterpret_cast<const char*>(base) + lo), b = read_transposed(reinterpret_cast<const char*>(base) + hi);
         return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     };
     auto read_x = [&](int slot, int j, int s) {

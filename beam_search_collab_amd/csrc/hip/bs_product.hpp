@@ -104,9 +104,10 @@ __device__ inline int place(int r, int c) {
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-__device__ inline s16x4 read_transposed(const char* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
-        reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p)));
+// For code that counts its moves to LDS by itself: the compiler takes every transposing read for one that may read what a move
+// writes, and puts a wait for all of the wave's moves before it, unless the read's pointer is known to have no alias.
+__device__ __forceinline__ s16x4 read_transposed(const char* __restrict p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
 }
 
 }  // namespace bse

@@ -479,8 +479,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     // is short too and half of a short prompt's tiles are such (passages: 74 us, 80 with two); two for heads of 128
     // (documents: 989 us, 1001 with one)
     constexpr int KB = DP <= 64 ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) char lds[2][2 * TILE];
-    __shared__ int flag;
+    // Dynamic: of two objects whose sizes it knows, the compiler would keep the moves apart, and then let every read of the
+    // tiles wait for all moves under way.
+    extern __shared__ __attribute__((aligned(16))) char tiles_[];
+    auto lds = [&](uint32_t i) { return tiles_ + (i & 1) * (2 * TILE); };
+    int& flag = *reinterpret_cast<int*>(tiles_ + 4 * TILE);
     const bs_attention_args& a = p.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
     const uint32_t tile = p.by_kv.quotient(blockIdx.x), kvh = blockIdx.x - tile * a.kv_heads;
@@ -504,7 +507,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     const uint32_t parts = (ke - full + BN - 1) / BN, tiles = parts + (full - kb) / BN;
     auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
     if (a.head_dim != DP) {  // the padding of the heads is never moved to
-        for (int i = threadIdx.x; i < 2 * 2 * TILE / 16; i += 256) reinterpret_cast<Vec<float, 4>*>(lds[0])[i] = Vec<float, 4>{};
+        for (int i = threadIdx.x; i < 2 * 2 * TILE / 16; i += 256) reinterpret_cast<Vec<float, 4>*>(tiles_)[i] = Vec<float, 4>{};
     }
     if (threadIdx.x == 0) flag = 0;
     settle();
@@ -518,9 +521,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
             front.any(u * BN, to);
     };
     if (tiles)
-        mover.any(start(0), lds[0]);
+        mover.any(start(0), lds(0));
     else if (Prefix)
-        bring(0, lds[0]);
+        bring(0, lds(0));
     const Place me = place_of(p, sq, kvh, row0 + wave * 32 + l, rows);
     Rows<T, DP> me_;
     me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
@@ -534,12 +537,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     Found<DP / 32> found;
     for (int pass = PLAIN; parts; ++pass) {
         for (uint32_t t = 0; t < parts; ++t) {
-            char* tk = lds[t & 1];
+            char* tk = lds(t);
             meet();  // tile t is in LDS, and nobody reads tile t - 1 any more
             if (t + 1 < tiles)
-                mover.any(start(t + 1), lds[~t & 1]);
+                mover.any(start(t + 1), lds(t + 1));
             else if (Prefix)
-                bring(t + 1 - tiles, lds[~t & 1]);
+                bring(t + 1 - tiles, lds(t + 1));
             if (start(t) + BN > all || pass != PLAIN) {
                 if (start(t) + BN > all) blank<S>(tk + TILE, all - start(t), BN, threadIdx.x, 256);  // start(t) < ke <= all
                 settle();
@@ -565,15 +568,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
             meet();
         }
         me_.clear();
-        mover.any(start(0), lds[0]);  // tile `parts` has landed, and is moved again
+        mover.any(start(0), lds(0));  // tile `parts` has landed, and is moved again
     }
     for (uint32_t t = parts; t < tiles; ++t) {
-        const char* tk = lds[t & 1];
+        const char* tk = lds(t);
         meet();
         if (t + 1 < tiles)
-            mover.near(kb + (t + 1 - parts) * BN, lds[~t & 1]);
+            mover.near(kb + (t + 1 - parts) * BN, lds(t + 1));
         else if (Prefix)
-            bring(t + 1 - tiles, lds[~t & 1]);
+            bring(t + 1 - tiles, lds(t + 1));
         if (reach) {
             // a loop of one turn: as a block of its own the step is scheduled apart from the moves (documents: 989 us, 1004
             // in one block with them)
@@ -583,9 +586,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     }
     if constexpr (Prefix) {
         for (uint32_t u = 0; u < shared_tiles; ++u) {
-            char* tk = lds[(tiles + u) & 1];
+            char* tk = lds(tiles + u);
             meet();
-            bring(u + 1, lds[~(tiles + u) & 1]);
+            bring(u + 1, lds(tiles + u + 1));
             if (u < shared_whole) {
                 if (wave0 < rows) {
 #pragma unroll 1
@@ -878,6 +881,15 @@ int check(const char* what, const bs_attention_args* a) {
     return BS_OK;
 }
 
+template <typename T, int DP, bool Prefix>
+int start_tiles(const Params& p, hipStream_t s) {
+    constexpr int LDS = 4 * BN * ROW<DP> + 16;  // two tiles of keys and values, and a flag
+    auto* k = attention_kernel<T, DP, Prefix>;
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), LDS, done)) return rc;
+    k<<<dim3(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits), 256, LDS, s>>>(p);
+    return BS_OK;
+}
 template <typename T, int DP, bool Near>
 int start_few(const Params& p, hipStream_t s) {
     constexpr int LDS = FEW_WAVES * 32768;
@@ -891,13 +903,7 @@ template <typename T, int DP>
 int start(const Params& p, hipStream_t s) {
     if (!near_of(p.a)) return start_few<T, DP, false>(p, s);  // rows too far apart for the other kernel's moves
     if (few_of(p.a)) return start_few<T, DP, true>(p, s);
-    attention_kernel<T, DP, false><<<dim3(static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), p.splits), 256, 0, s>>>(p);
-    return BS_OK;
-}
-template <typename T, int DP>
-int start_along(const Params& p, hipStream_t s) {
-    attention_kernel<T, DP, true><<<static_cast<uint32_t>(tiles_of(p.a, 128) * p.a.kv_heads), 256, 0, s>>>(p);
-    return BS_OK;
+    return start_tiles<T, DP, false>(p, s);
 }
 
 template <typename T>
@@ -965,7 +971,7 @@ template <typename T>
 int launch_prefix(const Params& p, void* workspace, hipStream_t s) {
     const uint32_t d = p.a.head_dim;
     if (along_of(p.a)) {
-        const int rc = d <= 32 ? start_along<T, 32>(p, s) : d <= 64 ? start_along<T, 64>(p, s) : d <= 96 ? start_along<T, 96>(p, s) : start_along<T, 128>(p, s);
+        const int rc = d <= 32 ? start_tiles<T, 32, true>(p, s) : d <= 64 ? start_tiles<T, 64, true>(p, s) : d <= 96 ? start_tiles<T, 96, true>(p, s) : start_tiles<T, 128, true>(p, s);
         return rc ? rc : launched("bs_attention_shared_prefix");
     }
     Apart x = apart(p.a, p.prefix);

@@ -25,7 +25,10 @@ struct Params {
     Divisor by_group, by_kv;
     uint32_t splits;   // pieces of the keys
     uint32_t piece;    // keys of a piece, a multiple of BN
-    uint32_t before;   // parts of a row that another launch writes, in front of these
+    uint32_t before;   // parts of a row that an earlier launch has written: in front of these, or if there is no
+                       // part_out, to be joined to the results (at front_out and front_stat, laid out alike)
+    const float* front_out;
+    const float2* front_stat;
     float* part_out;   // null, or where parts go: (before + splits) x q_tokens x heads x head_dim, sums of p v, unscaled
     float2* part_stat; // as many x q_tokens x heads: maximum (in units of log2) and sum
     bs_attention_prefix prefix; // keys that every row sees besides its sequence's
@@ -424,9 +427,41 @@ __device__ inline Place place_of(const Params& p, const Sequence& sq, uint32_t k
     return x;
 }
 
+// joins the parts that an earlier launch has left of row `at`
+template <typename T, int DP>
+__device__ inline void join_front(const Params& p, int64_t at, Rows<T, DP>& r, int h) {
+    const bs_attention_args& a = p.a;
+    const int64_t rows = static_cast<int64_t>(a.q_tokens) * a.heads;
+    float top = r.top;
+    for (uint32_t s = 0; s < p.before; ++s) top = fmaxf(top, p.front_stat[s * rows + at].x);
+    const float base = top == NONE ? 0.0f : top, own = __builtin_amdgcn_exp2f(r.top - base);
+    r.top = top;
+    r.sum *= own;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r.o[d][i] *= own;
+    for (uint32_t s = 0; s < p.before; ++s) {
+        const float2 st = p.front_stat[s * rows + at];
+        const float gain = __builtin_amdgcn_exp2f(st.x - base);
+        r.sum = fmaf(st.y, gain, r.sum);
+        const float* from = p.front_out + (s * rows + at) * a.head_dim;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t e = d * 32 + i * 8 + h * 4;
+                if (e >= a.head_dim) continue;
+                const f32x4 v = *reinterpret_cast<const f32x4*>(from + e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r.o[d][i * 4 + j] = fmaf(v[j], gain, r.o[d][i * 4 + j]);
+            }
+    }
+}
+
 // a row's results: parts to the workspace, or the output
 template <typename T, int DP>
-__device__ inline void write_rows(const Params& p, const Sequence& sq, const Place& me, const Rows<T, DP>& r, int h) {
+__device__ inline void write_rows(const Params& p, const Sequence& sq, const Place& me, Rows<T, DP>& r, int h) {
     if (!me.live) return;
     const bs_attention_args& a = p.a;
     const int64_t at = static_cast<int64_t>(sq.q0 + me.tok) * a.heads + me.head;
@@ -444,6 +479,7 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
             }
         return;
     }
+    if (p.before) join_front<T, DP>(p, at, r, h);
     const float over = reciprocal_of(r.sum);
     T* out = static_cast<T*>(a.out) + static_cast<int64_t>(sq.q0 + me.tok) * a.out_stride + static_cast<int64_t>(me.head) * a.out_head_stride;
 #pragma unroll
@@ -471,7 +507,7 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 // the documents: two groups of waves half a step apart, meeting between their phases (1244 against 1175), moves between
 // the products and exponentials instead of before them (1246 against 1142).
 //
-// Prefix: behind the sequence's own keys the tiles of the prefix, which every row sees, the last of them in part.
+// Prefix: every row sees the prefix's keys too, in the same pass.
 template <typename T, int DP, bool Prefix>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params p) {
     constexpr int ROWS = 128, S = ROW<DP>, TILE = BN * S;
@@ -504,26 +540,29 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     // The tiles that some row does not see whole come first, on a state of zeros, so that they can be taken again.
     const uint32_t seen = keys_of(a, sq, p.by_group.quotient(row0));  // by every row of the tile
     const uint32_t full = max(kb, min(ke, seen) / BN * BN);          // kb and pieces are multiples of BN
-    const uint32_t parts = (ke - full + BN - 1) / BN, tiles = parts + (full - kb) / BN;
-    auto start = [&](uint32_t t) { return t < parts ? full + t * BN : kb + (t - parts) * BN; };
+    const uint32_t parts = (ke - full + BN - 1) / BN, own_whole = (full - kb) / BN;
+    // The prefix: its last tile, if it is not whole, goes before those, and its whole tiles after the sequence's.
+    const uint32_t shared = Prefix ? p.prefix.tokens : 0, rest = shared % BN, extra = rest ? 1 : 0;
+    const uint32_t mixed = extra + parts, tiles = mixed + own_whole + shared / BN;
     if (a.head_dim != DP) {  // the padding of the heads is never moved to
         for (int i = threadIdx.x; i < 2 * 2 * TILE / 16; i += 256) reinterpret_cast<Vec<float, 4>*>(tiles_)[i] = Vec<float, 4>{};
     }
     if (threadIdx.x == 0) flag = 0;
     settle();
-    const Mover<S, BN, 256> mover(a, sq.k0, sq.nk, a.head_dim, kvh, threadIdx.x);
-    const uint32_t shared = Prefix ? p.prefix.tokens : 0, shared_whole = shared / BN, shared_tiles = (shared + BN - 1) / BN;
-    auto bring = [&](uint32_t u, char* to) {  // tile u of the prefix
-        const Mover<S, BN, 256> front(p.prefix, 0, shared, a.head_dim, kvh, threadIdx.x);
-        if (u < shared_whole)
-            front.near(u * BN, to);
-        else if (u < shared_tiles)
-            front.any(u * BN, to);
+    using Moves = Mover<S, BN, 256>;
+    const Moves mover(a, sq.k0, sq.nk, a.head_dim, kvh, threadIdx.x);
+    auto front = [&] { return Moves(p.prefix, 0, shared, a.head_dim, kvh, threadIdx.x); };
+    auto bring = [&](uint32_t t) {  // any tile
+        if (Prefix && t < extra)
+            front().any(shared - rest, lds(t));
+        else if (t < mixed)
+            mover.any(full + (t - extra) * BN, lds(t));
+        else if (!Prefix || t < mixed + own_whole)
+            mover.any(kb + (t - mixed) * BN, lds(t));
+        else
+            front().any((t - mixed - own_whole) * BN, lds(t));
     };
-    if (tiles)
-        mover.any(start(0), lds(0));
-    else if (Prefix)
-        bring(0, lds(0));
+    if (tiles) bring(0);
     const Place me = place_of(p, sq, kvh, row0 + wave * 32 + l, rows);
     Rows<T, DP> me_;
     me_.load(static_cast<const T*>(a.q) + static_cast<int64_t>(sq.q0 + me.tok) * a.q_stride + static_cast<int64_t>(me.head) * a.q_head_stride,
@@ -534,24 +573,26 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
     // keys up to which this wave's last row sees; a wave past the last row has nothing to do but its moves
     const uint32_t wave0 = row0 + wave * 32;
     const uint32_t reach = wave0 < rows ? min(ke, keys_of(a, sq, p.by_group.quotient(min(rows, wave0 + 32) - 1))) : 0;
+    const bool works = Prefix ? wave0 < rows : reach > 0;
     Found<DP / 32> found;
-    for (int pass = PLAIN; parts; ++pass) {
-        for (uint32_t t = 0; t < parts; ++t) {
+    for (int pass = PLAIN; mixed; ++pass) {
+        for (uint32_t t = 0; t < mixed; ++t) {
             char* tk = lds(t);
             meet();  // tile t is in LDS, and nobody reads tile t - 1 any more
-            if (t + 1 < tiles)
-                mover.any(start(t + 1), lds(t + 1));
-            else if (Prefix)
-                bring(t + 1 - tiles, lds(t + 1));
-            if (start(t) + BN > all || pass != PLAIN) {
-                if (start(t) + BN > all) blank<S>(tk + TILE, all - start(t), BN, threadIdx.x, 256);  // start(t) < ke <= all
+            if (t + 1 < tiles) bring(t + 1);
+            // the tile's first key, the first one past it that no row sees, those that this row and its wave see
+            const bool ahead = Prefix && t < extra;
+            const uint32_t j0 = ahead ? shared - rest : full + (t - extra) * BN, end = ahead ? shared : all;
+            const uint32_t see = ahead ? shared : mine, far = ahead ? (works ? shared : 0) : reach;
+            if (j0 + BN > end || pass != PLAIN) {
+                if (j0 + BN > end) blank<S>(tk + TILE, end - j0, BN, threadIdx.x, 256);  // j0 < end
                 settle();
                 if (pass != PLAIN) sift<T>(tk + TILE, TILE, pass, threadIdx.x, 256);
                 settle();
             }
 #pragma unroll 1
             for (int b = 0; b < BN; b += KB * 32)
-                if (reach > start(t) + b) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, start(t) + b, mine, scale_of(pass, scale), lane);
+                if (far > j0 + b) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, j0 + b, see, scale_of(pass, scale), lane);
         }
         if (pass == PLAIN) {
             if (seen == all) break;  // all rows see the same keys, and the others' values are blank
@@ -568,39 +609,29 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params
             meet();
         }
         me_.clear();
-        mover.any(start(0), lds(0));  // tile `parts` has landed, and is moved again
+        bring(0);  // tile `mixed` has landed, and is moved again
     }
-    for (uint32_t t = parts; t < tiles; ++t) {
+    Moves source = mover;
+    bool ahead = false;
+    for (uint32_t t = mixed; t < tiles; ++t) {
         const char* tk = lds(t);
         meet();
-        if (t + 1 < tiles)
-            mover.near(kb + (t + 1 - parts) * BN, lds(t + 1));
-        else if (Prefix)
-            bring(t + 1 - tiles, lds(t + 1));
-        if (reach) {
+        if (t + 1 < tiles) {
+            uint32_t j0 = kb + (t + 1 - mixed) * BN;
+            if constexpr (Prefix) {
+                if (t + 1 >= mixed + own_whole) {
+                    if (!ahead) source = front();
+                    ahead = true;
+                    j0 = (t + 1 - mixed - own_whole) * BN;
+                }
+            }
+            source.near(j0, lds(t + 1));
+        }
+        if (works) {
             // a loop of one turn: as a block of its own the step is scheduled apart from the moves (documents: 989 us, 1004
             // in one block with them)
 #pragma unroll 1
             for (int b = 0; b < BN; b += 64) me_.template step<2, false>(tk + b * S, tk + TILE + b * S, 0, 0, scale, lane);
-        }
-    }
-    if constexpr (Prefix) {
-        for (uint32_t u = 0; u < shared_tiles; ++u) {
-            char* tk = lds(tiles + u);
-            meet();
-            bring(u + 1, lds(tiles + u + 1));
-            if (u < shared_whole) {
-                if (wave0 < rows) {
-#pragma unroll 1
-                    for (int b = 0; b < BN; b += 64) me_.template step<2, false>(tk + b * S, tk + TILE + b * S, 0, 0, scale, lane);
-                }
-            } else {
-                blank<S>(tk + TILE, shared - u * BN, BN, threadIdx.x, 256);
-                settle();
-#pragma unroll 1
-                for (int b = 0; b < BN; b += KB * 32)
-                    if (wave0 < rows && u * BN + b < shared) me_.template step<KB, true>(tk + b * S, tk + TILE + b * S, u * BN + b, shared, scale, lane);
-            }
         }
     }
     me_.join_halves();
@@ -731,6 +762,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
     const uint32_t quads = a.head_dim / 4;
     for (uint32_t i = threadIdx.x; i < here * quads; i += W * 64) {
         const uint32_t r = i / quads, e = i % quads * 4;
+        const Place x = place_of(p, sq, kvh, row0 + r, rows);
+        const int64_t at = static_cast<int64_t>(sq.q0 + x.tok) * a.heads + x.head, all_rows = static_cast<int64_t>(a.q_tokens) * a.heads;
         float t = NONE, sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; ++w) t = fmaxf(t, stat[w][r].x);
@@ -740,8 +773,21 @@ __global__ __launch_bounds__(FEW_WAVES * 64, 1) void attention_few_kernel(Params
             sum += stat[w][r].y * __builtin_amdgcn_exp2f(stat[w][r].x - (t == NONE ? 0.0f : t));
             v += *reinterpret_cast<const f32x4*>(all_o + (w * 32 + r) * (DP + 4) + e);
         }
-        const Place x = place_of(p, sq, kvh, row0 + r, rows);
-        const int64_t at = static_cast<int64_t>(sq.q0 + x.tok) * a.heads + x.head;
+        if (p.front_out) {  // parts that an earlier launch has left
+            const float own = t;
+#pragma unroll 4
+            for (uint32_t s = 0; s < p.before; ++s) t = fmaxf(t, p.front_stat[s * all_rows + at].x);
+            const float base = t == NONE ? 0.0f : t, gain = __builtin_amdgcn_exp2f(own - base);
+            sum *= gain;
+            v *= gain;
+#pragma unroll 4
+            for (uint32_t s = 0; s < p.before; ++s) {
+                const float2 st = p.front_stat[s * all_rows + at];
+                const float g = __builtin_amdgcn_exp2f(st.x - base);
+                sum = fmaf(st.y, g, sum);
+                v += *reinterpret_cast<const f32x4*>(p.front_out + (s * all_rows + at) * a.head_dim + e) * g;
+            }
+        }
         if (p.part_out) {
             const int64_t slot = static_cast<int64_t>(p.before + blockIdx.y) * a.q_tokens * a.heads + at;
             *reinterpret_cast<f32x4*>(p.part_out + slot * a.head_dim + e) = v;
@@ -943,44 +989,85 @@ bs_attention_args over_prefix(const bs_attention_args& a, const bs_attention_pre
     return b;
 }
 // Whether the sequences' tiles go along the prefix, each for itself, instead of the rows of all sequences at once apart from
-// their own keys.
-bool along_of(const bs_attention_args& a) {
-    const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * (a.heads / a.kv_heads);
-    return rows / a.sequences >= 64 && tiles_of(a, 128) * a.kv_heads >= 2 * CUS;
+// their own keys.  Counted in keys of the prefix that a tile takes (34 ns for heads of 128): along, every sequence has tiles of
+// its own, of which the last is half empty; apart, there are as few tiles as the rows fill, cut into pieces of the prefix where
+// they leave compute units idle (256 keys at least), but every row's part is written and read again, 400 keys' time a tile, and
+// a launch more is 360.  Along and apart: 128 single tokens over 16384, 32 heads of 128 669 and 82 us, 256 x 12..24 tokens over
+// 1000 166 and 160, 24 x 150..300 over 8192 855 and 813, 4 x 50..100 over 4000 89 and 65, but over 1000 32 and 40, 24 x
+// 128..384 over 8191 901 and 939, 8 x 10..20 over 500 19.4 and 26.3, 16 x 6..40 over 100, 12 heads of 64 12.4 and 16.7.  Own keys
+// that are cut into pieces are always apart.
+bool along_of(const bs_attention_args& a, const bs_attention_prefix& f) {
+    uint32_t splits, piece;
+    split(a, splits, piece);
+    if (splits > 1) return false;
+    const double slots = (a.head_dim <= 64 ? 3.0 : 2.0) * CUS, rows = static_cast<double>(a.q_tokens) * (a.heads / a.kv_heads), n = f.tokens;
+    const double full = rows / 128 * a.kv_heads / slots;  // rounds of workgroups
+    const double own = std::max<double>(a.sequences, rows / 128 + a.sequences / 2.0) * a.kv_heads / slots;
+    const double along = std::max(1.0, own) * n, apart = std::max(full * n, std::min(n, 256.0)) + 400 * std::max(full, 1.0) + 360;
+    return along <= apart;
+}
+// Pieces of the prefix for the rows of all sequences: the number that takes the fewest rounds of workgroups, a piece's keys each
+// and 400 keys' time for the parts.  At least 256 keys, at most 256 MB of parts.
+void cut_prefix(const bs_attention_args& a, uint32_t keys, uint32_t& splits, uint32_t& piece) {
+    const uint64_t slots = (a.head_dim <= 64 ? 3 : 2) * CUS, rows = static_cast<uint64_t>(a.q_tokens) * (a.heads / a.kv_heads);
+    const uint64_t groups = (rows + 127) / 128 * a.kv_heads, row = static_cast<uint64_t>(a.q_tokens) * a.heads * (a.head_dim + 2) * sizeof(float);
+    const uint64_t most = std::min<uint64_t>({64, std::max<uint64_t>(1, keys / 256), std::max<uint64_t>(1, (1ull << 28) / row)});
+    double best = 0.0;
+    for (uint64_t n = 1; n <= most; ++n) {
+        const uint64_t each = ((keys + n - 1) / n + 127) / 128 * 128, pieces = (keys + each - 1) / each;
+        const double time = static_cast<double>((groups * pieces + slots - 1) / slots * each) + 400.0 * static_cast<double>(groups * pieces) / static_cast<double>(slots);
+        if (n > 1 && time >= best) continue;
+        best = time;
+        splits = static_cast<uint32_t>(pieces);
+        piece = static_cast<uint32_t>(each);
+    }
 }
 struct Apart {
     Params front, own;
+    uint32_t parts;  // of a row in the workspace
     uint64_t bytes;
 };
 Apart apart(const bs_attention_args& a, const bs_attention_prefix& f) {
     Apart x{};
     x.front.a = over_prefix(a, f);
     x.own.a = a;
-    split(x.front.a, x.front.splits, x.front.piece);
     split(x.own.a, x.own.splits, x.own.piece);
+    if (few_of(x.front.a))
+        split(x.front.a, x.front.splits, x.front.piece);
+    else
+        cut_prefix(a, f.tokens, x.front.splits, x.front.piece);
     x.own.before = x.front.splits;
     for (Params* p : {&x.front, &x.own}) {
         p->group = a.heads / a.kv_heads;
         p->by_group = Divisor(p->group);
         p->by_kv = Divisor(a.kv_heads);
     }
-    x.bytes = static_cast<uint64_t>(x.front.splits + x.own.splits) * a.q_tokens * a.heads * (a.head_dim + 2) * sizeof(float);
+    x.parts = x.front.splits + (x.own.splits > 1 ? x.own.splits : 0);
+    x.bytes = static_cast<uint64_t>(x.parts) * a.q_tokens * a.heads * (a.head_dim + 2) * sizeof(float);
     return x;
 }
 template <typename T>
 int launch_prefix(const Params& p, void* workspace, hipStream_t s) {
     const uint32_t d = p.a.head_dim;
-    if (along_of(p.a)) {
+    if (along_of(p.a, p.prefix)) {
         const int rc = d <= 32 ? start_tiles<T, 32, true>(p, s) : d <= 64 ? start_tiles<T, 64, true>(p, s) : d <= 96 ? start_tiles<T, 96, true>(p, s) : start_tiles<T, 128, true>(p, s);
         return rc ? rc : launched("bs_attention_shared_prefix");
     }
     Apart x = apart(p.a, p.prefix);
-    for (Params* q : {&x.front, &x.own}) {
-        q->part_out = static_cast<float*>(workspace);
-        q->part_stat = reinterpret_cast<float2*>(q->part_out + static_cast<uint64_t>(x.front.splits + x.own.splits) * p.a.q_tokens * p.a.heads * d);
-        if (const int rc = start_any<T>(*q, s)) return rc;
+    float* out = static_cast<float*>(workspace);
+    float2* stat = reinterpret_cast<float2*>(out + static_cast<uint64_t>(x.parts) * p.a.q_tokens * p.a.heads * d);
+    x.front.part_out = out;
+    x.front.part_stat = stat;
+    if (x.own.splits > 1) {
+        x.own.part_out = out;
+        x.own.part_stat = stat;
+    } else {  // the own keys' launch joins the prefix's parts itself
+        x.own.front_out = out;
+        x.own.front_stat = stat;
     }
-    join<T>(x.own, s);
+    if (const int rc = start_any<T>(x.front, s)) return rc;
+    if (const int rc = start_any<T>(x.own, s)) return rc;
+    if (x.own.splits > 1) join<T>(x.own, s);
     return launched("bs_attention_shared_prefix");
 }
 
@@ -1049,7 +1136,7 @@ extern "C" int bs_attention_shared_prefix_workspace(const bs_attention_args* arg
         *bytes = workspace_of(*args);
         return BS_OK;
     }
-    *bytes = along_of(*args) ? 0 : apart(*args, *prefix).bytes;
+    *bytes = along_of(*args, *prefix) ? 0 : apart(*args, *prefix).bytes;
     return BS_OK;
 } catch (...) {
     return bs_internal_exception();
@@ -1076,7 +1163,7 @@ extern "C" int bs_attention_shared_prefix(const bs_attention_args* args, const b
     p.by_group = Divisor(p.group);
     p.by_kv = Divisor(a.kv_heads);
     p.splits = 1;
-    if (!along_of(a)) {
+    if (!along_of(a, f)) {
         const uint64_t need = apart(a, f).bytes;
         if (!workspace || workspace_bytes < need) return refuse(what + ": the workspace must hold " + std::to_string(need) + " bytes");
         if (!aligned16(workspace)) return refuse(what + ": the workspace must be 16-byte aligned");

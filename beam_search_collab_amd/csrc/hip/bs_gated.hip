@@ -32,10 +32,10 @@ struct Params {
     void *dx, *dwg, *dwu;
     char* d;      // rows_up x 2 cols, rows past the last are 0
     char* tail;   // the last rows % 64 rows of x, then zeros: 64 x inner
-    float* parts; // splits x the result
     uint32_t rows, inner, cols;
     int act;
-    uint32_t splits;
+    uint32_t input_splits, weight_splits;  // pieces of the gradients' inner dimensions; > 1: their sums go to
+    float *input_parts, *weight_parts;     // splits x the result
 };
 
 // ------------------------------------------------------------------------------------------------ d
@@ -164,18 +164,18 @@ __device__ inline Vec<T, 8> read_across(const char* tile, int inner, int column,
 }
 
 // Tiles of any size and alignment.  Direct: operands are 16-byte aligned, whole steps go from memory to LDS without registers.
+// Tile `b` of the product; of its inner dimension piece y of `splits`, whose sums go to `parts` if there are several.
 template <typename T, int FORM, typename C, bool Direct>
-__global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_kernel(Params p) {
+__device__ inline void one_tile(const Params& p, char* lds, uint32_t b, uint32_t y, uint32_t splits, float* parts) {
     constexpr bool XT = FORM == WEIGHTS, WT = FORM != GATED;  // the operand's rows are columns in memory
     constexpr int OUT = FORM == GATED ? C::BN / 2 : C::BN;    // columns of the result in a tile
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     T* buf = reinterpret_cast<T*>(lds);
     const uint32_t rows = rows_of<FORM>(p), cols = cols_of<FORM>(p), inner = inner_of<FORM>(p);
     // Workgroup b runs on XCD b mod 8: each XCD takes a contiguous run of tiles, 8 tile rows high, so that
     // the tiles in flight on it share operands in its L2.
     const uint32_t mt = (rows + C::BM - 1) / C::BM, nt = (cols + OUT - 1) / OUT, total = mt * nt;
-    const uint32_t xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
-    const uint32_t id = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
+    const uint32_t xcd = b & 7, q8 = total >> 3, r8 = total & 7;
+    const uint32_t id = xcd * q8 + (xcd < r8 ? xcd : r8) + (b >> 3);
     const uint32_t band = id / (8 * nt), high = mt - band * 8 < 8 ? mt - band * 8 : 8, in = id - band * 8 * nt;
     const uint32_t m0 = (band * 8 + in % high) * C::BM, n0 = in / high * OUT;
 
@@ -223,8 +223,8 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_ke
         return line & 32 ? static_cast<const T*>(p.wu) + static_cast<int64_t>(c) * p.wus + k : static_cast<const T*>(p.wg) + static_cast<int64_t>(c) * p.wgs + k;
     };
     // this workgroup's piece: whole steps [begin, whole), and for the last piece what is left after them
-    const uint32_t allsteps = (inner + C::BK - 1) / C::BK, piece = (allsteps + p.splits - 1) / p.splits;
-    const uint32_t begin = blockIdx.y * piece, steps = min(begin + piece, allsteps), whole = min(steps, inner / C::BK);
+    const uint32_t allsteps = (inner + C::BK - 1) / C::BK, piece = (allsteps + splits - 1) / splits;
+    const uint32_t begin = y * piece, steps = min(begin + piece, allsteps), whole = min(steps, inner / C::BK);
     auto fetch = [&](uint32_t t, Vec<T, 8> (&v)[C::MOVES]) {
 #pragma unroll
         for (int i = 0; i < C::MOVES; ++i) {
@@ -391,8 +391,8 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_ke
             if (row >= rows || col >= cols) continue;
             if constexpr (FORM == GATED) {
                 write_gated<T, 8>(p, row, col, z, u);
-            } else if (p.splits > 1) {
-                float* part = p.parts + (static_cast<size_t>(blockIdx.y) * rows + row) * cols + col;
+            } else if (splits > 1) {
+                float* part = parts + (static_cast<size_t>(y) * rows + row) * cols + col;
                 store_some<float, 4>(part, f32x4{z[0], z[1], z[2], z[3]}, static_cast<int>(cols - col));
                 if (cols - col > 4) store_some<float, 4>(part + 4, f32x4{z[4], z[5], z[6], z[7]}, static_cast<int>(cols - col) - 4);
             } else {
@@ -400,6 +400,23 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_ke
             }
         }
         __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <typename T, typename C, bool Direct>
+__global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_kernel(Params p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    one_tile<T, GATED, C, Direct>(p, lds, blockIdx.x, 0, 1, nullptr);
+}
+// Both products of the gradients in one launch, `inputs` workgroups of dx first.
+template <typename T, typename C, bool Direct>
+__global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_backward_kernel(Params p, uint32_t input_tiles, uint32_t inputs, uint32_t weight_tiles) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if (blockIdx.x < inputs) {
+        one_tile<T, INPUT, C, Direct>(p, lds, blockIdx.x % input_tiles, blockIdx.x / input_tiles, p.input_splits, p.input_parts);
+    } else {
+        const uint32_t b = blockIdx.x - inputs;
+        one_tile<T, WEIGHTS, C, Direct>(p, lds, b % weight_tiles, b / weight_tiles, p.weight_splits, p.weight_parts);
     }
 }
 
@@ -411,9 +428,10 @@ __global__ __launch_bounds__(256) void gated_join_kernel(Params p) {
     const uint32_t row = static_cast<uint32_t>(at / across), col = static_cast<uint32_t>(at % across) * 4;
     if (row >= rows) return;
     const int n = static_cast<int>(cols - col);
-    const float* part = p.parts + static_cast<size_t>(row) * cols + col;
+    const uint32_t splits = FORM == INPUT ? p.input_splits : p.weight_splits;
+    const float* part = (FORM == INPUT ? p.input_parts : p.weight_parts) + static_cast<size_t>(row) * cols + col;
     f32x4 s = load_some<float, 4>(part, n);
-    for (uint32_t i = 1; i < p.splits; ++i) s += load_some<float, 4>(part + static_cast<size_t>(i) * rows * cols, n);
+    for (uint32_t i = 1; i < splits; ++i) s += load_some<float, 4>(part + static_cast<size_t>(i) * rows * cols, n);
     const float z[4] = {s[0], s[1], s[2], s[3]};
     write<T, FORM, 4>(p, row, col, z);
 }
@@ -774,27 +792,12 @@ constexpr uint32_t FEW = 32;
 
 uint64_t tiles_of(uint64_t rows, uint64_t cols, uint32_t high, uint32_t wide) { return (rows + high - 1) / high * ((cols + wide - 1) / wide); }
 
-// pieces of the inner dimension for tiles of 64, where they leave compute units idle
-uint32_t splits_of(uint64_t rows, uint64_t inner, uint64_t cols) {
-    const uint64_t tiles = tiles_of(rows, cols, 64, 64);
-    const uint64_t want = std::min<uint64_t>(2 * CUS / tiles, inner / 1024);
-    if (want < 2) return 1;
-    const uint64_t steps = (inner + 63) / 64, piece = (steps + want - 1) / want;
-    return static_cast<uint32_t>((steps + piece - 1) / piece);
-}
-
-template <typename T, int FORM, typename C, bool Direct>
+template <typename T, typename C, bool Direct>
 int start(const Params& p, hipStream_t s) {
-    auto* k = gated_kernel<T, FORM, C, Direct>;
+    auto* k = gated_kernel<T, C, Direct>;
     static std::atomic<uint64_t> done{0};
     if (const int rc = allow_lds(reinterpret_cast<const void*>(k), C::LDS, done)) return rc;
-    k<<<dim3(static_cast<uint32_t>(tiles_of(rows_of<FORM>(p), cols_of<FORM>(p), C::BM, FORM == GATED ? C::BN / 2 : C::BN)), p.splits), C::THREADS, C::LDS, s>>>(p);
-    if constexpr (FORM != GATED) {
-        if (p.splits > 1) {
-            const uint64_t quads = static_cast<uint64_t>(rows_of<FORM>(p)) * ((cols_of<FORM>(p) + 3) / 4);
-            gated_join_kernel<T, FORM><<<static_cast<uint32_t>((quads + 255) / 256), 256, 0, s>>>(p);
-        }
-    }
+    k<<<static_cast<uint32_t>(tiles_of(p.rows, p.cols, C::BM, C::BN / 2)), C::THREADS, C::LDS, s>>>(p);
     return BS_OK;
 }
 
@@ -824,41 +827,112 @@ int launch_forward(Params p, hipStream_t s) {
     const uint64_t big = tiles_of(p.rows, p.cols, 256, 128);
     if (direct && fill(big) >= 0.55f && p.rows >= 256 && p.cols >= 128 && p.inner % 64 == 0 && p.inner >= 128 && p.xs < (1 << 22) && p.wgs < (1 << 22) && p.wgs == p.wus)
         return start_big<T>(p, false, big, s);
-    if (tiles_of(p.rows, p.cols, 128, 64) >= CUS) return direct ? start<T, GATED, Mid, true>(p, s) : start<T, GATED, Mid, false>(p, s);
-    return direct ? start<T, GATED, Flat, true>(p, s) : start<T, GATED, Flat, false>(p, s);
+    if (tiles_of(p.rows, p.cols, 128, 64) >= CUS) return direct ? start<T, Mid, true>(p, s) : start<T, Mid, false>(p, s);
+    return direct ? start<T, Flat, true>(p, s) : start<T, Flat, false>(p, s);
 }
-template <typename T, int FORM>
-int launch_gradient(Params p, hipStream_t s) {
-    const uint64_t rows = rows_of<FORM>(p), cols = cols_of<FORM>(p);
-    // of INPUT: a step lies in one weight
-    const bool direct = p.cols % 64 == 0 && p.inner % 8 == 0 && (FORM == WEIGHTS ? rows16(p.x, p.xs) : rows16(p.wg, p.wgs) && rows16(p.wu, p.wus) && p.wgs == p.wus);
-    p.splits = splits_of(rows, inner_of<FORM>(p), cols);
-    if (p.splits == 1 && tiles_of(rows, cols, 128, 128) >= CUS) return direct ? start<T, FORM, Mid, true>(p, s) : start<T, FORM, Mid, false>(p, s);
-    return direct ? start<T, FORM, Small, true>(p, s) : start<T, FORM, Small, false>(p, s);
+// How the gradients' two products are cut: tiles of 256 (big), 128 or 64, and with the latter pieces of the inner dimensions.
+struct Plan {
+    bool big, mid;
+    uint32_t input_splits, weight_splits;
+    uint64_t input_tiles, weight_tiles;
+};
+// `dx`, `dw`: which are wanted; `big`: whether the operands' alignment and strides allow tiles of 256
+Plan plan_of(uint64_t rows, uint32_t inner, uint32_t cols, bool dx, bool dw, bool big) {
+    auto cut = [&](uint32_t size) {
+        Plan n{};
+        n.input_tiles = dx ? tiles_of(rows, inner, size, size) : 0;
+        n.weight_tiles = dw ? tiles_of(2ull * cols, inner, size, size) : 0;
+        n.input_splits = n.weight_splits = 1;
+        return n;
+    };
+    Plan n = cut(256);
+    if (big && rows >= 256 && cols >= 128 && cols % 64 == 0 && inner >= 256 && inner % 8 == 0) {
+        // A workgroup per compute unit takes its share of the tiles one after the other, dx's first.  Worth it where they are
+        // at work for 0.55 of the time.
+        const uint64_t most = (n.input_tiles + n.weight_tiles + CUS - 1) / CUS, first = std::min((n.input_tiles + CUS - 1) / CUS, most);
+        const uint64_t input_steps = cols / 32, weight_steps = (rows + 63) / 64, time = first * input_steps + (most - first) * weight_steps;
+        const uint64_t work = n.input_tiles * input_steps + n.weight_tiles * weight_steps;
+        if (static_cast<double>(work) >= 0.55 * static_cast<double>(time * CUS)) {
+            n.big = true;
+            return n;
+        }
+    }
+    // Two workgroups per compute unit, in one launch; pieces of an inner dimension about as long as their share of all
+    // steps, of 1024 elements at least.  Tiles of 128 and 64: gradients of 1000 x 1024 -> 2048 (320 tiles of 128) 36.3 and 40.4
+    // us, of 300 x 768 -> 2048 (210) 24.9 and 23.7.
+    n = cut(128);
+    n.mid = n.input_tiles + n.weight_tiles >= CUS;
+    if (!n.mid) n = cut(64);
+    const uint64_t input_steps = (2ull * cols + 63) / 64, weight_steps = (rows + 63) / 64;
+    const uint64_t share = std::max<uint64_t>(16, (n.input_tiles * input_steps + n.weight_tiles * weight_steps + 2 * CUS - 1) / (2 * CUS));
+    auto splits = [&](uint64_t steps) { return steps * 2 > share * 3 ? static_cast<uint32_t>((steps + share - 1) / share) : 1u; };
+    if (dx) n.input_splits = splits(input_steps);
+    if (dw) n.weight_splits = splits(weight_steps);
+    return n;
 }
-uint64_t big_backward(const Params& p) {
-    return (p.dx ? tiles_of(p.rows, p.inner, 256, 256) : 0) + (p.dwg ? tiles_of(2ull * p.cols, p.inner, 256, 256) : 0);
+uint64_t up16(uint64_t n) { return (n + 15) / 16 * 16; }
+// the workspace of the gradients: d, then x's tail or the pieces' sums of both products
+struct Space {
+    uint64_t d, input_parts, weight_parts;
+    uint64_t bytes() const { return d + std::max<uint64_t>(input_parts + weight_parts, tail); }
+    uint64_t tail;
+};
+Space space_of(const Plan& n, uint64_t rows, uint32_t inner, uint32_t cols) {
+    Space s{};
+    s.d = up16((rows + 63) / 64 * 64 * 2 * cols * 2);
+    s.input_parts = n.input_splits > 1 ? up16(n.input_splits * rows * inner * 4) : 0;
+    s.weight_parts = n.weight_splits > 1 ? up16(n.weight_splits * 2ull * cols * inner * 4) : 0;
+    s.tail = n.big ? 128ull * inner : 0;
+    return s;
+}
+// Whether tiles of 256 are taken depends on more than the sizes: the larger of both.
+uint64_t space_for(uint64_t rows, uint32_t inner, uint32_t cols, bool dx, bool dw) {
+    return std::max(space_of(plan_of(rows, inner, cols, dx, dw, true), rows, inner, cols).bytes(),
+                    space_of(plan_of(rows, inner, cols, dx, dw, false), rows, inner, cols).bytes());
+}
+
+template <typename T, typename C, bool Direct>
+int start_backward(const Params& p, const Plan& n, hipStream_t s) {
+    auto* k = gated_backward_kernel<T, C, Direct>;
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), C::LDS, done)) return rc;
+    const uint64_t inputs = n.input_tiles * n.input_splits, all = inputs + n.weight_tiles * n.weight_splits;
+    k<<<static_cast<uint32_t>(all), C::THREADS, C::LDS, s>>>(p, static_cast<uint32_t>(std::max<uint64_t>(n.input_tiles, 1)), static_cast<uint32_t>(inputs),
+                                                            static_cast<uint32_t>(std::max<uint64_t>(n.weight_tiles, 1)));
+    auto join = [&](auto* kernel, uint64_t rows) { kernel<<<static_cast<uint32_t>((rows * ((p.inner + 3) / 4) + 255) / 256), 256, 0, s>>>(p); };
+    if (n.input_splits > 1) join(gated_join_kernel<T, INPUT>, p.rows);
+    if (n.weight_splits > 1) join(gated_join_kernel<T, WEIGHTS>, 2ull * p.cols);
+    return BS_OK;
 }
 template <typename T>
-int launch_backward(const Params& p, hipStream_t s) {
-    const bool big = rows16(p.x, p.xs) && rows16(p.wg, p.wgs) && rows16(p.wu, p.wus) && p.wgs == p.wus && p.xs < (1 << 22) && p.wgs < (1 << 22) && p.cols < (1 << 21) &&
-                     p.rows >= 256 && p.cols >= 128 && p.cols % 64 == 0 && p.inner >= 256 && p.inner % 8 == 0 && fill(big_backward(p)) >= 0.55f;
-    const uint32_t rows_up = (p.rows + 63) / 64 * 64, tail_rows = big && p.rows % 64 ? 64 : 0;
-    const uint64_t chunks = static_cast<uint64_t>(rows_up) * ((p.cols + 7) / 8) + static_cast<uint64_t>(tail_rows) * ((p.inner + 7) / 8);
-    gated_slopes_kernel<T><<<static_cast<uint32_t>(std::min<uint64_t>((chunks + 255) / 256, 1u << 22)), 256, 0, s>>>(p, rows_up, tail_rows);
-    if (big) return start_big<T>(p, true, big_backward(p), s);
-    if (p.dx)
-        if (const int rc = launch_gradient<T, INPUT>(p, s)) return rc;
-    if (p.dwg)
-        if (const int rc = launch_gradient<T, WEIGHTS>(p, s)) return rc;
-    return BS_OK;
+int launch_backward(Params p, char* workspace, hipStream_t s) {
+    const bool aligned = rows16(p.x, p.xs) && rows16(p.wg, p.wgs) && rows16(p.wu, p.wus) && p.wgs == p.wus;
+    const bool near = p.xs < (1 << 22) && p.wgs < (1 << 22) && p.cols < (1 << 21);
+    const Plan n = plan_of(p.rows, p.inner, p.cols, p.dx, p.dwg, aligned && near);
+    const Space space = space_of(n, p.rows, p.inner, p.cols);
+    p.d = workspace;
+    p.tail = workspace + space.d;
+    p.input_parts = reinterpret_cast<float*>(workspace + space.d);
+    p.weight_parts = reinterpret_cast<float*>(workspace + space.d + space.input_parts);
+    p.input_splits = n.input_splits;
+    p.weight_splits = n.weight_splits;
+    const uint32_t rows_up = (p.rows + 63) / 64 * 64, tail_rows = n.big && p.rows % 64 ? 64 : 0;
+    if (p.rows) {
+        const uint64_t chunks = static_cast<uint64_t>(rows_up) * ((p.cols + 7) / 8) + static_cast<uint64_t>(tail_rows) * ((p.inner + 7) / 8);
+        gated_slopes_kernel<T><<<static_cast<uint32_t>(std::min<uint64_t>((chunks + 255) / 256, 1u << 22)), 256, 0, s>>>(p, rows_up, tail_rows);
+    }
+    if (n.big) return start_big<T>(p, true, n.input_tiles + n.weight_tiles, s);
+    // a step of dx's inner dimension lies in one weight
+    const bool direct = aligned && p.cols % 64 == 0 && p.inner % 8 == 0;
+    if (n.mid) return direct ? start_backward<T, Mid, true>(p, n, s) : start_backward<T, Mid, false>(p, n, s);
+    return direct ? start_backward<T, Small, true>(p, n, s) : start_backward<T, Small, false>(p, n, s);
 }
 
 int check(const std::string& what, uint64_t rows, uint32_t inner, uint32_t cols) {
     if (rows > 0x7FFFFFFFull) return refuse(what + ": rows must be < 2^31");
     if (inner == 0 || inner > (1u << 24) || cols == 0 || cols > (1u << 23)) return refuse(what + ": inner must be in 1..2^24, cols in 1..2^23");
     // A grid of 2^32 threads is cut short without an error.  Tiles of 64 x 64 results by 256 threads are the most.
-    if (tiles_of(rows, std::max(inner, cols), 64, 64) * 256 > 0xFFFFFFFFull || tiles_of(2 * static_cast<uint64_t>(cols), inner, 64, 64) * 256 > 0xFFFFFFFFull)
+    if ((tiles_of(rows, std::max(inner, cols), 64, 64) + tiles_of(2ull * cols, inner, 64, 64)) * 256 > 0xFFFFFFFFull)
         return refuse(what + ": the sizes are too large for one launch");
     return BS_OK;
 }
@@ -867,14 +941,6 @@ int check_rows(const std::string& what, const char* name, const void* p, int64_t
     if (stride < row) return refuse(what + ": rows of " + name + " overlap (a stride is shorter than its row)");
     if (stride >= (1 << 24)) return refuse(what + ": strides must be < 2^24");
     return BS_OK;
-}
-
-// the workspace of the gradients: d, then x's tail or the pieces' sums of the one product and, in the same place, of the other
-uint64_t up16(uint64_t n) { return (n + 15) / 16 * 16; }
-uint64_t d_bytes(uint64_t rows, uint32_t cols) { return up16((rows + 63) / 64 * 64 * 2 * cols * 2); }
-uint64_t parts_bytes(uint64_t rows, uint32_t inner, uint32_t cols) {
-    const uint64_t a = splits_of(rows, 2ull * cols, inner), b = splits_of(2ull * cols, rows, inner);
-    return std::max<uint64_t>(128ull * inner, std::max(a > 1 ? a * rows * inner * 4 : 0, b > 1 ? b * 2 * cols * inner * 4 : 0));
 }
 
 }  // namespace
@@ -894,7 +960,7 @@ extern "C" int bs_gated(const void* x, int64_t x_stride, const void* w_gate, int
     Params p{};
     p.x = x, p.wg = w_gate, p.wu = w_up, p.h = out, p.gate = gate, p.up = up;
     p.xs = x_stride, p.wgs = w_gate_stride, p.wus = w_up_stride, p.hs = out_stride;
-    p.rows = static_cast<uint32_t>(rows), p.inner = inner, p.cols = cols, p.act = activation, p.splits = 1;
+    p.rows = static_cast<uint32_t>(rows), p.inner = inner, p.cols = cols, p.act = activation;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int rc = type == BS_F16 ? launch_forward<f16>(p, s) : launch_forward<bf16>(p, s);
     return rc ? rc : launched("bs_gated");
@@ -905,7 +971,7 @@ extern "C" int bs_gated(const void* x, int64_t x_stride, const void* w_gate, int
 extern "C" int bs_gated_backward_workspace(uint64_t rows, uint32_t inner, uint32_t cols, uint64_t* bytes) try {
     if (!bytes) return refuse("bs_gated_backward_workspace: bytes is null");
     if (const int rc = check("bs_gated_backward_workspace", rows, inner, cols)) return rc;
-    *bytes = rows ? d_bytes(rows, cols) + parts_bytes(rows, inner, cols) : 0;
+    *bytes = rows ? std::max(space_for(rows, inner, cols, true, true), space_for(rows, inner, cols, true, false)) : 0;
     return BS_OK;
 } catch (...) {
     return bs_internal_exception();
@@ -925,7 +991,7 @@ extern "C" int bs_gated_backward(const void* dh, int64_t dh_stride, const void* 
     Params p{};
     p.x = x, p.wg = w_gate, p.wu = w_up, p.dh = dh, p.g = gate, p.u = up, p.dx = dx, p.dwg = dw_gate, p.dwu = dw_up;
     p.xs = x_stride, p.wgs = w_gate_stride, p.wus = w_up_stride, p.dhs = dh_stride, p.gs = gate_stride, p.us = up_stride;
-    p.rows = static_cast<uint32_t>(rows), p.inner = inner, p.cols = cols, p.act = activation, p.splits = 1;
+    p.rows = static_cast<uint32_t>(rows), p.inner = inner, p.cols = cols, p.act = activation;
     if (rows) {
         if (const int rc = check_rows(what, "dh", dh, dh_stride, cols)) return rc;
         if (const int rc = check_rows(what, "x", x, x_stride, inner)) return rc;
@@ -933,18 +999,14 @@ extern "C" int bs_gated_backward(const void* dh, int64_t dh_stride, const void* 
         if (const int rc = check_rows(what, "w_up", w_up, w_up_stride, inner)) return rc;
         if (const int rc = check_rows(what, "gate", gate, gate_stride, cols)) return rc;
         if (const int rc = check_rows(what, "up", up, up_stride, cols)) return rc;
-        const uint64_t need = d_bytes(rows, cols) + parts_bytes(rows, inner, cols);
+        const uint64_t need = space_for(rows, inner, cols, dx, dw_gate);
         if (!workspace || workspace_bytes < need) return refuse(what + ": the workspace must hold " + std::to_string(need) + " bytes");
         if (!aligned16(workspace)) return refuse(what + ": the workspace must be 16-byte aligned");
-        p.d = static_cast<char*>(workspace);
-        p.tail = p.d + d_bytes(rows, cols);
-        p.parts = reinterpret_cast<float*>(p.tail);
-        const int rc = type == BS_F16 ? launch_backward<f16>(p, s) : launch_backward<bf16>(p, s);
-        return rc ? rc : launched("bs_gated_backward");
+    } else if (!dw_gate) {
+        return BS_OK;
     }
-    if (!dw_gate) return BS_OK;
-    // no rows: the weights' gradients are 0, the sums of no pieces' steps
-    const int rc = type == BS_F16 ? start<f16, WEIGHTS, Small, false>(p, s) : start<bf16, WEIGHTS, Small, false>(p, s);
+    // without rows the weights' gradients are 0, sums of no steps
+    const int rc = type == BS_F16 ? launch_backward<f16>(p, static_cast<char*>(workspace), s) : launch_backward<bf16>(p, static_cast<char*>(workspace), s);
     return rc ? rc : launched("bs_gated_backward");
 } catch (...) {
     return bs_internal_exception();

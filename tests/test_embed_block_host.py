@@ -138,7 +138,7 @@ def test_attention_shared_prefix_refuses_arguments(change, text):
 
 
 def test_attention_shared_prefix_asks_for_its_workspace():
-    hip, a, f, n = _lib.hip(), attention_args(), prefix_args(), C.c_uint64(0)
+    hip, a, f, n = _lib.hip(), attention_args(), prefix_args(tokens=100000), C.c_uint64(0)
     assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), C.byref(n)) == 0 and n.value > 0
     refused(hip.bs_attention_shared_prefix(C.byref(a), C.byref(f), None, 0, None), "the workspace must hold")
     refused(hip.bs_attention_shared_prefix(C.byref(a), C.byref(f), PTR, n.value - 1, None), "the workspace must hold")
@@ -148,6 +148,7 @@ def test_attention_shared_prefix_asks_for_its_workspace():
     refused(hip.bs_attention_shared_prefix_workspace(C.byref(a), None, C.byref(n)), "prefix is null")
     refused(hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), None), "bytes is null")
     assert hip.bs_attention_shared_prefix(C.byref(attention_args(q_tokens=0)), C.byref(f), None, 0, None) == 0
+    assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(prefix_args()), C.byref(n)) == 0 and n.value == 0  # one pass
     b = C.c_uint64(1)  # of no prefix: attention's
     assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(prefix_args(tokens=0)), C.byref(n)) == 0
     assert hip.bs_attention_workspace(C.byref(a), C.byref(b)) == 0 and b.value == n.value

@@ -59,6 +59,12 @@ __device__ inline Vec<T, N> load_any(const T* p) {
     __builtin_memcpy(&v, p, sizeof(v));
     return v;
 }
+// the same for elements that the kernel reads once: they do not displace others from the caches
+template <typename T, int N>
+__device__ inline Vec<T, N> load_once(const T* p) {
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
 template <typename T, int N>
 __device__ inline void store_any(T* p, Vec<T, N> v) {
     __builtin_memcpy(p, &v, sizeof(v));

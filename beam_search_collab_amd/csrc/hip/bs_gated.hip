@@ -436,62 +436,70 @@ __global__ __launch_bounds__(256) void gated_join_kernel(Params p) {
     write<T, FORM, 4>(p, row, col, z);
 }
 
-// Few rows: both weights are read once, from memory to registers, and bound the time.  A workgroup has 16 rows of each, its
-// eight waves a contiguous piece each of the inner dimension; x (MT x 16 rows) comes from the L2.
-template <typename T, int MT>
+// Few rows: both weights are read once, from memory to registers, and bound the time.  A workgroup has P x 16 rows of each, its
+// eight waves a contiguous piece each of the inner dimension; x (MT x 16 rows) comes from the L2, as often as there are
+// workgroups.
+template <typename T, int MT, int P>
 __global__ __launch_bounds__(512) void gated_few_kernel(Params p) {
-    __shared__ f32x4 join[8][2 * MT][64];
+    constexpr int NT = 2 * P;  // tiles of 16 rows: of wg, wu, wg, ..
+    __shared__ f32x4 join[8][NT * MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-    const uint32_t n0 = blockIdx.x * 16;
+    const uint32_t n0 = blockIdx.x * (P * 16);
     // rows past the end repeat the last one: their products are not stored
-    const uint32_t n = min(n0 + l, p.cols - 1);
-    const T *wp[2] = {static_cast<const T*>(p.wg) + static_cast<int64_t>(n) * p.wgs + g * 8, static_cast<const T*>(p.wu) + static_cast<int64_t>(n) * p.wus + g * 8}, *xp[MT];
+    const T *wp[NT], *xp[MT];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const uint32_t n = min(n0 + i * 16 + l, p.cols - 1);
+        wp[2 * i] = static_cast<const T*>(p.wg) + static_cast<int64_t>(n) * p.wgs + g * 8;
+        wp[2 * i + 1] = static_cast<const T*>(p.wu) + static_cast<int64_t>(n) * p.wus + g * 8;
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) xp[i] = static_cast<const T*>(p.x) + static_cast<int64_t>(min(static_cast<uint32_t>(i * 16 + l), p.rows - 1)) * p.xs + g * 8;
-    f32x4 acc[2][MT] = {};
+    f32x4 acc[NT][MT] = {};
     const uint32_t steps = (p.inner + 31) / 32, piece = (steps + 7) / 8, begin = wave * piece;
     const uint32_t end = min(begin + piece, steps), whole = min(end, p.inner / 32);
     constexpr int U = 8;  // steps in flight
     uint32_t t = begin;
     for (; t + U <= whole; t += U) {
-        Vec<T, 8> a[U][2], b[U][MT];
+        Vec<T, 8> a[U][NT], b[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) a[u][i] = load_any<T, 8>(wp[i] + (t + u) * 32);
+            for (int i = 0; i < NT; ++i) a[u][i] = load_any<T, 8>(wp[i] + (t + u) * 32);
 #pragma unroll
             for (int i = 0; i < MT; ++i) b[u][i] = load_any<T, 8>(xp[i] + (t + u) * 32);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int j = 0; j < MT; ++j) acc[i][j] = Mma16<T>::go(a[u][i], b[u][j], acc[i][j]);
     }
     for (; t < end; ++t) {
         const int left = static_cast<int>(p.inner - t * 32) - g * 8;
-        Vec<T, 8> a[2], b[MT];
+        Vec<T, 8> a[NT], b[MT];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) a[i] = left > 0 ? load_some<T, 8>(wp[i] + t * 32, left) : Vec<T, 8>{};
+        for (int i = 0; i < NT; ++i) a[i] = left > 0 ? load_some<T, 8>(wp[i] + t * 32, left) : Vec<T, 8>{};
 #pragma unroll
         for (int i = 0; i < MT; ++i) b[i] = left > 0 ? load_some<T, 8>(xp[i] + t * 32, left) : Vec<T, 8>{};
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int j = 0; j < MT; ++j) acc[i][j] = Mma16<T>::go(a[i], b[j], acc[i][j]);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < MT; ++j) join[wave][i * MT + j][lane] = acc[i][j];
     __syncthreads();
-    if (wave >= MT) return;
-    // wave j: rows 16 j + l, columns 4 g to + 3; the waves' sums in order
-    f32x4 s = join[0][wave][lane], r = join[0][MT + wave][lane];
+    if (wave >= P * MT) return;
+    // wave i MT + j: rows 16 j + l, columns 16 i + 4 g to + 3; the waves' sums in order
+    const int gate = wave / MT * 2 * MT + wave % MT, up = gate + MT;
+    f32x4 s = join[0][gate][lane], r = join[0][up][lane];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += join[k][wave][lane], r += join[k][MT + wave][lane];
-    const uint32_t row = wave * 16 + l, col = n0 + g * 4;
+    for (int k = 1; k < 8; ++k) s += join[k][gate][lane], r += join[k][up][lane];
+    const uint32_t row = wave % MT * 16 + l, col = n0 + wave / MT * 16 + g * 4;
     float z[4] = {s[0], s[1], s[2], s[3]};
     const float u[4] = {r[0], r[1], r[2], r[3]};
     if (row < p.rows && col < p.cols) write_gated<T, 4>(p, row, col, z, u);
@@ -521,7 +529,7 @@ __device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint3
     if (first >= count) return;
     T* buf = reinterpret_cast<T*>(lds);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 31, h = lane >> 5;
-    float* turn = reinterpret_cast<float*>(lds + 2 * STEP * 2) + wave * 1024;
+    char* turn = lds + 2 * STEP * 2 + wave * 4096;
     const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
     auto swizzle = [](int r, int c) { return c ^ ((r >> 1) & 7); };
     const uint32_t rows = rows_of<FORM>(p), cols = cols_of<FORM>(p);
@@ -676,75 +684,78 @@ __device__ inline void big_tiles(const Params& p, char* lds, uint32_t run, uint3
             });
             slot ^= 1;
         }
-        // results: 16 rows at a time through the wave's 4 KB, then 8 adjacent columns a lane (GATED: of both products)
+        // Results, rounded, 32 x 32 at a time through the wave's 4 KB, of which each takes half: a lane that has 4 adjacent
+        // columns of one row eight columns apart then has 8 of two rows.  A row's chunks of 16 bytes are spread over the banks.
         const uint32_t ms = min(m0, rows - 256), ns = min(n0, cols - OUT);
-        auto put = [&](auto J, int half) {
-            constexpr int j = decltype(J)::value;
-            if ((l >> 4) == half) {
+        const int rr = lane >> 2, cc = lane & 3;
+        auto put = [&](int half, const f32x16& z) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<f32x4*>(turn + (l & 15) * 64 + ((i * 8 + q * 2 + h) ^ (l & 15)) * 4) =
-                            f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
-            }
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<Vec<T, 4>*>(turn + half * 2048 + l * 64 + ((q ^ ((l >> 2) & 3)) << 4) + h * 8) =
+                    Vec<T, 4>{static_cast<T>(z[q * 4]), static_cast<T>(z[q * 4 + 1]), static_cast<T>(z[q * 4 + 2]), static_cast<T>(z[q * 4 + 3])};
         };
-        auto take = [&](int rr, int chunk, float (&z)[8]) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(turn + rr * 64 + ((chunk + e / 4) ^ rr) * 4);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) z[e + x] = v[x];
-            }
+        struct Two {
+            Vec<T, 8> of[2];
         };
-        auto give = [&](T* row, uint32_t col, const float (&z)[8]) {  // those from n0 on
-            Vec<T, 8> o;
+        auto take = [&](int half) {
+            Two v;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(z[e]);
-            if (col >= n0) {
-                store_any<T, 8>(row + col, o);
-            } else {
+            for (int k = 0; k < 2; ++k) v.of[k] = *reinterpret_cast<const Vec<T, 8>*>(turn + half * 2048 + (k * 16 + rr) * 64 + ((cc ^ ((rr >> 2) & 3)) << 4));
+            return v;
+        };
+        auto give = [&](auto row_at, uint32_t row, uint32_t col, const Two& v) {  // rows row and row + 16; what lies from m0 and n0 on
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (col + e >= n0) row[col + e] = o[e];
+            for (int k = 0; k < 2; ++k) {
+                if (row + k * 16 < m0) continue;
+                T* to = row_at(row + k * 16);
+                if (col >= n0) {
+                    store_any<T, 8>(to + col, v.of[k]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (col + e >= n0) to[col + e] = v.of[k][e];
+                }
             }
         };
 #pragma unroll 1
-        for (int g = 0; g < 8; ++g) {  // not unrolled: the epilogue's code stays in the instruction cache
-            const int half = g & 1;
-            switch (g >> 1) {
-                case 0: put(std::integral_constant<int, 0>(), half); break;
-                case 1: put(std::integral_constant<int, 1>(), half); break;
-                case 2: put(std::integral_constant<int, 2>(), half); break;
-                default: put(std::integral_constant<int, 3>(), half); break;
+        for (int j = 0; j < 4; ++j) {  // not unrolled: the epilogue's code stays in the instruction cache
+            f32x16 z, u;
+            switch (j) {
+                case 0: z = acc[0][0], u = acc[1][0]; break;
+                case 1: z = acc[0][1], u = acc[1][1]; break;
+                case 2: z = acc[0][2], u = acc[1][2]; break;
+                default: z = acc[0][3], u = acc[1][3]; break;
             }
-            __builtin_amdgcn_wave_barrier();
-            float z[8];
+            const uint32_t row = ms + (XT ? (j >> 1) * 128 + (wave >> 2) * 64 + (j & 1) * 32 : wm + j * 32) + rr;
             if constexpr (FORM == GATED) {
-                const int rr = lane >> 2, cc = (lane & 3) * 2;
-                const uint32_t row = ms + wm + g * 16 + rr, col = ns + wn / 2 + cc * 4;
-                float u[8];
-                take(rr, cc, z);
-                take(rr, 8 + cc, u);
-                if (row >= m0) {
-                    if (p.gate) {
-                        give(static_cast<T*>(p.gate) + static_cast<size_t>(row) * p.cols, col, z);
-                        give(static_cast<T*>(p.up) + static_cast<size_t>(row) * p.cols, col, u);
-                    }
-                    activate(z, p.act);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] *= u[e];
-                    give(static_cast<T*>(p.h) + static_cast<int64_t>(row) * p.hs, col, z);
+                const uint32_t col = ns + wn / 2 + cc * 8;
+                if (p.gate) {
+                    put(0, z);
+                    put(1, u);
+                    __builtin_amdgcn_wave_barrier();
+                    const Two a = take(0), b = take(1);
+                    give([&](uint32_t r) { return static_cast<T*>(p.gate) + static_cast<size_t>(r) * p.cols; }, row, col, a);
+                    give([&](uint32_t r) { return static_cast<T*>(p.up) + static_cast<size_t>(r) * p.cols; }, row, col, b);
+                    __builtin_amdgcn_wave_barrier();
                 }
+                float g[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) g[e] = z[e];
+                activate(g, p.act);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) z[e] = g[e] * u[e];
+                put(0, z);
+                __builtin_amdgcn_wave_barrier();
+                give([&](uint32_t r) { return static_cast<T*>(p.h) + static_cast<int64_t>(r) * p.hs; }, row, col, take(0));
             } else {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int rr = q * 8 + (lane >> 3), cc = (lane & 7) * 2;
-                    const uint32_t row = ms + (XT ? (g >> 2) * 128 + (wave >> 2) * 64 + (g & 3) * 16 : wm + g * 16) + rr;
-                    const uint32_t col = ns + (cc >> 3) * 128 + (wave & 3) * 32 + (cc & 7) * 4;
-                    take(rr, cc, z);
-                    if (row >= m0) give(row_of<T, FORM>(p, row), col, z);
-                }
+                const uint32_t col = ns + (wave & 3) * 32 + cc * 8;
+                put(0, z);
+                put(1, u);
+                __builtin_amdgcn_wave_barrier();
+                const Two a = take(0), b = take(1);
+                auto at = [&](uint32_t r) { return row_of<T, FORM>(p, r); };
+                give(at, row, col, a);
+                give(at, row, col + 128, b);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -784,9 +795,13 @@ __global__ __launch_bounds__(512, 2) void gated_big_backward_kernel(Params p) {
     big_tiles<T, WEIGHTS>(p, lds, b.run, first - a.count, b.count, stride);
 }
 
+// Mid and Small: two workgroups per compute unit.  Flat and Narrow: GATED's waves have 64 rows of W; Narrow has a workgroup for
+// every tile of 64 x 32 results, where tiles of Flat (64 x 64) leave compute units idle: 64 x 4096 -> 8192 34 and 56 us, 128 x
+// 4096 -> 4096 21.8 and 36.3, 200 x 2048 -> 4096 16.5 and 20.1, but 300 x 4096 -> 4096 (320 tiles of 64) 47 and 37.
 using Mid = Tile<128, 128, 2, 2, 32, 4, 2>;
 using Small = Tile<64, 64, 2, 2, 64, 4, 2>;
-using Flat = Tile<64, 128, 2, 2, 64, 3, 2>;  // of GATED, whose waves have 64 rows of W
+using Narrow = Tile<64, 64, 2, 1, 64, 4, 2>;
+using Flat = Tile<64, 128, 2, 2, 64, 3, 2>;
 
 constexpr uint32_t FEW = 32;
 
@@ -817,10 +832,14 @@ float fill(uint64_t tiles) { return static_cast<float>(tiles) / static_cast<floa
 template <typename T>
 int launch_forward(Params p, hipStream_t s) {
     if (p.rows <= FEW) {
+        // 32 columns a workgroup, half the reads of x, where that leaves a workgroup for every compute unit: 17 x 4096 -> 8192
+        // takes 30.6 us, 35.7 with 16
         if (p.rows <= 16)
-            gated_few_kernel<T, 1><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
+            gated_few_kernel<T, 1, 1><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
+        else if (p.cols >= 32 * CUS)
+            gated_few_kernel<T, 2, 2><<<(p.cols + 31) / 32, 512, 0, s>>>(p);
         else
-            gated_few_kernel<T, 2><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
+            gated_few_kernel<T, 2, 1><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
         return BS_OK;
     }
     const bool direct = rows16(p.x, p.xs) && rows16(p.wg, p.wgs) && rows16(p.wu, p.wus);
@@ -828,6 +847,7 @@ int launch_forward(Params p, hipStream_t s) {
     if (direct && fill(big) >= 0.55f && p.rows >= 256 && p.cols >= 128 && p.inner % 64 == 0 && p.inner >= 128 && p.xs < (1 << 22) && p.wgs < (1 << 22) && p.wgs == p.wus)
         return start_big<T>(p, false, big, s);
     if (tiles_of(p.rows, p.cols, 128, 64) >= CUS) return direct ? start<T, Mid, true>(p, s) : start<T, Mid, false>(p, s);
+    if (tiles_of(p.rows, p.cols, 64, 64) <= CUS) return direct ? start<T, Narrow, true>(p, s) : start<T, Narrow, false>(p, s);
     return direct ? start<T, Flat, true>(p, s) : start<T, Flat, false>(p, s);
 }
 // How the gradients' two products are cut: tiles of 256 (big), 128 or 64, and with the latter pieces of the inner dimensions.

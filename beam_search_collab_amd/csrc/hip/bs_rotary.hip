@@ -75,13 +75,8 @@ __device__ inline Places places_of(const Params& p, uint32_t u) {
     }
     return x;
 }
-// N elements that nobody reads again: they leave the caches to the results, which attention reads next (32768 tokens of 32 +
-// 8 heads of 128 in bf16: 176 us without, 162 with it)
-template <typename T, int N>
-__device__ inline Vec<T, N> load_once(const T* p) {
-    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
-}
+// Read once: they leave the caches to the results, which attention reads next (32768 tokens of 32 + 8 heads of 128 in bf16: 176
+// us otherwise, 162 so)
 template <typename T, int N, int K>
 __device__ inline void load(const T* head, const Places (&at)[K], bool live, Raw<T, N, K>& x) {
 #pragma unroll

@@ -468,11 +468,9 @@ def head_norm_rotary_backward(dq: torch.Tensor, dk: Optional[torch.Tensor], q: t
         gs += (0, 0)
     size = 0
     if params and eps is not None:
-        dim = q.shape[2]
-        both = q.new_empty((2 if k is not None else 1, dim), dtype=wt)
-        dwq = both[0]
+        dwq = q.new_empty((q.shape[2],), dtype=wt) if q_weight is None else torch.empty_like(q_weight)
         if k is not None:
-            dwk = both[1]
+            dwk = torch.empty_like(dwq)
         size = _rotary_workspace(*sizes[:5], sizes[7])
         ws = q.new_empty((size,), dtype=torch.uint8)
     a = _lib.HeadNormRotaryArgs(qp, kp, dq.data_ptr(), dkp, y.data_ptr(), zp, wq, wk, None if dwq is None else dwq.data_ptr(),

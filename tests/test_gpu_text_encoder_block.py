@@ -658,3 +658,208 @@ def test_attention_shared_prefix_refusals(gpu):
     ]:
         with pytest.raises(ValueError, match=text):
             call()
+
+
+# ---------------------------------------------------------------- on both sides of the rules that choose a kernel
+
+@pytest.mark.parametrize("rows,inner,cols", [
+    (32, 300, 8191), (32, 300, 8192), (16, 300, 8192), (17, 260, 8205), (32, 64, 100),       # few rows, by 16 and by 32 columns
+    (33, 320, 8192), (33, 320, 8200), (64, 256, 8224), (65, 256, 4096),                      # 256 and 257 narrow tiles
+    (256, 96, 8192), (256, 96, 8128), (128, 100, 16384), (128, 100, 16321),                  # 256 and 254 tiles of 128 x 64
+    (2816, 128, 1664), (2816, 128, 1537), (2816, 64, 1664), (2816, 192, 1663), (2560, 128, 1792), (300, 256, 9088), (256, 128, 17920)])  # 143 and 140 of 256 x 128
+def test_gated_on_both_sides_of_the_rules(gpu, rows, inner, cols):
+    x, wg, wu = gated_case(400, rows, inner, cols, BF16)
+    h, gate, up = embed.gated(x, wg, wu, activation="gelu_tanh", save=True)
+    check_gated(x, wg, wu, "gelu_tanh", h, gate, up)
+    # weights whose strides differ, so that another kernel takes them
+    wide = torch.zeros(cols, inner + 8, dtype=BF16, device="cuda")
+    wide[:, :inner] = wu
+    other = embed.gated(x, wg, wide[:, :inner], activation="gelu_tanh")
+    check_gated(x, wg, wu, "gelu_tanh", other)
+
+
+@pytest.mark.parametrize("rows,inner,cols", [
+    (256, 256, 128), (256, 4096, 2304), (255, 4096, 2304), (3000, 520, 2048), (3008, 520, 2048), (2999, 1024, 1024),  # large tiles, with a tail and without
+    (520, 264, 8192), (9000, 256, 192), (16390, 256, 256), (700, 2304, 1088),
+    (1000, 512, 2048), (1000, 512, 1984), (600, 600, 1536), (2500, 64, 128), (20000, 64, 64), (70, 64, 8192), (64, 72, 5000)])  # tiles of 128 and 64, pieces of either product
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gated_backward_on_both_sides_of_the_rules(gpu, rows, inner, cols, dtype):
+    x, wg, wu = gated_case(410, rows, inner, cols, dtype)
+    gate, up, dh = rand(414, rows, cols, dtype=dtype, std=1.5), rand(415, rows, cols, dtype=dtype), rand(416, rows, cols, dtype=dtype, std=0.3)
+    got = embed.gated_backward(dh, x, wg, wu, gate, up)
+    check_gated_backward(dh, x, wg, wu, gate, up, "silu", *got)
+    assert all(torch.equal(a, b) for a, b in zip(got, embed.gated_backward(dh, x, wg, wu, gate, up)))
+    wide = torch.zeros(cols, inner + 8, dtype=dtype, device="cuda")
+    wide[:, :inner] = wu
+    dx, _, _ = embed.gated_backward(dh, x, wg, wide[:, :inner], gate, up, params=False)
+    check_gated_backward(dh, x, wg, wu, gate, up, "silu", dx, None, None)
+
+
+def test_gated_backward_of_a_tail_beside_a_row_that_is_not_finite(gpu):
+    """large tiles: the rows behind the last one are zeros, not repetitions of it"""
+    rows, inner, cols = 3001, 512, 2048
+    x, wg, wu = gated_case(420, rows, inner, cols, BF16)
+    gate, up, dh = (rand(423 + i, rows, cols, dtype=BF16) for i in range(3))
+    x[-1, 5] = math.inf
+    _, dwg, dwu = embed.gated_backward(dh, x, wg, wu, gate, up, activation="none")
+    for dw, d in ((dwg, dh[-1] * up[-1]), (dwu, dh[-1] * gate[-1])):
+        want = torch.where(d == 0, math.nan, torch.sign(d.float()) * math.inf)
+        assert torch.equal(torch.nan_to_num(dw[:, 5].float(), nan=7.0), torch.nan_to_num(want, nan=7.0))
+        assert torch.isfinite(dw[:, :5]).all() and torch.isfinite(dw[:, 6:]).all()
+
+
+@pytest.mark.parametrize("nq,nk,prefix,heads,kv,dim", [
+    ([1] * 8, [40] * 8, 1015, 8, 1, 64), ([1] * 8, [40] * 8, 1017, 8, 1, 64), ([1] * 8, [40] * 8, 700, 8, 8, 128),  # one pass, or the prefix apart
+    ([20] * 8, [20] * 8, 900, 32, 8, 128), ([20] * 8, [20] * 8, 2000, 32, 8, 128), ([4] * 3, [4] * 3, 6000, 4, 4, 32),
+    ([1], [5000], 100, 4, 1, 64), ([40], [3000], 3000, 4, 4, 96), ([1], [0], 20000, 8, 1, 64), ([1, 1], [3, 900], 9000, 9, 1, 64)])  # own keys in pieces; single tokens
+def test_attention_shared_prefix_on_both_sides_of_the_rules(gpu, nq, nk, prefix, heads, kv, dim):
+    for causal in (True, False):
+        behind_prefix(430, nq, nk, prefix, heads, kv, dim, BF16, causal)
+
+
+def test_past_32_bit_offsets(gpu):
+    """rows and heads 2^31 bytes apart, keys in the last gigabytes of a long prefix"""
+    buf = torch.empty((3 << 30) + 4096, dtype=BF16, device="cuda")
+    x = buf.as_strided((4, 2, 64), (1 << 30, 128, 1))
+    x.copy_(rand(440, 4, 2, 64))
+    f, w = embed.rotary_frequencies(64), rand(441, 64)
+    want, _ = embed.head_norm_rotary(x.contiguous(), None, None, f, w)
+    got, _ = embed.head_norm_rotary(x, None, None, f, w)
+    assert torch.equal(got, want)
+    heads = buf.as_strided((2, 4, 64), (128, 1 << 30, 1))
+    assert torch.equal(embed.head_norm_rotary(heads, None, torch.zeros(2, dtype=torch.int32, device="cuda"), None, w)[0].transpose(0, 1).contiguous(),
+                       embed.head_norm_rotary(x, None, torch.zeros(4, dtype=torch.int32, device="cuda"), None, w)[0])
+    dy = rand(442, 4, 2, 64, dtype=BF16)
+    a, b = embed.head_norm_rotary_backward(dy, None, x, None, None, f, w), embed.head_norm_rotary_backward(dy, None, x.contiguous(), None, None, f, w)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+    embed.head_norm_rotary(x, None, None, f, w, out=(x, None))
+    assert torch.equal(x, want)
+    stride = (1 << 22) - 8
+    pk, pv = buf.as_strided((700, 1, 64), (stride, 64, 1)), buf.as_strided((700, 1, 64), (stride, 64, 1), 128)
+    pk.copy_(rand(443, 700, 1, 64))
+    pv.copy_(rand(444, 700, 1, 64))
+    for n in (1, 5, 300):
+        q, k, v, _, _ = prefix_case(445, [n], [n], 1, 2, 1, 64, BF16)
+        out, lse = embed.attention_shared_prefix(q, k, v, pk, pv, lse=True)
+        check_prefix(q, k, v, pk.contiguous(), pv.contiguous(), [n], [n], True, 0.125, out, lse)
+        back = embed.attention_shared_prefix(q, pk, pv, k, v, offsets([n]), offsets([700]))
+        check_prefix(q, pk.contiguous(), pv.contiguous(), k, v, [n], [700], True, 0.125, back, None)
+    x = buf.as_strided((4, 512), ((1 << 24) - 8, 1))
+    x.copy_(rand(450, 4, 512))
+    _, wg, wu = gated_case(451, 4, 512, 96, BF16)
+    assert torch.equal(embed.gated(x, wg, wu), embed.gated(x.contiguous(), wg, wu))
+
+
+# ---------------------------------------------------------------- together
+
+class Block:
+    """a block of an encoder as these operators make it"""
+
+    def __init__(self, width=256, heads=8, kv=2, dim=32, hidden=512, dtype=BF16):
+        def weight(seed, rows, cols):
+            return rand(seed, rows, cols, dtype=dtype, std=cols ** -0.5)
+        self.heads, self.kv, self.dim = heads, kv, dim
+        self.qkv, self.mix = weight(500, (heads + 2 * kv) * dim, width), weight(501, width, heads * dim)
+        self.both, self.down = weight(502, 2 * hidden, width), weight(503, width, hidden)
+        self.n1, self.n2 = 1 + 0.1 * rand(504, width), 1 + 0.1 * rand(505, width)
+        self.nq, self.nk = 1 + 0.1 * rand(506, dim), 1 + 0.1 * rand(507, dim)
+        self.f = embed.rotary_frequencies(dim)
+
+    def heads_of(self, x, positions):
+        h, kv = self.heads, self.kv
+        t = embed.linear(embed.layer_norm(x, self.n1), self.qkv).unflatten(1, (h + 2 * kv, self.dim))
+        q, k = embed.head_norm_rotary(t[:, :h], t[:, h:h + kv], positions, self.f, self.nq, self.nk)
+        return q, k, t[:, h + kv:]
+
+    def rest(self, x, o):
+        x = embed.linear(o.flatten(1), self.mix, residual=x)
+        hidden = self.down.shape[1]
+        h, gate, up = embed.gated(embed.layer_norm(x, self.n2), self.both[:hidden], self.both[hidden:], save=True)
+        return embed.linear(h, self.down, residual=x), (x, h, gate, up)
+
+
+def test_a_block_behind_a_prefix_is_the_block_over_all(gpu):
+    """sequences encoded behind the cached keys of their prefix, and whole: the same vectors, up to a rounding of every
+    operator's on both ways (10 of them, none of which a block of norms and unit weights magnifies in the mean)"""
+    b, prefix, lengths = Block(), 70, [5, 40, 1, 23]
+    front, tails = rand(510, prefix, 256, dtype=BF16), [rand(511 + i, n, 256, dtype=BF16) for i, n in enumerate(lengths)]
+    pos = torch.arange(prefix, dtype=torch.int32, device="cuda")
+    _, pk, pv = b.heads_of(front, pos)
+    x = torch.cat(tails)
+    q, k, v = b.heads_of(x, torch.cat([prefix + torch.arange(n, dtype=torch.int32, device="cuda") for n in lengths]))
+    y, _ = b.rest(x, embed.attention_shared_prefix(q, k, v, pk, pv, offsets(lengths)))
+    whole = torch.cat([torch.cat([front, t]) for t in tails])
+    q, k, v = b.heads_of(whole, torch.cat([torch.arange(prefix + n, dtype=torch.int32, device="cuda") for n in lengths]))
+    z, _ = b.rest(whole, embed.attention(q, k, v, offsets([prefix + n for n in lengths])))
+    z = torch.cat([t[prefix:] for t in z.split([prefix + n for n in lengths])])
+    assert (y.double() - z.double()).square().mean().sqrt() <= 10 * U[BF16] * z.double().square().mean().sqrt()
+
+
+def test_results_together_on_another_stream_and_in_a_graph(gpu):
+    b, lengths = Block(), [200, 1, 60, 39]
+    x, off = rand(520, 300, 256, dtype=BF16), offsets(lengths)
+    pos = torch.cat([90 + torch.arange(n, dtype=torch.int32, device="cuda") for n in lengths])
+    pk, pv = rand(521, 900, 2, 32, dtype=BF16), rand(522, 900, 2, 32, dtype=BF16)
+    one = offsets([1, 1, 1, 1])
+
+    def step():
+        q, k, v = b.heads_of(x, pos)
+        o = embed.attention_shared_prefix(q, k, v, pk, pv, off, longest_q=200, longest_k=200)
+        last = embed.attention_shared_prefix(q[:4], k, v, pk, pv, one, off, longest_q=1, longest_k=200)
+        y, (mid, h, gate, up) = b.rest(x, o)
+        hidden = b.down.shape[1]
+        grads = embed.gated_backward(h, mid, b.both[:hidden], b.both[hidden:], gate, up)
+        turned_back = embed.head_norm_rotary_backward(o, k, q, k, pos, b.f, b.nq, b.nk)
+        return (y, last, *grads, *turned_back)
+    want = step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:  # two at once
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(step())
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for g in got for a, c in zip(g, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for t in range(3):
+        x.copy_(rand(530 + t, 300, 256))
+        pk.copy_(rand(540 + t, 900, 2, 32))
+        graph.replay()
+        torch.cuda.synchronize()
+        copies = [a.clone() for a in captured]
+        want = step()
+        assert all(torch.equal(a, c) for a, c in zip(copies, want))
+
+
+def test_two_graphs_with_workspaces_of_their_own(gpu):
+    """captured one after the other, replayed in turn on two streams"""
+    def case(seed):
+        x, wg, wu = gated_case(seed, 300, 256, 512, BF16)
+        gate, up, dh = (rand(seed + 3 + i, 300, 512, dtype=BF16) for i in range(3))
+        q, k, v, pk, pv = prefix_case(seed + 10, [1] * 30, [5] * 30, 3000, 8, 2, 64, BF16)
+        off, one = offsets([5] * 30), offsets([1] * 30)
+
+        def run():
+            return (*embed.gated_backward(dh, x, wg, wu, gate, up), embed.attention_shared_prefix(q, k, v, pk, pv, one, off, longest_q=1, longest_k=5))
+        return run
+    runs = [case(600), case(650)]
+    want = [r() for r in runs]
+    graphs, outs = [], []
+    for r in runs:
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            outs.append(r())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(3):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, w))

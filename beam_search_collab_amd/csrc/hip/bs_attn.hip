@@ -499,7 +499,7 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 // run under a tile's products.  Two workgroups per compute unit (three for heads up to 64): one's matrix
 // instructions run under the other's exponentials.  (Three for heads of 64: passages below 90 to 83 us; four spill: 144.)
 //
-// Two causal documents of 8192 and 7500 tokens, 32 heads of 128, 8 key/value heads, bf16: 973 us (992 TFLOP/s), the
+// Two causal documents of 8192 and 7500 tokens, 32 heads of 128, 8 key/value heads, bf16: 929 us (1038 TFLOP/s), the
 // vector and matrix pipes half busy each (0.50, 0.47): a wave's exponentials and its products do not overlap, only two
 // waves' do.  96 passages of 37..512 tokens, 16 heads of 64: 69 us, the vector pipe busy for 0.43 of the time (170
 // instructions beside 16 matrix instructions a tile, 270 with masks) and waves waiting for 0.40 of theirs, on the four
@@ -507,7 +507,8 @@ __device__ inline void write_rows(const Params& p, const Sequence& sq, const Pla
 // the documents: two groups of waves half a step apart, meeting between their phases (1244 against 1175), moves between
 // the products and exponentials instead of before them (1246 against 1142).
 //
-// Prefix: every row sees the prefix's keys too, in the same pass.
+// Prefix: every row sees the prefix's keys too, in the same pass.  24 chunks of 128..384 tokens behind 8191 keys, as documents:
+// 909 us (947 TFLOP/s), 0.9 of the documents' rate: their 1632 tiles make 3.2 rounds of workgroups.
 template <typename T, int DP, bool Prefix>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void attention_kernel(Params p) {
     constexpr int ROWS = 128, S = ROW<DP>, TILE = BN * S;

@@ -3,7 +3,8 @@
  *
  * The index of bs_hip.h holds float32 vectors and is searched with float32 vectors; these are
  * the operators of the text encoder that makes both, on the GPU and stream that search them:
- * attention over packed sequences, products with their epilogue, layer norm and its gradients.
+ * attention over packed sequences, also behind a shared prefix, products with their epilogue, gated
+ * products, layer norm, norms of heads with rotary positions, and gradients of the latter three.
  * The reference starts from vectors in files and has no counterpart.
  *
  * Conventions

@@ -61,7 +61,7 @@ __device__ inline void act_and_slope(float z, int act, float& a, float& slope) {
         halves_of_one(-2.0f * LOG2E * 0.79788456080286536f * fmaf(0.044715f * q, z, z), s, rest);
         a = z * s;
         const float bend = s * rest;
-        slope = bend == 0.0f ? s : fmaf(z * bend, 1.59576912160573072f * fmaf(3.0f * 0.044715f, q, 1.0f), s);
+        slope = bend == 0.0f ? s : fmaf(z * bend, 2.0f * 0.79788456080286536f * fmaf(3.0f * 0.044715f, q, 1.0f), s);
     } else if (act == BS_ACT_SILU) {  // z s, s = 1 / (1 + exp(-z)): slope s + z s (1 - s)
         float s, rest;
         halves_of_one(-LOG2E * z, s, rest);
@@ -327,7 +327,7 @@ __device__ inline void one_tile(const Params& p, char* lds, uint32_t b, uint32_t
         }
         meet<0>();
         __syncthreads();
-        if (steps > whole) {
+        if (steps > whole && begin <= whole) {
             Vec<T, 8> v[C::MOVES];
             fetch(whole, v);
             put(0, v);
@@ -991,7 +991,8 @@ extern "C" int bs_gated(const void* x, int64_t x_stride, const void* w_gate, int
 extern "C" int bs_gated_backward_workspace(uint64_t rows, uint32_t inner, uint32_t cols, uint64_t* bytes) try {
     if (!bytes) return refuse("bs_gated_backward_workspace: bytes is null");
     if (const int rc = check("bs_gated_backward_workspace", rows, inner, cols)) return rc;
-    *bytes = rows ? std::max(space_for(rows, inner, cols, true, true), space_for(rows, inner, cols, true, false)) : 0;
+    // whichever gradients are asked for
+    *bytes = rows ? std::max({space_for(rows, inner, cols, true, true), space_for(rows, inner, cols, true, false), space_for(rows, inner, cols, false, true)}) : 0;
     return BS_OK;
 } catch (...) {
     return bs_internal_exception();

@@ -125,8 +125,8 @@ int bs_attention_workspace(const bs_attention_args* args, uint64_t* bytes);
  * first `rotary` elements are turned in pairs i = 0 .. rotary / 2 - 1 and the others are n:
  *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin),  angle = position * frequencies[i]
  * where a pair is (i, i + rotary / 2), or (2 i, 2 i + 1) if `interleaved`.  Angles are reduced in
- * float64, so far positions lose nothing; squares are summed in float32.  Elements of a head
- * are contiguous; *_out may be the call's own q and k (or q_grad and k_grad) with their strides. */
+ * float64, so far positions lose nothing; squares are summed in float32, which holds those of
+ * elements up to 2^60.  Elements of a head are contiguous; *_out may be the call's own q and k (or q_grad and k_grad) with their strides. */
 typedef struct {
     const void* q;
     const void* k;
@@ -178,7 +178,8 @@ int bs_gated(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate
              int activation, void* stream);
 
 /* Its gradients from dh, the gradient of out, and the saved gate and up:
- *   dgate = dh up act'(gate),  dup = dh act(gate), both rounded to `type` for their products
+ *   dgate = dh up act'(gate),  dup = dh act(gate), both rounded to `type` for their products (so in
+ *   BS_F16 they are infinite past 65504 and lose bits below 2^-14)
  *   dx = dgate w_gate + dup w_up,  dw_gate = dgate^T x,  dw_up = dup^T x
  * (relu's slope at 0 is 0).  dx (rows x inner) may be NULL, dw_gate and dw_up (cols x inner) too,
  * both or neither; all contiguous.  The sums over the rows have a fixed order.  workspace:

@@ -152,3 +152,14 @@ def test_attention_shared_prefix_asks_for_its_workspace():
     b = C.c_uint64(1)  # of no prefix: attention's
     assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(prefix_args(tokens=0)), C.byref(n)) == 0
     assert hip.bs_attention_workspace(C.byref(a), C.byref(b)) == 0 and b.value == n.value
+
+
+@pytest.mark.parametrize("rows,inner,cols", [(4, 8, 8), (300, 768, 2048), (20000, 64, 64), (70, 64, 8192), (3001, 512, 2048), (9000, 256, 192), (777, 1000, 900)])
+def test_gated_workspace_is_enough_for_either_gradient(rows, inner, cols):
+    """a call that is refused for its workspace says how much it wants"""
+    hip, n = _lib.hip(), C.c_uint64(0)
+    assert hip.bs_gated_backward_workspace(rows, inner, cols, C.byref(n)) == 0
+    for dx, dwg, dwu in ((PTR, PTR, PTR), (PTR, None, None), (None, PTR, PTR)):
+        rc = hip.bs_gated_backward(PTR, cols, PTR, inner, PTR, inner, PTR, inner, PTR, cols, PTR, cols, dx, dwg, dwu, rows, inner, cols, 2, 4, None, 0, None)
+        refused(rc, "the workspace must hold")
+        assert int(hip.bs_last_error().decode().split("hold ")[1].split(" ")[0]) <= n.value

@@ -95,8 +95,8 @@ def _rows(what: str, name: str, t: torch.Tensor) -> Tuple[int, int, int]:
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
-    """a contiguous tensor of x's shape and type (empty_like is the faster call, and keeps x's order)"""
-    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    """a contiguous tensor of x's shape and type"""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)  # 1.2 us, new_empty 1.7
 
 
 def _vector(what: str, name: str, t: torch.Tensor, n: int, *types):
@@ -285,7 +285,7 @@ def _attention_args(what, q, k, v, q_offsets, k_offsets, causal, scale, longest_
         if k_offsets is not q_offsets:
             _offsets(what, "k_offsets", k_offsets, n)
     if out is None:
-        o, ot, oh = q.new_empty((tq, heads, dim)), heads * dim, dim
+        o, ot, oh = _like(q), heads * dim, dim
     else:
         o = out
         if o.shape != q.shape or o.dtype != type_ or (dim > 1 and o.stride(2) != 1):
@@ -413,8 +413,7 @@ def _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, la
 
 def _rotary_out(what, x, name, out):
     if out is None:
-        o = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
-        return o, (o.shape[1] * o.shape[2], o.shape[2])
+        return _like(x), (x.shape[1] * x.shape[2], x.shape[2])
     return out, _heads(what, name, out, x.shape, x.dtype)
 
 
@@ -468,7 +467,7 @@ def head_norm_rotary_backward(dq: torch.Tensor, dk: Optional[torch.Tensor], q: t
         gs += (0, 0)
     size = 0
     if params and eps is not None:
-        dwq = q.new_empty((q.shape[2],), dtype=wt) if q_weight is None else torch.empty_like(q_weight)
+        dwq = q.new_empty((q.shape[2],), dtype=wt) if q_weight is None else _like(q_weight)
         if k is not None:
             dwk = torch.empty_like(dwq)
         size = _rotary_workspace(*sizes[:5], sizes[7])

@@ -77,7 +77,7 @@ __device__ inline void act_and_slope(float z, int act, float& a, float& slope) {
 // for their products, as every operand of a matrix product is: off by half a unit each, at random, which gives a sum of n of
 // them the error that the same sum of rounded inputs has.
 template <typename T>
-__global__ __launch_bounds__(256) void gated_slopes_kernel(Params p, uint32_t rows_up, uint32_t tail_rows) {
+__global__ __launch_bounds__(256) void gated_slopes_kernel(Params p, uint32_t rows_up, uint32_t tail_rows, Divisor by_across) {
     const uint32_t across = (p.cols + 7) / 8, wide = (p.inner + 7) / 8;
     const uint64_t all = static_cast<uint64_t>(rows_up) * across, more = static_cast<uint64_t>(tail_rows) * wide;
     T* d = reinterpret_cast<T*>(p.d);
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void gated_slopes_kernel(Params p, uint32_t ro
             store_some<T, 8>(reinterpret_cast<T*>(p.tail) + static_cast<size_t>(r) * p.inner + c, v, n);
             continue;
         }
-        const uint32_t row = static_cast<uint32_t>(i / across), c = static_cast<uint32_t>(i % across) * 8;
+        const uint32_t row = all >> 31 ? static_cast<uint32_t>(i / across) : by_across.quotient(static_cast<uint32_t>(i)), c = static_cast<uint32_t>(i - static_cast<uint64_t>(row) * across) * 8;
         const int n = static_cast<int>(p.cols - c);
         Vec<T, 8> dg = {}, du = {};
         if (row < p.rows) {
@@ -409,14 +409,15 @@ __global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_ke
     one_tile<T, GATED, C, Direct>(p, lds, blockIdx.x, 0, 1, nullptr);
 }
 // Both products of the gradients in one launch, `inputs` workgroups of dx first.
-template <typename T, typename C, bool Direct>
-__global__ __launch_bounds__(C::THREADS, C::PER_CU * C::WAVES / 4) void gated_backward_kernel(Params p, uint32_t input_tiles, uint32_t inputs, uint32_t weight_tiles) {
+template <typename T, typename CI, typename CW, bool Direct>
+__global__ __launch_bounds__(256, 2) void gated_backward_kernel(Params p, uint32_t input_tiles, uint32_t inputs, uint32_t weight_tiles) {
+    static_assert(CI::THREADS == 256 && CW::THREADS == 256 && CI::PER_CU == 2 && CW::PER_CU == 2, "of one launch");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     if (blockIdx.x < inputs) {
-        one_tile<T, INPUT, C, Direct>(p, lds, blockIdx.x % input_tiles, blockIdx.x / input_tiles, p.input_splits, p.input_parts);
+        one_tile<T, INPUT, CI, Direct>(p, lds, blockIdx.x % input_tiles, blockIdx.x / input_tiles, p.input_splits, p.input_parts);
     } else {
         const uint32_t b = blockIdx.x - inputs;
-        one_tile<T, WEIGHTS, C, Direct>(p, lds, b % weight_tiles, b / weight_tiles, p.weight_splits, p.weight_parts);
+        one_tile<T, WEIGHTS, CW, Direct>(p, lds, b % weight_tiles, b / weight_tiles, p.weight_splits, p.weight_parts);
     }
 }
 
@@ -852,7 +853,7 @@ int launch_forward(Params p, hipStream_t s) {
 }
 // How the gradients' two products are cut: tiles of 256 (big), 128 or 64, and with the latter pieces of the inner dimensions.
 struct Plan {
-    bool big, mid;
+    bool big, input_mid, weight_mid;
     uint32_t input_splits, weight_splits;
     uint64_t input_tiles, weight_tiles;
 };
@@ -868,26 +869,49 @@ Plan plan_of(uint64_t rows, uint32_t inner, uint32_t cols, bool dx, bool dw, boo
     Plan n = cut(256);
     if (big && rows >= 256 && cols >= 128 && cols % 64 == 0 && inner >= 256 && inner % 8 == 0) {
         // A workgroup per compute unit takes its share of the tiles one after the other, dx's first.  Worth it where they are
-        // at work for 0.55 of the time.
-        const uint64_t most = (n.input_tiles + n.weight_tiles + CUS - 1) / CUS, first = std::min((n.input_tiles + CUS - 1) / CUS, most);
-        const uint64_t input_steps = cols / 32, weight_steps = (rows + 63) / 64, time = first * input_steps + (most - first) * weight_steps;
+        // at work for 0.55 of the time, which they are not where one product has few long tiles: 20000 x 256 -> 256 takes 340 us
+        // with them (2 tiles of 313 steps beside 79 of 8), 43 with smaller ones.
+        const uint64_t most = (n.input_tiles + n.weight_tiles + CUS - 1) / CUS, input_steps = cols / 32, weight_steps = (rows + 63) / 64;
+        // the workgroups with the most and with the fewest tiles of dx
+        const uint64_t more = std::min((n.input_tiles + CUS - 1) / CUS, most), less = n.weight_tiles ? n.input_tiles / CUS : more;
+        const uint64_t time = std::max(more * input_steps + (most - more) * weight_steps, less * input_steps + (most - less) * weight_steps);
         const uint64_t work = n.input_tiles * input_steps + n.weight_tiles * weight_steps;
         if (static_cast<double>(work) >= 0.55 * static_cast<double>(time * CUS)) {
             n.big = true;
             return n;
         }
     }
-    // Two workgroups per compute unit, in one launch; pieces of an inner dimension about as long as their share of all
-    // steps, of 1024 elements at least.  Tiles of 128 and 64: gradients of 1000 x 1024 -> 2048 (320 tiles of 128) 36.3 and 40.4
-    // us, of 300 x 768 -> 2048 (210) 24.9 and 23.7.
-    n = cut(128);
-    n.mid = n.input_tiles + n.weight_tiles >= CUS;
-    if (!n.mid) n = cut(64);
+    // Two workgroups per compute unit, in one launch, of tiles of 64 or 128 for either product, and pieces of an inner dimension
+    // about as long as their share of all work, of 1024 elements at least: what takes the least time, by the microseconds of a
+    // workgroup's start and of 64 inner elements, and of the launch that joins pieces and its bytes.  Against tiles of 64 alone
+    // below a tile of 128 for every compute unit: 300 x 768 -> 2048 20.9 and 23.6 us, 1000 x 1024 -> 2048 34.8 and 37.4, 2000 x
+    // 256 -> 1024 21.2 and 24.5, but 256 x 2048 -> 2048 28.9 and 26.8.
+    constexpr double START = 2.5, SMALL = 0.45, MID = 1.4, JOIN = 4.0, BYTES = 4e6;
     const uint64_t input_steps = (2ull * cols + 63) / 64, weight_steps = (rows + 63) / 64;
-    const uint64_t share = std::max<uint64_t>(16, (n.input_tiles * input_steps + n.weight_tiles * weight_steps + 2 * CUS - 1) / (2 * CUS));
-    auto splits = [&](uint64_t steps) { return steps * 2 > share * 3 ? static_cast<uint32_t>((steps + share - 1) / share) : 1u; };
-    if (dx) n.input_splits = splits(input_steps);
-    if (dw) n.weight_splits = splits(weight_steps);
+    double best = 0.0;
+    for (int way = 0; way < 16; ++way) {
+        Plan c{};
+        c.input_mid = way & 1;
+        c.weight_mid = way >> 1 & 1;
+        c.input_tiles = dx ? tiles_of(rows, inner, c.input_mid ? 128 : 64, c.input_mid ? 128 : 64) : 0;
+        c.weight_tiles = dw ? tiles_of(2ull * cols, inner, c.weight_mid ? 128 : 64, c.weight_mid ? 128 : 64) : 0;
+        const double a = c.input_mid ? MID : SMALL, b = c.weight_mid ? MID : SMALL;
+        const double work = static_cast<double>(c.input_tiles * input_steps) * a + static_cast<double>(c.weight_tiles * weight_steps) * b;
+        const auto splits = [&](bool cut, uint64_t steps, double step) {
+            const uint64_t share = std::max<uint64_t>(16, static_cast<uint64_t>(work / (2 * CUS) / step));
+            return cut && steps > share ? static_cast<uint32_t>((steps + share - 1) / share) : 1u;
+        };
+        c.input_splits = splits(dx && (way & 4), input_steps, a);
+        c.weight_splits = splits(dw && (way & 8), weight_steps, b);
+        const double longest = std::max(dx ? a * static_cast<double>(input_steps) / c.input_splits : 0.0, dw ? b * static_cast<double>(weight_steps) / c.weight_splits : 0.0);
+        const double groups = static_cast<double>(c.input_tiles * c.input_splits + c.weight_tiles * c.weight_splits);
+        double time = std::max((work + START * groups) / (2 * CUS), longest + START);
+        if (c.input_splits > 1) time += JOIN + 8.0 * static_cast<double>(rows * inner) * c.input_splits / BYTES;
+        if (c.weight_splits > 1) time += JOIN + 16.0 * static_cast<double>(static_cast<uint64_t>(cols) * inner) * c.weight_splits / BYTES;
+        if (way && time >= best) continue;
+        best = time;
+        n = c;
+    }
     return n;
 }
 uint64_t up16(uint64_t n) { return (n + 15) / 16 * 16; }
@@ -911,13 +935,14 @@ uint64_t space_for(uint64_t rows, uint32_t inner, uint32_t cols, bool dx, bool d
                     space_of(plan_of(rows, inner, cols, dx, dw, false), rows, inner, cols).bytes());
 }
 
-template <typename T, typename C, bool Direct>
+template <typename T, typename CI, typename CW, bool Direct>
 int start_backward(const Params& p, const Plan& n, hipStream_t s) {
-    auto* k = gated_backward_kernel<T, C, Direct>;
+    constexpr int LDS = std::max(CI::LDS, CW::LDS);
+    auto* k = gated_backward_kernel<T, CI, CW, Direct>;
     static std::atomic<uint64_t> done{0};
-    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), C::LDS, done)) return rc;
+    if (const int rc = allow_lds(reinterpret_cast<const void*>(k), LDS, done)) return rc;
     const uint64_t inputs = n.input_tiles * n.input_splits, all = inputs + n.weight_tiles * n.weight_splits;
-    k<<<static_cast<uint32_t>(all), C::THREADS, C::LDS, s>>>(p, static_cast<uint32_t>(std::max<uint64_t>(n.input_tiles, 1)), static_cast<uint32_t>(inputs),
+    k<<<static_cast<uint32_t>(all), 256, LDS, s>>>(p, static_cast<uint32_t>(std::max<uint64_t>(n.input_tiles, 1)), static_cast<uint32_t>(inputs),
                                                             static_cast<uint32_t>(std::max<uint64_t>(n.weight_tiles, 1)));
     auto join = [&](auto* kernel, uint64_t rows) { kernel<<<static_cast<uint32_t>((rows * ((p.inner + 3) / 4) + 255) / 256), 256, 0, s>>>(p); };
     if (n.input_splits > 1) join(gated_join_kernel<T, INPUT>, p.rows);
@@ -939,13 +964,16 @@ int launch_backward(Params p, char* workspace, hipStream_t s) {
     const uint32_t rows_up = (p.rows + 63) / 64 * 64, tail_rows = n.big && p.rows % 64 ? 64 : 0;
     if (p.rows) {
         const uint64_t chunks = static_cast<uint64_t>(rows_up) * ((p.cols + 7) / 8) + static_cast<uint64_t>(tail_rows) * ((p.inner + 7) / 8);
-        gated_slopes_kernel<T><<<static_cast<uint32_t>(std::min<uint64_t>((chunks + 255) / 256, 1u << 22)), 256, 0, s>>>(p, rows_up, tail_rows);
+        gated_slopes_kernel<T><<<static_cast<uint32_t>(std::min<uint64_t>((chunks + 255) / 256, 1u << 22)), 256, 0, s>>>(p, rows_up, tail_rows, Divisor((p.cols + 7) / 8));
     }
     if (n.big) return start_big<T>(p, true, n.input_tiles + n.weight_tiles, s);
     // a step of dx's inner dimension lies in one weight
     const bool direct = aligned && p.cols % 64 == 0 && p.inner % 8 == 0;
-    if (n.mid) return direct ? start_backward<T, Mid, true>(p, n, s) : start_backward<T, Mid, false>(p, n, s);
-    return direct ? start_backward<T, Small, true>(p, n, s) : start_backward<T, Small, false>(p, n, s);
+    if (n.input_mid)
+        return n.weight_mid ? direct ? start_backward<T, Mid, Mid, true>(p, n, s) : start_backward<T, Mid, Mid, false>(p, n, s)
+                            : direct ? start_backward<T, Mid, Small, true>(p, n, s) : start_backward<T, Mid, Small, false>(p, n, s);
+    return n.weight_mid ? direct ? start_backward<T, Small, Mid, true>(p, n, s) : start_backward<T, Small, Mid, false>(p, n, s)
+                        : direct ? start_backward<T, Small, Small, true>(p, n, s) : start_backward<T, Small, Small, false>(p, n, s);
 }
 
 int check(const std::string& what, uint64_t rows, uint32_t inner, uint32_t cols) {

@@ -75,7 +75,7 @@ __device__ inline void act_and_slope(float z, int act, float& a, float& slope) {
 
 // d, 8 columns a thread; the rows past the last are 0 and so are those of x's tail.  dg and du are rounded to the inputs' type
 // for their products, as every operand of a matrix product is: off by half a unit each, at random, which gives a sum of n of
-// them the error that the same sum of rounded inputs has.
+// them the error that the same sum of rounded inputs has.  Memory bounds it: 8191 x 4096 takes 52 us, 335 MB at 6.5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_slopes_kernel(Params p, uint32_t rows_up, uint32_t tail_rows, Divisor by_across) {
     const uint32_t across = (p.cols + 7) / 8, wide = (p.inner + 7) / 8;
@@ -163,7 +163,8 @@ __device__ inline Vec<T, 8> read_across(const char* tile, int inner, int column,
     return __builtin_bit_cast(Vec<T, 8>, Vec<short, 8>{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
 }
 
-// Tiles of any size and alignment.  Direct: operands are 16-byte aligned, whole steps go from memory to LDS without registers.
+// Tiles of any size and alignment, two workgroups per compute unit.  1000 x 1024 -> 4096 takes 24 us (700 TFLOP/s), 300 x 768 ->
+// 2048 8.7, most of it the latency of its 12 steps and a launch.  Direct: operands are 16-byte aligned, whole steps go from memory to LDS without registers.
 // Tile `b` of the product; of its inner dimension piece y of `splits`, whose sums go to `parts` if there are several.
 template <typename T, int FORM, typename C, bool Direct>
 __device__ inline void one_tile(const Params& p, char* lds, uint32_t b, uint32_t y, uint32_t splits, float* parts) {
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(Params p) {
 
 // Few rows: both weights are read once, from memory to registers, and bound the time.  A workgroup has P x 16 rows of each, its
 // eight waves a contiguous piece each of the inner dimension; x (MT x 16 rows) comes from the L2, as often as there are
-// workgroups.
+// workgroups.  One row of 4096 -> 8192 takes 27.5 us (4.9 TB/s), 17 rows 30.7; 8 more steps' loads ahead spill (106 us).
 template <typename T, int MT, int P>
 __global__ __launch_bounds__(512) void gated_few_kernel(Params p) {
     constexpr int NT = 2 * P;  // tiles of 16 rows: of wg, wu, wg, ..
@@ -520,6 +521,14 @@ __global__ __launch_bounds__(512) void gated_few_kernel(Params p) {
 // weights' gradients of 8192 x 4096 -> 4096 took 726 us), and lie in LDS as 64 inner elements x 128 rows.  A workgroup goes through its tiles without a break: the moves of the next tile's first steps are under way
 // while a tile's results are written.  A tile that would pass an edge is shifted back inside and does not write what its
 // neighbour writes.
+//
+// 8192 x 4096 -> 8192 takes 820-850 us by box (1290-1340 TFLOP/s; the library reaches 1407 at 8192 x 8192 x 8192), the matrix
+// pipe busy for 0.75 of the time.  A step takes 3250 cycles, 2048 of them matrix instructions and as many LDS traffic (196 KB
+// read, 64 KB moved, 128 bytes a cycle); with half as many meetings it takes as long.  A tile's first step takes 2500 more, behind
+// its predecessor's writes, and its results 4800 cycles, with gelu 10800, with gate and up written too 14200: a fifth of the time
+// at 1024 inner elements (8191 x 1024 -> 4096: 150-155 us).  Waiting for the next tile's moves before those writes, or counting
+// the writes apart, did not pay (168 and 163 against 151-155).  Gradients of 8192 x 4096 -> 4096: 870 us with the pass for d, 1270
+// TFLOP/s.
 //
 // The tiles run .. run + count - 1 of the product, 8 tile rows high; this workgroup's are those from `first` on, `stride` apart.
 template <typename T, int FORM>

@@ -164,8 +164,9 @@ __device__ inline Vec<T, 8> read_across(const char* tile, int inner, int column,
 }
 
 // Tiles of any size and alignment, two workgroups per compute unit.  1000 x 1024 -> 4096 takes 24 us (700 TFLOP/s), 300 x 768 ->
-// 2048 8.7, most of it the latency of its 12 steps and a launch.  Direct: operands are 16-byte aligned, whole steps go from memory to LDS without registers.
-// Tile `b` of the product; of its inner dimension piece y of `splits`, whose sums go to `parts` if there are several.
+// 2048 8.7, most of it the latency of its 12 steps and a launch.  Direct: operands are 16-byte aligned, whole steps go from
+// memory to LDS without registers.  Tile `b` of the product; of its inner dimension piece y of `splits`, whose sums go to `parts`
+// if there are several.
 template <typename T, int FORM, typename C, bool Direct>
 __device__ inline void one_tile(const Params& p, char* lds, uint32_t b, uint32_t y, uint32_t splits, float* parts) {
     constexpr bool XT = FORM == WEIGHTS, WT = FORM != GATED;  // the operand's rows are columns in memory

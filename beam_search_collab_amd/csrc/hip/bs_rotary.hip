@@ -8,7 +8,7 @@
 // rotary / 2) or 2 N neighbours, so that both partners of a pair are the lane's.
 //
 // Memory bounds both directions.  32768 tokens of 32 + 8 heads of 128 in bf16, columns of a product 48 heads wide: 156 us, 4.3
-// TB/s (a copy reaches 5.0); the gradients of 16384 with float32 weights: 124 us, 4.1 TB/s.  Weights in LDS instead of
+// TB/s (a copy reaches 5.0); the gradients of 16384 with float32 weights: 122 us, 4.1 TB/s.  Weights in LDS instead of
 // registers and queries and keys in workgroups of their own took the first from 198 us to 176, the second from 182 to 151.
 #include "bs_embed.hpp"
 
@@ -180,9 +180,20 @@ __device__ inline void turn(const Params& p, const float* table, const Places (&
         }
     }
 }
-// sum over a head's lanes
+// Sum over a head's lanes, the same bits in all of them.  Exchanges within 16 lanes are operands of the additions (by 4 and 8: a
+// mirror of 8 and 16 lanes, whose halves hold one value each by then); with all of them through LDS the gradients of 16384
+// tokens take 124 us instead of 122.
+template <int Control>
+__device__ inline float from_lane(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), Control, 0xF, 0xF, true));
+}
 __device__ inline float head_sum(float v, uint32_t lanes) {
-    for (uint32_t m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m);
+    if (lanes >= 2) v += from_lane<0xB1>(v);    // quad_perm 1 0 3 2
+    if (lanes >= 4) v += from_lane<0x4E>(v);    // quad_perm 2 3 0 1
+    if (lanes >= 8) v += from_lane<0x141>(v);   // row_half_mirror
+    if (lanes >= 16) v += from_lane<0x140>(v);  // row_mirror
+    if (lanes >= 32) v += __shfl_xor(v, 16);
+    if (lanes >= 64) v += __shfl_xor(v, 32);
     return v;
 }
 template <int N, int K>

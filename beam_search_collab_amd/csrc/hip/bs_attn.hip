@@ -1025,6 +1025,7 @@ void cut_prefix(const bs_attention_args& a, uint32_t keys, uint32_t& splits, uin
 }
 struct Apart {
     Params front, own;
+    bool joins;      // the own keys' launch joins the prefix's parts itself, else a third one does
     uint32_t parts;  // of a row in the workspace
     uint64_t bytes;
 };
@@ -1043,7 +1044,12 @@ Apart apart(const bs_attention_args& a, const bs_attention_prefix& f) {
         p->by_group = Divisor(p->group);
         p->by_kv = Divisor(a.kv_heads);
     }
-    x.parts = x.front.splits + (x.own.splits > 1 ? x.own.splits : 0);
+    // A lane of the prompts' kernel takes a row's parts one after the other, a thread of the single tokens' kernel four at a
+    // time.  By itself and by a third launch: 15 tokens, 46 parts of 13676 keys 86 and 26 us, 655 tokens, 7 to 12 parts of 9187
+    // 108 and 70; but 49 x 2..97, 4 parts of 12775 83 and 92; 128 single tokens, 16 parts of 16384 80 and 82.5, 64, 16 parts
+    // of 4000 26.0 and 28.0.
+    x.joins = x.own.splits == 1 && x.front.splits <= (few_of(a) ? 16u : 6u);
+    x.parts = x.front.splits + (x.joins ? 0 : x.own.splits);
     x.bytes = static_cast<uint64_t>(x.parts) * a.q_tokens * a.heads * (a.head_dim + 2) * sizeof(float);
     return x;
 }
@@ -1059,16 +1065,16 @@ int launch_prefix(const Params& p, void* workspace, hipStream_t s) {
     float2* stat = reinterpret_cast<float2*>(out + static_cast<uint64_t>(x.parts) * p.a.q_tokens * p.a.heads * d);
     x.front.part_out = out;
     x.front.part_stat = stat;
-    if (x.own.splits > 1) {
-        x.own.part_out = out;
-        x.own.part_stat = stat;
-    } else {  // the own keys' launch joins the prefix's parts itself
+    if (x.joins) {
         x.own.front_out = out;
         x.own.front_stat = stat;
+    } else {
+        x.own.part_out = out;
+        x.own.part_stat = stat;
     }
     if (const int rc = start_any<T>(x.front, s)) return rc;
     if (const int rc = start_any<T>(x.own, s)) return rc;
-    if (x.own.splits > 1) join<T>(x.own, s);
+    if (!x.joins) join<T>(x.own, s);
     return launched("bs_attention_shared_prefix");
 }
 

@@ -864,3 +864,11 @@ def test_two_graphs_with_workspaces_of_their_own(gpu):
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert all(torch.equal(a, b) for a, b in zip(o, w))
+
+
+@pytest.mark.parametrize("nq,nk,prefix,heads,kv,dim", [
+    ([5] * 3, [2, 3, 1], 13676, 8, 8, 80), ([5] * 40, [1] * 40, 9187, 12, 4, 128), ([2, 97, 40, 1] * 8, [2, 97, 40, 1] * 8, 9000, 8, 8, 32),  # many parts of a row, six and fewer
+    ([1] * 16, [3] * 16, 4096, 8, 2, 64), ([1] * 16, [3] * 16, 12000, 8, 2, 64)])
+def test_attention_shared_prefix_of_many_parts(gpu, nq, nk, prefix, heads, kv, dim):
+    for dtype in (BF16, F16):
+        behind_prefix(700, nq, nk, prefix, heads, kv, dim, dtype)

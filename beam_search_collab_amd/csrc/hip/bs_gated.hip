@@ -838,13 +838,13 @@ int start_big(const Params& p, bool backward, uint64_t tiles, hipStream_t s) {
     k<<<tiles < CUS ? static_cast<uint32_t>(tiles + 7) / 8 * 8 : CUS, 512, LDS, s>>>(p);
     return BS_OK;
 }
-float fill(uint64_t tiles) { return static_cast<float>(tiles) / static_cast<float>((tiles + CUS - 1) / CUS * CUS); }
 
 template <typename T>
 int launch_forward(Params p, hipStream_t s) {
     if (p.rows <= FEW) {
-        // 32 columns a workgroup, half the reads of x, where that leaves a workgroup for every compute unit: 17 x 4096 -> 8192
-        // takes 30.6 us, 35.7 with 16
+        // Up to 32 rows: with 64, 64 x 4096 -> 8192 would take 39 us, 34 with tiles; 48 x 1024 -> 4096 8.5 either way.  32
+        // columns a workgroup, half the reads of x, where that leaves a workgroup for every compute unit: 17 x 4096 -> 8192
+        // takes 30.6 us, 35.7 with 16.
         if (p.rows <= 16)
             gated_few_kernel<T, 1, 1><<<(p.cols + 15) / 16, 512, 0, s>>>(p);
         else if (p.cols >= 32 * CUS)
@@ -854,10 +854,16 @@ int launch_forward(Params p, hipStream_t s) {
         return BS_OK;
     }
     const bool direct = rows16(p.x, p.xs) && rows16(p.wg, p.wgs) && rows16(p.wu, p.wus);
-    const uint64_t big = tiles_of(p.rows, p.cols, 256, 128);
-    if (direct && fill(big) >= 0.55f && p.rows >= 256 && p.cols >= 128 && p.inner % 64 == 0 && p.inner >= 128 && p.xs < (1 << 22) && p.wgs < (1 << 22) && p.wgs == p.wus)
+    // Tiles of 256 where they take fewer rounds of workgroups than tiles of 128, of which two share a compute unit.  256 and
+    // 128: 2560 x 4096 -> 1792 (140 and 560 tiles) 73 and 104 us, 4096 x 1024 -> 1280 25.4 and 32.0, 4200 x 1024 -> 2048 (272
+    // and 1056) 53 and 56, 5000 x 4096 -> 2048 169 and 202, but 2048 x 4096 -> 1792 (112 and 448) 73 and 70, 1500 x 2048 ->
+    // 2048 39.6 and 35.7.  128 and 64: 1500 x 2048 -> 2048 (384 tiles of 128) 35.7 and 40.6, but 2048 x 1024 -> 1024 (256)
+    // 14.6 and 13.4.
+    const uint64_t big = tiles_of(p.rows, p.cols, 256, 128), mid = tiles_of(p.rows, p.cols, 128, 64);
+    if (direct && (big + CUS - 1) / CUS < (mid + 2 * CUS - 1) / (2 * CUS) && p.rows >= 256 && p.cols >= 128 && p.inner % 64 == 0 &&
+        p.inner >= 128 && p.xs < (1 << 22) && p.wgs < (1 << 22) && p.wgs == p.wus)
         return start_big<T>(p, false, big, s);
-    if (tiles_of(p.rows, p.cols, 128, 64) >= CUS) return direct ? start<T, Mid, true>(p, s) : start<T, Mid, false>(p, s);
+    if (mid > CUS) return direct ? start<T, Mid, true>(p, s) : start<T, Mid, false>(p, s);
     if (tiles_of(p.rows, p.cols, 64, 64) <= CUS) return direct ? start<T, Narrow, true>(p, s) : start<T, Narrow, false>(p, s);
     return direct ? start<T, Flat, true>(p, s) : start<T, Flat, false>(p, s);
 }

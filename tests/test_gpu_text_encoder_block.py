@@ -666,8 +666,9 @@ def test_attention_shared_prefix_refusals(gpu):
 @pytest.mark.parametrize("rows,inner,cols", [
     (32, 300, 8191), (32, 300, 8192), (16, 300, 8192), (17, 260, 8205), (32, 64, 100),       # few rows, by 16 and by 32 columns
     (33, 320, 8192), (33, 320, 8200), (64, 256, 8224), (65, 256, 4096),                      # 256 and 257 narrow tiles
-    (256, 96, 8192), (256, 96, 8128), (128, 100, 16384), (128, 100, 16321),                  # 256 and 254 tiles of 128 x 64
-    (2816, 128, 1664), (2816, 128, 1537), (2816, 64, 1664), (2816, 192, 1663), (2560, 128, 1792), (300, 256, 9088), (256, 128, 17920)])  # 143 and 140 of 256 x 128
+    (256, 96, 8192), (256, 96, 8128), (256, 96, 8256), (128, 100, 16384), (128, 100, 16321), (128, 100, 16385),  # 256 tiles of 128 x 64 and more
+    (2816, 128, 1664), (2816, 128, 1537), (2816, 64, 1664), (2816, 192, 1663), (2560, 128, 1792), (300, 256, 9088), (256, 128, 17920),
+    (2048, 128, 2048), (2049, 128, 2048), (2304, 128, 1920), (4352, 128, 1984)])  # 128 tiles of 256 x 128 (512 of 128 x 64) and more, 272
 def test_gated_on_both_sides_of_the_rules(gpu, rows, inner, cols):
     x, wg, wu = gated_case(400, rows, inner, cols, BF16)
     h, gate, up = embed.gated(x, wg, wu, activation="gelu_tanh", save=True)

@@ -1012,7 +1012,7 @@ bool along_of(const bs_attention_args& a, const bs_attention_prefix& f) {
 void cut_prefix(const bs_attention_args& a, uint32_t keys, uint32_t& splits, uint32_t& piece) {
     const uint64_t slots = (a.head_dim <= 64 ? 3 : 2) * CUS, rows = static_cast<uint64_t>(a.q_tokens) * (a.heads / a.kv_heads);
     const uint64_t groups = (rows + 127) / 128 * a.kv_heads, row = static_cast<uint64_t>(a.q_tokens) * a.heads * (a.head_dim + 2) * sizeof(float);
-    const uint64_t most = std::min<uint64_t>({64, std::max<uint64_t>(1, keys / 256), std::max<uint64_t>(1, (1ull << 28) / row)});
+    const uint64_t most = std::min<uint64_t>({64, std::max<uint64_t>(1, keys / 256), std::max<uint64_t>(1, (1ull << 28) / std::max<uint64_t>(row, 1))});
     double best = 0.0;
     for (uint64_t n = 1; n <= most; ++n) {
         const uint64_t each = ((keys + n - 1) / n + 127) / 128 * 128, pieces = (keys + each - 1) / each;
@@ -1141,6 +1141,10 @@ extern "C" int bs_attention_shared_prefix_workspace(const bs_attention_args* arg
     if (const int rc = check_prefix(what, args, prefix)) return rc;
     if (prefix->tokens == 0) {
         *bytes = workspace_of(*args);
+        return BS_OK;
+    }
+    if (args->q_tokens == 0) {
+        *bytes = 0;
         return BS_OK;
     }
     *bytes = along_of(*args, *prefix) ? 0 : apart(*args, *prefix).bytes;

@@ -163,3 +163,18 @@ def test_gated_workspace_is_enough_for_either_gradient(rows, inner, cols):
         rc = hip.bs_gated_backward(PTR, cols, PTR, inner, PTR, inner, PTR, inner, PTR, cols, PTR, cols, dx, dwg, dwu, rows, inner, cols, 2, 4, None, 0, None)
         refused(rc, "the workspace must hold")
         assert int(hip.bs_last_error().decode().split("hold ")[1].split(" ")[0]) <= n.value
+
+
+@pytest.mark.parametrize("group", [1, 8, 9, 16, 64])
+@pytest.mark.parametrize("tokens", [1, 100, 1016, 1017, 16384])
+def test_attention_shared_prefix_of_no_queries_needs_no_workspace(group, tokens):
+    """whichever way queries behind such a prefix would take: 64 of them take both"""
+    hip, n = _lib.hip(), C.c_uint64(1)
+    for kv_heads in (1, 4):
+        for sequences in (1, 3):
+            a = attention_args(q_tokens=0, heads=group * kv_heads, kv_heads=kv_heads, sequences=sequences, q_offsets=PTR, k_offsets=PTR)
+            f = prefix_args(tokens=tokens)
+            assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), C.byref(n)) == 0 and n.value == 0
+            assert hip.bs_attention_shared_prefix(C.byref(a), C.byref(f), None, 0, None) == 0
+            a.q_tokens = 64
+            assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), C.byref(n)) == 0 and (n.value > 0 or tokens <= 1017)

@@ -873,3 +873,13 @@ def test_two_graphs_with_workspaces_of_their_own(gpu):
 def test_attention_shared_prefix_of_many_parts(gpu, nq, nk, prefix, heads, kv, dim):
     for dtype in (BF16, F16):
         behind_prefix(700, nq, nk, prefix, heads, kv, dim, dtype)
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 4), (8, 1), (9, 1), (16, 1), (40, 4)])
+@pytest.mark.parametrize("prefix", [0, 100, 1017, 16384])
+def test_attention_shared_prefix_of_no_queries(gpu, heads, kv, prefix):
+    q, k, p = (rand(440 + i, n, h, 64, dtype=BF16) for i, (n, h) in enumerate([(0, heads), (5, kv), (prefix, kv)]))
+    for off in (None, offsets([0]), offsets([0, 0, 0])):
+        own = offsets([5] if off is None or len(off) == 2 else [2, 0, 3])
+        out, lse = embed.attention_shared_prefix(q, k, k, p, p, off, None if off is None else own, lse=True)
+        assert out.shape == q.shape and out.dtype == BF16 and lse.shape == (0, heads)

@@ -40,11 +40,13 @@ struct Params {
 
 // ------------------------------------------------------------------------------------------------ d
 
-// 1 / (1 + e) and e / (1 + e) for e = 2^v, neither by a difference
+// 1 / (1 + e) and e / (1 + e) for e = 2^v, neither by a difference; 0 and 1 past 2^126, for a 1 / (1 + e) that stopped at 2^-126
+// would give far gates values and slopes that grow with them
 __device__ inline void halves_of_one(float v, float& s, float& rest) {
     const float e = __builtin_amdgcn_exp2f(fminf(v, 126.0f));
     s = __builtin_amdgcn_rcpf(1.0f + e);
     rest = e * s;
+    s = v > 126.0f ? 0.0f : s;
 }
 // an activation and its slope
 __device__ inline void act_and_slope(float z, int act, float& a, float& slope) {

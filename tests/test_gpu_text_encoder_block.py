@@ -883,3 +883,38 @@ def test_attention_shared_prefix_of_no_queries(gpu, heads, kv, prefix):
         own = offsets([5] if off is None or len(off) == 2 else [2, 0, 3])
         out, lse = embed.attention_shared_prefix(q, k, k, p, p, off, None if off is None else own, lse=True)
         assert out.shape == q.shape and out.dtype == BF16 and lse.shape == (0, heads)
+
+
+def every_value(dtype):
+    """all 65536 values of a 16-bit type, one row"""
+    return torch.arange(1 << 16, device="cuda").to(torch.int16).view(dtype)[None]
+
+
+def gate_gradients(gate, act):
+    """dup and dgate for ones in the other places, as the weights' gradients of one row that is 1"""
+    one, w = torch.ones(1, 1, dtype=gate.dtype, device="cuda"), torch.ones(gate.shape[1], 1, dtype=gate.dtype, device="cuda")
+    _, slope, value = embed.gated_backward(torch.ones_like(gate), one, w, w, gate, torch.ones_like(gate), activation=act)
+    return value[:, 0], slope[:, 0]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gated_slopes_of_every_finite_gate(gpu, act, dtype):
+    gate = every_value(dtype)
+    z = gate[0].double()
+    # value z s and slope s + z s (1 - s) w' of s = 1 / (1 + exp(-w))
+    k = 2 * math.sqrt(2 / math.pi)
+    w, bend = (z, 1.0) if act == "silu" else (k * (z + 0.044715 * z ** 3), k * (1 + 3 * 0.044715 * z * z))
+    s, rest = torch.sigmoid(w), torch.sigmoid(-w)
+    # w in float32, 6 roundings at most, each 1 unit of w in the exponent; the exponential, the sum and the reciprocal, 5, and
+    # two products
+    part = 6 * E * w.abs() + 8 * E
+    # exp(-w) from 2^126 on: 1 / (1 + exp(-w)) is below float32's normal range and may be 0
+    lost = torch.where(w <= -126 * math.log(2), 1.0, 0.0)
+    floor = 2.0 ** -126 if dtype == BF16 else TINY[dtype]  # bfloat16 below the normal range: matrix products may take it as 0
+    value, slope = gate_gradients(gate, act)
+    fine = torch.isfinite(z)
+    want, whole = z * s, s + (z * s * rest * bend).abs()
+    near(value[fine], want[fine], ((part + U[dtype] + lost) * want.abs() + floor)[fine])
+    want = s + z * s * rest * bend
+    near(slope[fine], want[fine], ((2 * part + 8 * E + lost) * whole + U[dtype] * want.abs() + floor)[fine])

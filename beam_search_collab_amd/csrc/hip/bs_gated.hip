@@ -52,7 +52,7 @@ __device__ inline void halves_of_one(float v, float& s, float& rest) {
 __device__ inline void act_and_slope(float z, int act, float& a, float& slope) {
     if (act == BS_ACT_RELU) {
         a = z < 0.0f ? 0.0f : z;
-        slope = z > 0.0f ? 1.0f : 0.0f;
+        slope = z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;  // NaN as it is
     } else if (act == BS_ACT_GELU) {  // P = (1 + erf(z / sqrt 2)) / 2: slope P + z exp(-z^2 / 2) / sqrt(2 pi)
         const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E)), part = gelu_part(z, e);
         a = z * part;

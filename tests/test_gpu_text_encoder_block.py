@@ -918,3 +918,16 @@ def test_gated_slopes_of_every_finite_gate(gpu, act, dtype):
     near(value[fine], want[fine], ((part + U[dtype] + lost) * want.abs() + floor)[fine])
     want = s + z * s * rest * bend
     near(slope[fine], want[fine], ((2 * part + 8 * E + lost) * whole + U[dtype] * want.abs() + floor)[fine])
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gated_gradients_of_nan_gates_are_nan(gpu, act, dtype):
+    gate = every_value(dtype)
+    value, slope = gate_gradients(gate, act)
+    assert torch.isnan(value[torch.isnan(gate[0])]).all()
+    assert torch.isnan(slope[torch.isnan(gate[0])]).all() if act != "none" else (slope == 1).all()
+    if act == "relu":
+        fine = ~torch.isnan(gate[0])
+        large = fine & ((gate[0].double().abs() >= 2.0 ** -126) | (gate[0] == 0))  # bfloat16 below the normal range
+        assert torch.equal(slope[fine], (gate[0] > 0).to(dtype)[fine]) and torch.equal(value[large], torch.relu(gate[0])[large])

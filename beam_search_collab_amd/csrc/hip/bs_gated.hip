@@ -48,27 +48,29 @@ __device__ inline void halves_of_one(float v, float& s, float& rest) {
     rest = e * s;
     s = v > 126.0f ? 0.0f : s;
 }
-// an activation and its slope
+// An activation and its slope.  An infinite gate, a finite product past the type's range (65504 in float16) that the forward call
+// took as it was, has their limits: factors that vanish there are not multiplied by it.
 __device__ inline void act_and_slope(float z, int act, float& a, float& slope) {
     if (act == BS_ACT_RELU) {
         a = z < 0.0f ? 0.0f : z;
         slope = z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;  // NaN as it is
     } else if (act == BS_ACT_GELU) {  // P = (1 + erf(z / sqrt 2)) / 2: slope P + z exp(-z^2 / 2) / sqrt(2 pi)
         const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E)), part = gelu_part(z, e);
-        a = z * part;
-        slope = fmaf(z * 0.3989422804014327f, e, part);
+        a = part == 0.0f ? 0.0f : z * part;
+        slope = e == 0.0f ? part : fmaf(z * 0.3989422804014327f, e, part);
     } else if (act == BS_ACT_GELU_TANH) {  // z s, s = 1 / (1 + exp(-2 v)): slope s + z s (1 - s) 2 v'
         const float q = z * z;
         float s, rest;
         halves_of_one(-2.0f * LOG2E * 0.79788456080286536f * fmaf(0.044715f * q, z, z), s, rest);
-        a = z * s;
+        a = s == 0.0f ? 0.0f : z * s;
         const float bend = s * rest;
         slope = bend == 0.0f ? s : fmaf(z * bend, 2.0f * 0.79788456080286536f * fmaf(3.0f * 0.044715f, q, 1.0f), s);
     } else if (act == BS_ACT_SILU) {  // z s, s = 1 / (1 + exp(-z)): slope s + z s (1 - s)
         float s, rest;
         halves_of_one(-LOG2E * z, s, rest);
-        a = z * s;
-        slope = fmaf(z * rest, s, s);
+        a = s == 0.0f ? 0.0f : z * s;
+        const float bend = s * rest;
+        slope = bend == 0.0f ? s : fmaf(z, bend, s);
     } else {
         a = z;
         slope = 1.0f;

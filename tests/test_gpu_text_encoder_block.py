@@ -931,3 +931,22 @@ def test_gated_gradients_of_nan_gates_are_nan(gpu, act, dtype):
         fine = ~torch.isnan(gate[0])
         large = fine & ((gate[0].double().abs() >= 2.0 ** -126) | (gate[0] == 0))  # bfloat16 below the normal range
         assert torch.equal(slope[fine], (gate[0] > 0).to(dtype)[fine]) and torch.equal(value[large], torch.relu(gate[0])[large])
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gated_gradients_of_infinite_gates_are_the_limits(gpu, act, dtype):
+    gate = torch.tensor([[math.inf, -math.inf]], dtype=dtype, device="cuda")
+    value, slope = gate_gradients(gate, act)
+    assert value.tolist() == [math.inf, -math.inf if act == "none" else 0.0]
+    assert slope.tolist() == [1.0, 1.0 if act == "none" else 0.0]
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_gated_gradients_of_products_past_float16(gpu, act):
+    """gates that float16 saves as -infinity: the forward call's result and its gradients are 0, not NaN"""
+    x, w = torch.full((3, 64), 200.0, dtype=F16, device="cuda"), torch.full((40, 64), 20.0, dtype=F16, device="cuda")
+    h, gate, up = embed.gated(x, -w, 0.001 * w, activation=act, save=True)
+    assert (gate == -math.inf).all() and (h == 0).all() and torch.isfinite(up).all()
+    for g in embed.gated_backward(torch.ones_like(h), x, -w, 0.001 * w, gate, up, activation=act):
+        assert (g == 0).all()

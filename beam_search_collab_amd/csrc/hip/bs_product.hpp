@@ -32,15 +32,18 @@ struct Mma16<bf16> {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// z (1 + erf(z / sqrt 2)) / 2 by formula 7.1.26 of Abramowitz and Stegun's handbook: with x = |z| / sqrt 2,
-// t = 1 / (1 + p x), erfc(x) = t (a1 + t (a2 + .. )) exp(-x^2), off by 1.5e-7 at most, so by 1.3 units of 2^-24
-// |z| here; the halves and roots are in the constants.  That is absolute: a result far below 1 is off by 7e-4 of itself at
-// z = -4.2 and 3e-3 at -5.7, which float32 results show (1 + erf in float32 is off by 2e-3 and loses all of it there).
-// 8191 x 1024 -> 4096: 92 us, 102 us with the library's erff.
+// z (1 + erf(z / sqrt 2)) / 2 in the form of formula 7.1.26 of Abramowitz and Stegun's handbook: with x = |z| / sqrt 2 and t = 1 /
+// (1 + p |z|), erfc(x) / 2 = t P(t) exp(-x^2).  Its five coefficients are off by 1.5e-7 of 1, which is 7e-4 of the result at
+// z = -4.2 and 3e-2 at -12, several roundings of a 16-bit type.  Those here are of degree 6, the least squares over |z| <= 13.5
+// reweighted until the largest of the errors against 7e-8 exp(x^2) and 4e-6 of erfc(x) is least: off by 2.8e-6 of itself and by
+// 1.6e-7, float32 roundings included (the five: 2.4e-7), beside the rounding of the exponent, 1.5 z^2 units of 2^-24 of a result
+// below 0.  Past z = -13.2, where exp(-x^2) is below float32's normal range, the result may be 0.  8191 x 1024 -> 4096:
+// 87 us, 84 with five coefficients (another card: 92, and 102 with the library's erff).
 __device__ inline float gelu_part(float z, float e) {  // (1 + erf(z / sqrt 2)) / 2 for e = exp(-z^2 / 2)
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, fabsf(z), 1.0f));
-    const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
-    const float rest = q * e;  // erfc(x) / 2
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.348f, fabsf(z), 1.0f));
+    float q = fmaf(t, 0.044490628f, -0.18701635f);
+    q = fmaf(t, fmaf(t, fmaf(t, q, 0.22043395f), 0.0022022785f), 0.14531076f);
+    const float rest = t * fmaf(t, fmaf(t, q, 0.13556218f), 0.13901654f) * e;  // erfc(x) / 2
     return z < 0.0f ? rest : 1.0f - rest;
 }
 __device__ inline float gelu(float z) { return z * gelu_part(z, __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E))); }

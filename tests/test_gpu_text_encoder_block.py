@@ -950,3 +950,32 @@ def test_gated_gradients_of_products_past_float16(gpu, act):
     assert (gate == -math.inf).all() and (h == 0).all() and torch.isfinite(up).all()
     for g in embed.gated_backward(torch.ones_like(h), x, -w, 0.001 * w, gate, up, activation=act):
         assert (g == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gelu_of_every_value_is_near_itself(gpu, dtype):
+    """also where it is far below 1: of products with a large factor beside it, of float32 results and of gradients"""
+    gate = every_value(dtype)[0]
+    gate = gate[gate.abs() < 200]
+    z = gate.double()
+    lower, density = torch.special.erfc(-z / math.sqrt(2)) / 2, torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    # the formula is off by 2.7e-6, 45 E, of erfc; its reciprocal, 4 E, weighs 2.3 times, its seven sums and products 1.8 times; the
+    # exponent's three roundings, of its square's halves; the exponential, two products
+    part = (1.5 * z * z + 45 + 4 * 2.3 + 14 * 1.8 + 6) * E
+    lost = torch.where(z <= -13.2, 1.0, 0.0)  # exp(-z^2 / 2) is below float32's normal range
+    low = 2.0 ** -126
+    want = z * lower
+    one = torch.ones(1, 1, dtype=dtype, device="cuda")
+    got = embed.linear(gate[:, None], one, activation="gelu", out_dtype=F32)[:, 0]
+    near(got, want, (part + lost) * want.abs() + low)
+    near(embed.linear(gate[:, None], one, activation="gelu")[:, 0], want, (part + U[dtype] + lost) * want.abs() + max(low, TINY[dtype]))
+    for factor in (1.0, 2.0 ** 14):  # the latter brings out what float16 has no bits for
+        x = torch.stack([gate, torch.full_like(gate, factor)], 1)
+        w = torch.eye(2, dtype=dtype, device="cuda")
+        fine = (want * factor).abs() < 60000  # float16's largest number
+        tol = (part + U[dtype] + 2 * E + lost) * want.abs() * factor + max(low * factor, TINY[dtype])
+        near(embed.gated(x, w[:1], w[1:], activation="gelu")[fine, 0], want[fine] * factor, tol[fine])
+    value, slope = gate_gradients(gate[None], "gelu")
+    near(value, want, (part + U[dtype] + lost) * want.abs() + max(low, TINY[dtype]))
+    whole = lower + z.abs() * density
+    near(slope, lower + z * density, (part + 6 * E + lost) * whole + U[dtype] * (lower + z * density).abs() + max(low, TINY[dtype]))

@@ -178,3 +178,26 @@ def test_attention_shared_prefix_of_no_queries_needs_no_workspace(group, tokens)
             assert hip.bs_attention_shared_prefix(C.byref(a), C.byref(f), None, 0, None) == 0
             a.q_tokens = 64
             assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(f), C.byref(n)) == 0 and (n.value > 0 or tokens <= 1017)
+
+
+def test_python_refuses_sizes_past_32_bits(monkeypatch):
+    """the structures of the C calls hold sizes in 32 bits: 2^32 + 8 tokens would be taken for 8"""
+    import torch
+    from beam_search_collab_amd import embed
+    monkeypatch.setattr(embed, "_gpu", lambda what, *tensors: 0)
+    far = (1 << 32) + 8
+
+    def t(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+    q, k = t(8, 2, 8), t(8, 1, 8)
+    for call in (lambda: embed.layer_norm(t(1, far)), lambda: embed.layer_norm_backward(t(1, far), t(1, far), t(1), t(1)),
+                 lambda: embed.linear(t(1, far), t(4, far)), lambda: embed.linear(t(1, 8), t(far, 8)),
+                 lambda: embed.gated(t(1, far), t(4, far), t(4, far)), lambda: embed.gated(t(1, 8), t(far, 8), t(far, 8)),
+                 lambda: embed.gated_backward(t(1, far), t(1, 8), t(far, 8), t(far, 8), t(1, far), t(1, far)),
+                 lambda: embed.head_norm_rotary(t(far, 1, 8)), lambda: embed.head_norm_rotary(t(1, far, 8)), lambda: embed.head_norm_rotary(t(1, 1, far)),
+                 lambda: embed.head_norm_rotary(t(8, 1, 8), t(8, far, 8)), lambda: embed.head_norm_rotary_backward(t(far, 1, 8), None, t(far, 1, 8)),
+                 lambda: embed.attention(t(far, 1, 8), k, k), lambda: embed.attention(q, t(far, 1, 8), t(far, 1, 8)),
+                 lambda: embed.attention(t(8, far, 8), k, k), lambda: embed.attention(q, t(8, far, 8), t(8, far, 8)),
+                 lambda: embed.attention_shared_prefix(q, k, k, t(far, 1, 8), t(far, 1, 8)), lambda: embed.attention_shared_prefix(t(far, 1, 8), k, k, k, k)):
+        with pytest.raises(ValueError, match="sizes must be < 2.31"):
+            call()

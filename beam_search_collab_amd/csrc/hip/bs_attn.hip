@@ -899,7 +899,7 @@ void split(const bs_attention_args& a, uint32_t& splits, uint32_t& piece) {
     }
     piece = static_cast<uint32_t>(std::min<uint64_t>((want + 127) / 128 * 128, (static_cast<uint64_t>(longest) + 127) / 128 * 128));
     if (piece == 0) piece = 128;
-    // at most 256 MB of parts: with many sequences the pieces are for their different lengths alone
+    // at most 256 MB of parts, or one for every row: with many sequences the pieces are for their different lengths alone
     const uint64_t row = rows * (a.head_dim + 2) * sizeof(float);
     const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(65535, (1ull << 28) / std::max<uint64_t>(row, 1)));
     if ((longest + piece - 1) / piece > most) piece = static_cast<uint32_t>((longest + most - 1) / most + 127) / 128 * 128;
@@ -1008,7 +1008,7 @@ bool along_of(const bs_attention_args& a, const bs_attention_prefix& f) {
     return along <= apart;
 }
 // Pieces of the prefix for the rows of all sequences: the number that takes the fewest rounds of workgroups, a piece's keys each
-// and 400 keys' time for the parts.  At least 256 keys, at most 256 MB of parts.
+// and 400 keys' time for the parts.  At least 256 keys, and at most 256 MB of parts or, where that is more, one for every row.
 void cut_prefix(const bs_attention_args& a, uint32_t keys, uint32_t& splits, uint32_t& piece) {
     const uint64_t slots = (a.head_dim <= 64 ? 3 : 2) * CUS, rows = static_cast<uint64_t>(a.q_tokens) * (a.heads / a.kv_heads);
     const uint64_t groups = (rows + 127) / 128 * a.kv_heads, row = static_cast<uint64_t>(a.q_tokens) * a.heads * (a.head_dim + 2) * sizeof(float);

@@ -196,7 +196,9 @@ int bs_gated_backward_workspace(uint64_t rows, uint32_t inner, uint32_t cols, ui
  * by each tile of rows where they fill tiles.  Its type, kv_heads and head_dim are args'; a prefix
  * of 0 tokens is bs_attention.  A query's own keys may be none.  Strides of keys and values, the
  * prefix's too, are < 2^22.  Queries outside every sequence may be read, not written.
- * workspace: bs_attention_shared_prefix_workspace bytes for the same sizes, 16-byte aligned. */
+ * workspace: bs_attention_shared_prefix_workspace bytes for the same sizes, 16-byte aligned; up to
+ * twice 256 MB, or twice q_tokens heads (head_dim + 2) 4 bytes where that is more (a part for every
+ * row over the prefix, and one over the own keys): 1.7 GB for 100000 single tokens, 32 heads of 128. */
 typedef struct {
     const void* k;
     const void* v;

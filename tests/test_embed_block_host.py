@@ -201,3 +201,13 @@ def test_python_refuses_sizes_past_32_bits(monkeypatch):
                  lambda: embed.attention_shared_prefix(q, k, k, t(far, 1, 8), t(far, 1, 8)), lambda: embed.attention_shared_prefix(t(far, 1, 8), k, k, k, k)):
         with pytest.raises(ValueError, match="sizes must be < 2.31"):
             call()
+
+
+@pytest.mark.parametrize("q,k,sequences,heads,kv,dim,longest,prefix", [
+    (100000, 100000, 100000, 32, 8, 128, 0, 1000), (20000, 5000000, 20000, 32, 8, 128, 300, 1000), (4294, 66527, 65, 8, 1, 128, 66527, 85984),
+    (2677, 57278, 2, 32, 8, 64, 57278, 50665), (1, 1 << 30, 1, 64, 1, 128, 0, 1 << 30), (3, 5, 1, 2, 1, 32, 0, 100000)])
+def test_attention_shared_prefix_workspace_stays_within_its_bound(q, k, sequences, heads, kv, dim, longest, prefix):
+    hip, n = _lib.hip(), C.c_uint64(0)
+    a = attention_args(q_tokens=q, k_tokens=k, sequences=sequences, heads=heads, kv_heads=kv, head_dim=dim, longest_k=longest)
+    assert hip.bs_attention_shared_prefix_workspace(C.byref(a), C.byref(prefix_args(tokens=prefix)), C.byref(n)) == 0
+    assert 0 < n.value <= 2 * max(1 << 28, q * heads * (dim + 2) * 4)

@@ -14,7 +14,9 @@
 They take and return torch tensors on the GPU and run on torch's current stream, so that a float32
 result can go to GPUGraph.search_device on the same stream without a copy or a wait.  Every call goes
 through libbs_hip.so (include/bs_embed.h); wrong arguments raise ValueError.  The features of a row are
-contiguous, rows may lie any distance apart (slices of a wider tensor are taken as they are).
+contiguous, rows may lie any distance apart (slices of a wider tensor are taken as they are) but not on
+one another: a gradient that is a broadcast view is made contiguous first.  `out` overlaps no input except
+where the call says so.
 Autograd does not see the calls: tensors that require a gradient are refused while it records, and taken
 under torch.no_grad(); the *_backward calls are made by hand or from a torch.autograd.Function.
 Workspaces and results come from torch's allocator, so the calls can be captured in a torch.cuda.graph.
@@ -70,10 +72,9 @@ def _gpu(what: str, x: torch.Tensor, *tensors) -> int:
     return dev
 
 
-def _sizes(what: str, *sizes: int):
-    """ctypes would cut what has more than 32 bits without a word"""
-    if max(sizes) > 0x7FFFFFFF:
-        _fail(f"{what}: sizes must be < 2^31, got {max(sizes)}")
+def _too_large(what: str, *sizes: int):
+    """refuses the sizes: ctypes would cut what has more than 32 bits without a word"""
+    _fail(f"{what}: sizes must be < 2^31, got {max(sizes)}")
 
 
 def _rows(what: str, name: str, t: torch.Tensor) -> Tuple[int, int, int]:
@@ -83,7 +84,7 @@ def _rows(what: str, name: str, t: torch.Tensor) -> Tuple[int, int, int]:
         _fail(f"{what}: {name} must have at least one dimension")
     m = t.shape[-1]
     if m > 0x7FFFFFFF:
-        _sizes(what, m)
+        _too_large(what, m)
     if t.is_contiguous():
         return (t.numel() // m if m else 0), m, m
     if t.dim() != 2:
@@ -226,7 +227,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         _fail(f"{what}: weight must be cols x inner of x's type")
     n, inner, xs = _rows(what, "x", x)
     cols, k, ws = _rows(what, "weight", weight)
-    _sizes(what, cols)
+    if cols > 0x7FFFFFFF:
+        _too_large(what, cols)
     if k != inner:
         _fail(f"{what}: x has {inner} features, weight {k}")
     if bias is not None:
@@ -273,7 +275,8 @@ def _attention_args(what, q, k, v, q_offsets, k_offsets, causal, scale, longest_
     dev = _gpu(what, q, k, v, q_offsets, k_offsets, out, *others)
     tq, heads, dim = q.shape
     tk, kv_heads, kdim = k.shape
-    _sizes(what, tq, heads, dim, tk, kv_heads)
+    if (tq | heads | dim | tk | kv_heads) > 0x7FFFFFFF:  # a call costs 0.3 us
+        _too_large(what, tq, heads, dim, tk, kv_heads)
     qt, qh, qe = q.stride()
     kt, kh, ke = k.stride()
     vt, vh, ve = v.stride()
@@ -382,14 +385,16 @@ def _rotary_args(what, q, k, positions, frequencies, q_weight, k_weight, eps, la
         _fail(f"{what}: q must be a float32, float16 or bfloat16 tensor")
     strides = _heads(what, "q", q, None, type_)
     tokens, heads, dim = q.shape
-    _sizes(what, tokens, heads, dim)
+    if (tokens | heads | dim) > 0x7FFFFFFF:
+        _too_large(what, tokens, heads, dim)
     kv = rotary = norm = 0
     kp = pp = fp = wq = wk = None
     wt = torch.float32
     if k is not None:
         kv = k.shape[1] if k.dim() == 3 else 0
         strides += _heads(what, "k", k, (tokens, kv, dim), type_)
-        _sizes(what, kv)
+        if kv > 0x7FFFFFFF:
+            _too_large(what, kv)
         kp = k.data_ptr()
     else:
         strides += (0, 0)
@@ -513,7 +518,8 @@ def _gated_sizes(what, x, w_gate, w_up, activation):
     if w_gate.dim() != 2 or w_gate.dtype != type_ or w_up.shape != w_gate.shape or w_up.dtype != type_:
         _fail(f"{what}: w_gate and w_up must be cols x inner, both of x's type")
     cols, k, gs = _rows(what, "w_gate", w_gate)
-    _sizes(what, cols)
+    if cols > 0x7FFFFFFF:
+        _too_large(what, cols)
     if k != inner:
         _fail(f"{what}: x has {inner} features, w_gate and w_up {k}")
     return TYPES[type_], act, n, inner, cols, xs, gs, _rows(what, "w_up", w_up)[2]
@@ -600,7 +606,8 @@ def attention_shared_prefix(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     if prefix_k.shape[2] > 1 and not pe == ve == 1:
         _fail(f"{what}: the elements of a head of prefix_k and prefix_v must be contiguous")
     tokens = prefix_k.shape[0]
-    _sizes(what, tokens)
+    if tokens > 0x7FFFFFFF:
+        _too_large(what, tokens)
     f = _lib.AttentionPrefix(prefix_k.data_ptr(), prefix_v.data_ptr(), pt, ph, vt, vh, tokens)
     size = _prefix_workspace(tokens, *sizes)
     space = q.new_empty((size,), dtype=torch.uint8) if size else None

@@ -126,7 +126,9 @@ int bs_attention_workspace(const bs_attention_args* args, uint64_t* bytes);
  *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin),  angle = position * frequencies[i]
  * where a pair is (i, i + rotary / 2), or (2 i, 2 i + 1) if `interleaved`.  Angles are reduced in
  * float64, so far positions lose nothing; squares are summed in float32, which holds those of
- * elements up to 2^60.  Elements of a head are contiguous; *_out may be the call's own q and k (or q_grad and k_grad) with their strides. */
+ * elements up to 2^60 and, where eps does not cover them (as 0), of heads whose largest element is
+ * 2^-60 or more.  Elements of a head are contiguous; *_out may be the call's own q and k (or q_grad
+ * and k_grad) with their strides. */
 typedef struct {
     const void* q;
     const void* k;

@@ -183,8 +183,9 @@ int bs_gated(const void* x, int64_t x_stride, const void* w_gate, int64_t w_gate
  *   dgate = dh up act'(gate),  dup = dh act(gate), both rounded to `type` for their products (so in
  *   BS_F16 they are infinite past 65504 and lose bits below 2^-14)
  *   dx = dgate w_gate + dup w_up,  dw_gate = dgate^T x,  dw_up = dup^T x
- * (relu's slope at 0 is 0; infinite gates have the activations' limits).  dx (rows x inner) may be NULL, dw_gate and dw_up (cols x inner) too,
- * both or neither; all contiguous.  The sums over the rows have a fixed order.  workspace:
+ * (relu's slope at 0 is 0; infinite gates have the activations' limits; factors are multiplied in
+ * float32 in this order, so dh up has to lie within its range).  dx (rows x inner) may be NULL,
+ * dw_gate and dw_up (cols x inner) too, both or neither; all contiguous.  The sums over the rows have a fixed order.  workspace:
  * bs_gated_backward_workspace bytes, 16-byte aligned. */
 int bs_gated_backward(const void* dh, int64_t dh_stride, const void* x, int64_t x_stride, const void* w_gate,
                       int64_t w_gate_stride, const void* w_up, int64_t w_up_stride, const void* gate, int64_t gate_stride,
